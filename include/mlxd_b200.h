@@ -41,7 +41,8 @@ enum mlxd_geom {
   MLXD_GEOM_AFFINE = 2  /* core::image::affine, mlx/data/core/image/ImageTransform.cpp:75-111 */
 };
 
-enum mlxd_dtype { MLXD_U8 = 0, MLXD_F32 = 1 };
+/* Batches are MLXD_U8 or MLXD_F32; the attention operators at the end take the others. */
+enum mlxd_dtype { MLXD_U8 = 0, MLXD_F32 = 1, MLXD_BF16 = 2, MLXD_F16 = 3, MLXD_I32 = 4, MLXD_I64 = 5 };
 enum mlxd_mem { MLXD_MEM_HOST = 0, MLXD_MEM_DEVICE = 1 };
 
 /*
@@ -268,6 +269,102 @@ MLXD_API int mlxd_cast_scale_normalise(
     const float* mean, const float* std_, float* dst);
 
 MLXD_API int mlxd_stats_get(mlxd_ctx* ctx, mlxd_stats* out);
+
+/* ---- attention over batches of images and clips ----------------------------
+ * What a model does with a batch once its patches are projected: queries and
+ * keys are turned by where a patch lies (time, row, column), normalised per
+ * head, and text reads the images.  The reference stops at the batch and has
+ * no counterpart.  All memory is device memory of `device`; everything is
+ * queued on the caller's CUDA stream (NULL: the default stream) and may be
+ * captured into a graph.  Nothing is allocated: the calls that need scratch
+ * memory take a workspace, whose contents matter only during the call.  The
+ * structs are read before the call returns.  Results do not depend on the
+ * order in which blocks run: there are no atomic sums. */
+
+/* A [batch, tokens, heads, head_dim] tensor, head_dim contiguous, the other
+ * strides in elements and free (views of a joint projection, for instance). */
+typedef struct mlxd_heads {
+  void* data;
+  int64_t stride_batch, stride_token, stride_head;
+} mlxd_heads;
+
+#define MLXD_ROTARY_MAX_AXES 4
+#define MLXD_ROTARY_MAX_HEAD_DIM 256
+
+/* Rotary positions with several axes.  The pairs of a head are dealt to the
+ * axes: sections[a] pairs to axis a, in order (interleaved == 0) or one in
+ * turn to every axis that has some left (interleaved == 1).  Pair i turns by
+ * the angle float32(position of its axis) * frequencies[i], a float32 product;
+ * (x, y) -> (x cos - y sin, y cos + x sin), inverse: the other way round, which
+ * is the gradient too.  Pairs are (i, i + P), or (2i, 2i + 1) if `adjacent`, with
+ * P = the sum of the sections; elements from 2P on pass through unturned.
+ *
+ * k may be absent (k_heads == 0).  q_out and k_out may be q and k themselves
+ * (same pointer, same strides); other overlaps are not allowed. */
+typedef struct mlxd_rotary_desc {
+  int32_t dtype;                 /* of q, k and their results: MLXD_F32, MLXD_BF16 or MLXD_F16 */
+  int32_t batch, tokens, q_heads, k_heads;
+  int32_t head_dim;              /* even, at most MLXD_ROTARY_MAX_HEAD_DIM */
+  mlxd_heads q, k, q_out, k_out;
+  const void* positions;         /* [n_axes, batch, tokens] */
+  int32_t positions_dtype;       /* MLXD_I32, MLXD_I64 or MLXD_F32 */
+  int64_t positions_stride_axis, positions_stride_batch, positions_stride_token;
+  const float* frequencies;      /* [P] */
+  int32_t n_axes;
+  int32_t sections[MLXD_ROTARY_MAX_AXES];
+  int32_t adjacent, interleaved, inverse;
+  /* the norm in the same pass (mlxd_qk_norm_rotary and its backward): x / sqrt(mean(x^2) + eps) * weight for each head,
+   * ahead of the rotation */
+  const void* q_weight;          /* [head_dim], NULL: all ones */
+  const void* k_weight;
+  int32_t weight_dtype;          /* MLXD_F32, MLXD_BF16 or MLXD_F16 */
+  float eps;
+  /* backward only: the gradients of the results come in here; those of q and k leave in q_out and k_out */
+  mlxd_heads q_grad, k_grad;
+  void* q_weight_grad;           /* [head_dim] of weight_dtype, NULL where the weight is */
+  void* k_weight_grad;
+  void* workspace;               /* mlxd_qk_norm_rotary_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} mlxd_rotary_desc;
+
+MLXD_API int mlxd_rotary(int device, void* cuda_stream, const mlxd_rotary_desc* d);
+MLXD_API int mlxd_qk_norm_rotary(int device, void* cuda_stream, const mlxd_rotary_desc* d);
+/* Bytes that the backward pass needs for the sums of the weights' gradients. */
+MLXD_API int mlxd_qk_norm_rotary_workspace(int device, const mlxd_rotary_desc* d, size_t* bytes);
+MLXD_API int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const mlxd_rotary_desc* d);
+
+#define MLXD_CROSS_MAX_HEAD_DIM 128
+
+/* Cross attention: softmax(scale * q k^T) v, q of `q_tokens` and k, v of
+ * `kv_tokens` tokens; query head h reads key head h / (q_heads / kv_heads).
+ * Sample b reads its first lengths[b] keys (NULL: all; values outside
+ * 0..kv_tokens are taken as the nearest of them), of these the ones whose byte
+ * in key_mask [batch, kv_tokens] is not 0 (NULL: all).  What lies in k and v
+ * where nothing is read has no effect, whatever it is.  A sample with no key
+ * to read gets zeros, -infinity in lse, and gradients of zero.
+ *
+ * lse [batch, q_heads, q_tokens] float32 is the natural logarithm of each
+ * row's sum of exponentials; NULL where no backward pass follows. */
+typedef struct mlxd_cross_desc {
+  int32_t dtype;                 /* of every tensor here: MLXD_BF16 or MLXD_F16 */
+  int32_t batch, q_tokens, kv_tokens, q_heads, kv_heads;
+  int32_t head_dim;              /* a multiple of 8, at most MLXD_CROSS_MAX_HEAD_DIM */
+  float scale;
+  mlxd_heads q, k, v, out;       /* data 16-byte aligned, strides multiples of 8 */
+  float* lse;
+  const void* lengths;
+  int32_t lengths_dtype;         /* MLXD_I32 or MLXD_I64 */
+  const uint8_t* key_mask;
+  int64_t key_mask_stride;       /* between two samples */
+  /* backward only: out and lse as the forward pass left them */
+  mlxd_heads dout, dq, dk, dv;
+  void* workspace;               /* mlxd_cross_attention_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} mlxd_cross_desc;
+
+MLXD_API int mlxd_cross_attention_workspace(int device, const mlxd_cross_desc* d, int backward, size_t* bytes);
+MLXD_API int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cross_desc* d);
+MLXD_API int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libmlxd_b200.so")
 
 OK, ERR_INVALID, ERR_CUDA, ERR_NOMEM, ERR_TIMEOUT, ERR_UNSUPPORTED, ERR_DEVICE = range(7)
 GEOM_NONE, GEOM_RESIZE, GEOM_AFFINE = 0, 1, 2
-U8, F32 = 0, 1
+U8, F32, BF16, F16, I32, I64 = range(6)
 MEM_HOST, MEM_DEVICE = 0, 1
 
 
@@ -61,6 +61,36 @@ class Stats(ctypes.Structure):
         "kernel_ns", "timed_launches", "algo_src_bytes", "algo_dst_bytes", "h2d_ns", "d2h_ns", "host_stage_ns")]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_batch", ctypes.c_int64), ("stride_token", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "tokens", "q_heads", "k_heads", "head_dim")] + [
+        ("q", Heads), ("k", Heads), ("q_out", Heads), ("k_out", Heads),
+        ("positions", ctypes.c_void_p), ("positions_dtype", ctypes.c_int32),
+        ("positions_stride_axis", ctypes.c_int64), ("positions_stride_batch", ctypes.c_int64),
+        ("positions_stride_token", ctypes.c_int64),
+        ("frequencies", ctypes.c_void_p), ("n_axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
+        ("adjacent", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("q_grad", Heads), ("k_grad", Heads), ("q_weight_grad", ctypes.c_void_p), ("k_weight_grad", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class CrossDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "dtype", "batch", "q_tokens", "kv_tokens", "q_heads", "kv_heads", "head_dim")] + [
+        ("scale", ctypes.c_float), ("q", Heads), ("k", Heads), ("v", Heads), ("out", Heads), ("lse", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p), ("lengths_dtype", ctypes.c_int32),
+        ("key_mask", ctypes.c_void_p), ("key_mask_stride", ctypes.c_int64),
+        ("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # numpy mirror of SampleDesc so a whole batch of descriptors is one array
 SAMPLE_DTYPE = np.dtype([
     ("src", np.uint64), ("src_h", np.int32), ("src_w", np.int32),
@@ -79,6 +109,8 @@ EXPORTS = [
     "mlxd_batch_pad", "mlxd_cast_scale_normalise", "mlxd_stats_get",
     "mlxd_device_alloc", "mlxd_device_free", "mlxd_ctx_set_timing", "mlxd_fused_batch_noalloc",
     "mlxd_noalloc_status", "mlxd_stream_status", "mlxd_device_pci_bus_id",
+    "mlxd_rotary", "mlxd_qk_norm_rotary", "mlxd_qk_norm_rotary_workspace", "mlxd_qk_norm_rotary_backward",
+    "mlxd_cross_attention", "mlxd_cross_attention_workspace", "mlxd_cross_attention_backward",
 ]
 NOALLOC_MAX_SAMPLES = 1024
 
@@ -132,6 +164,13 @@ def load():
     lib.mlxd_noalloc_status.argtypes = [i32, vp, ctypes.POINTER(ctypes.c_int32)]
     lib.mlxd_stream_status.argtypes = [vp, vp, ctypes.POINTER(ctypes.c_int32)]
     lib.mlxd_device_pci_bus_id.argtypes = [i32, ctypes.c_char_p, ctypes.c_size_t]
+    size_p = ctypes.POINTER(ctypes.c_size_t)
+    for name in ("mlxd_rotary", "mlxd_qk_norm_rotary", "mlxd_qk_norm_rotary_backward"):
+        getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(RotaryDesc)]
+    lib.mlxd_qk_norm_rotary_workspace.argtypes = [i32, ctypes.POINTER(RotaryDesc), size_p]
+    for name in ("mlxd_cross_attention", "mlxd_cross_attention_backward"):
+        getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(CrossDesc)]
+    lib.mlxd_cross_attention_workspace.argtypes = [i32, ctypes.POINTER(CrossDesc), i32, size_p]
     _lib = lib
     return lib
 
