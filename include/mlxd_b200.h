@@ -349,7 +349,7 @@ typedef struct mlxd_cross_desc {
   int32_t dtype;                 /* of every tensor here: MLXD_BF16 or MLXD_F16 */
   int32_t batch, q_tokens, kv_tokens, q_heads, kv_heads;
   int32_t head_dim;              /* a multiple of 8, at most MLXD_CROSS_MAX_HEAD_DIM */
-  float scale;
+  float scale;                   /* positive */
   mlxd_heads q, k, v, out;       /* data 16-byte aligned, strides multiples of 8 */
   float* lse;
   const void* lengths;
@@ -365,6 +365,11 @@ typedef struct mlxd_cross_desc {
 MLXD_API int mlxd_cross_attention_workspace(int device, const mlxd_cross_desc* d, int backward, size_t* bytes);
 MLXD_API int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cross_desc* d);
 MLXD_API int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d);
+
+/* Self-check word of the kernels of cross attention on this device: waits for `cuda_stream`, stores the word in *status
+ * (0 = clean; 1: a kernel gave up waiting for its own copies or products, which none does unless the device is at fault),
+ * clears it, and returns MLXD_ERR_DEVICE when it was set.  Not under capture. */
+MLXD_API int mlxd_attention_status(int device, void* cuda_stream, int32_t* status);
 
 #ifdef __cplusplus
 }

@@ -111,6 +111,7 @@ EXPORTS = [
     "mlxd_noalloc_status", "mlxd_stream_status", "mlxd_device_pci_bus_id",
     "mlxd_rotary", "mlxd_qk_norm_rotary", "mlxd_qk_norm_rotary_workspace", "mlxd_qk_norm_rotary_backward",
     "mlxd_cross_attention", "mlxd_cross_attention_workspace", "mlxd_cross_attention_backward",
+    "mlxd_attention_status",
 ]
 NOALLOC_MAX_SAMPLES = 1024
 
@@ -171,6 +172,7 @@ def load():
     for name in ("mlxd_cross_attention", "mlxd_cross_attention_backward"):
         getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(CrossDesc)]
     lib.mlxd_cross_attention_workspace.argtypes = [i32, ctypes.POINTER(CrossDesc), i32, size_p]
+    lib.mlxd_attention_status.argtypes = [i32, vp, ctypes.POINTER(ctypes.c_int32)]
     _lib = lib
     return lib
 
@@ -228,6 +230,16 @@ def noalloc_status(device, stream):
     lib = load()
     word = ctypes.c_int32(-1)
     rc = lib.mlxd_noalloc_status(device, ctypes.c_void_p(stream), ctypes.byref(word))
+    if rc not in (OK, ERR_DEVICE):
+        raise MlxdError(rc, lib.mlxd_last_error().decode())
+    return word.value
+
+
+def attention_status(device, stream):
+    """mlxd_attention_status: waits for the stream, returns the self-check word of cross attention's kernels (0 = clean)."""
+    lib = load()
+    word = ctypes.c_int32(-1)
+    rc = lib.mlxd_attention_status(device, ctypes.c_void_p(stream), ctypes.byref(word))
     if rc not in (OK, ERR_DEVICE):
         raise MlxdError(rc, lib.mlxd_last_error().decode())
     return word.value

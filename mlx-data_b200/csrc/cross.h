@@ -1,0 +1,48 @@
+// What the parts of cross attention share.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/mlxd_b200.h"
+
+namespace mlxd {
+
+struct Heads {
+  char* data;
+  int64_t batch, token, head;   // strides in elements
+};
+
+struct CrossParams {
+  Heads q, k, v, out, dout, dq, dk, dv;
+  float* lse;
+  float* delta;                 // [batch, q_heads, q_tokens]: sum of dout * out over a row
+  const void* lengths;
+  int lengths_dtype;
+  const uint8_t* key_mask;
+  int64_t key_mask_stride;
+  int batch, q_tokens, kv_tokens, q_heads, kv_heads, group, head_dim;
+  float scale;
+  int* status;                  // set where a wait ran out
+};
+
+// Tensor maps of a call: boxes of 64 elements by 128 tokens, 128-byte swizzle.
+struct CrossMaps {
+  CUtensorMap q, k, v, out;
+};
+
+int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map);
+
+cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int length_of(const CrossParams& p, int b) {
+  if (!p.lengths) return p.kv_tokens;
+  const int64_t n = p.lengths_dtype == MLXD_I64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
+  return static_cast<int>(n < 0 ? 0 : n > p.kv_tokens ? p.kv_tokens : n);
+}
+#endif
+
+}  // namespace mlxd

@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "attention.h"
+#include "cross.h"
 
 namespace mlxd {
 
@@ -13,29 +14,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kMaxDims = MLXD_CROSS_MAX_HEAD_DIM / 32;   // of a head, for a lane
-
-struct Heads {
-  char* data;
-  int64_t batch, token, head;   // strides in elements
-};
-
-struct CrossParams {
-  Heads q, k, v, out, dout, dq, dk, dv;
-  float* lse;
-  float* delta;                 // [batch, q_heads, q_tokens]: sum of dout * out over a row
-  const void* lengths;
-  int lengths_dtype;
-  const uint8_t* key_mask;
-  int64_t key_mask_stride;
-  int batch, q_tokens, kv_tokens, q_heads, kv_heads, group, head_dim;
-  float scale;
-};
-
-__device__ int length_of(const CrossParams& p, int b) {
-  if (!p.lengths) return p.kv_tokens;
-  const int64_t n = p.lengths_dtype == MLXD_I64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
-  return static_cast<int>(n < 0 ? 0 : n > p.kv_tokens ? p.kv_tokens : n);
-}
 
 __device__ bool is_read(const CrossParams& p, int b, int key) {
   return !p.key_mask || p.key_mask[b * p.key_mask_stride + key];
@@ -64,32 +42,6 @@ __device__ float dot(const float (&a)[kMaxDims], const float (&b)[kMaxDims]) {
   for (int i = 0; i < kMaxDims; i++) s += a[i] * b[i];
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   return s;
-}
-
-// One warp a query row.
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) cross_forward_kernel(const __grid_constant__ CrossParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  if (id >= static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens) return;
-  const int s = id % p.q_tokens, h = id / p.q_tokens % p.q_heads, b = id / p.q_tokens / p.q_heads;
-  float q[kMaxDims], o[kMaxDims] = {}, m = -INFINITY, l = 0;
-  load_row(row_of<T>(p.q, b, s, h), p.head_dim, lane, q);
-  const int n = length_of(p, b);
-  for (int key = 0; key < n; key++) {
-    if (!is_read(p, b, key)) continue;
-    float k[kMaxDims], v[kMaxDims];
-    load_row(row_of<T>(p.k, b, key, h / p.group), p.head_dim, lane, k);
-    load_row(row_of<T>(p.v, b, key, h / p.group), p.head_dim, lane, v);
-    const float x = dot(q, k) * p.scale;
-    const float top = fmaxf(m, x), keep = expf(m - top), e = expf(x - top);
-    m = top;
-    l = l * keep + e;
-    for (int i = 0; i < kMaxDims; i++) o[i] = o[i] * keep + e * v[i];
-  }
-  for (int i = 0; i < kMaxDims; i++) o[i] = l > 0 ? o[i] / l : 0.0f;
-  store_row(const_cast<T*>(row_of<T>(p.out, b, s, h)), p.head_dim, lane, o);
-  if (p.lse && !lane) p.lse[id] = l > 0 ? m + logf(l) : -INFINITY;
 }
 
 // One warp a query row: its delta and the gradient of q.
@@ -170,6 +122,23 @@ int check_sizes(const char* entry, const mlxd_cross_desc* d) {
   return MLXD_OK;
 }
 
+// Set by a kernel whose wait for its own copies or products ran out.
+__device__ int attention_status;
+
+int status_word(int device, int** word) {
+  constexpr int kDevices = 64;
+  static std::atomic<int*> known[kDevices];
+  if (device < 0 || device >= kDevices) return fail(MLXD_ERR_INVALID, "device index out of range");
+  *word = known[device].load(std::memory_order_relaxed);
+  if (!*word) {
+    void* at = nullptr;
+    MLXD_CUDA(cudaGetSymbolAddress(&at, attention_status));
+    *word = static_cast<int*>(at);
+    known[device].store(*word, std::memory_order_relaxed);
+  }
+  return MLXD_OK;
+}
+
 Heads heads_of(const mlxd_heads& h) {
   return Heads{static_cast<char*>(h.data), h.stride_batch, h.stride_token, h.stride_head};
 }
@@ -178,7 +147,7 @@ int params_of(const char* entry, const mlxd_cross_desc* d, bool backward, CrossP
   const auto bad = [&](const std::string& what) { return fail(MLXD_ERR_INVALID, std::string(entry) + ": " + what); };
   const int rc = check_sizes(entry, d);
   if (rc != MLXD_OK) return rc;
-  if (!std::isfinite(d->scale)) return bad("scale must be finite");
+  if (!std::isfinite(d->scale) || d->scale <= 0) return bad("scale must be positive and finite");
   if (d->lengths && d->lengths_dtype != MLXD_I32 && d->lengths_dtype != MLXD_I64) return bad("lengths must be int32 or int64");
   const int b = d->batch, t = d->q_tokens, n = d->kv_tokens, hq = d->q_heads, hk = d->kv_heads;
   struct { const mlxd_heads* h; bool query; const char* name; } need[] = {
@@ -228,6 +197,34 @@ unsigned blocks_of(int64_t warps) {
 }
 
 }  // namespace
+
+// The driver's encoder, found through the runtime: the library links against no driver library.
+int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  Encode encode = known.load(std::memory_order_relaxed);
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    MLXD_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !f) return fail(MLXD_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    encode = reinterpret_cast<Encode>(f);
+    known.store(encode, std::memory_order_relaxed);
+  }
+  const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
+  // strides of dimensions that are not stepped along may be anything; the encoder wants multiples of 16 bytes
+  const auto bytes = [](int64_t stride, int size) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : 16); };
+  const cuuint64_t strides[3] = {bytes(h.token, tokens), bytes(h.head, heads), bytes(h.batch, batch)};
+  const cuuint32_t box[4] = {64, 128, 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, dtype == MLXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, h.data, sizes,
+                            strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MLXD_ERR_INVALID, "cross_attention: a tensor's strides do not fit a tensor map (status " + std::to_string(r) + ")");
+  return MLXD_OK;
+}
+
 }  // namespace mlxd
 
 using namespace mlxd;
@@ -246,16 +243,37 @@ extern "C" int mlxd_cross_attention_workspace(int device, const mlxd_cross_desc*
 extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cross_desc* d) {
   return guarded("cross_attention", [&] {
     CrossParams p;
-    const int rc = params_of("cross_attention", d, false, p);
+    int rc = params_of("cross_attention", d, false, p);
     if (rc != MLXD_OK) return rc;
-    const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens;
-    if (!rows) return static_cast<int>(MLXD_OK);
+    if (!p.batch || !p.q_tokens) return static_cast<int>(MLXD_OK);
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    if (d->dtype == MLXD_F16) cross_forward_kernel<__half><<<blocks_of(rows), 32 * kWarps, 0, s>>>(p);
-    else cross_forward_kernel<__nv_bfloat16><<<blocks_of(rows), 32 * kWarps, 0, s>>>(p);
-    MLXD_CUDA(cudaGetLastError());
+    rc = status_word(device, &p.status);
+    CrossMaps maps;
+    if (rc == MLXD_OK) rc = cross_map(p.q, d->dtype, p.batch, p.q_tokens, p.q_heads, p.head_dim, &maps.q);
+    if (rc == MLXD_OK) rc = cross_map(p.out, d->dtype, p.batch, p.q_tokens, p.q_heads, p.head_dim, &maps.out);
+    if (rc == MLXD_OK && p.kv_tokens) rc = cross_map(p.k, d->dtype, p.batch, p.kv_tokens, p.kv_heads, p.head_dim, &maps.k);
+    if (rc == MLXD_OK && p.kv_tokens) rc = cross_map(p.v, d->dtype, p.batch, p.kv_tokens, p.kv_heads, p.head_dim, &maps.v);
+    if (rc != MLXD_OK) return rc;
+    MLXD_CUDA(launch_cross_forward(p, maps, d->dtype, s));
     return static_cast<int>(MLXD_OK);
+  });
+}
+
+extern "C" int mlxd_attention_status(int device, void* cuda_stream, int32_t* status) {
+  return guarded("attention_status", [&] {
+    if (!status) return fail(MLXD_ERR_INVALID, "attention_status: no place for the result");
+    MLXD_ON_DEVICE(device);
+    int* word = nullptr;
+    const int rc = status_word(device, &word);
+    if (rc != MLXD_OK) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    int32_t got = 0;
+    MLXD_CUDA(cudaMemcpyAsync(&got, word, sizeof(got), cudaMemcpyDeviceToHost, s));
+    MLXD_CUDA(cudaMemsetAsync(word, 0, sizeof(got), s));
+    MLXD_CUDA(cudaStreamSynchronize(s));
+    *status = got;
+    return got ? fail(MLXD_ERR_DEVICE, "attention: a kernel gave up waiting for its own copies or products; its results are not valid") : static_cast<int>(MLXD_OK);
   });
 }
 

@@ -1,0 +1,313 @@
+// Cross attention of many queries: two tiles of 128 query rows a CTA against tiles of 128 keys.
+#include "cross.h"
+#include "sm100.cuh"
+
+namespace mlxd {
+
+namespace {
+
+constexpr int kThreads = 384;          // two warpgroups of softmax, then warps for copies, products, masks
+constexpr int kMaskRing = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+// A row's reference maximum is moved, and what is summed so far scaled, only where the maximum has grown by more than
+// 2^8: the result is the same quotient, and 2^8 is far from the largest float16.
+constexpr float kSlack = 8.0f;
+
+template <int kDim>
+struct Sizes {
+  static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
+  static constexpr int kBoxes = kDim / 64;
+  static constexpr int kSlots = kDim == 128 ? 5 : 8;       // of the ring of keys and values
+  static constexpr int kShared = (2 + kSlots) * kTile + 1024;
+};
+
+template <class T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
+  using S = Sizes<kDim>;
+  extern __shared__ uint8_t shared[];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2];
+  __shared__ uint32_t mask_words[kMaskRing][4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t tiles_at = (smem_address(shared) + 1023) & ~1023u, ring_at = tiles_at + 2 * S::kTile;
+  const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
+                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
+
+  const int q_tiles = (p.q_tokens + 255) / 256;
+  const int q0 = blockIdx.x % q_tiles * 256, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
+  const int length = length_of(p, batch), n = (length + 127) / 128;
+  const int rows = p.q_tokens - q0 > 128 ? 2 : 1;   // tiles of query rows
+  // tiles of keys of which some may not be read: every one under a mask, else the last
+  const auto partial = [&](int j) { return p.key_mask != nullptr || (j + 1) * 128 > length; };
+  const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
+
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (int t = 0; t < 2; t++) {
+      barrier_init(q_full + 8 * t, 1);
+      barrier_init(s_full + 8 * t, 1);
+      barrier_init(p_full + 8 * t, 128);
+      barrier_init(o_full + 8 * t, 1);
+      barrier_init(staged_full + 8 * t, 128);
+    }
+    for (int i = 0; i < S::kSlots; i++) {
+      barrier_init(full + 8 * i, 1);
+      barrier_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kMaskRing; i++) {
+      barrier_init(masked + 8 * i, 1);
+      barrier_init(landed + 8 * i, 1);
+    }
+    barrier_init_done();
+  }
+  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t o_column = 256;   // scores of tile t in columns 128 t, results in 256 + 128 t
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 8 && lane == 0 && n) {
+      // -------------------------------------------------- copies
+      for (int t = 0; t < rows; t++) {
+        barrier_expect(q_full + 8 * t, S::kTile);
+        for (int x = 0; x < S::kBoxes; x++) {
+          tile_load(tiles_at + t * S::kTile + x * kBoxBytes, &maps.q, 64 * x, q0 + 128 * t, head, batch, q_full + 8 * t);
+        }
+      }
+      int issued = 0;
+      for (; issued < 2 * n; issued++) {   // keys of tile 0, values of tile 0, keys of tile 1, ...
+        const int slot = issued % S::kSlots, use = issued / S::kSlots, j = issued / 2;
+        if (use && !barrier_wait(empty + 8 * slot, (use - 1) & 1, &failed)) break;
+        // values of a tile that is not read as a whole go by way of the mask warp
+        const uint32_t bar = issued & 1 && partial(j) ? landed + 8 * (ring_of(j) % kMaskRing) : full + 8 * slot;
+        barrier_expect(bar, S::kTile);
+        for (int x = 0; x < S::kBoxes; x++) {
+          tile_load(ring_at + slot * S::kTile + x * kBoxBytes, issued & 1 ? &maps.v : &maps.k, 64 * x, j * 128,
+                    head / p.group, batch, bar);
+        }
+      }
+      if (failed) {   // what is under way still lands before the CTA ends
+        for (int t = 0; t < rows; t++) {
+          for (int i = 0; i < kWaitTries && !barrier_try(q_full + 8 * t, 0); i++) {}
+        }
+        for (int k = max(0, issued - S::kSlots); k < issued; k++) {
+          const int r = ring_of(k / 2);
+          const bool masks = k & 1 && partial(k / 2);
+          const uint32_t bar = masks ? landed + 8 * (r % kMaskRing) : full + 8 * (k % S::kSlots);
+          for (int i = 0; i < kWaitTries && !barrier_try(bar, (masks ? r / kMaskRing : k / S::kSlots) & 1); i++) {}
+        }
+      }
+    } else if (warp == 9 && lane == 0 && n) {
+      // -------------------------------------------------- products
+      constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
+      const int steps = (p.head_dim + 15) / 16;
+      const auto item_full = [&](int item) { return barrier_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
+      const auto slot_of = [&](int item) { return ring_at + item % S::kSlots * S::kTile; };
+      const auto scores = [&](int t, int j) {   // S = Q K^T
+        for (int k = 0; k < steps; k++) {
+          const uint32_t at = k / 4 * kBoxBytes + k % 4 * 32;
+          product(tmem + 128 * t, at_address(tile_descriptor(16), tiles_at + t * S::kTile + at),
+                  at_address(tile_descriptor(16), slot_of(2 * j) + at), kScores, k > 0);
+        }
+        products_done(s_full + 8 * t);
+      };
+      bool going = item_full(0);
+      for (int t = 0; t < rows && going; t++) {
+        going = barrier_wait(q_full + 8 * t, 0, &failed);
+        if (going) scores(t, 0);
+      }
+      if (going) products_done(empty + 0);
+      for (int j = 0; j < n && going; j++) {
+        going = item_full(2 * j + 1) && (j + 1 == n || item_full(2 * j + 2));
+        for (int t = 0; t < rows && going; t++) {
+          going = barrier_wait(p_full + 8 * t, j & 1, &failed);
+          if (!going) break;
+          tmem_after_sync();
+          // O += P V, P where the scores were
+          for (int k = 0; k < 8; k++) {
+            product_from_tmem(tmem + o_column + 128 * t, tmem + 128 * t + 8 * k,
+                              at_address(tile_descriptor(kBoxBytes), slot_of(2 * j + 1) + 2048 * k), kResults, j > 0 || k > 0);
+          }
+          if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
+          // products run in the order in which they are issued: these scores overwrite P after it has been read
+          if (j + 1 < n) scores(t, j + 1);
+          else products_done(o_full + 8 * t);
+        }
+        if (going && j + 1 < n) products_done(empty + 8 * ((2 * j + 2) % S::kSlots));
+      }
+    } else if (warp == 10) {
+      // -------------------------------------------------- masks: which keys are read, and zeros where values are not
+      for (int j = 0; j < n; j++) {
+        if (!partial(j)) continue;
+        uint32_t words[4];
+        for (int i = 0; i < 4; i++) {
+          const int key = j * 128 + i * 32 + lane;
+          words[i] = __ballot_sync(~0u, key < length && (!p.key_mask || p.key_mask[batch * p.key_mask_stride + key]));
+        }
+        const int item = 2 * j + 1, r = ring_of(j);
+        if (!warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed)) break;
+        const uint32_t values = ring_at + item % S::kSlots * S::kTile;
+        for (int i = 0; i < 4; i++) {
+          if (lane == 0) mask_words[r % kMaskRing][i] = words[i];
+          // 8 lanes a row of 128 bytes
+          for (int row = lane / 8; row < 32; row += 4) {
+            if (words[i] >> row & 1) continue;
+            for (int x = 0; x < S::kBoxes; x++) {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                           : : "r"(values + x * kBoxBytes + (32 * i + row) * 128 + (lane & 7) * 16), "r"(0) : "memory");
+            }
+          }
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) {
+          barrier_arrive(full + 8 * (item % S::kSlots));
+          barrier_arrive(masked + 8 * (r % kMaskRing));
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------------------------------------------- softmax: a thread owns a row
+    const int t = warp / 4, row = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const uint32_t mine = tmem + 128 * t + lanes, result = tmem + o_column + 128 * t + lanes;
+    if (t < rows) {
+      const float c = p.scale * kLog2e;
+      float top = -INFINITY, total = 0;
+      bool going = true;
+      for (int j = 0; j < n; j++) {
+        going = warp_wait(s_full + 8 * t, j & 1, &failed);
+        if (!going) break;
+        tmem_after_sync();
+        uint32_t s[128];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tmem_load<32>(mine + 32 * i, s + 32 * i);
+        tmem_loaded();
+        if (partial(j)) {
+          const int r = ring_of(j);
+          going = warp_wait(masked + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed);
+          if (!going) break;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t word = mask_words[r % kMaskRing][i];
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+              if (!(word >> k & 1)) s[32 * i + k] = __float_as_uint(-INFINITY);
+            }
+          }
+        }
+        float most[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          most[i] = __uint_as_float(s[i]);
+#pragma unroll
+          for (int k = 1; k < 32; k++) most[i] = fmaxf(most[i], __uint_as_float(s[i + 4 * k]));
+        }
+        const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if (j == 0) {
+          top = now;
+        } else {
+          const bool grows = (now - top) * c > kSlack;   // also from -infinity; not where both are
+          if (__any_sync(~0u, grows)) {
+            const float keep = grows ? exp2_of((top - now) * c) : 1.0f;
+            if (grows) top = now;
+            total *= keep;
+            // the products of tile j - 1 were done before the scores of tile j
+#pragma unroll
+            for (int x = 0; x < kDim; x += 32) {
+              uint32_t o[32];
+              tmem_load<32>(result + x, o);
+              tmem_loaded();
+#pragma unroll
+              for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+              tmem_store<32>(result + x, o);
+            }
+          }
+        }
+        const float base = top == -INFINITY ? 0.0f : -top * c;
+        float2 sum[2] = {};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int k = 0; k < 32; k++) {
+            float2 x = make_float2(__uint_as_float(s[64 * i + 2 * k]), __uint_as_float(s[64 * i + 2 * k + 1]));
+            x = fma2(x, make_float2(c, c), make_float2(base, base));
+            x.x = exp2_of(x.x);
+            x.y = exp2_of(x.y);
+            sum[k & 1] = add2(sum[k & 1], x);
+            packed[k] = pack2<T>(x.x, x.y);
+          }
+          tmem_store<32>(mine + 32 * i, packed);
+        }
+        sum[0] = add2(sum[0], sum[1]);
+        total += sum[0].x + sum[0].y;
+        tmem_stored();
+        tmem_before_sync();
+        barrier_arrive(p_full + 8 * t);
+      }
+      if (n && going) going = warp_wait(o_full + 8 * t, 0, &failed);
+      if (going) {
+        tmem_after_sync();
+        const float by = total > 0 ? 1.0f / total : 0.0f;
+        const uint32_t staged = tiles_at + t * S::kTile;   // the queries are no longer needed
+#pragma unroll
+        for (int x = 0; x < kDim; x += 32) {
+          uint32_t o[32] = {};
+          if (n) {
+            tmem_load<32>(result + x, o);
+            tmem_loaded();
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by);
+            const int unit = (x + k) % 64 / 8;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         : : "r"(staged + (x + k) / 64 * kBoxBytes + row * 128 + ((unit ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          }
+        }
+        if (p.lse && q0 + 128 * t + row < p.q_tokens) {
+          p.lse[(static_cast<int64_t>(batch) * p.q_heads + head) * p.q_tokens + q0 + 128 * t + row] =
+              total > 0 ? top * p.scale + logf(total) : -INFINITY;
+        }
+        fence_async_proxy();
+        barrier_arrive(staged_full + 8 * t);
+        if (row == 0 && barrier_wait(staged_full + 8 * t, 0, &failed)) {
+          for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(&maps.out, 64 * x, q0 + 128 * t, head, batch, staged + x * kBoxBytes);
+          tile_stores_read();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tmem_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_free<512>(tmem);
+  if (threadIdx.x == 0 && failed) *p.status = 1;
+}
+
+template <class T, int kDim>
+cudaError_t launch(const CrossParams& p, const CrossMaps& maps, cudaStream_t stream) {
+  constexpr int bytes = Sizes<kDim>::kShared;
+  const cudaError_t e = cudaFuncSetAttribute(cross_forward_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  const unsigned blocks = static_cast<unsigned>((p.q_tokens + 255) / 256) * p.q_heads * p.batch;
+  cross_forward_kernel<T, kDim><<<blocks, kThreads, bytes, stream>>>(p, maps);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream) {
+  if (dtype == MLXD_F16) return p.head_dim > 64 ? launch<__half, 128>(p, maps, stream) : launch<__half, 64>(p, maps, stream);
+  return p.head_dim > 64 ? launch<__nv_bfloat16, 128>(p, maps, stream) : launch<__nv_bfloat16, 64>(p, maps, stream);
+}
+
+}  // namespace mlxd

@@ -1,0 +1,218 @@
+// What the attention kernels need of sm_100a: barriers in shared memory, copies of tensor tiles, matrix products whose
+// accumulators lie in tensor memory.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+namespace mlxd {
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// ---------------------------------------------------------------- barriers
+__device__ __forceinline__ void barrier_init(uint32_t bar, int arrivals) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" : : "r"(bar), "r"(arrivals) : "memory");
+}
+
+__device__ __forceinline__ void barrier_init_done() {
+  asm volatile("fence.mbarrier_init.release.cluster;" : : : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" : : "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" : : "r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      "selp.b32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity), "r"(20000) : "memory");
+  return done;
+}
+
+// Every wait ends: after about two seconds (a try sleeps for 20 us at most) it sets `failed`, which ends the waits of
+// the CTA's other warps too, and returns false; the caller then leaves its loop.
+constexpr int kWaitTries = 100000;
+
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  if (barrier_try(bar, parity)) return true;
+  for (int i = 0; i < kWaitTries; i++) {
+    if (barrier_try(bar, parity)) return true;
+    if (*failed) return false;
+  }
+  *failed = 1;
+  return false;
+}
+
+// The same for a whole warp, which goes on or gives up as one.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  return __all_sync(~0u, barrier_wait(bar, parity, failed));
+}
+
+// Writes of this thread to shared memory are seen by copies and matrix products that are issued after this (and after a
+// barrier, where another thread issues them).
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" : : : "memory");
+}
+
+// ---------------------------------------------------------------- copies of tiles: tensors are [batch][head][token][element]
+__device__ __forceinline__ void tile_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" : : "l"(map) : "memory");
+}
+
+__device__ __forceinline__ void tile_load(uint32_t to, const CUtensorMap* map, int element, int token, int head, int batch, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      : : "r"(to), "l"(map), "r"(element), "r"(token), "r"(head), "r"(batch), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tile_store(const CUtensorMap* map, int element, int token, int head, int batch, uint32_t from) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
+               : : "l"(map), "r"(element), "r"(token), "r"(head), "r"(batch), "r"(from) : "memory");
+}
+
+__device__ __forceinline__ void tile_stores_read() {
+  asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;" : : : "memory");
+}
+
+// ---------------------------------------------------------------- tensor memory
+// kColumns columns of 128 lanes of 32 bits; a whole warp allocates and frees.
+template <int kColumns>
+__device__ __forceinline__ void tmem_alloc(uint32_t to_smem) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" : : "r"(to_smem), "n"(kColumns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+
+template <int kColumns>
+__device__ __forceinline__ void tmem_free(uint32_t at) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" : : "r"(at), "n"(kColumns));
+}
+
+// kN consecutive columns of a thread's lane.  A warp reaches lanes 32 * (warp % 4) to + 31; `at` carries the first of them in its
+// upper half.
+template <int kN> __device__ void tmem_load(uint32_t at, uint32_t* v);
+template <int kN> __device__ void tmem_store(uint32_t at, const uint32_t* v);
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t at, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at));
+}
+template <>
+__device__ __forceinline__ void tmem_store<16>(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" : : "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at) : "memory");
+}
+template <>
+__device__ __forceinline__ void tmem_load<32>(uint32_t at, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]) : "r"(at));
+}
+template <>
+__device__ __forceinline__ void tmem_store<32>(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" : : "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" : : : "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" : : : "memory"); }
+__device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" : : : "memory"); }
+__device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" : : : "memory"); }
+
+// ---------------------------------------------------------------- matrix products
+// Tiles lie in shared memory as the copies leave them: boxes of 64 elements (128 bytes) by 128 tokens, the 16-byte units of a row
+// exchanged by the row's number modulo 8 (128-byte swizzle), boxes of the elements 64 to 127 behind those of 0 to 63.
+constexpr int kBoxBytes = 128 * 128;
+
+// The constant part of a descriptor: 128-byte swizzle, version 1, 1024 bytes from eight tokens to the next eight.
+// `along`: bytes to the next 64 elements where they are the operand's rows (or columns of the result) instead of what is
+// summed over.
+__host__ __device__ constexpr uint64_t tile_descriptor(uint32_t along) {
+  return (uint64_t{2} << 61) | (uint64_t{1} << 46) | (uint64_t{1024 >> 4} << 32) | (static_cast<uint64_t>(along >> 4) << 16);
+}
+
+__device__ __forceinline__ uint64_t at_address(uint64_t descriptor, uint32_t address) {
+  return descriptor | ((address & 0x3ffff) >> 4);
+}
+
+// Instruction descriptor: float32 accumulators, A and B of one 16-bit type; `b_tokens`: B is summed over its tokens (its elements
+// are the columns of the result).
+template <class T>
+__host__ __device__ constexpr uint32_t product_descriptor(int m, int n, bool b_tokens) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  return (1u << 4) | (type << 7) | (type << 10) | (b_tokens ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// One product of 16 along what is summed: D (+)= A B, A and B in shared memory.
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t how, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+      : : "r"(d), "l"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+
+// The same with A in tensor memory, two 16-bit values a column.
+__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t how, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      : : "r"(d), "r"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+
+// The barrier gets an arrival when every product this thread has issued is done.
+__device__ __forceinline__ void products_done(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" : : "r"(bar) : "memory");
+}
+
+// ---------------------------------------------------------------- arithmetic
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// a * b + c for two floats at once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+// Two floats rounded to 16 bits each, the first in the lower half.
+template <class T> __device__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+}  // namespace mlxd
