@@ -30,12 +30,14 @@ struct CrossParams {
 
 // Tensor maps of a call: boxes of 64 elements by 128 tokens, 128-byte swizzle.
 struct CrossMaps {
-  CUtensorMap q, k, v, out;
+  CUtensorMap q, k, v, out, dout, dq, dk, dv;   // forward: the first four; backward: all but out
 };
 
 int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map);
 
 cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
+
+cudaError_t launch_cross_backward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ int length_of(const CrossParams& p, int b) {

@@ -1,7 +1,4 @@
 // Cross attention: entry points, checks, launches.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <cmath>
 #include <cstring>
 
@@ -11,92 +8,6 @@
 namespace mlxd {
 
 namespace {
-
-constexpr int kWarps = 4;
-constexpr int kMaxDims = MLXD_CROSS_MAX_HEAD_DIM / 32;   // of a head, for a lane
-
-__device__ bool is_read(const CrossParams& p, int b, int key) {
-  return !p.key_mask || p.key_mask[b * p.key_mask_stride + key];
-}
-
-template <class T> __device__ const T* row_of(const Heads& h, int64_t b, int64_t s, int64_t head) {
-  return reinterpret_cast<const T*>(h.data) + b * h.batch + s * h.token + head * h.head;
-}
-
-template <class T> __device__ T from_float(float v);
-template <> __device__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <class T> __device__ void load_row(const T* x, int d, int lane, float (&v)[kMaxDims]) {
-  for (int i = 0; i < kMaxDims; i++) v[i] = lane + 32 * i < d ? static_cast<float>(x[lane + 32 * i]) : 0.0f;
-}
-
-template <class T> __device__ void store_row(T* x, int d, int lane, const float (&v)[kMaxDims]) {
-  for (int i = 0; i < kMaxDims; i++) {
-    if (lane + 32 * i < d) x[lane + 32 * i] = from_float<T>(v[i]);
-  }
-}
-
-__device__ float dot(const float (&a)[kMaxDims], const float (&b)[kMaxDims]) {
-  float s = 0;
-  for (int i = 0; i < kMaxDims; i++) s += a[i] * b[i];
-  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-  return s;
-}
-
-// One warp a query row: its delta and the gradient of q.
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) cross_dq_kernel(const __grid_constant__ CrossParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  if (id >= static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens) return;
-  const int s = id % p.q_tokens, h = id / p.q_tokens % p.q_heads, b = id / p.q_tokens / p.q_heads;
-  float q[kMaxDims], o[kMaxDims], g[kMaxDims], dq[kMaxDims] = {};
-  load_row(row_of<T>(p.q, b, s, h), p.head_dim, lane, q);
-  load_row(row_of<T>(p.out, b, s, h), p.head_dim, lane, o);
-  load_row(row_of<T>(p.dout, b, s, h), p.head_dim, lane, g);
-  const float delta = dot(o, g), lse = p.lse[id];
-  if (!lane) p.delta[id] = delta;
-  const int n = length_of(p, b);
-  for (int key = 0; key < n; key++) {
-    if (!is_read(p, b, key)) continue;
-    float k[kMaxDims], v[kMaxDims];
-    load_row(row_of<T>(p.k, b, key, h / p.group), p.head_dim, lane, k);
-    load_row(row_of<T>(p.v, b, key, h / p.group), p.head_dim, lane, v);
-    const float w = expf(dot(q, k) * p.scale - lse), ds = w * (dot(g, v) - delta) * p.scale;
-    for (int i = 0; i < kMaxDims; i++) dq[i] += ds * k[i];
-  }
-  store_row(const_cast<T*>(row_of<T>(p.dq, b, s, h)), p.head_dim, lane, dq);
-}
-
-// One warp a key: the gradients of k and v, summed over the query heads that share it.
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) cross_dkv_kernel(const __grid_constant__ CrossParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  if (id >= static_cast<int64_t>(p.batch) * p.kv_heads * p.kv_tokens) return;
-  const int key = id % p.kv_tokens, hk = id / p.kv_tokens % p.kv_heads, b = id / p.kv_tokens / p.kv_heads;
-  float k[kMaxDims], v[kMaxDims], dk[kMaxDims] = {}, dv[kMaxDims] = {};
-  if (key < length_of(p, b) && is_read(p, b, key)) {
-    load_row(row_of<T>(p.k, b, key, hk), p.head_dim, lane, k);
-    load_row(row_of<T>(p.v, b, key, hk), p.head_dim, lane, v);
-    for (int h = hk * p.group; h < (hk + 1) * p.group; h++) {
-      for (int s = 0; s < p.q_tokens; s++) {
-        const int64_t row = (static_cast<int64_t>(b) * p.q_heads + h) * p.q_tokens + s;
-        float q[kMaxDims], g[kMaxDims];
-        load_row(row_of<T>(p.q, b, s, h), p.head_dim, lane, q);
-        load_row(row_of<T>(p.dout, b, s, h), p.head_dim, lane, g);
-        const float w = expf(dot(q, k) * p.scale - p.lse[row]), ds = w * (dot(g, v) - p.delta[row]) * p.scale;
-        for (int i = 0; i < kMaxDims; i++) {
-          dv[i] += w * g[i];
-          dk[i] += ds * q[i];
-        }
-      }
-    }
-  }
-  store_row(const_cast<T*>(row_of<T>(p.dk, b, key, hk)), p.head_dim, lane, dk);
-  store_row(const_cast<T*>(row_of<T>(p.dv, b, key, hk)), p.head_dim, lane, dv);
-}
 
 // Tensors as the copies into shared memory want them: 16-byte units throughout.  Strides of dimensions that are not
 // stepped along do not matter.
@@ -119,6 +30,7 @@ int check_sizes(const char* entry, const mlxd_cross_desc* d) {
   if (static_cast<int64_t>(d->batch) * d->q_heads > (1 << 24) || static_cast<int64_t>(d->batch) * d->q_heads * d->q_tokens > (int64_t{1} << 33)) {
     return bad("too many rows");
   }
+  if (static_cast<int64_t>(d->batch) * d->kv_heads * ((static_cast<int64_t>(d->kv_tokens) + 127) / 128) > INT32_MAX) return bad("too many keys");
   return MLXD_OK;
 }
 
@@ -192,8 +104,19 @@ size_t workspace_bytes(const mlxd_cross_desc* d, bool backward) {
   return backward ? sizeof(float) * d->batch * d->q_heads * d->q_tokens : 0;
 }
 
-unsigned blocks_of(int64_t warps) {
-  return static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+// Maps of the tensors that a pass copies or stores by tiles; those of empty tensors are left as they are.
+int maps_of(const CrossParams& p, int dtype, bool backward, CrossMaps& m) {
+  struct { const Heads* h; bool query; CUtensorMap* map; } all[] = {
+      {&p.q, true, &m.q}, {&p.k, false, &m.k}, {&p.v, false, &m.v}, {&p.out, true, &m.out},
+      {&p.dout, true, &m.dout}, {&p.dq, true, &m.dq}, {&p.dk, false, &m.dk}, {&p.dv, false, &m.dv}};
+  for (int i = 0; i < (backward ? 8 : 4); i++) {
+    const auto& x = all[i];
+    const int tokens = x.query ? p.q_tokens : p.kv_tokens;
+    if (!tokens || (backward && i == 3)) continue;
+    const int rc = cross_map(*x.h, dtype, p.batch, tokens, x.query ? p.q_heads : p.kv_heads, p.head_dim, x.map);
+    if (rc != MLXD_OK) return rc;
+  }
+  return MLXD_OK;
 }
 
 }  // namespace
@@ -250,10 +173,7 @@ extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cr
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     rc = status_word(device, &p.status);
     CrossMaps maps;
-    if (rc == MLXD_OK) rc = cross_map(p.q, d->dtype, p.batch, p.q_tokens, p.q_heads, p.head_dim, &maps.q);
-    if (rc == MLXD_OK) rc = cross_map(p.out, d->dtype, p.batch, p.q_tokens, p.q_heads, p.head_dim, &maps.out);
-    if (rc == MLXD_OK && p.kv_tokens) rc = cross_map(p.k, d->dtype, p.batch, p.kv_tokens, p.kv_heads, p.head_dim, &maps.k);
-    if (rc == MLXD_OK && p.kv_tokens) rc = cross_map(p.v, d->dtype, p.batch, p.kv_tokens, p.kv_heads, p.head_dim, &maps.v);
+    if (rc == MLXD_OK) rc = maps_of(p, d->dtype, false, maps);
     if (rc != MLXD_OK) return rc;
     MLXD_CUDA(launch_cross_forward(p, maps, d->dtype, s));
     return static_cast<int>(MLXD_OK);
@@ -280,25 +200,18 @@ extern "C" int mlxd_attention_status(int device, void* cuda_stream, int32_t* sta
 extern "C" int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d) {
   return guarded("cross_attention_backward", [&] {
     CrossParams p;
-    const int rc = params_of("cross_attention_backward", d, true, p);
+    int rc = params_of("cross_attention_backward", d, true, p);
     if (rc != MLXD_OK) return rc;
     const size_t need = workspace_bytes(d, true);
     if (need && (!d->workspace || d->workspace_bytes < need)) return fail(MLXD_ERR_INVALID, "cross_attention_backward: workspace too small");
     p.delta = static_cast<float*>(d->workspace);
-    const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens;
-    const int64_t keys = static_cast<int64_t>(p.batch) * p.kv_heads * p.kv_tokens;
+    if (!p.batch) return static_cast<int>(MLXD_OK);
     MLXD_ON_DEVICE(device);
-    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    if (rows) {
-      if (d->dtype == MLXD_F16) cross_dq_kernel<__half><<<blocks_of(rows), 32 * kWarps, 0, s>>>(p);
-      else cross_dq_kernel<__nv_bfloat16><<<blocks_of(rows), 32 * kWarps, 0, s>>>(p);
-      MLXD_CUDA(cudaGetLastError());
-    }
-    if (keys) {
-      if (d->dtype == MLXD_F16) cross_dkv_kernel<__half><<<blocks_of(keys), 32 * kWarps, 0, s>>>(p);
-      else cross_dkv_kernel<__nv_bfloat16><<<blocks_of(keys), 32 * kWarps, 0, s>>>(p);
-      MLXD_CUDA(cudaGetLastError());
-    }
+    rc = status_word(device, &p.status);
+    CrossMaps maps;
+    if (rc == MLXD_OK) rc = maps_of(p, d->dtype, true, maps);
+    if (rc != MLXD_OK) return rc;
+    MLXD_CUDA(launch_cross_backward(p, maps, d->dtype, static_cast<cudaStream_t>(cuda_stream)));
     return static_cast<int>(MLXD_OK);
   });
 }

@@ -18,19 +18,19 @@ struct Sizes {
   static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
   static constexpr int kBoxes = kDim / 64;
   static constexpr int kSlots = kDim == 128 ? 5 : 8;       // of the ring of keys and values
-  static constexpr int kShared = (2 + kSlots) * kTile + 1024;
+  static constexpr int kShared = (2 + kSlots) * kTile;
 };
 
 template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
-  extern __shared__ uint8_t shared[];
+  extern __shared__ __align__(1024) uint8_t shared[];
   __shared__ uint64_t bars[2 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const uint32_t tiles_at = (smem_address(shared) + 1023) & ~1023u, ring_at = tiles_at + 2 * S::kTile;
+  const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
                  p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
 
