@@ -27,6 +27,7 @@ int check_sizes(const char* entry, const mlxd_cross_desc* d) {
   if (d->head_dim < 8 || d->head_dim % 8 || d->head_dim > MLXD_CROSS_MAX_HEAD_DIM) {
     return bad("head_dim must be a multiple of 8 up to " + std::to_string(MLXD_CROSS_MAX_HEAD_DIM) + " (got " + std::to_string(d->head_dim) + ")");
   }
+  if (d->q_tokens > (1 << 30) || d->kv_tokens > (1 << 30)) return bad("more than 2^30 tokens");
   if (static_cast<int64_t>(d->batch) * d->q_heads > (1 << 24) || static_cast<int64_t>(d->batch) * d->q_heads * d->q_tokens > (int64_t{1} << 33)) {
     return bad("too many rows");
   }
@@ -55,6 +56,33 @@ Heads heads_of(const mlxd_heads& h) {
   return Heads{static_cast<char*>(h.data), h.stride_batch, h.stride_token, h.stride_head};
 }
 
+CrossParams sizes_of(const mlxd_cross_desc* d) {
+  CrossParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.batch = d->batch;
+  p.q_tokens = d->q_tokens;
+  p.kv_tokens = d->kv_tokens;
+  p.q_heads = d->q_heads;
+  p.kv_heads = d->kv_heads;
+  p.group = d->q_heads / d->kv_heads;
+  p.head_dim = d->head_dim;
+  p.scale = d->scale;
+  return p;
+}
+
+int workspace_of(int device, const CrossParams& p, bool backward, size_t* bytes) {
+  *bytes = 0;
+  if (backward) {
+    *bytes = sizeof(float) * p.batch * p.q_heads * p.q_tokens;
+  } else if (p.batch && p.q_tokens && takes_steps(p)) {
+    int sms = 0;
+    const int rc = device_sms(device, &sms);
+    if (rc != MLXD_OK) return rc;
+    *bytes = step_workspace(p, sms);
+  }
+  return MLXD_OK;
+}
+
 int params_of(const char* entry, const mlxd_cross_desc* d, bool backward, CrossParams& p) {
   const auto bad = [&](const std::string& what) { return fail(MLXD_ERR_INVALID, std::string(entry) + ": " + what); };
   const int rc = check_sizes(entry, d);
@@ -75,7 +103,7 @@ int params_of(const char* entry, const mlxd_cross_desc* d, bool backward, CrossP
     }
   }
   if (backward && b && t && !d->lse) return bad("lse is needed");
-  std::memset(&p, 0, sizeof(p));
+  p = sizes_of(d);
   p.q = heads_of(d->q);
   p.k = heads_of(d->k);
   p.v = heads_of(d->v);
@@ -89,19 +117,7 @@ int params_of(const char* entry, const mlxd_cross_desc* d, bool backward, CrossP
   p.lengths_dtype = d->lengths_dtype;
   p.key_mask = d->key_mask;
   p.key_mask_stride = d->key_mask_stride;
-  p.batch = b;
-  p.q_tokens = t;
-  p.kv_tokens = n;
-  p.q_heads = hq;
-  p.kv_heads = hk;
-  p.group = hq / hk;
-  p.head_dim = d->head_dim;
-  p.scale = d->scale;
   return MLXD_OK;
-}
-
-size_t workspace_bytes(const mlxd_cross_desc* d, bool backward) {
-  return backward ? sizeof(float) * d->batch * d->q_heads * d->q_tokens : 0;
 }
 
 // Maps of the tensors that a pass copies or stores by tiles; those of empty tensors are left as they are.
@@ -154,12 +170,10 @@ using namespace mlxd;
 
 extern "C" int mlxd_cross_attention_workspace(int device, const mlxd_cross_desc* d, int backward, size_t* bytes) {
   return guarded("cross_attention_workspace", [&] {
-    (void)device;
-    const int rc = check_sizes("cross_attention_workspace", d);
+    int rc = check_sizes("cross_attention_workspace", d);
     if (rc != MLXD_OK) return rc;
     if (!bytes) return fail(MLXD_ERR_INVALID, "cross_attention_workspace: no place for the result");
-    *bytes = workspace_bytes(d, backward != 0);
-    return static_cast<int>(MLXD_OK);
+    return workspace_of(device, sizes_of(d), backward != 0, bytes);
   });
 }
 
@@ -169,13 +183,45 @@ extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cr
     int rc = params_of("cross_attention", d, false, p);
     if (rc != MLXD_OK) return rc;
     if (!p.batch || !p.q_tokens) return static_cast<int>(MLXD_OK);
+    size_t need = 0;
+    rc = workspace_of(device, p, false, &need);
+    if (rc != MLXD_OK) return rc;
+    if (need && (!d->workspace || d->workspace_bytes < need)) return fail(MLXD_ERR_INVALID, "cross_attention: workspace too small");
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    if (takes_steps(p)) {
+      int sms = 0;
+      rc = device_sms(device, &sms);
+      if (rc != MLXD_OK) return rc;
+      MLXD_CUDA(launch_cross_step(p, d->workspace, sms, d->dtype, s));
+      return static_cast<int>(MLXD_OK);
+    }
     rc = status_word(device, &p.status);
     CrossMaps maps;
     if (rc == MLXD_OK) rc = maps_of(p, d->dtype, false, maps);
     if (rc != MLXD_OK) return rc;
     MLXD_CUDA(launch_cross_forward(p, maps, d->dtype, s));
+    return static_cast<int>(MLXD_OK);
+  });
+}
+
+extern "C" int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d) {
+  return guarded("cross_attention_backward", [&] {
+    CrossParams p;
+    int rc = params_of("cross_attention_backward", d, true, p);
+    if (rc != MLXD_OK) return rc;
+    size_t need = 0;
+    rc = workspace_of(device, p, true, &need);
+    if (rc != MLXD_OK) return rc;
+    if (need && (!d->workspace || d->workspace_bytes < need)) return fail(MLXD_ERR_INVALID, "cross_attention_backward: workspace too small");
+    p.delta = static_cast<float*>(d->workspace);
+    if (!p.batch) return static_cast<int>(MLXD_OK);
+    MLXD_ON_DEVICE(device);
+    rc = status_word(device, &p.status);
+    CrossMaps maps;
+    if (rc == MLXD_OK) rc = maps_of(p, d->dtype, true, maps);
+    if (rc != MLXD_OK) return rc;
+    MLXD_CUDA(launch_cross_backward(p, maps, d->dtype, static_cast<cudaStream_t>(cuda_stream)));
     return static_cast<int>(MLXD_OK);
   });
 }
@@ -194,24 +240,5 @@ extern "C" int mlxd_attention_status(int device, void* cuda_stream, int32_t* sta
     MLXD_CUDA(cudaStreamSynchronize(s));
     *status = got;
     return got ? fail(MLXD_ERR_DEVICE, "attention: a kernel gave up waiting for its own copies or products; its results are not valid") : static_cast<int>(MLXD_OK);
-  });
-}
-
-extern "C" int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d) {
-  return guarded("cross_attention_backward", [&] {
-    CrossParams p;
-    int rc = params_of("cross_attention_backward", d, true, p);
-    if (rc != MLXD_OK) return rc;
-    const size_t need = workspace_bytes(d, true);
-    if (need && (!d->workspace || d->workspace_bytes < need)) return fail(MLXD_ERR_INVALID, "cross_attention_backward: workspace too small");
-    p.delta = static_cast<float*>(d->workspace);
-    if (!p.batch) return static_cast<int>(MLXD_OK);
-    MLXD_ON_DEVICE(device);
-    rc = status_word(device, &p.status);
-    CrossMaps maps;
-    if (rc == MLXD_OK) rc = maps_of(p, d->dtype, true, maps);
-    if (rc != MLXD_OK) return rc;
-    MLXD_CUDA(launch_cross_backward(p, maps, d->dtype, static_cast<cudaStream_t>(cuda_stream)));
-    return static_cast<int>(MLXD_OK);
   });
 }
