@@ -19,22 +19,6 @@ struct Sizes {
   static constexpr int kShared = (2 + kSlots) * kTile;
 };
 
-// D (+)= A B of two tiles in shared memory, both summed over their elements.
-template <class S>
-__device__ __forceinline__ void product_of_tiles(uint32_t d, uint32_t a, uint32_t b, uint32_t how, int steps) {
-  for (int k = 0; k < steps; k++) {
-    const uint32_t at = k / 4 * kBoxBytes + k % 4 * 32;
-    product(d, at_address(tile_descriptor(16), a + at), at_address(tile_descriptor(16), b + at), how, k > 0);
-  }
-}
-
-// D (+)= A B, A 128 x 128 in tensor memory in two halves of 64 columns each (of which 32 are used), B a tile summed over its tokens.
-__device__ __forceinline__ void product_over_tokens(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
-  for (int k = 0; k < 8; k++) {
-    product_from_tmem(d, a + k / 4 * 64 + k % 4 * 8, at_address(tile_descriptor(kBoxBytes), b + 2048 * k), how, add || k > 0);
-  }
-}
-
 template <class S>
 __device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* map, int token, int head, int batch, uint32_t bar) {
   barrier_expect(bar, S::kTile);
@@ -49,7 +33,7 @@ __device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, f
     uint32_t o[32] = {};
     if (!zero) {
       tmem_load<32>(tmem + x, o);
-      tmem_loaded();
+      tmem_loaded(o);
     }
 #pragma unroll
     for (int k = 0; k < 32; k += 8) {
@@ -81,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   __shared__ float delta_parts[2][128];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 16, ds_full = dp_full + 8, done = ds_full + 8, delta_full = done + 8,
@@ -136,40 +120,45 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
           for (int i = 0; i < kWaitTries && !barrier_try(bar, (masks ? r / kMaskRing : k / S::kSlots) & 1); i++) {}
         }
       }
-    } else if (warp == 9 && lane == 0 && n) {
+    } else if (warp == 9 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return barrier_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
-      const auto slot_of = [&](int item) { return ring_at + item % S::kSlots * S::kTile; };
+      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
+      const uint32_t queries = low_half(at_address(tile_descriptor(16), q_at)), grads = low_half(at_address(tile_descriptor(16), do_at)),
+                     ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
+      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
       const auto scores = [&](int j) {
-        product_of_tiles<S>(tmem + 128 * (j & 1), q_at, slot_of(2 * j), kScores, steps);
+        product_of_tiles<kDim>(tmem + 128 * (j & 1), queries, ring + slot_of(2 * j), kScores, steps);
         products_done(s_full + 8 * (j & 1));
       };
       const auto dp = [&](int j) {
-        product_of_tiles<S>(tmem + dp_column, do_at, slot_of(2 * j + 1), kScores, steps);
+        product_of_tiles<kDim>(tmem + dp_column, grads, ring + slot_of(2 * j + 1), kScores, steps);
         products_done(dp_full);
         products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
       };
-      bool going = barrier_wait(q_full, 0, &failed) && item_full(0);
-      if (going) scores(0);
-      going = going && barrier_wait(do_full, 0, &failed) && item_full(1);
-      if (going) dp(0);
+      bool going = warp_wait(q_full, 0, &failed) && item_full(0);
+      if (going && elected()) scores(0);
+      __syncwarp();
+      going = going && warp_wait(do_full, 0, &failed) && item_full(1);
+      if (going && elected()) dp(0);
+      __syncwarp();
       going = going && (n == 1 || item_full(2));
-      if (going && n > 1) scores(1);
+      if (going && n > 1 && elected()) scores(1);
+      __syncwarp();
       for (int j = 0; j < n && going; j++) {
-        going = (j + 1 >= n || item_full(2 * j + 3)) && barrier_wait(ds_full, j & 1, &failed);
+        going = (j + 1 >= n || item_full(2 * j + 3)) && (j + 2 >= n || item_full(2 * j + 4)) && warp_wait(ds_full, j & 1, &failed);
         if (!going) break;
         tmem_after_sync();
-        if (j + 1 < n) dp(j + 1);
-        product_over_tokens(tmem + dq_column, tmem + 128 * (j & 1), slot_of(2 * j), kResults, j > 0);
-        products_done(empty + 8 * (2 * j % S::kSlots));
-        if (j + 2 < n) {
-          going = item_full(2 * j + 4);
-          if (going) scores(j + 2);   // overwrites dS of tile j after it has been read
+        if (elected()) {
+          if (j + 1 < n) dp(j + 1);
+          product_over_tokens(tmem + dq_column, tmem + 128 * (j & 1), ring_tokens + slot_of(2 * j), kResults, j > 0);
+          products_done(empty + 8 * (2 * j % S::kSlots));
+          if (j + 2 < n) scores(j + 2);   // overwrites dS of tile j after it has been read
+          if (j + 1 == n) products_done(done);
         }
+        __syncwarp();
       }
-      if (going) products_done(done);
     } else if (warp == 10) {
       // -------------------------------------------------- masks: which keys are read, and zeros where they are not
       for (int j = 0; j < n; j++) {
@@ -238,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
       tmem_after_sync();
       tmem_load<32>(mine, s);
       tmem_load<32>(mine + 32, s + 32);
-      tmem_loaded();
+      tmem_loaded(s);
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {
         const float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), make_float2(c, c), make_float2(base, base));
@@ -260,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
       for (int i = 0; i < 2; i++) {
         uint32_t d[32], packed[16];
         tmem_load<32>(tmem + dp_column + 64 * half + 32 * i + lanes, d);
-        tmem_loaded();
+        tmem_loaded(d);
         if (words[i] == ~0u) {
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
@@ -308,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   __shared__ float4 stats[2][2][32];      // of the queries of a tile: -lse * log2(e), delta
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
   const uint32_t k_full = smem_address(bars), v_full = k_full + 8, full = k_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, done = ds_full + 8,
@@ -354,40 +343,50 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
           for (int i = 0; i < kWaitTries && !barrier_try(full + 8 * (k % S::kSlots), k / S::kSlots & 1); i++) {}
         }
       }
-    } else if (warp == 9 && lane == 0 && n) {
+    } else if (warp == 9 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return barrier_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
-      const auto slot_of = [&](int item) { return ring_at + item % S::kSlots * S::kTile; };
+      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
+      const uint32_t keys = low_half(at_address(tile_descriptor(16), k_at)), values = low_half(at_address(tile_descriptor(16), v_at)),
+                     ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
+      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
       const auto scores = [&](int i) {
-        product_of_tiles<S>(tmem, k_at, slot_of(2 * i), kScores, steps);
+        product_of_tiles<kDim>(tmem, keys, ring + slot_of(2 * i), kScores, steps);
         products_done(s_full);
       };
       const auto dp = [&](int i) {
-        product_of_tiles<S>(tmem + dp_column, v_at, slot_of(2 * i + 1), kScores, steps);
+        product_of_tiles<kDim>(tmem + dp_column, values, ring + slot_of(2 * i + 1), kScores, steps);
         products_done(dp_full);
       };
-      bool going = barrier_wait(k_full, 0, &failed) && item_full(0);
-      if (going) scores(0);
-      going = going && barrier_wait(v_full, 0, &failed) && item_full(1);
-      if (going) dp(0);
+      bool going = warp_wait(k_full, 0, &failed) && item_full(0);
+      if (going && elected()) scores(0);
+      __syncwarp();
+      going = going && warp_wait(v_full, 0, &failed) && item_full(1);
+      if (going && elected()) dp(0);
+      __syncwarp();
       for (int i = 0; i < n && going; i++) {
         const bool more = i + 1 < n;
-        going = (!more || item_full(2 * i + 2)) && barrier_wait(p_full, i & 1, &failed);
+        going = (!more || item_full(2 * i + 2)) && warp_wait(p_full, i & 1, &failed);
         if (!going) break;
         tmem_after_sync();
-        product_over_tokens(tmem + dv_column, tmem, slot_of(2 * i + 1), kResults, i > 0);
-        if (more) scores(i + 1);   // overwrites P after it has been read
-        products_done(empty + 8 * ((2 * i + 1) % S::kSlots));
-        going = (!more || item_full(2 * i + 3)) && barrier_wait(ds_full, i & 1, &failed);
+        if (elected()) {
+          product_over_tokens(tmem + dv_column, tmem, ring_tokens + slot_of(2 * i + 1), kResults, i > 0);
+          if (more) scores(i + 1);   // overwrites P after it has been read
+          products_done(empty + 8 * ((2 * i + 1) % S::kSlots));
+        }
+        __syncwarp();
+        going = (!more || item_full(2 * i + 3)) && warp_wait(ds_full, i & 1, &failed);
         if (!going) break;
         tmem_after_sync();
-        product_over_tokens(tmem + dk_column, tmem + dp_column, slot_of(2 * i), kResults, i > 0);
-        if (more) dp(i + 1);
-        products_done(empty + 8 * (2 * i % S::kSlots));
+        if (elected()) {
+          product_over_tokens(tmem + dk_column, tmem + dp_column, ring_tokens + slot_of(2 * i), kResults, i > 0);
+          if (more) dp(i + 1);
+          products_done(empty + 8 * (2 * i % S::kSlots));
+          if (!more) products_done(done);
+        }
+        __syncwarp();
       }
-      if (going) products_done(done);
     } else if (warp == 10) {
       // -------------------------------------------------- what is known of the queries; -infinity makes P = 0 where there is none
       for (int i = 0; i < n; i++) {
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       tmem_after_sync();
       tmem_load<32>(mine, s);
       tmem_load<32>(mine + 32, s + 32);
-      tmem_loaded();
+      tmem_loaded(s);
       const float4* lse = stats[i & 1][0] + 16 * half;
       const float4* delta = stats[i & 1][1] + 16 * half;
 #pragma unroll
@@ -454,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       for (int x = 0; x < 2; x++) {
         uint32_t d[32], packed[16];
         tmem_load<32>(mine + dp_column + 32 * x, d);
-        tmem_loaded();
+        tmem_loaded(d);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 l = delta[8 * x + k / 4];

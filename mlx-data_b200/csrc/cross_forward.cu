@@ -21,6 +21,51 @@ struct Sizes {
   static constexpr int kShared = (2 + kSlots) * kTile;
 };
 
+// 64 scores of a row; -infinity where a key is not read.
+__device__ __forceinline__ void load_scores(uint32_t at, uint32_t word0, uint32_t word1, uint32_t (&s)[64]) {
+  tmem_load<32>(at, s);
+  tmem_load<32>(at + 32, s + 32);
+  tmem_loaded(s);
+  if ((word0 & word1) != ~0u) {
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+      if (!(word0 >> k & 1)) s[k] = __float_as_uint(-INFINITY);
+      if (!(word1 >> k & 1)) s[32 + k] = __float_as_uint(-INFINITY);
+    }
+  }
+}
+
+__device__ __forceinline__ float most_of(const uint32_t (&s)[64]) {
+  float most[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    most[i] = __uint_as_float(s[i]);
+#pragma unroll
+    for (int k = 1; k < 16; k++) most[i] = fmaxf(most[i], __uint_as_float(s[i + 4 * k]));
+  }
+  return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+}
+
+// exp(score - maximum) of 64 scores, as 2^(c s + base): summed in float32, rounded to 16 bits for the products, stored in the
+// first 32 columns of where they came from.
+template <class T>
+__device__ __forceinline__ void weigh(const uint32_t (&s)[64], float c, float base, float2 (&sum)[2], uint32_t to) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      float2 x = make_float2(__uint_as_float(s[32 * i + 2 * k]), __uint_as_float(s[32 * i + 2 * k + 1]));
+      x = fma2(x, make_float2(c, c), make_float2(base, base));
+      x.x = exp2_of(x.x);
+      x.y = exp2_of(x.y);
+      sum[k & 1] = add2(sum[k & 1], x);
+      packed[k] = pack2<T>(x.x, x.y);
+    }
+    tmem_store<16>(to + 16 * i, packed);
+  }
+}
+
 template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
@@ -29,7 +74,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
                  p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
@@ -101,43 +146,47 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
           for (int i = 0; i < kWaitTries && !barrier_try(bar, (masks ? r / kMaskRing : k / S::kSlots) & 1); i++) {}
         }
       }
-    } else if (warp == 9 && lane == 0 && n) {
+    } else if (warp == 9 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return barrier_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
-      const auto slot_of = [&](int item) { return ring_at + item % S::kSlots * S::kTile; };
+      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
+      const uint32_t queries = low_half(at_address(tile_descriptor(16), tiles_at)), keys = low_half(at_address(tile_descriptor(16), ring_at)),
+                     values = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
+      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
       const auto scores = [&](int t, int j) {   // S = Q K^T
-        for (int k = 0; k < steps; k++) {
-          const uint32_t at = k / 4 * kBoxBytes + k % 4 * 32;
-          product(tmem + 128 * t, at_address(tile_descriptor(16), tiles_at + t * S::kTile + at),
-                  at_address(tile_descriptor(16), slot_of(2 * j) + at), kScores, k > 0);
-        }
+        product_of_tiles<kDim>(tmem + 128 * t, queries + (t * S::kTile >> 4), keys + slot_of(2 * j), kScores, steps);
         products_done(s_full + 8 * t);
       };
       bool going = item_full(0);
       for (int t = 0; t < rows && going; t++) {
-        going = barrier_wait(q_full + 8 * t, 0, &failed);
-        if (going) scores(t, 0);
+        going = warp_wait(q_full + 8 * t, 0, &failed);
+        if (going && elected()) {
+          scores(t, 0);
+          if (t + 1 == rows) products_done(empty + 0);
+        }
+        __syncwarp();
       }
-      if (going) products_done(empty + 0);
       for (int j = 0; j < n && going; j++) {
         going = item_full(2 * j + 1) && (j + 1 == n || item_full(2 * j + 2));
         for (int t = 0; t < rows && going; t++) {
-          going = barrier_wait(p_full + 8 * t, j & 1, &failed);
+          going = warp_wait(p_full + 8 * t, j & 1, &failed);
           if (!going) break;
           tmem_after_sync();
-          // O += P V, P where the scores were
-          for (int k = 0; k < 8; k++) {
-            product_from_tmem(tmem + o_column + 128 * t, tmem + 128 * t + 8 * k,
-                              at_address(tile_descriptor(kBoxBytes), slot_of(2 * j + 1) + 2048 * k), kResults, j > 0 || k > 0);
+          if (elected()) {
+            // O += P V, P where the scores were
+            product_over_tokens(tmem + o_column + 128 * t, tmem + 128 * t, values + slot_of(2 * j + 1), kResults, j > 0);
+            if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
+            // products run in the order in which they are issued: these scores overwrite P after it has been read
+            if (j + 1 < n) {
+              scores(t, j + 1);
+              if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 2) % S::kSlots));
+            } else {
+              products_done(o_full + 8 * t);
+            }
           }
-          if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
-          // products run in the order in which they are issued: these scores overwrite P after it has been read
-          if (j + 1 < n) scores(t, j + 1);
-          else products_done(o_full + 8 * t);
+          __syncwarp();
         }
-        if (going && j + 1 < n) products_done(empty + 8 * ((2 * j + 2) % S::kSlots));
       }
     } else if (warp == 10) {
       // -------------------------------------------------- masks: which keys are read, and zeros where values are not
@@ -184,31 +233,20 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         going = warp_wait(s_full + 8 * t, j & 1, &failed);
         if (!going) break;
         tmem_after_sync();
-        uint32_t s[128];
-#pragma unroll
-        for (int i = 0; i < 4; i++) tmem_load<32>(mine + 32 * i, s + 32 * i);
-        tmem_loaded();
+        uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
         if (partial(j)) {
           const int r = ring_of(j);
           going = warp_wait(masked + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed);
           if (!going) break;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t word = mask_words[r % kMaskRing][i];
-#pragma unroll
-            for (int k = 0; k < 32; k++) {
-              if (!(word >> k & 1)) s[32 * i + k] = __float_as_uint(-INFINITY);
-            }
-          }
+          for (int i = 0; i < 4; i++) words[i] = mask_words[r % kMaskRing][i];
         }
-        float most[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          most[i] = __uint_as_float(s[i]);
-#pragma unroll
-          for (int k = 1; k < 32; k++) most[i] = fmaxf(most[i], __uint_as_float(s[i + 4 * k]));
-        }
-        const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        // 64 scores at a time: the second half for its maximum, the first for both, the second again for its exponentials
+        uint32_t s[64];
+        load_scores(mine + 64, words[2], words[3], s);
+        float now = most_of(s);
+        load_scores(mine, words[0], words[1], s);
+        now = fmaxf(now, most_of(s));
         if (j == 0) {
           top = now;
         } else {
@@ -218,33 +256,22 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
             if (grows) top = now;
             total *= keep;
             // the products of tile j - 1 were done before the scores of tile j
+#pragma unroll 1
+            for (int x = 0; x < kDim; x += 16) {
+              uint32_t o[16];
+              tmem_load<16>(result + x, o);
+              tmem_loaded(o);
 #pragma unroll
-            for (int x = 0; x < kDim; x += 32) {
-              uint32_t o[32];
-              tmem_load<32>(result + x, o);
-              tmem_loaded();
-#pragma unroll
-              for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-              tmem_store<32>(result + x, o);
+              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+              tmem_store<16>(result + x, o);
             }
           }
         }
         const float base = top == -INFINITY ? 0.0f : -top * c;
         float2 sum[2] = {};
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          uint32_t packed[32];
-#pragma unroll
-          for (int k = 0; k < 32; k++) {
-            float2 x = make_float2(__uint_as_float(s[64 * i + 2 * k]), __uint_as_float(s[64 * i + 2 * k + 1]));
-            x = fma2(x, make_float2(c, c), make_float2(base, base));
-            x.x = exp2_of(x.x);
-            x.y = exp2_of(x.y);
-            sum[k & 1] = add2(sum[k & 1], x);
-            packed[k] = pack2<T>(x.x, x.y);
-          }
-          tmem_store<32>(mine + 32 * i, packed);
-        }
+        weigh<T>(s, c, base, sum, mine);
+        load_scores(mine + 64, words[2], words[3], s);
+        weigh<T>(s, c, base, sum, mine + 64);
         sum[0] = add2(sum[0], sum[1]);
         total += sum[0].x + sum[0].y;
         tmem_stored();
@@ -261,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
           uint32_t o[32] = {};
           if (n) {
             tmem_load<32>(result + x, o);
-            tmem_loaded();
+            tmem_loaded(o);
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {

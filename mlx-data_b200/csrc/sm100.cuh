@@ -122,7 +122,18 @@ __device__ __forceinline__ void tmem_store<32>(uint32_t at, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" : : "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(at) : "memory");
 }
 
-__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" : : : "memory"); }
+// Waits for this thread's loads.  The registers they go to are named here, so that nothing that reads them is moved ahead of
+// the wait: a load is under way until then, whatever the compiler thinks of its operands.
+__device__ __forceinline__ void tmem_loaded(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) : : "memory");
+}
+__device__ __forceinline__ void tmem_loaded(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) : : "memory");
+}
+__device__ __forceinline__ void tmem_loaded(uint32_t (&v)[64]) {
+  tmem_loaded(reinterpret_cast<uint32_t (&)[32]>(v));
+  asm volatile("" : "+r"(v[32]), "+r"(v[33]), "+r"(v[34]), "+r"(v[35]), "+r"(v[36]), "+r"(v[37]), "+r"(v[38]), "+r"(v[39]), "+r"(v[40]), "+r"(v[41]), "+r"(v[42]), "+r"(v[43]), "+r"(v[44]), "+r"(v[45]), "+r"(v[46]), "+r"(v[47]), "+r"(v[48]), "+r"(v[49]), "+r"(v[50]), "+r"(v[51]), "+r"(v[52]), "+r"(v[53]), "+r"(v[54]), "+r"(v[55]), "+r"(v[56]), "+r"(v[57]), "+r"(v[58]), "+r"(v[59]), "+r"(v[60]), "+r"(v[61]), "+r"(v[62]), "+r"(v[63]) : : "memory");
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" : : : "memory"); }
 __device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" : : : "memory"); }
 __device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" : : : "memory"); }
@@ -151,20 +162,52 @@ __host__ __device__ constexpr uint32_t product_descriptor(int m, int n, bool b_t
   return (1u << 4) | (type << 7) | (type << 10) | (b_tokens ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// True in one thread of a warp that runs together.  Products are issued behind this, by a warp whose threads have taken every
+// branch and wait before it together.
+__device__ __forceinline__ bool elected() {
+  uint32_t is;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is;
+}
+
+// The half of a descriptor that changes: what lies `bytes` (a multiple of 16) further has `bytes >> 4` added, and nothing is carried,
+// since shared memory ends below 2^18.
+__device__ __forceinline__ uint32_t low_half(uint64_t descriptor) { return static_cast<uint32_t>(descriptor); }
+constexpr uint32_t kHighHalf = static_cast<uint32_t>(tile_descriptor(16) >> 32);
+
 // One product of 16 along what is summed: D (+)= A B, A and B in shared memory.
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t how, bool add) {
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-      : : "r"(d), "l"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) : "memory");
+      "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %5, 0;\n"
+      "mov.b64 a, {%1, %4};\nmov.b64 b, {%2, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}"
+      : : "r"(d), "r"(a), "r"(b), "r"(how), "r"(kHighHalf), "r"(static_cast<uint32_t>(add)) : "memory");
 }
 
 // The same with A in tensor memory, two 16-bit values a column.
-__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t how, bool add) {
+__device__ __forceinline__ void product_from_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      : : "r"(d), "r"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) : "memory");
+      "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %5, 0;\n"
+      "mov.b64 b, {%2, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}"
+      : : "r"(d), "r"(a), "r"(b), "r"(how), "r"(kHighHalf), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+
+// D = A B of two tiles in shared memory, both summed over their elements, `steps` times 16 of them.
+template <int kDim>
+__device__ __forceinline__ void product_of_tiles(uint32_t d, uint32_t a, uint32_t b, uint32_t how, int steps) {
+#pragma unroll
+  for (int k = 0; k < kDim / 16; k++) {
+    const uint32_t at = (k / 4 * kBoxBytes + k % 4 * 32) >> 4;
+    if (k < steps) product(d, a + at, b + at, how, k > 0);
+  }
+}
+
+// D (+)= A B, A 128 x 128 in tensor memory, each half of 64 of its columns in the first 32 columns of 64; B a tile summed over
+// its tokens.
+__device__ __forceinline__ void product_over_tokens(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) product_from_tmem(d, a + k / 4 * 64 + k % 4 * 8, b + (2048 * k >> 4), how, add || k > 0);
 }
 
 // The barrier gets an arrival when every product this thread has issued is done.
