@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, done}) barrier_init(bar, 1);
-    for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 256);
+    for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
       barrier_init(empty + 8 * i, 1);
@@ -152,7 +152,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
         tmem_after_sync();
         if (elected()) {
           if (j + 1 < n) dp(j + 1);
-          product_over_tokens(tmem + dq_column, tmem + 128 * (j & 1), ring_tokens + slot_of(2 * j), kResults, j > 0);
+          const uint32_t ds = tmem + 128 * (j & 1), k = ring_tokens + slot_of(2 * j);
+          product_over_tokens(tmem + dq_column, ds, k, kResults, j > 0);
+          product_over_tokens(tmem + dq_column, ds + 64, k + kHalfTokens, kResults, true);
           products_done(empty + 8 * (2 * j % S::kSlots));
           if (j + 2 < n) scores(j + 2);   // overwrites dS of tile j after it has been read
           if (j + 1 == n) products_done(done);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
       }
     }
     delta_parts[half][row] = part;
-    barrier_arrive(delta_full);
+    warp_arrive(delta_full, lane);
     bool going = warp_wait(delta_full, 0, &failed);
     const float delta = going ? delta_parts[0][row] + delta_parts[1][row] : 0.0f;
     if (there && half == 0) p.delta[stat] = delta;
@@ -269,14 +271,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
       }
       tmem_stored();
       tmem_before_sync();
-      barrier_arrive(ds_full);
+      warp_arrive(ds_full, lane);
     }
     if (n && going) going = warp_wait(done, 0, &failed);
     if (going) {
       tmem_after_sync();
       if (half == 0) stage_row<T, kDim>(tmem + dq_column + lanes, q_at, row, p.scale, n == 0);
       fence_async_proxy();
-      barrier_arrive(staged_full);
+      warp_arrive(staged_full, lane);
       if (threadIdx.x == 0 && barrier_wait(staged_full, 0, &failed)) store_tile<S>(&maps.dq, p.head_dim, q0, head, batch, q_at);
     }
   }
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8}) barrier_init(bar, 1);
-    for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 256);
+    for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 8);
     for (const uint32_t bar : {stats_empty, stats_empty + 8}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
@@ -371,7 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          product_over_tokens(tmem + dv_column, tmem, ring_tokens + slot_of(2 * i + 1), kResults, i > 0);
+          const uint32_t g = ring_tokens + slot_of(2 * i + 1);
+          product_over_tokens(tmem + dv_column, tmem, g, kResults, i > 0);
+          product_over_tokens(tmem + dv_column, tmem + 64, g + kHalfTokens, kResults, true);
           if (more) scores(i + 1);   // overwrites P after it has been read
           products_done(empty + 8 * ((2 * i + 1) % S::kSlots));
         }
@@ -380,7 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          product_over_tokens(tmem + dk_column, tmem + dp_column, ring_tokens + slot_of(2 * i), kResults, i > 0);
+          const uint32_t q = ring_tokens + slot_of(2 * i);
+          product_over_tokens(tmem + dk_column, tmem + dp_column, q, kResults, i > 0);
+          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, q + kHalfTokens, kResults, true);
           if (more) dp(i + 1);
           products_done(empty + 8 * (2 * i % S::kSlots));
           if (!more) products_done(done);
@@ -445,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       }
       tmem_stored();
       tmem_before_sync();
-      barrier_arrive(p_full);
+      warp_arrive(p_full, lane);
       going = warp_wait(dp_full, i & 1, &failed);
       if (!going) break;
       tmem_after_sync();
@@ -467,11 +473,10 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
         }
         tmem_store<16>(mine + dp_column + 16 * x, packed);
       }
-      __syncwarp();
-      if (lane == 0) barrier_arrive(stats_empty + 8 * (i & 1));
+      warp_arrive(stats_empty + 8 * (i & 1), lane);
       tmem_stored();
       tmem_before_sync();
-      barrier_arrive(ds_full);
+      warp_arrive(ds_full, lane);
     }
     if (n && going) going = warp_wait(done, 0, &failed);
     if (going) {   // the first warpgroup stores dV, the second dK, out of the ring, which is no longer needed
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       const uint32_t staged = ring_at + half * S::kTile;
       stage_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, staged, row, half ? p.scale : 1.0f, n == 0);
       fence_async_proxy();
-      barrier_arrive(staged_full);
+      warp_arrive(staged_full, lane);
       if (row == 0 && barrier_wait(staged_full, 0, &failed)) store_tile<S>(half ? &maps.dk : &maps.dv, p.head_dim, k0, kv_head, batch, staged);
     }
   }

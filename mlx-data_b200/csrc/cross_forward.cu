@@ -12,7 +12,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference maximum is moved, and what is summed so far scaled, only where the maximum has grown by more than
 // 2^8: the result is the same quotient, and 2^8 is far from the largest float16.
 constexpr float kSlack = 8.0f;
-
 template <int kDim>
 struct Sizes {
   static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
@@ -33,6 +32,14 @@ __device__ __forceinline__ void load_scores(uint32_t at, uint32_t word0, uint32_
       if (!(word1 >> k & 1)) s[32 + k] = __float_as_uint(-INFINITY);
     }
   }
+}
+
+__device__ __forceinline__ void swap_halves(uint32_t (&words)[4]) {
+  const uint32_t a = words[0], b = words[1];
+  words[0] = words[2];
+  words[1] = words[3];
+  words[2] = a;
+  words[3] = b;
 }
 
 __device__ __forceinline__ float most_of(const uint32_t (&s)[64]) {
@@ -70,14 +77,14 @@ template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 8 + 2 * kMaskRing + 2];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
-                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
+                 p_full = s_full + 16, o_full = p_full + 32, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
 
   const int q_tiles = (p.q_tokens + 255) / 256;
   const int q0 = blockIdx.x % q_tiles * 256, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
@@ -92,9 +99,10 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
-      barrier_init(p_full + 8 * t, 128);
+      barrier_init(p_full + 8 * t, 4);         // the first half of a tile's keys
+      barrier_init(p_full + 16 + 8 * t, 4);    // the second
       barrier_init(o_full + 8 * t, 1);
-      barrier_init(staged_full + 8 * t, 128);
+      barrier_init(staged_full + 8 * t, 4);
     }
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
@@ -150,15 +158,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
       const uint32_t queries = low_half(at_address(tile_descriptor(16), tiles_at)), keys = low_half(at_address(tile_descriptor(16), ring_at)),
                      values = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
-      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
-      const auto scores = [&](int t, int j) {   // S = Q K^T
-        product_of_tiles<kDim>(tmem + 128 * t, queries + (t * S::kTile >> 4), keys + slot_of(2 * j), kScores, steps);
+      const auto scores = [&](int t, uint32_t slot) {   // S = Q K^T
+        product_of_tiles<kDim>(tmem + 128 * t, queries + t * (S::kTile >> 4), keys + slot * (S::kTile >> 4), kScores, steps);
         products_done(s_full + 8 * t);
       };
-      bool going = item_full(0);
+      Ring<S::kSlots> at;                               // the item that is needed next
+      bool going = warp_wait(full, 0, &failed);
       for (int t = 0; t < rows && going; t++) {
         going = warp_wait(q_full + 8 * t, 0, &failed);
         if (going && elected()) {
@@ -167,20 +174,34 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         }
         __syncwarp();
       }
+      at.next();
+#pragma unroll 1
       for (int j = 0; j < n && going; j++) {
-        going = item_full(2 * j + 1) && (j + 1 == n || item_full(2 * j + 2));
+        const uint32_t v_slot = at.slot;
+        going = warp_wait(full + 8 * v_slot, at.phase, &failed);
+        at.next();
+        const uint32_t k_slot = at.slot;
+        if (j + 1 < n) going = going && warp_wait(full + 8 * k_slot, at.phase, &failed);
+        at.next();
+#pragma unroll 1
         for (int t = 0; t < rows && going; t++) {
+          // O += P V, P where the scores were; the first half of the keys while the second is being worked on
+          const uint32_t o = tmem + o_column + 128 * t, v = values + v_slot * (S::kTile >> 4);
           going = warp_wait(p_full + 8 * t, j & 1, &failed);
           if (!going) break;
           tmem_after_sync();
+          if (elected()) product_over_tokens(o, tmem + 128 * t, v, kResults, j > 0);
+          __syncwarp();
+          going = warp_wait(p_full + 16 + 8 * t, j & 1, &failed);
+          if (!going) break;
+          tmem_after_sync();
           if (elected()) {
-            // O += P V, P where the scores were
-            product_over_tokens(tmem + o_column + 128 * t, tmem + 128 * t, values + slot_of(2 * j + 1), kResults, j > 0);
-            if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
+            product_over_tokens(o, tmem + 128 * t + 64, v + kHalfTokens, kResults, true);
+            if (t + 1 == rows) products_done(empty + 8 * v_slot);
             // products run in the order in which they are issued: these scores overwrite P after it has been read
             if (j + 1 < n) {
-              scores(t, j + 1);
-              if (t + 1 == rows) products_done(empty + 8 * ((2 * j + 2) % S::kSlots));
+              scores(t, k_slot);
+              if (t + 1 == rows) products_done(empty + 8 * k_slot);
             } else {
               products_done(o_full + 8 * t);
             }
@@ -241,12 +262,16 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
 #pragma unroll
           for (int i = 0; i < 4; i++) words[i] = mask_words[r % kMaskRing][i];
         }
-        // 64 scores at a time: the second half for its maximum, the first for both, the second again for its exponentials
+        // 64 scores at a time, read twice: for their maximum and for their exponentials.  Loops, not copies of their bodies: the
+        // roles of a CTA share the instruction caches, and the warp that issues products suffers when they do not fit.
         uint32_t s[64];
-        load_scores(mine + 64, words[2], words[3], s);
-        float now = most_of(s);
-        load_scores(mine, words[0], words[1], s);
-        now = fmaxf(now, most_of(s));
+        float now = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          load_scores(mine + 64 * h, words[0], words[1], s);
+          now = fmaxf(now, most_of(s));
+          swap_halves(words);
+        }
         if (j == 0) {
           top = now;
         } else {
@@ -269,14 +294,17 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         }
         const float base = top == -INFINITY ? 0.0f : -top * c;
         float2 sum[2] = {};
-        weigh<T>(s, c, base, sum, mine);
-        load_scores(mine + 64, words[2], words[3], s);
-        weigh<T>(s, c, base, sum, mine + 64);
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          load_scores(mine + 64 * h, words[0], words[1], s);
+          weigh<T>(s, c, base, sum, mine + 64 * h);
+          swap_halves(words);
+          tmem_stored();
+          tmem_before_sync();
+          warp_arrive(p_full + 16 * h + 8 * t, lane);
+        }
         sum[0] = add2(sum[0], sum[1]);
         total += sum[0].x + sum[0].y;
-        tmem_stored();
-        tmem_before_sync();
-        barrier_arrive(p_full + 8 * t);
       }
       if (n && going) going = warp_wait(o_full + 8 * t, 0, &failed);
       if (going) {
@@ -305,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
               total > 0 ? top * p.scale + logf(total) : -INFINITY;
         }
         fence_async_proxy();
-        barrier_arrive(staged_full + 8 * t);
+        warp_arrive(staged_full + 8 * t, lane);
         if (row == 0 && barrier_wait(staged_full + 8 * t, 0, &failed)) {
           for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(&maps.out, 64 * x, q0 + 128 * t, head, batch, staged + x * kBoxBytes);
           tile_stores_read();

@@ -62,6 +62,24 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(~0u, barrier_wait(bar, parity, failed));
 }
 
+// Where one is in a ring of kSlots slots: the slot, and the parity of its use.
+template <int kSlots>
+struct Ring {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == kSlots) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// One arrival for a warp, after what its threads did.  (An arrival of every thread is served one at a time.)
+__device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
+  __syncwarp();
+  if (lane == 0) barrier_arrive(bar);
+}
+
 // Writes of this thread to shared memory are seen by copies and matrix products that are issued after this (and after a
 // barrier, where another thread issues them).
 __device__ __forceinline__ void fence_async_proxy() {
@@ -203,11 +221,12 @@ __device__ __forceinline__ void product_of_tiles(uint32_t d, uint32_t a, uint32_
   }
 }
 
-// D (+)= A B, A 128 x 128 in tensor memory, each half of 64 of its columns in the first 32 columns of 64; B a tile summed over
-// its tokens.
+// D (+)= A B over 64 tokens: A 128 x 64 in 32 columns of tensor memory, B half a tile summed over its tokens (the second half lies
+// kHalfTokens further).
+constexpr uint32_t kHalfTokens = 4 * 2048 >> 4;
 __device__ __forceinline__ void product_over_tokens(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
 #pragma unroll
-  for (int k = 0; k < 8; k++) product_from_tmem(d, a + k / 4 * 64 + k % 4 * 8, b + (2048 * k >> 4), how, add || k > 0);
+  for (int k = 0; k < 4; k++) product_from_tmem(d, a + k * 8, b + (2048 * k >> 4), how, add || k > 0);
 }
 
 // The barrier gets an arrival when every product this thread has issued is done.
