@@ -7,12 +7,14 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "sm100.cuh"
 
 namespace mlxd {
 
 namespace {
 
 constexpr int kWarps = 4;                                // of a CTA
+constexpr int kBackwardBlocks = 3;                       // CTAs of an SM in the backward pass
 constexpr int kMaxPairs = MLXD_ROTARY_MAX_HEAD_DIM / 2;
 
 struct Heads {
@@ -33,7 +35,9 @@ struct RotaryParams {
   int positions_dtype, weight_dtype, adjacent;
   float sign, eps;              // sign: -1 turns back
   int lanes;                    // of a warp for one head, a power of two
-  int parts, part_heads;        // forward: a token's heads are cut into so many parts
+  int q_rounds, k_rounds;       // forward: rounds of 32 / lanes heads of a token,
+  int parts, part_rounds;       // cut into so many parts
+  float inverse_dim;            // 1 / head_dim
   int q_blocks;                 // backward: CTAs that take queries
   uint32_t axes[kMaxPairs / 16];   // axis of a pair, two bits each
 };
@@ -82,9 +86,10 @@ __device__ void elements_of(const RotaryParams& p, int i, int& lo, int& hi) {
   }
 }
 
-// How a warp lies over a head.  A lane owns units of kV pairs: two vectors of kV elements (the low and the high elements of its
-// pairs, or, where pairs are neighbours, 2 kV elements in a row).  kL lanes cover a head, so a warp takes 32 / kL heads at once;
-// kUnits > 1 only where a lane takes single pairs (kV == 1) of a head of more than 64 elements.
+// How a warp lies over a head.  A lane owns kN pairs of a head: kUnits units of kV pairs, whose elements are two vectors of kV (the low
+// and the high elements of its pairs, or, where pairs are neighbours, 2 kV elements in a row).  p.lanes lanes cover a head, so a
+// warp takes 32 / lanes heads at once; kUnits > 1 only where a lane takes single pairs (kV == 1) of a head of more than 64 elements.
+// Arithmetic runs on two pairs at once (f32x2).
 template <class T, int kV>
 struct alignas(sizeof(T) * kV) Vec {
   T v[kV];
@@ -92,9 +97,18 @@ struct alignas(sizeof(T) * kV) Vec {
 
 template <class T, int kV, int kUnits, bool kAdjacent>
 struct Lane {
+  static constexpr int kN = kV * kUnits;
   int at[kUnits][2];            // first elements of the two vectors
   bool owns[kUnits];
-  float2 turn[kUnits * kV];     // cos, sin of the pairs
+
+  struct Raw {
+    Vec<T, kV> v[kUnits][2];
+  };
+
+  // Elements a and b of the lane's pairs.
+  struct Pairs {
+    float a[kN], b[kN];
+  };
 
   __device__ Lane(const RotaryParams& p, int first) {
     for (int k = 0; k < kUnits; k++) {
@@ -112,22 +126,18 @@ struct Lane {
     }
   }
 
-  // The warp works out each angle of its token once, in `table`, and every lane takes those of its pairs.
-  __device__ void angles(const RotaryParams& p, int lane, int first, uint32_t row, float2* table) {
-    const uint32_t b = row / p.tokens, s = row - b * p.tokens;
-    for (int i = lane; i < p.head_dim / 2; i += 32) table[i] = unit_of(p, i, b, s);
-    __syncwarp();
+  // Cosines and sines of the lane's pairs out of the warp's table.
+  __device__ void angles(const float2* table, int first, Pairs& u) const {
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
 #pragma unroll
-      for (int j = 0; j < kV; j++) turn[k * kV + j] = owns[k] ? table[(first + 32 * k) * kV + j] : make_float2(1.0f, 0.0f);
+      for (int j = 0; j < kV; j++) {
+        const float2 x = owns[k] ? table[(first + 32 * k) * kV + j] : make_float2(1.0f, 0.0f);
+        u.a[k * kV + j] = x.x;
+        u.b[k * kV + j] = x.y;
+      }
     }
-    __syncwarp();
   }
-
-  struct Raw {
-    Vec<T, kV> v[kUnits][2];
-  };
 
   __device__ void load(const T* x, bool there, Raw& r) const {
 #pragma unroll
@@ -139,112 +149,164 @@ struct Lane {
     }
   }
 
-  __device__ void widen(const Raw& r, float (&e)[kUnits][2 * kV]) const {
+  // Where in a unit's 2 kV elements those of pair j are.
+  static __device__ constexpr int low(int j) { return kAdjacent ? 2 * j : j; }
+  static __device__ constexpr int high(int j) { return kAdjacent ? 2 * j + 1 : kV + j; }
+
+  // Lanes beyond the head hold zeros: their part of `r` is zero from the beginning and never loaded.
+  __device__ void widen(const Raw& r, Pairs& e) const {
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
+      if constexpr (sizeof(T) == 2 && kV > 1) {
 #pragma unroll
-      for (int j = 0; j < kV; j++) {
-        e[k][j] = owns[k] ? to_float(r.v[k][0].v[j]) : 0.0f;
-        e[k][kV + j] = owns[k] ? to_float(r.v[k][1].v[j]) : 0.0f;
+        for (int i = 0; i < kV; i++) {   // words of two elements: first those of the low vector
+          const float2 x = unpack2<T>(reinterpret_cast<const uint32_t*>(r.v[k])[i]);
+          if (kAdjacent) {
+            e.a[k * kV + i] = x.x;
+            e.b[k * kV + i] = x.y;
+          } else {
+            float* to = i < kV / 2 ? e.a : e.b;
+            to[k * kV + 2 * i % kV] = x.x;
+            to[k * kV + 2 * i % kV + 1] = x.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kV; j++) {
+          e.a[k * kV + j] = to_float(r.v[k][low(j) / kV].v[low(j) % kV]);
+          e.b[k * kV + j] = to_float(r.v[k][high(j) / kV].v[high(j) % kV]);
+        }
       }
     }
   }
 
-  __device__ void store(T* x, const float (&e)[kUnits][2 * kV]) const {
+  __device__ void store(T* x, const Pairs& e) const {
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
       if (!owns[k]) continue;
       Vec<T, kV> v[2];
+      if constexpr (sizeof(T) == 2 && kV > 1) {
 #pragma unroll
-      for (int j = 0; j < kV; j++) {
-        v[0].v[j] = from_float<T>(e[k][j]);
-        v[1].v[j] = from_float<T>(e[k][kV + j]);
+        for (int i = 0; i < kV; i++) {
+          const float* from = i < kV / 2 ? e.a : e.b;
+          reinterpret_cast<uint32_t*>(v)[i] = kAdjacent ? pack2<T>(e.a[k * kV + i], e.b[k * kV + i])
+                                                        : pack2<T>(from[k * kV + 2 * i % kV], from[k * kV + 2 * i % kV + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kV; j++) {
+          v[low(j) / kV].v[low(j) % kV] = from_float<T>(e.a[k * kV + j]);
+          v[high(j) / kV].v[high(j) % kV] = from_float<T>(e.b[k * kV + j]);
+        }
       }
       *reinterpret_cast<Vec<T, kV>*>(x + at[k][0]) = v[0];
       *reinterpret_cast<Vec<T, kV>*>(x + at[k][1]) = v[1];
     }
   }
 
-  __device__ void turned(float (&e)[kUnits][2 * kV]) const {
+  // Values of a vector over the head (weights in shared memory) at the lane's elements.
+  __device__ void gather(const float* w, Pairs& e) const {
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
 #pragma unroll
       for (int j = 0; j < kV; j++) {
-        const int lo = kAdjacent ? 2 * j : j, hi = kAdjacent ? 2 * j + 1 : kV + j;
-        const float2 u = turn[k * kV + j];
-        const float a = e[k][lo], b = e[k][hi];
-        e[k][lo] = a * u.x - b * u.y;
-        e[k][hi] = b * u.x + a * u.y;
-      }
-    }
-  }
-
-  __device__ void weights(const void* w, int dtype, float (&e)[kUnits][2 * kV]) const {
-#pragma unroll
-    for (int k = 0; k < kUnits; k++) {
-#pragma unroll
-      for (int j = 0; j < kV; j++) {
-        e[k][j] = owns[k] ? weight_at(w, dtype, at[k][0] + j) : 0.0f;
-        e[k][kV + j] = owns[k] ? weight_at(w, dtype, at[k][1] + j) : 0.0f;
+        e.a[k * kV + j] = owns[k] ? w[at[k][low(j) / kV] + low(j) % kV] : 0.0f;
+        e.b[k * kV + j] = owns[k] ? w[at[k][high(j) / kV] + high(j) % kV] : 0.0f;
       }
     }
   }
 };
+
+// Two neighbouring values of an array.
+__device__ __forceinline__ float2 two(const float* v, int i) { return make_float2(v[i], v[i + 1]); }
+__device__ __forceinline__ void put(float* v, int i, float2 x) {
+  v[i] = x.x;
+  v[i + 1] = x.y;
+}
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 __device__ float lanes_sum(float v, int lanes) {
   for (int d = lanes >> 1; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
   return v;
 }
 
-// One warp a token, or a part of its heads where tokens are few: cosines and sines once, then its heads, 32 / lanes at a time.
-// The next heads are loaded while these are worked on.
+__device__ void read_weights(const RotaryParams& p, float (&w)[2][MLXD_ROTARY_MAX_HEAD_DIM]) {
+  for (int i = threadIdx.x; i < p.head_dim; i += 32 * kWarps) {
+    w[0][i] = weight_at(p.q_weight, p.weight_dtype, i);
+    w[1][i] = weight_at(p.k_weight, p.weight_dtype, i);
+  }
+  __syncthreads();
+}
+
+// One warp a token, or a part of its heads where tokens are few: each angle of the token once, then its heads, 32 / lanes at a time,
+// queries first.  The next heads are loaded while these are worked on.
 template <class T, int kV, int kUnits, bool kAdjacent, bool kNorm>
 __global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ float2 table[kWarps][kMaxPairs];
-  const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), warp = threadIdx.x / 32;
-  const uint32_t item = blockIdx.x * kWarps + warp;
-  const uint32_t row = item / p.parts, part = item - row * p.parts;
-  if (row >= p.rows) return;
-  const int64_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
-  Lane<T, kV, kUnits, kAdjacent> me(p, first);
-  const int step = 32 / p.lanes;
-  const int heads = p.q_heads + p.k_heads, end = min(heads, static_cast<int>(part + 1) * p.part_heads);
-  const auto source = [&](int h) {
-    const bool is_k = h >= p.q_heads;
-    const Heads& x = is_k ? p.k : p.q;
-    return reinterpret_cast<const T*>(x.data) + b * x.batch + s * x.token + (is_k ? h - p.q_heads : h) * x.head;
-  };
-  typename Lane<T, kV, kUnits, kAdjacent>::Raw raw;
-  int h = part * p.part_heads + lane / p.lanes;
-  me.load(source(h), h < end, raw);
-  me.angles(p, lane, first, row, table[warp]);
-  float w[kUnits][2 * kV];
-  int held = -1;   // whose weights are in w
-  for (int base = part * p.part_heads; base < end; base += step, h += step) {
-    float e[kUnits][2 * kV];
-    me.widen(raw, e);
-    const bool is_k = h >= p.q_heads;
-    me.load(source(h + step), h + step < end, raw);
-    if (kNorm) {
-      if (held != is_k) me.weights(is_k ? p.k_weight : p.q_weight, p.weight_dtype, w);
-      held = is_k;
-      float sum = 0;
+  using L = Lane<T, kV, kUnits, kAdjacent>;
+  __shared__ float2 tables[kWarps][kMaxPairs];
+  __shared__ float weights[2][kNorm ? MLXD_ROTARY_MAX_HEAD_DIM : 1];
+  const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), mine = lane / p.lanes, at_once = 32 / p.lanes;
+  float2* table = tables[threadIdx.x / 32];
+  const L me(p, first);
+  if constexpr (kNorm) read_weights(p, weights);
+  const uint32_t items = static_cast<uint32_t>(p.rows) * p.parts;
+  const uint32_t item = blockIdx.x * kWarps + threadIdx.x / 32;
+  if (item < items) {
+    const uint32_t row = p.parts == 1 ? item : item / p.parts, part = item - row * p.parts;
+    const uint32_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
+    // rounds of a token: those of its queries, then those of its keys; this warp has `from` to `to` - 1 of them
+    const int from = part * p.part_rounds, to = min(p.q_rounds + p.k_rounds, from + p.part_rounds);
+    const int first_of[2] = {min(from, p.q_rounds), max(from, p.q_rounds) - p.q_rounds};
+    const int last_of[2] = {min(to, p.q_rounds), max(to, p.q_rounds) - p.q_rounds};
+    typename L::Raw raw = {}, keys = {};
+    const auto source = [&](const Heads& x, int round) {
+      return reinterpret_cast<const T*>(x.data) + b * x.batch + s * x.token + (round * at_once + mine) * x.head;
+    };
+    me.load(source(p.q, first_of[0]), first_of[0] < last_of[0] && first_of[0] * at_once + mine < p.q_heads, raw);
+    me.load(source(p.k, first_of[1]), first_of[1] < last_of[1] && first_of[1] * at_once + mine < p.k_heads, keys);
+    for (int i = lane; i < p.head_dim / 2; i += 32) table[i] = unit_of(p, i, b, s);
+    __syncwarp();
+    typename L::Pairs u, w;
+    me.angles(table, first, u);
+#pragma unroll 1
+    for (int is_k = 0; is_k < 2; is_k++) {
+      const Heads& in = is_k ? p.k : p.q;
+      const Heads& out = is_k ? p.k_out : p.q_out;
+      const int heads = is_k ? p.k_heads : p.q_heads, last = last_of[is_k];
+      int round = first_of[is_k];
+      if (round >= last) continue;
+      if (is_k) raw = keys;
+      if constexpr (kNorm) me.gather(weights[is_k], w);
+      const T* x = source(in, round);
+      T* y = reinterpret_cast<T*>(out.data) + b * out.batch + s * out.token + (round * at_once + mine) * out.head;
+      const int64_t step = at_once * in.head, out_step = at_once * out.head;
+#pragma unroll 1
+      for (int h = round * at_once + mine; round < last; round++, h += at_once) {
+        typename L::Pairs e;
+        me.widen(raw, e);
+        x += step;
+        me.load(x, round + 1 < last && h + at_once < heads, raw);
+        if constexpr (kNorm) {
+          float2 sum = {};
 #pragma unroll
-      for (int k = 0; k < kUnits; k++) {
+          for (int i = 0; i < L::kN; i += 2) sum = fma2(two(e.a, i), two(e.a, i), fma2(two(e.b, i), two(e.b, i), sum));
+          const float2 r = both(rsqrtf(lanes_sum(sum.x + sum.y, p.lanes) * p.inverse_dim + p.eps));
 #pragma unroll
-        for (int j = 0; j < 2 * kV; j++) sum += e[k][j] * e[k][j];
+          for (int i = 0; i < L::kN; i += 2) {
+            put(e.a, i, mul2(mul2(two(e.a, i), r), two(w.a, i)));
+            put(e.b, i, mul2(mul2(two(e.b, i), r), two(w.b, i)));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < L::kN; i += 2) {
+          const float2 a = two(e.a, i), c = two(e.b, i), cos = two(u.a, i), sin = two(u.b, i);
+          put(e.a, i, fma2(c, neg2(sin), mul2(a, cos)));
+          put(e.b, i, fma2(a, sin, mul2(c, cos)));
+        }
+        if (h < heads) me.store(y, e);
+        y += out_step;
       }
-      const float r = rsqrtf(lanes_sum(sum, p.lanes) / p.head_dim + p.eps);
-#pragma unroll
-      for (int k = 0; k < kUnits; k++) {
-#pragma unroll
-        for (int j = 0; j < 2 * kV; j++) e[k][j] *= r * w[k][j];
-      }
-    }
-    me.turned(e);
-    if (h < end) {
-      const Heads& y = is_k ? p.k_out : p.q_out;
-      me.store(reinterpret_cast<T*>(y.data) + b * y.batch + s * y.token + (is_k ? h - p.q_heads : h) * y.head, e);
     }
   }
 }
@@ -252,88 +314,93 @@ __global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const __grid_consta
 // The first p.q_blocks CTAs take the tokens' queries, the others their keys, so that a lane holds the sums of one weight's
 // gradient: over all tokens it meets, then over the lanes and warps of the CTA in a fixed order, one row of p.partial a CTA.
 template <class T, int kV, int kUnits, bool kAdjacent>
-__global__ void __launch_bounds__(32 * kWarps, 4) norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ float2 table[kWarps][kMaxPairs];
-  const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), warp = threadIdx.x / 32;
+__global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
+  using L = Lane<T, kV, kUnits, kAdjacent>;
+  __shared__ float2 tables[kWarps][kMaxPairs];
+  __shared__ float weights[2][MLXD_ROTARY_MAX_HEAD_DIM];
+  const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), mine = lane / p.lanes, at_once = 32 / p.lanes;
+  float2* table = tables[threadIdx.x / 32];
   const bool is_k = static_cast<int>(blockIdx.x) >= p.q_blocks;
-  const Heads& in = is_k ? p.k : p.q;
-  const Heads& gr = is_k ? p.k_grad : p.q_grad;
-  const Heads& out = is_k ? p.k_out : p.q_out;
+  const Heads in = is_k ? p.k : p.q, gr = is_k ? p.k_grad : p.q_grad, out = is_k ? p.k_out : p.q_out;
   const int heads = is_k ? p.k_heads : p.q_heads;
   const uint32_t block = is_k ? blockIdx.x - p.q_blocks : blockIdx.x;
   const uint32_t stride = (is_k ? gridDim.x - p.q_blocks : p.q_blocks) * kWarps;
-  Lane<T, kV, kUnits, kAdjacent> me(p, first);
-  const int step = 32 / p.lanes;
-  float w[kUnits][2 * kV], dw[kUnits][2 * kV] = {};
-  me.weights(is_k ? p.k_weight : p.q_weight, p.weight_dtype, w);
-  for (uint32_t row = block * kWarps + warp; row < p.rows; row += stride) {
-    const int64_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
-    const T* x = reinterpret_cast<const T*>(in.data) + b * in.batch + s * in.token;
-    const T* dy = reinterpret_cast<const T*>(gr.data) + b * gr.batch + s * gr.token;
-    T* dx = reinterpret_cast<T*>(out.data) + b * out.batch + s * out.token;
-    typename Lane<T, kV, kUnits, kAdjacent>::Raw rx, rg;
-    int h = lane / p.lanes;
-    me.load(x + h * in.head, h < heads, rx);
-    me.load(dy + h * gr.head, h < heads, rg);
-    me.angles(p, lane, first, row, table[warp]);
-    for (int base = 0; base < heads; base += step, h += step) {
-      float e[kUnits][2 * kV], g[kUnits][2 * kV];
+  const L me(p, first);
+  read_weights(p, weights);
+  typename L::Pairs w, dw = {};
+  me.gather(weights[is_k], w);
+  for (uint32_t row = block * kWarps + threadIdx.x / 32; row < p.rows; row += stride) {
+    const uint32_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
+    const T* x = reinterpret_cast<const T*>(in.data) + b * in.batch + s * in.token + mine * in.head;
+    const T* dy = reinterpret_cast<const T*>(gr.data) + b * gr.batch + s * gr.token + mine * gr.head;
+    T* dx = reinterpret_cast<T*>(out.data) + b * out.batch + s * out.token + mine * out.head;
+    typename L::Raw rx = {}, rg = {};
+    me.load(x, mine < heads, rx);
+    me.load(dy, mine < heads, rg);
+    for (int i = lane; i < p.head_dim / 2; i += 32) table[i] = unit_of(p, i, b, s);
+    __syncwarp();
+    typename L::Pairs u;
+    me.angles(table, first, u);
+    for (int h = mine; h - mine < heads; h += at_once) {
+      typename L::Pairs e, g;
       me.widen(rx, e);
       me.widen(rg, g);
-      me.load(x + (h + step) * in.head, h + step < heads, rx);
-      me.load(dy + (h + step) * gr.head, h + step < heads, rg);
-      me.turned(g);
-      float sum = 0, dot = 0;
+      x += at_once * in.head;
+      dy += at_once * gr.head;
+      me.load(x, h + at_once < heads, rx);
+      me.load(dy, h + at_once < heads, rg);
+      float2 sum = {}, dot = {};
 #pragma unroll
-      for (int k = 0; k < kUnits; k++) {
-#pragma unroll
-        for (int j = 0; j < 2 * kV; j++) {
-          sum += e[k][j] * e[k][j];
-          dot += g[k][j] * w[k][j] * e[k][j];
-        }
+      for (int i = 0; i < L::kN; i += 2) {
+        const float2 a = two(g.a, i), c = two(g.b, i), cos = two(u.a, i), sin = two(u.b, i), f = two(e.a, i), k = two(e.b, i);
+        const float2 ga = fma2(c, neg2(sin), mul2(a, cos)), gb = fma2(a, sin, mul2(c, cos));
+        put(g.a, i, ga);
+        put(g.b, i, gb);
+        sum = fma2(f, f, fma2(k, k, sum));
+        dot = fma2(mul2(ga, two(w.a, i)), f, fma2(mul2(gb, two(w.b, i)), k, dot));
       }
-      const float r = rsqrtf(lanes_sum(sum, p.lanes) / p.head_dim + p.eps);
-      const float m = lanes_sum(dot, p.lanes) * r / p.head_dim;   // mean(g w n)
+      const float r = rsqrtf(lanes_sum(sum.x + sum.y, p.lanes) * p.inverse_dim + p.eps);
+      const float m = lanes_sum(dot.x + dot.y, p.lanes) * r * p.inverse_dim;   // mean(g w n)
       if (h < heads) {
 #pragma unroll
-        for (int k = 0; k < kUnits; k++) {
-#pragma unroll
-          for (int j = 0; j < 2 * kV; j++) {
-            const float n = e[k][j] * r;
-            dw[k][j] += g[k][j] * n;
-            e[k][j] = r * (g[k][j] * w[k][j] - n * m);
-          }
+        for (int i = 0; i < L::kN; i += 2) {   // n = x r, dw += g n, dx = r (g w - n m)
+          const float2 na = mul2(two(e.a, i), both(r)), nb = mul2(two(e.b, i), both(r)), ga = two(g.a, i), gb = two(g.b, i);
+          put(dw.a, i, fma2(ga, na, two(dw.a, i)));
+          put(dw.b, i, fma2(gb, nb, two(dw.b, i)));
+          put(e.a, i, mul2(both(r), fma2(na, both(-m), mul2(ga, two(w.a, i)))));
+          put(e.b, i, mul2(both(r), fma2(nb, both(-m), mul2(gb, two(w.b, i)))));
         }
-        me.store(dx + h * out.head, e);
+        me.store(dx, e);
       }
+      dx += at_once * out.head;
     }
+    __syncwarp();
   }
   if (is_k ? !p.k_weight : !p.q_weight) return;
   // lanes that hold the same elements of other heads, then the warps
 #pragma unroll
-  for (int k = 0; k < kUnits; k++) {
-#pragma unroll
-    for (int j = 0; j < 2 * kV; j++) {
-      for (int d = p.lanes; d < 32; d <<= 1) dw[k][j] += __shfl_xor_sync(~0u, dw[k][j], d);
+  for (int i = 0; i < L::kN; i++) {
+    for (int d = p.lanes; d < 32; d <<= 1) {
+      dw.a[i] += __shfl_xor_sync(~0u, dw.a[i], d);
+      dw.b[i] += __shfl_xor_sync(~0u, dw.b[i], d);
     }
   }
-  float* part = reinterpret_cast<float*>(table[warp]);   // head_dim values fit: 2 * kMaxPairs
-  __syncwarp();
+  float* part = reinterpret_cast<float*>(table);   // head_dim values fit: 2 * kMaxPairs
   if (lane < p.lanes) {
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
       if (!me.owns[k]) continue;
 #pragma unroll
       for (int j = 0; j < kV; j++) {
-        part[me.at[k][0] + j] = dw[k][j];
-        part[me.at[k][1] + j] = dw[k][kV + j];
+        part[me.at[k][L::low(j) / kV] + L::low(j) % kV] = dw.a[k * kV + j];
+        part[me.at[k][L::high(j) / kV] + L::high(j) % kV] = dw.b[k * kV + j];
       }
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < p.head_dim; i += 32 * kWarps) {
     float sum = 0;
-    for (int v = 0; v < kWarps; v++) sum += reinterpret_cast<const float*>(table[v])[i];
+    for (int v = 0; v < kWarps; v++) sum += reinterpret_cast<const float*>(tables[v])[i];
     p.partial[static_cast<int64_t>(blockIdx.x) * p.head_dim + i] = sum;
   }
 }
@@ -368,11 +435,11 @@ bool absent(const mlxd_heads& h) {
   return h.data == nullptr;
 }
 
-// CTAs of the backward pass: queries' and keys' in proportion to their heads, four of each SM at most.
+// CTAs of the backward pass: queries' and keys' in proportion to their heads, kBackwardBlocks of each SM at most.
 void backward_blocks(int64_t rows, int q_heads, int k_heads, int sms, int* q_blocks, int* blocks) {
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>((rows + kWarps - 1) / kWarps, 4 * sms));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>((rows + kWarps - 1) / kWarps, kBackwardBlocks * sms));
   const int heads = q_heads + k_heads;
-  const auto share = [&](int h) { return h ? static_cast<int>(std::max<int64_t>(1, std::min(most, (4 * sms * static_cast<int64_t>(h) + heads / 2) / heads))) : 0; };
+  const auto share = [&](int h) { return h ? static_cast<int>(std::max<int64_t>(1, std::min(most, (kBackwardBlocks * sms * static_cast<int64_t>(h) + heads / 2) / heads))) : 0; };
   *q_blocks = share(q_heads);
   *blocks = *q_blocks + share(k_heads);
 }
@@ -457,6 +524,7 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
   // the backward pass turns the gradient back
   p.sign = (d->inverse != 0) != (pass == Pass::kBackward) ? -1.0f : 1.0f;
   p.eps = d->eps;
+  p.inverse_dim = 1.0f / d->head_dim;
   return MLXD_OK;
 }
 
@@ -514,18 +582,20 @@ int forward(const char* entry, int device, void* stream, const mlxd_rotary_desc*
   RotaryParams p;
   int rc = params_of(entry, d, pass, p);
   if (rc != MLXD_OK) return rc;
-  const int heads = p.q_heads + p.k_heads;
-  if (!p.rows || !heads) return MLXD_OK;
+  if (!p.rows || !(p.q_heads + p.k_heads)) return MLXD_OK;
   int sms = 0;
   rc = device_sms(device, &sms);
   if (rc != MLXD_OK) return rc;
   const int v = vector_of(p, dtype_bytes(d->dtype), false);
   p.lanes = lanes_of(p.head_dim / 2 / v);
   // a token's heads are shared out among warps until there are 32 warps for every SM
-  const int at_once = 32 / p.lanes, groups = (heads + at_once - 1) / at_once;
-  const int64_t parts = std::min<int64_t>(groups, std::max<int64_t>(1, 32 * sms / p.rows));
-  p.part_heads = static_cast<int>((groups + parts - 1) / parts) * at_once;
-  p.parts = (heads + p.part_heads - 1) / p.part_heads;
+  const int at_once = 32 / p.lanes;
+  p.q_rounds = (p.q_heads + at_once - 1) / at_once;
+  p.k_rounds = (p.k_heads + at_once - 1) / at_once;
+  const int rounds = p.q_rounds + p.k_rounds;
+  const int64_t parts = std::min<int64_t>(rounds, std::max<int64_t>(1, 32 * sms / p.rows));
+  p.part_rounds = static_cast<int>((rounds + parts - 1) / parts);
+  p.parts = (rounds + p.part_rounds - 1) / p.part_rounds;
   MLXD_ON_DEVICE(device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned blocks = static_cast<unsigned>((p.rows * p.parts + kWarps - 1) / kWarps);
