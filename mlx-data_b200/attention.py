@@ -10,15 +10,28 @@ their work on torch's current stream of the tensors' device; results are new con
 float32 and results rounded once to the tensors' type.  The same call gives the same bits again.  Wrong arguments raise
 ``ValueError``; there is no CPU path.
 """
-from ._c import attention as _ops
+import importlib
 
 __all__ = ["rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "cross_attention", "cross_attention_backward"]
 
+
+
+class _Operators:
+    """The compiled module, loaded on first use: importing the package does not import torch."""
+
+    def __getattr__(self, name):
+        global _ops
+        importlib.import_module("torch")
+        _ops = importlib.import_module("._attention", __package__)
+        return getattr(_ops, name)
+
+
+_ops = _Operators()
 _functions = None
 
 
 def _autograd():
-    """The autograd functions, made on first use: importing the package does not import torch."""
+    """The autograd functions, made on first use."""
     global _functions
     if _functions is None:
         import torch
@@ -66,11 +79,15 @@ def _autograd():
                 q, k, v, out, lse, lengths, key_mask = ctx.saved_tensors
                 return (*_ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.scale), None, None, None)
 
-        def wanted(*tensors):
-            return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
-
-        _functions = Rotary, QkNormRotary, CrossAttention, wanted
+        _functions = Rotary, QkNormRotary, CrossAttention
     return _functions
+
+
+def _wants_gradient(*tensors):
+    for t in tensors:
+        if getattr(t, "requires_grad", False):
+            return importlib.import_module("torch").is_grad_enabled()
+    return False
 
 
 def rotary(q, k, positions, frequencies, sections, *, inverse=False, adjacent=False, interleaved=False):
@@ -84,9 +101,8 @@ def rotary(q, k, positions, frequencies, sections, *, inverse=False, adjacent=Fa
     Pairs are elements (i, i + pairs), or (2 i, 2 i + 1) (``adjacent``); elements from 2 * pairs on stay as they are.
     ``inverse`` turns back, which is also the gradient.
     """
-    fn, _, _, wanted = _autograd()
-    if wanted(q, k):
-        return fn.apply(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
+    if _wants_gradient(q, k):
+        return _autograd()[0].apply(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
     return _ops.rotary(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
 
 
@@ -96,9 +112,8 @@ def qk_norm_rotary(q, k, positions, frequencies, sections, q_weight=None, k_weig
 
     ``q_weight`` and ``k_weight`` [head_dim] of one type, float32, bfloat16 or float16; None stands for ones.
     """
-    _, fn, _, wanted = _autograd()
-    if wanted(q, k, q_weight, k_weight):
-        return fn.apply(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
+    if _wants_gradient(q, k, q_weight, k_weight):
+        return _autograd()[1].apply(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
     return _ops.qk_norm_rotary(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
 
 
@@ -122,9 +137,8 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale=None, return_
     Returns the result, or with ``return_lse`` also the logarithm of each row's sum of exponentials, float32
     [batch, q_heads, tokens], which ``cross_attention_backward`` takes.
     """
-    _, _, fn, wanted = _autograd()
-    if wanted(q, k, v):
-        out, lse = fn.apply(q, k, v, lengths, key_mask, scale)
+    if _wants_gradient(q, k, v):
+        out, lse = _autograd()[2].apply(q, k, v, lengths, key_mask, scale)
         return (out, lse) if return_lse else out
     return _ops.cross_attention(q, k, v, lengths, key_mask, scale, return_lse)
 

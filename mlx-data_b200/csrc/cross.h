@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/mlxd_b200.h"
@@ -26,12 +27,24 @@ struct CrossParams {
   int batch, q_tokens, kv_tokens, q_heads, kv_heads, group, head_dim;
   float scale;
   int* status;                  // set where a wait ran out
+  int device;
 };
 
 // Tensor maps of a call: boxes of 64 elements by 128 tokens, 128-byte swizzle.
 struct CrossMaps {
   CUtensorMap q, k, v, out, dout, dq, dk, dv;   // forward: the first four; backward: all but out
 };
+
+// Raises a kernel's limit of shared memory, once per device.
+template <auto kKernel>
+cudaError_t allow_shared(int bytes, int device) {
+  static std::atomic<uint64_t> done{0};   // of this kernel, a bit for each device
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map);
 

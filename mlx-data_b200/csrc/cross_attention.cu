@@ -189,6 +189,7 @@ extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cr
     if (need && (!d->workspace || d->workspace_bytes < need)) return fail(MLXD_ERR_INVALID, "cross_attention: workspace too small");
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    p.device = device;
     if (takes_steps(p)) {
       int sms = 0;
       rc = device_sms(device, &sms);
@@ -217,6 +218,7 @@ extern "C" int mlxd_cross_attention_backward(int device, void* cuda_stream, cons
     p.delta = static_cast<float*>(d->workspace);
     if (!p.batch) return static_cast<int>(MLXD_OK);
     MLXD_ON_DEVICE(device);
+    p.device = device;
     rc = status_word(device, &p.status);
     CrossMaps maps;
     if (rc == MLXD_OK) rc = maps_of(p, d->dtype, true, maps);

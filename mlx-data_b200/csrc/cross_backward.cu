@@ -499,12 +499,12 @@ template <class T, int kDim>
 cudaError_t launch(const CrossParams& p, const CrossMaps& maps, cudaStream_t stream) {
   constexpr int bytes = Sizes<kDim>::kShared;
   if (p.q_tokens) {
-    const cudaError_t e = cudaFuncSetAttribute(cross_dq_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = allow_shared<cross_dq_kernel<T, kDim>>(bytes, p.device);
     if (e != cudaSuccess) return e;
     cross_dq_kernel<T, kDim><<<static_cast<unsigned>((p.q_tokens + 127) / 128) * p.q_heads * p.batch, kThreads, bytes, stream>>>(p, maps);
   }
   if (p.kv_tokens) {
-    const cudaError_t e = cudaFuncSetAttribute(cross_dkv_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = allow_shared<cross_dkv_kernel<T, kDim>>(bytes, p.device);
     if (e != cudaSuccess) return e;
     cross_dkv_kernel<T, kDim><<<static_cast<unsigned>((p.kv_tokens + 127) / 128) * p.kv_heads * p.batch, kThreads, bytes, stream>>>(p, maps);
   }

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
 template <class T, int kDim>
 cudaError_t launch(const CrossParams& p, const CrossMaps& maps, cudaStream_t stream) {
   constexpr int bytes = Sizes<kDim>::kShared;
-  const cudaError_t e = cudaFuncSetAttribute(cross_forward_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = allow_shared<cross_forward_kernel<T, kDim>>(bytes, p.device);
   if (e != cudaSuccess) return e;
   const unsigned blocks = static_cast<unsigned>((p.q_tokens + 255) / 256) * p.q_heads * p.batch;
   cross_forward_kernel<T, kDim><<<blocks, kThreads, bytes, stream>>>(p, maps);

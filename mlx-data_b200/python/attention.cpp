@@ -1,14 +1,17 @@
-// The attention operators on torch tensors: checks, results and workspaces, calls of the C ABI.
+// The module `_attention`: the attention operators on torch tensors - checks, results and workspaces, calls of the C ABI.
 //
-// Tensors are read through their Python methods (torch is no build dependency); results and workspaces come from the
-// tensors' own allocator (new_empty), so torch's rules for memory and streams hold for them.
-#include "python/attention.h"
+// A module of its own because it is built against torch: a call of a few microseconds has no time for reading tensors through
+// their Python methods.  The pipeline's module `_c` knows nothing of torch.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <pybind11/pybind11.h>
 
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
-#include <vector>
 
 #include "../../include/mlxd_b200.h"
 
@@ -30,110 +33,70 @@ void check(int rc) {
   throw std::runtime_error(std::string("mlx-data GPU path: ") + mlxd_last_error());
 }
 
-py::object steal(PyObject* o) {
-  if (!o) {
-    throw py::error_already_set();
-  }
-  return py::reinterpret_steal<py::object>(o);
+// Work is queued on torch's current stream of the tensors' device.
+void* stream_of(int device) {
+  return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
 }
 
-// What is asked of torch, looked up once.  Never freed: it outlives the interpreter's own teardown.
-struct Torch {
-  py::object bf16, f16, f32, i32, i64, u8, boolean, raw_stream, current_stream, empty;
-  PyObject *shape, *stride, *dtype, *data_ptr, *get_device, *is_contiguous, *contiguous, *clone, *new_empty, *cuda_stream, *is_cuda;
-
-  Torch() {
-    const py::module_ t = py::module_::import("torch");
-    bf16 = t.attr("bfloat16");
-    f16 = t.attr("float16");
-    f32 = t.attr("float32");
-    i32 = t.attr("int32");
-    i64 = t.attr("int64");
-    u8 = t.attr("uint8");
-    boolean = t.attr("bool");
-    empty = t.attr("empty");
-    current_stream = t.attr("cuda").attr("current_stream");
-    const py::object c = t.attr("_C");
-    raw_stream = py::getattr(c, "_cuda_getCurrentRawStream", py::none());
-    shape = PyUnicode_InternFromString("shape");
-    stride = PyUnicode_InternFromString("stride");
-    dtype = PyUnicode_InternFromString("dtype");
-    data_ptr = PyUnicode_InternFromString("data_ptr");
-    get_device = PyUnicode_InternFromString("get_device");
-    is_contiguous = PyUnicode_InternFromString("is_contiguous");
-    contiguous = PyUnicode_InternFromString("contiguous");
-    clone = PyUnicode_InternFromString("clone");
-    new_empty = PyUnicode_InternFromString("new_empty");
-    cuda_stream = PyUnicode_InternFromString("cuda_stream");
-    is_cuda = PyUnicode_InternFromString("is_cuda");
-  }
-
-  // Work is queued on torch's current stream of the tensors' device.
-  void* stream_of(int device) const {
-    if (!raw_stream.is_none()) {
-      return reinterpret_cast<void*>(raw_stream(device).cast<uintptr_t>());
-    }
-    return reinterpret_cast<void*>(current_stream(device).attr("cuda_stream").cast<uintptr_t>());
-  }
-};
-
-const Torch& torch() {
-  static const Torch* t = new Torch();
-  return *t;
+py::object wrapped(const at::Tensor& t) {
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(t));
 }
 
 constexpr int kMaxDims = 4;
 
 // A tensor in GPU memory.
 struct Tensor {
-  py::object obj;
-  PyObject* dtype = nullptr;   // of torch, kept alive there
+  at::Tensor t;
   char* data = nullptr;
   int device = -1, dims = 0;
   int64_t size[kMaxDims], stride[kMaxDims];
 
   void read(const char* op, const char* name, const py::object& o) {
-    const Torch& t = torch();
-    obj = o;
-    if (!PyObject_HasAttr(o.ptr(), t.data_ptr) || !PyObject_HasAttr(o.ptr(), t.get_device)) {
+    if (!THPVariable_Check(o.ptr())) {
       bad(op, std::string(name) + " must be a torch tensor");
     }
-    device = static_cast<int>(PyLong_AsLong(steal(PyObject_CallMethodNoArgs(o.ptr(), t.get_device)).ptr()));
-    if (device < 0) {
+    set(op, name, THPVariable_Unpack(o.ptr()));
+  }
+
+  void set(const char* op, const char* name, const at::Tensor& from) {
+    t = from;
+    if (!t.is_cuda()) {
       bad(op, std::string(name) + " must be in GPU memory (there is no CPU path)");
     }
-    data = reinterpret_cast<char*>(PyLong_AsUnsignedLongLong(steal(PyObject_CallMethodNoArgs(o.ptr(), t.data_ptr)).ptr()));
-    dtype = steal(PyObject_GetAttr(o.ptr(), t.dtype)).ptr();
-    const py::object shape = steal(PyObject_GetAttr(o.ptr(), t.shape));
-    const py::object strides = steal(PyObject_CallMethodNoArgs(o.ptr(), t.stride));
-    const Py_ssize_t n = PyTuple_Size(shape.ptr());
-    if (n < 1 || n > kMaxDims || PyTuple_Size(strides.ptr()) != n) {
-      PyErr_Clear();
-      bad(op, std::string(name) + " has " + std::to_string(n) + " dimensions");
+    if (t.layout() != at::kStrided || t.is_conj() || t.is_neg()) {
+      bad(op, std::string(name) + " must be an ordinary strided tensor");
     }
-    dims = static_cast<int>(n);
+    device = t.get_device();
+    data = static_cast<char*>(t.data_ptr());
+    const auto sizes = t.sizes(), strides = t.strides();
+    if (sizes.size() < 1 || sizes.size() > kMaxDims) {
+      bad(op, std::string(name) + " has " + std::to_string(sizes.size()) + " dimensions");
+    }
+    dims = static_cast<int>(sizes.size());
     for (int i = 0; i < dims; i++) {
-      size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), i));
-      stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(strides.ptr(), i));
-    }
-    if (PyErr_Occurred()) {
-      throw py::error_already_set();
+      size[i] = sizes[i];
+      stride[i] = strides[i];
     }
   }
 
   int kind() const {   // mlxd_dtype; -1: another type
-    const Torch& t = torch();
-    if (dtype == t.bf16.ptr()) return MLXD_BF16;
-    if (dtype == t.f16.ptr()) return MLXD_F16;
-    if (dtype == t.f32.ptr()) return MLXD_F32;
-    if (dtype == t.i64.ptr()) return MLXD_I64;
-    if (dtype == t.i32.ptr()) return MLXD_I32;
-    if (dtype == t.u8.ptr() || dtype == t.boolean.ptr()) return MLXD_U8;
-    return -1;
+    switch (t.scalar_type()) {
+      case at::kBFloat16: return MLXD_BF16;
+      case at::kHalf: return MLXD_F16;
+      case at::kFloat: return MLXD_F32;
+      case at::kLong: return MLXD_I64;
+      case at::kInt: return MLXD_I32;
+      case at::kByte: case at::kBool: return MLXD_U8;
+      default: return -1;
+    }
   }
 
   std::string text() const {
-    return py::str(py::tuple(obj.attr("shape"))).cast<std::string>();
+    std::string s = "(";
+    for (int i = 0; i < dims; i++) {
+      s += (i ? ", " : "") + std::to_string(size[i]);
+    }
+    return s + ")";
   }
 };
 
@@ -167,9 +130,8 @@ struct HeadsTensor : Tensor {
       }
     }
     if (!fits) {
-      const Torch& t = torch();
-      const bool dense = steal(PyObject_CallMethodNoArgs(o.ptr(), t.is_contiguous)).ptr() == Py_True;
-      read(op, name, steal(PyObject_CallMethodNoArgs(o.ptr(), dense ? t.clone : t.contiguous)));
+      const at::Tensor copy = t.is_contiguous() ? t.clone() : t.contiguous();
+      set(op, name, copy);
       layout(op, name);
     }
   }
@@ -191,27 +153,25 @@ struct HeadsTensor : Tensor {
   }
 
   void same_kind(const char* op, const char* name, const HeadsTensor& like, const char* other) const {
-    if (dtype != like.dtype || device != like.device) {
+    if (t.scalar_type() != like.t.scalar_type() || device != like.device) {
       bad(op, std::string(name) + " must have the type and device of " + other);
     }
   }
 };
 
 // A new tensor of `like`'s shape, type and device, contiguous.
-py::object empty_like(const HeadsTensor& like, mlxd_heads* view) {
-  const Torch& t = torch();
-  const py::object shape = steal(PyObject_GetAttr(like.obj.ptr(), t.shape));
-  py::object o = steal(PyObject_CallMethodOneArg(like.obj.ptr(), t.new_empty, shape.ptr()));
-  view->data = reinterpret_cast<void*>(PyLong_AsUnsignedLongLong(steal(PyObject_CallMethodNoArgs(o.ptr(), t.data_ptr)).ptr()));
+at::Tensor empty_like(const HeadsTensor& like, mlxd_heads* view) {
+  at::Tensor o = at::empty(like.t.sizes(), like.t.options().requires_grad(false));
+  view->data = o.data_ptr();
   view->stride_head = like.dim;
   view->stride_token = like.heads * like.dim;
   view->stride_batch = like.tokens * view->stride_token;
   return o;
 }
 
-py::object empty_bytes(const HeadsTensor& like, size_t bytes, const py::object& dtype, void** data) {
-  py::object o = torch().empty(py::make_tuple(bytes), py::arg("dtype") = dtype, py::arg("device") = like.obj.attr("device"));
-  *data = reinterpret_cast<void*>(o.attr("data_ptr")().cast<uintptr_t>());
+at::Tensor empty_bytes(const HeadsTensor& like, size_t bytes, void** data) {
+  at::Tensor o = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(like.t.device()));
+  *data = o.data_ptr();
   return o;
 }
 
@@ -298,7 +258,7 @@ struct Rotary {
   void weights(const py::object& q_weight_, const py::object& k_weight_, double eps) {
     weight("q_weight", q_weight_, q_weight, &d.q_weight);
     weight("k_weight", k_weight_, k_weight, &d.k_weight);
-    if (d.q_weight && d.k_weight && q_weight.dtype != k_weight.dtype) {
+    if (d.q_weight && d.k_weight && q_weight.t.scalar_type() != k_weight.t.scalar_type()) {
       bad(op, "q_weight and k_weight must have one type");
     }
     d.weight_dtype = d.q_weight ? q_weight.kind() : d.k_weight ? k_weight.kind() : MLXD_F32;
@@ -306,12 +266,13 @@ struct Rotary {
   }
 
   py::tuple results(int (*call)(int, void*, const mlxd_rotary_desc*)) {
-    py::object q_out = empty_like(q, &d.q_out), k_out = py::none();
+    const at::Tensor q_out = empty_like(q, &d.q_out);
+    at::Tensor k_out;
     if (has_k) {
       k_out = empty_like(k, &d.k_out);
     }
-    check(call(q.device, torch().stream_of(q.device), &d));
-    return py::make_tuple(q_out, k_out);
+    check(call(q.device, stream_of(q.device), &d));
+    return py::make_tuple(wrapped(q_out), has_k ? wrapped(k_out) : py::none());
   }
 };
 
@@ -353,12 +314,10 @@ py::tuple qk_norm_rotary_backward(const py::object& q_grad, const py::object& k_
     gk.same_shape(r.op, "k_grad", r.k, "k");
     r.d.k_grad = gk.view();
   }
-  const Torch& t = torch();
-  py::object wq = py::none(), wk = py::none(), work;
+  at::Tensor wq, wk;
   const auto grad_of = [&](const Tensor& w, void** at) {
-    const py::object shape = steal(PyObject_GetAttr(w.obj.ptr(), t.shape));
-    py::object o = steal(PyObject_CallMethodOneArg(w.obj.ptr(), t.new_empty, shape.ptr()));
-    *at = reinterpret_cast<void*>(PyLong_AsUnsignedLongLong(steal(PyObject_CallMethodNoArgs(o.ptr(), t.data_ptr)).ptr()));
+    at::Tensor o = at::empty(w.t.sizes(), w.t.options().requires_grad(false));
+    *at = o.data_ptr();
     return o;
   };
   if (r.d.q_weight) {
@@ -368,9 +327,9 @@ py::tuple qk_norm_rotary_backward(const py::object& q_grad, const py::object& k_
     wk = grad_of(r.k_weight, &r.d.k_weight_grad);
   }
   check(mlxd_qk_norm_rotary_workspace(r.q.device, &r.d, &r.d.workspace_bytes));
-  work = empty_bytes(r.q, r.d.workspace_bytes, t.u8, &r.d.workspace);
+  const at::Tensor work = empty_bytes(r.q, r.d.workspace_bytes, &r.d.workspace);
   const py::tuple x = r.results(mlxd_qk_norm_rotary_backward);
-  return py::make_tuple(x[0], x[1], wq, wk);
+  return py::make_tuple(x[0], x[1], wq.defined() ? wrapped(wq) : py::none(), wk.defined() ? wrapped(wk) : py::none());
 }
 
 // ---------------------------------------------------------------- cross attention
@@ -379,7 +338,6 @@ struct Cross {
   mlxd_cross_desc d{};
   HeadsTensor q, k, v;
   Tensor lengths, mask;
-  py::object copied_mask;
 
   void inputs(const py::object& q_, const py::object& k_, const py::object& v_, const py::object& lengths_, const py::object& mask_,
               const py::object& scale) {
@@ -420,16 +378,16 @@ struct Cross {
         bad(op, "key_mask must be bool [batch, keys] on q's device");
       }
       if (mask.size[1] > 1 && mask.stride[1] != 1) {
-        mask.read(op, "key_mask", steal(PyObject_CallMethodNoArgs(mask_.ptr(), torch().contiguous)));
+        mask.set(op, "key_mask", at::Tensor(mask.t.contiguous()));
       }
       d.key_mask = reinterpret_cast<const uint8_t*>(mask.data);
       d.key_mask_stride = mask.stride[0];
     }
   }
 
-  py::object workspace(bool backward) {
+  at::Tensor workspace(bool backward) {
     check(mlxd_cross_attention_workspace(q.device, &d, backward, &d.workspace_bytes));
-    return d.workspace_bytes ? empty_bytes(q, d.workspace_bytes, torch().u8, &d.workspace) : py::object(py::none());
+    return d.workspace_bytes ? empty_bytes(q, d.workspace_bytes, &d.workspace) : at::Tensor();
   }
 };
 
@@ -437,21 +395,18 @@ py::object cross_attention(const py::object& q, const py::object& k, const py::o
                            const py::object& key_mask, const py::object& scale, bool return_lse) {
   Cross c{"cross_attention"};
   c.inputs(q, k, v, lengths, key_mask, scale);
-  const py::object work = c.workspace(false);
-  const py::object out = empty_like(c.q, &c.d.out);
-  py::object lse;
+  const at::Tensor work = c.workspace(false);
+  const at::Tensor out = empty_like(c.q, &c.d.out);
+  at::Tensor lse;
   if (return_lse) {
-    void* at = nullptr;
-    lse = torch().empty(py::make_tuple(c.d.batch, c.d.q_heads, c.d.q_tokens), py::arg("dtype") = torch().f32,
-                        py::arg("device") = c.q.obj.attr("device"));
-    at = reinterpret_cast<void*>(lse.attr("data_ptr")().cast<uintptr_t>());
-    c.d.lse = static_cast<float*>(at);
+    lse = at::empty({c.d.batch, c.d.q_heads, c.d.q_tokens}, at::TensorOptions().dtype(at::kFloat).device(c.q.t.device()));
+    c.d.lse = static_cast<float*>(lse.data_ptr());
   }
-  check(mlxd_cross_attention(c.q.device, torch().stream_of(c.q.device), &c.d));
+  check(mlxd_cross_attention(c.q.device, stream_of(c.q.device), &c.d));
   if (return_lse) {
-    return py::make_tuple(out, lse);
+    return py::make_tuple(wrapped(out), wrapped(lse));
   }
-  return out;
+  return wrapped(out);
 }
 
 py::tuple cross_attention_backward(const py::object& dout, const py::object& q, const py::object& k, const py::object& v,
@@ -469,20 +424,20 @@ py::tuple cross_attention_backward(const py::object& dout, const py::object& q, 
   Tensor l;
   l.read(c.op, "lse", lse);
   if (l.kind() != MLXD_F32 || l.dims != 3 || l.size[0] != c.d.batch || l.size[1] != c.d.q_heads || l.size[2] != c.d.q_tokens ||
-      l.device != c.q.device || steal(PyObject_CallMethodNoArgs(lse.ptr(), torch().is_contiguous)).ptr() != Py_True) {
+      l.device != c.q.device || !l.t.is_contiguous()) {
     bad(c.op, "lse must be what cross_attention returned: contiguous float32 [batch, q_heads, tokens]");
   }
   c.d.lse = reinterpret_cast<float*>(l.data);
-  const py::object work = c.workspace(true);
-  const py::object dq = empty_like(c.q, &c.d.dq), dk = empty_like(c.k, &c.d.dk), dv = empty_like(c.v, &c.d.dv);
-  check(mlxd_cross_attention_backward(c.q.device, torch().stream_of(c.q.device), &c.d));
-  return py::make_tuple(dq, dk, dv);
+  const at::Tensor work = c.workspace(true);
+  const at::Tensor dq = empty_like(c.q, &c.d.dq), dk = empty_like(c.k, &c.d.dk), dv = empty_like(c.v, &c.d.dv);
+  check(mlxd_cross_attention_backward(c.q.device, stream_of(c.q.device), &c.d));
+  return py::make_tuple(wrapped(dq), wrapped(dk), wrapped(dv));
 }
 
 }  // namespace
 
-void bind_attention(py::module_& m) {
-  py::module_ a = m.def_submodule("attention", "The attention operators without gradients of their own; see the package's attention.py");
+PYBIND11_MODULE(_attention, a) {
+  a.doc() = "The attention operators without gradients of their own; see attention.py";
   a.def("rotary", &rotary, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("frequencies"), py::arg("sections"),
         py::arg("inverse"), py::arg("adjacent"), py::arg("interleaved"));
   a.def("qk_norm_rotary", &qk_norm_rotary, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("frequencies"),

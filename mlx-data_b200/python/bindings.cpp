@@ -18,7 +18,6 @@
 #include "mlx/data/core/image/Jpeg.h"
 #include "mlx/data/core/image/Png.h"
 #include "mlx/data/gpu/Runtime.h"
-#include "python/attention.h"
 
 namespace py = pybind11;
 using namespace mlx::data;
@@ -761,6 +760,4 @@ PYBIND11_MODULE(_c, m) {
     d["host_stage_ns"] = s.host_stage_ns;
     return d;
   });
-
-  bind_attention(m);
 }
