@@ -63,6 +63,23 @@ __device__ __forceinline__ int length_of(const CrossParams& p, int b) {
   const int64_t n = p.lengths_dtype == MLXD_I64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
   return static_cast<int>(n < 0 ? 0 : n > p.kv_tokens ? p.kv_tokens : n);
 }
+
+// The end of a sample's last key that is read, found by the whole CTA from the back: the padding below the images of a batch
+// ends a sample's keys under a mask too.  `reach` (shared) is 0 before, for all threads.
+__device__ __forceinline__ int reach_of(const CrossParams& p, int b, int length, int* reach) {
+  if (!p.key_mask) return length;
+  const uint8_t* mask = p.key_mask + b * p.key_mask_stride;
+  for (int end = length; end > 0; end -= blockDim.x) {
+    const int key = end - 1 - static_cast<int>(threadIdx.x);
+    const int most = __reduce_max_sync(~0u, key >= 0 && mask[key] ? key + 1 : 0);
+    if (most && (threadIdx.x & 31) == 0) atomicMax(reach, most);
+    __syncthreads();
+    const int found = *reach;
+    __syncthreads();
+    if (found) return found;
+  }
+  return 0;
+}
 #endif
 
 }  // namespace mlxd

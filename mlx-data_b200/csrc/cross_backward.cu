@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ float delta_parts[2][128];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed;
+  __shared__ int failed, reach;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
@@ -73,12 +73,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
 
   const int q_tiles = (p.q_tokens + 127) / 128;
   const int q0 = blockIdx.x % q_tiles * 128, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
-  const int length = length_of(p, batch), n = (length + 127) / 128;
-  const auto partial = [&](int j) { return p.key_mask != nullptr || (j + 1) * 128 > length; };
-  const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
-
   if (threadIdx.x == 0) {
-    failed = 0;
+    failed = reach = 0;
     for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, done}) barrier_init(bar, 1);
     for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
@@ -96,6 +92,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = tmem_slot, dp_column = 256, dq_column = 384;   // scores in 0 and 128
+  const int length = reach_of(p, batch, length_of(p, batch), &reach), n = (length + 127) / 128;
+  const auto partial = [&](int j) { return p.key_mask != nullptr || (j + 1) * 128 > length; };
+  const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -298,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + 1];
   __shared__ float4 stats[2][2][32];      // of the queries of a tile: -lse * log2(e), delta
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed;
+  __shared__ int failed, reach;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
   const uint32_t k_full = smem_address(bars), v_full = k_full + 8, full = k_full + 16, empty = full + 8 * S::kSlots,
@@ -307,11 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
 
   const int k_tiles = (p.kv_tokens + 127) / 128;
   const int k0 = blockIdx.x % k_tiles * 128, kv_head = blockIdx.x / k_tiles % p.kv_heads, batch = blockIdx.x / k_tiles / p.kv_heads;
-  const int length = length_of(p, batch), q_tiles = (p.q_tokens + 127) / 128;
-  const int n = k0 < length ? q_tiles * p.group : 0;   // tiles of queries, head by head
+  const int q_tiles = (p.q_tokens + 127) / 128;
 
   if (threadIdx.x == 0) {
-    failed = 0;
+    failed = reach = 0;
     for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8}) barrier_init(bar, 1);
     for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 8);
     for (const uint32_t bar : {stats_empty, stats_empty + 8}) barrier_init(bar, 8);
@@ -326,6 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = tmem_slot, dp_column = 128, dv_column = 256, dk_column = 384;   // scores in 0
+  const int length = reach_of(p, batch, length_of(p, batch), &reach);
+  const int n = k0 < length ? q_tiles * p.group : 0;   // tiles of queries, head by head
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");

@@ -20,18 +20,23 @@ struct Sizes {
   static constexpr int kShared = (2 + kSlots) * kTile;
 };
 
-// 64 scores of a row; -infinity where a key is not read.
-__device__ __forceinline__ void load_scores(uint32_t at, uint32_t word0, uint32_t word1, uint32_t (&s)[64]) {
+// 64 scores of a row.
+__device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[64]) {
   tmem_load<32>(at, s);
   tmem_load<32>(at + 32, s + 32);
   tmem_loaded(s);
-  if ((word0 & word1) != ~0u) {
+}
+
+// -infinity where a key is not read, in tensor memory too, where the scores are read again.
+__device__ __forceinline__ void mask_scores(uint32_t at, uint32_t word0, uint32_t word1, uint32_t (&s)[64]) {
 #pragma unroll
-    for (int k = 0; k < 32; k++) {
-      if (!(word0 >> k & 1)) s[k] = __float_as_uint(-INFINITY);
-      if (!(word1 >> k & 1)) s[32 + k] = __float_as_uint(-INFINITY);
-    }
+  for (int k = 0; k < 32; k++) {
+    if (!(word0 >> k & 1)) s[k] = __float_as_uint(-INFINITY);
+    if (!(word1 >> k & 1)) s[32 + k] = __float_as_uint(-INFINITY);
   }
+  tmem_store<32>(at, s);
+  tmem_store<32>(at + 32, s + 32);
+  tmem_stored();
 }
 
 __device__ __forceinline__ void swap_halves(uint32_t (&words)[4]) {
@@ -80,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   __shared__ uint64_t bars[2 + 2 * S::kSlots + 8 + 2 * kMaskRing + 2];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed;
+  __shared__ int failed, reach;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
@@ -88,14 +93,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
 
   const int q_tiles = (p.q_tokens + 255) / 256;
   const int q0 = blockIdx.x % q_tiles * 256, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
-  const int length = length_of(p, batch), n = (length + 127) / 128;
   const int rows = p.q_tokens - q0 > 128 ? 2 : 1;   // tiles of query rows
-  // tiles of keys of which some may not be read: every one under a mask, else the last
-  const auto partial = [&](int j) { return p.key_mask != nullptr || (j + 1) * 128 > length; };
-  const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
-
   if (threadIdx.x == 0) {
-    failed = 0;
+    failed = reach = 0;
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
@@ -119,6 +119,10 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = tmem_slot;
+  const int length = reach_of(p, batch, length_of(p, batch), &reach), n = (length + 127) / 128;
+  // tiles of keys of which some may not be read: every one under a mask, else the last
+  const auto partial = [&](int j) { return p.key_mask != nullptr || (j + 1) * 128 > length; };
+  const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
   const uint32_t o_column = 256;   // scores of tile t in columns 128 t, results in 256 + 128 t
 
   if (warp >= 8) {
@@ -268,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         float now = -INFINITY;
 #pragma unroll 1
         for (int h = 0; h < 2; h++) {
-          load_scores(mine + 64 * h, words[0], words[1], s);
+          load_scores(mine + 64 * h, s);
+          if ((words[0] & words[1]) != ~0u) mask_scores(mine + 64 * h, words[0], words[1], s);
           now = fmaxf(now, most_of(s));
           swap_halves(words);
         }
@@ -296,9 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         float2 sum[2] = {};
 #pragma unroll 1
         for (int h = 0; h < 2; h++) {
-          load_scores(mine + 64 * h, words[0], words[1], s);
+          load_scores(mine + 64 * h, s);
           weigh<T>(s, c, base, sum, mine + 64 * h);
-          swap_halves(words);
           tmem_stored();
           tmem_before_sync();
           warp_arrive(p_full + 16 * h + 8 * t, lane);
