@@ -6,12 +6,17 @@ namespace mlxd {
 
 namespace {
 
-constexpr int kThreads = 384;          // two warpgroups of softmax, then warps for copies, products, masks
+constexpr int kThreads = 640;          // four warpgroups of softmax, then warps for copies, products, masks
 constexpr int kMaskRing = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference maximum is moved, and what is summed so far scaled, only where the maximum has grown by more than
 // 2^8: the result is the same quotient, and 2^8 is far from the largest float16.
 constexpr float kSlack = 8.0f;
+// Of eight pairs of exponentials so many are worked out by multiply-adds: the pipe of exponentials is what a tile of scores waits
+// for.  Measured for 0, 1, 2, 3: 388, 376, 382, 398 us (2 x 2048 tokens, 6404 keys, 32 heads of 128), 246, 232, 232, 272 us (4096
+// keys, heads of 64): above one in eight the issue of instructions takes as long.
+constexpr int kByFma = 1;
+
 template <int kDim>
 struct Sizes {
   static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
@@ -27,24 +32,13 @@ __device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[64]) {
   tmem_loaded(s);
 }
 
-// -infinity where a key is not read, in tensor memory too, where the scores are read again.
-__device__ __forceinline__ void mask_scores(uint32_t at, uint32_t word0, uint32_t word1, uint32_t (&s)[64]) {
+// -infinity where a key is not read.
+__device__ __forceinline__ void mask_scores(uint32_t word0, uint32_t word1, uint32_t (&s)[64]) {
 #pragma unroll
   for (int k = 0; k < 32; k++) {
     if (!(word0 >> k & 1)) s[k] = __float_as_uint(-INFINITY);
     if (!(word1 >> k & 1)) s[32 + k] = __float_as_uint(-INFINITY);
   }
-  tmem_store<32>(at, s);
-  tmem_store<32>(at + 32, s + 32);
-  tmem_stored();
-}
-
-__device__ __forceinline__ void swap_halves(uint32_t (&words)[4]) {
-  const uint32_t a = words[0], b = words[1];
-  words[0] = words[2];
-  words[1] = words[3];
-  words[2] = a;
-  words[3] = b;
 }
 
 __device__ __forceinline__ float most_of(const uint32_t (&s)[64]) {
@@ -69,8 +63,12 @@ __device__ __forceinline__ void weigh(const uint32_t (&s)[64], float c, float ba
     for (int k = 0; k < 16; k++) {
       float2 x = make_float2(__uint_as_float(s[32 * i + 2 * k]), __uint_as_float(s[32 * i + 2 * k + 1]));
       x = fma2(x, make_float2(c, c), make_float2(base, base));
-      x.x = exp2_of(x.x);
-      x.y = exp2_of(x.y);
+      if (k % 8 < kByFma) {
+        x = exp2_by_fma(x);
+      } else {
+        x.x = exp2_of(x.x);
+        x.y = exp2_of(x.y);
+      }
       sum[k & 1] = add2(sum[k & 1], x);
       packed[k] = pack2<T>(x.x, x.y);
     }
@@ -84,12 +82,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   extern __shared__ __align__(1024) uint8_t shared[];
   __shared__ uint64_t bars[2 + 2 * S::kSlots + 8 + 2 * kMaskRing + 2];
   __shared__ uint32_t mask_words[kMaskRing][4];
+  __shared__ float exchange[2][2][128];   // of a row's two threads: maxima, sums at last
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, reach;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
-                 p_full = s_full + 16, o_full = p_full + 32, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
+                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
 
   const int q_tiles = (p.q_tokens + 255) / 256;
   const int q0 = blockIdx.x % q_tiles * 256, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
@@ -99,10 +98,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
-      barrier_init(p_full + 8 * t, 4);         // the first half of a tile's keys
-      barrier_init(p_full + 16 + 8 * t, 4);    // the second
+      barrier_init(p_full + 8 * t, 8);
       barrier_init(o_full + 8 * t, 1);
-      barrier_init(staged_full + 8 * t, 4);
+      barrier_init(staged_full + 8 * t, 8);
     }
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
@@ -114,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
     }
     barrier_init_done();
   }
-  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  if (warp == 17) tmem_alloc<512>(smem_address(&tmem_slot));
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
@@ -125,9 +123,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   const auto ring_of = [&](int j) { return p.key_mask ? j : 0; };
   const uint32_t o_column = 256;   // scores of tile t in columns 128 t, results in 256 + 128 t
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    if (warp == 8 && lane == 0 && n) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16 && lane == 0 && n) {
       // -------------------------------------------------- copies
       for (int t = 0; t < rows; t++) {
         barrier_expect(q_full + 8 * t, S::kTile);
@@ -158,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
           for (int i = 0; i < kWaitTries && !barrier_try(bar, (masks ? r / kMaskRing : k / S::kSlots) & 1); i++) {}
         }
       }
-    } else if (warp == 9 && n) {
+    } else if (warp == 17 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
@@ -179,41 +177,44 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         __syncwarp();
       }
       at.next();
+      // The tensor cores run a product or two behind the thread that issues them, so between two groups of products there is one
+      // look at barriers and no more: with the last group of a tile of keys, at those of the next one's tiles too.
+      Ring<S::kSlots> v = at, k = at;
+      k.next();
+      going = going && warp_wait3(full + 8 * v.slot, v.phase, n > 1 ? full + 8 * k.slot : 0, k.phase, 0, 0, &failed);
 #pragma unroll 1
       for (int j = 0; j < n && going; j++) {
-        const uint32_t v_slot = at.slot;
-        going = warp_wait(full + 8 * v_slot, at.phase, &failed);
-        at.next();
-        const uint32_t k_slot = at.slot;
-        if (j + 1 < n) going = going && warp_wait(full + 8 * k_slot, at.phase, &failed);
-        at.next();
+        Ring<S::kSlots> next_v = k, next_k;
+        next_v.next();
+        next_k = next_v;
+        next_k.next();
 #pragma unroll 1
         for (int t = 0; t < rows && going; t++) {
-          // O += P V, P where the scores were; the first half of the keys while the second is being worked on
-          const uint32_t o = tmem + o_column + 128 * t, v = values + v_slot * (S::kTile >> 4);
-          going = warp_wait(p_full + 8 * t, j & 1, &failed);
-          if (!going) break;
-          tmem_after_sync();
-          if (elected()) product_over_tokens(o, tmem + 128 * t, v, kResults, j > 0);
-          __syncwarp();
-          going = warp_wait(p_full + 16 + 8 * t, j & 1, &failed);
+          // O += P V, P where the scores were, when both halves of the keys have been weighed
+          const uint32_t o = tmem + o_column + 128 * t, values_at = values + v.slot * (S::kTile >> 4);
+          const bool last = t + 1 == rows;
+          going = warp_wait3(p_full + 8 * t, j & 1, last && j + 1 < n ? full + 8 * next_v.slot : 0, next_v.phase,
+                             last && j + 2 < n ? full + 8 * next_k.slot : 0, next_k.phase, &failed);
           if (!going) break;
           tmem_after_sync();
           if (elected()) {
-            product_over_tokens(o, tmem + 128 * t + 64, v + kHalfTokens, kResults, true);
-            if (t + 1 == rows) products_done(empty + 8 * v_slot);
+            product_over_tokens(o, tmem + 128 * t, values_at, kResults, j > 0);
+            product_over_tokens(o, tmem + 128 * t + 64, values_at + kHalfTokens, kResults, true);
+            if (last) products_done(empty + 8 * v.slot);
             // products run in the order in which they are issued: these scores overwrite P after it has been read
             if (j + 1 < n) {
-              scores(t, k_slot);
-              if (t + 1 == rows) products_done(empty + 8 * k_slot);
+              scores(t, k.slot);
+              if (last) products_done(empty + 8 * k.slot);
             } else {
               products_done(o_full + 8 * t);
             }
           }
           __syncwarp();
         }
+        v = next_v;
+        k = next_k;
       }
-    } else if (warp == 10) {
+    } else if (warp == 19) {
       // -------------------------------------------------- masks: which keys are read, and zeros where values are not
       for (int j = 0; j < n; j++) {
         if (!partial(j)) continue;
@@ -245,38 +246,32 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---------------------------------------------------- softmax: a thread owns a row
-    const int t = warp / 4, row = threadIdx.x & 127;
-    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    const uint32_t mine = tmem + 128 * t + lanes, result = tmem + o_column + 128 * t + lanes;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---------------------------------------------------- softmax: a row belongs to two threads, one for each half of the keys of a tile
+    // A wait that ran out does not end the loop: the two warps of a row's threads meet at a barrier for every tile.
+    const int t = warp / 8, half = warp / 4 % 2, part = warp % 4, row = 32 * part + lane;
+    const uint32_t lanes = static_cast<uint32_t>(32 * part) << 16;
+    const uint32_t mine = tmem + 128 * t + 64 * half + lanes, result = tmem + o_column + 128 * t + half * (kDim / 2) + lanes;
     if (t < rows) {
       const float c = p.scale * kLog2e;
       float top = -INFINITY, total = 0;
-      bool going = true;
-      for (int j = 0; j < n; j++) {
-        going = warp_wait(s_full + 8 * t, j & 1, &failed);
-        if (!going) break;
-        tmem_after_sync();
-        uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
-        if (partial(j)) {
-          const int r = ring_of(j);
-          going = warp_wait(masked + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed);
-          if (!going) break;
-#pragma unroll
-          for (int i = 0; i < 4; i++) words[i] = mask_words[r % kMaskRing][i];
-        }
-        // 64 scores at a time, read twice: for their maximum and for their exponentials.  Loops, not copies of their bodies: the
-        // roles of a CTA share the instruction caches, and the warp that issues products suffers when they do not fit.
-        uint32_t s[64];
-        float now = -INFINITY;
 #pragma unroll 1
-        for (int h = 0; h < 2; h++) {
-          load_scores(mine + 64 * h, s);
-          if ((words[0] & words[1]) != ~0u) mask_scores(mine + 64 * h, words[0], words[1], s);
-          now = fmaxf(now, most_of(s));
-          swap_halves(words);
+      for (int j = 0; j < n; j++) {
+        uint32_t s[64];
+        warp_wait(s_full + 8 * t, j & 1, &failed);
+        tmem_after_sync();
+        load_scores(mine, s);
+        if (partial(j)) {
+          const int r = ring_of(j) % kMaskRing;
+          warp_wait(masked + 8 * r, ring_of(j) / kMaskRing & 1, &failed);
+          const uint32_t word0 = mask_words[r][2 * half], word1 = mask_words[r][2 * half + 1];
+          if ((word0 & word1) != ~0u) mask_scores(word0, word1, s);
         }
+        // what lay in `exchange` has been read: these scores were worked out after the other thread's weights of the tile before
+        float now = most_of(s);
+        exchange[t][half][row] = now;
+        asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");
+        now = fmaxf(now, exchange[t][half ^ 1][row]);
         if (j == 0) {
           top = now;
         } else {
@@ -285,9 +280,9 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
             const float keep = grows ? exp2_of((top - now) * c) : 1.0f;
             if (grows) top = now;
             total *= keep;
-            // the products of tile j - 1 were done before the scores of tile j
+            // this thread's half of the results; the products of tile j - 1 were done before the scores of tile j
 #pragma unroll 1
-            for (int x = 0; x < kDim; x += 16) {
+            for (int x = 0; x < kDim / 2; x += 16) {
               uint32_t o[16];
               tmem_load<16>(result + x, o);
               tmem_loaded(o);
@@ -299,24 +294,23 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         }
         const float base = top == -INFINITY ? 0.0f : -top * c;
         float2 sum[2] = {};
-#pragma unroll 1
-        for (int h = 0; h < 2; h++) {
-          load_scores(mine + 64 * h, s);
-          weigh<T>(s, c, base, sum, mine + 64 * h);
-          tmem_stored();
-          tmem_before_sync();
-          warp_arrive(p_full + 16 * h + 8 * t, lane);
-        }
+        weigh<T>(s, c, base, sum, mine);
         sum[0] = add2(sum[0], sum[1]);
         total += sum[0].x + sum[0].y;
+        tmem_stored();
+        tmem_before_sync();
+        warp_arrive(p_full + 8 * t, lane);
       }
-      if (n && going) going = warp_wait(o_full + 8 * t, 0, &failed);
-      if (going) {
+      const bool done = !n || warp_wait(o_full + 8 * t, 0, &failed);
+      exchange[t][half][row] = total;
+      asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");
+      total += exchange[t][half ^ 1][row];
+      if (done) {
         tmem_after_sync();
         const float by = total > 0 ? 1.0f / total : 0.0f;
         const uint32_t staged = tiles_at + t * S::kTile;   // the queries are no longer needed
 #pragma unroll
-        for (int x = 0; x < kDim; x += 32) {
+        for (int x = 0; x < kDim / 2; x += 32) {
           uint32_t o[32] = {};
           if (n) {
             tmem_load<32>(result + x, o);
@@ -327,18 +321,18 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) w[i] = pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by);
-            const int unit = (x + k) % 64 / 8;
+            const int column = half * (kDim / 2) + x + k;
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                         : : "r"(staged + (x + k) / 64 * kBoxBytes + row * 128 + ((unit ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                         : : "r"(staged + column / 64 * kBoxBytes + row * 128 + ((column % 64 / 8 ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           }
         }
-        if (p.lse && q0 + 128 * t + row < p.q_tokens) {
+        if (p.lse && half == 0 && q0 + 128 * t + row < p.q_tokens) {
           p.lse[(static_cast<int64_t>(batch) * p.q_heads + head) * p.q_tokens + q0 + 128 * t + row] =
               total > 0 ? top * p.scale + logf(total) : -INFINITY;
         }
         fence_async_proxy();
         warp_arrive(staged_full + 8 * t, lane);
-        if (row == 0 && barrier_wait(staged_full + 8 * t, 0, &failed)) {
+        if (row == 0 && half == 0 && barrier_wait(staged_full + 8 * t, 0, &failed)) {
           for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(&maps.out, 64 * x, q0 + 128 * t, head, batch, staged + x * kBoxBytes);
           tile_stores_read();
         }
@@ -348,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   __syncwarp();
   tmem_before_sync();
   __syncthreads();
-  if (warp == 9) tmem_free<512>(tmem);
+  if (warp == 17) tmem_free<512>(tmem);
   if (threadIdx.x == 0 && failed) *p.status = 1;
 }
 

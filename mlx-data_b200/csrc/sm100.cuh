@@ -74,6 +74,14 @@ struct Ring {
   }
 };
 
+// The same for several barriers at once: where they are ready, as they mostly are, one look costs what a look at one costs.  A barrier
+// of 0 is none.
+__device__ __forceinline__ bool warp_wait3(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, uint32_t bar2, uint32_t parity2, volatile int* failed) {
+  const bool a = barrier_try(bar0, parity0), b = !bar1 || barrier_try(bar1, parity1), c = !bar2 || barrier_try(bar2, parity2);
+  if (__all_sync(~0u, a && b && c)) return true;
+  return warp_wait(bar0, parity0, failed) && (!bar1 || warp_wait(bar1, parity1, failed)) && (!bar2 || warp_wait(bar2, parity2, failed));
+}
+
 // One arrival for a warp, after what its threads did.  (An arrival of every thread is served one at a time.)
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
   __syncwarp();
@@ -262,6 +270,22 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;"
       : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
+}
+
+// 2^x for two floats at once on the pipe of multiply-adds, which has time where the one for exponentials has not: x = n + f with n the
+// nearest integer (by adding 1.5 * 2^23), 2^f = 1 + f q(f) with the cubic q of least largest relative error on [-1/2, 1/2] (2.9e-6, by
+// exchange), n added to the exponent.  -infinity gives 0; what is not a number gives something that is not finite.
+__device__ __forceinline__ float2 exp2_by_fma(float2 x) {
+  constexpr float kRound = 12582912.0f;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.0f));
+  const float2 t = add2(x, make_float2(kRound, kRound)), n = add2(t, make_float2(-kRound, -kRound));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 q = fma2(f, make_float2(0.009582853f, 0.009582853f), make_float2(0.055906426f, 0.055906426f));
+  q = fma2(f, q, make_float2(0.24024099f, 0.24024099f));
+  q = fma2(f, q, make_float2(0.6931242f, 0.6931242f));
+  q = fma2(f, q, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
 }
 
 // Two floats rounded to 16 bits each, the first in the lower half.
