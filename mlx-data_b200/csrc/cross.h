@@ -51,7 +51,7 @@ int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int d
 cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
 
 // Few queries: whether a call is one, and how it runs.
-bool takes_steps(const CrossParams& p);
+bool takes_steps(const CrossParams& p, int sms);
 size_t step_workspace(const CrossParams& p, int sms);
 cudaError_t launch_cross_step(const CrossParams& p, void* workspace, int sms, int dtype, cudaStream_t stream);
 

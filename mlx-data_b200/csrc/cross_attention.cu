@@ -74,11 +74,11 @@ int workspace_of(int device, const CrossParams& p, bool backward, size_t* bytes)
   *bytes = 0;
   if (backward) {
     *bytes = sizeof(float) * p.batch * p.q_heads * p.q_tokens;
-  } else if (p.batch && p.q_tokens && takes_steps(p)) {
+  } else if (p.batch && p.q_tokens) {
     int sms = 0;
     const int rc = device_sms(device, &sms);
     if (rc != MLXD_OK) return rc;
-    *bytes = step_workspace(p, sms);
+    if (takes_steps(p, sms)) *bytes = step_workspace(p, sms);
   }
   return MLXD_OK;
 }
@@ -190,10 +190,10 @@ extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cr
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     p.device = device;
-    if (takes_steps(p)) {
-      int sms = 0;
-      rc = device_sms(device, &sms);
-      if (rc != MLXD_OK) return rc;
+    int sms = 0;
+    rc = device_sms(device, &sms);
+    if (rc != MLXD_OK) return rc;
+    if (takes_steps(p, sms)) {
       MLXD_CUDA(launch_cross_step(p, d->workspace, sms, d->dtype, s));
       return static_cast<int>(MLXD_OK);
     }

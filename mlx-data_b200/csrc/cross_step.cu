@@ -233,30 +233,35 @@ __global__ void __launch_bounds__(32 * kWarps, 2) cross_step_kernel(const __grid
   }
 }
 
-// One CTA a row: its parts, weighted by exp(lse).
-template <class T>
-__global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__ StepParams sp) {
+// One CTA a row: its parts, weighted by exp(lse), dealt among its warps.  Sixteen where parts are many (235 parts: 18 us, four 28); four
+// otherwise, whose registers fit beside the CTAs that work the parts out, so that they are there when those end (8.5 us, else 10.8).
+constexpr int kManyParts = 32;
+
+template <class T, int kJoinWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __grid_constant__ StepParams sp) {
   const CrossParams& p = sp.p;
-  __shared__ float4 sums[4][32];
-  __shared__ float tops[4], totals[4];
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float tops[kJoinWarps], totals[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int64_t all = static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens, stat = blockIdx.x;
   const int token = stat % p.q_tokens, head = stat / p.q_tokens % p.q_heads, batch = stat / p.q_tokens / p.q_heads;
   const int parts = (length_of(p, batch) + sp.split_keys - 1) / sp.split_keys;
   asm volatile("griddepcontrol.wait;" : : : "memory");
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 128) top = fmaxf(top, sp.part_lse[i * all + stat]);
+  for (int i = threadIdx.x; i < parts; i += 32 * kJoinWarps) top = fmaxf(top, sp.part_lse[i * all + stat]);
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   if (lane == 0) tops[warp] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; i++) top = fmaxf(top, tops[i]);
   float4 o = {};
   float total = 0;
   const bool there = 4 * lane < p.head_dim;
   if (top > -INFINITY) {
-    for (int i = warp; i < parts; i += 4) {
+#pragma unroll 4
+    for (int i = warp; i < parts; i += kJoinWarps) {
       const float w = exp2_of((sp.part_lse[i * all + stat] - top) * kLog2e);
-      const float4 x = there ? *reinterpret_cast<const float4*>(sp.part_out + (i * all + stat) * p.head_dim + 4 * lane) : o;
+      const float4 x = there ? *reinterpret_cast<const float4*>(sp.part_out + (i * all + stat) * p.head_dim + 4 * lane) : make_float4(0, 0, 0, 0);
       total += w;
       o.x += w * x.x;
       o.y += w * x.y;
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
   if (lane == 0) totals[warp] = total;
   __syncthreads();
   if (warp) return;
-  for (int i = 1; i < 4; i++) {
+  for (int i = 1; i < kJoinWarps; i++) {
     total += totals[i];
     o.x += sums[i][lane].x;
     o.y += sums[i][lane].y;
@@ -283,11 +288,11 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
   if (lane == 0 && p.lse) p.lse[stat] = total > 0 ? top + logf(total) : -INFINITY;
 }
 
-// Keys of a CTA: 512, fewer (down to one round of its warps) while CTAs are fewer than two an SM, more while they are over four
+// Keys of a CTA: 2048 (sixteen sequences of up to 6404 keys: 57 us, with 1024 60, with 512 66), fewer (down to one round of its warps) while CTAs are fewer than two an SM, more while they are over four
 // an SM and a row would have over 64 parts.
 void split(const CrossParams& p, int sms, int* split_keys, int* splits) {
   const int64_t base = static_cast<int64_t>(p.batch) * p.kv_heads * ((static_cast<int64_t>(p.q_tokens) * p.group + kRows - 1) / kRows);
-  int64_t keys = 512;
+  int64_t keys = 2048;
   const auto parts = [&] { return (p.kv_tokens + keys - 1) / keys; };
   while (keys > kWarps * kKeys && base * parts() < 2 * sms) keys /= 2;
   while (parts() > 64 && base * parts() > 4 * sms) keys *= 2;
@@ -306,20 +311,29 @@ cudaError_t launch(const StepParams& sp, cudaStream_t stream) {
   // begins while the parts are being worked out and waits for them on the device
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(p.batch) * p.q_heads * p.q_tokens);
-  config.blockDim = dim3(128);
+  const bool many = sp.splits > kManyParts;
+  config.blockDim = dim3(many ? 512 : 128);
   config.stream = stream;
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &early;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, cross_join_kernel<T>, sp);
+  return many ? cudaLaunchKernelEx(&config, cross_join_kernel<T, 16>, sp) : cudaLaunchKernelEx(&config, cross_join_kernel<T, 4>, sp);
 }
 
 }  // namespace
 
-bool takes_steps(const CrossParams& p) {
-  return static_cast<int64_t>(p.q_tokens) * p.group <= 64 && static_cast<int64_t>(p.batch) * p.kv_heads <= 65535;
+// Both ways, by what they were measured to take, in us beyond what they share: few queries 2, 1.5 for 16 rows, and keys and values once
+// for every 16 rows at 4.5 TB/s; many queries 3, and 1.5 for each tile of 128 keys of each round of CTAs.  32 heads on 8, 1601 keys:
+// 16 rows 10.2 and 26.1 us, 64 rows 16.3 and 26.2, 256 rows 29.1 and 26.3; 8 x 16 heads of 64, 1024 keys: 16 rows 12.5 and 15.8,
+// 32 rows 20.1 and 15.8; 4 x 4 heads, 6404 keys: 64 rows 41 and 90, 256 rows 160 and 90.
+bool takes_steps(const CrossParams& p, int sms) {
+  const int64_t sixteens = (static_cast<int64_t>(p.q_tokens) * p.group + kRows - 1) / kRows;
+  if (sixteens > 64 || static_cast<int64_t>(p.batch) * p.kv_heads > 65535) return false;
+  const double bytes = 4.0 * p.batch * p.kv_heads * p.kv_tokens * p.head_dim;
+  const int64_t ctas = static_cast<int64_t>(p.batch) * p.q_heads * ((p.q_tokens + 255) / 256), tiles = (p.kv_tokens + 127) / 128;
+  return 2 + sixteens * (1.5 + bytes / 4.5e6) < 3 + 1.5 * ((ctas + sms - 1) / sms) * tiles;
 }
 
 size_t step_workspace(const CrossParams& p, int sms) {
