@@ -1,4 +1,13 @@
 // Cross attention of many queries: two tiles of 128 query rows a CTA against tiles of 128 keys.
+//
+// One pass over the keys with a running maximum m and sum l of each row: S = Q K^T, P = 2^(c S - c m) with c = scale log2(e), O = O + P V,
+// O and l scaled where m moves; at last O / l.  4 Sq Sk D operations, so the tensor cores are the floor; the exponentials (one
+// for 4 D operations) take as long at D = 128 and twice as long at 64.  Scores and results stay in tensor memory (512 columns: two tiles of
+// 128 scores and 128 results each), weights go back where their scores were and are an operand from there.  While one tile of rows is in
+// the tensor cores the other is with the softmax.  A row belongs to two threads, so that a tile's softmax takes half as long: it and the
+// products of a tile follow one another (about 1600 and 1300 cycles, of which 1024 are products), and a tile waits for both.
+// Measured: 2 x 2048 tokens, 6404 keys, 32 heads on 8, D = 128: 388 us, 1106 TFLOP/s (68 % of the measured rate; 436 us where calls
+// follow one another for long and the power cap lowers the clock); D = 64, 4096 keys: 222 us, 619.
 #include "cross.h"
 #include "sm100.cuh"
 
@@ -9,7 +18,7 @@ namespace {
 constexpr int kThreads = 640;          // four warpgroups of softmax, then warps for copies, products, masks
 constexpr int kMaskRing = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-// A row's reference maximum is moved, and what is summed so far scaled, only where the maximum has grown by more than
+// A row's reference maximum is moved, and what is summed so far scaled, only where its weight has grown by more than
 // 2^8: the result is the same quotient, and 2^8 is far from the largest float16.
 constexpr float kSlack = 8.0f;
 // Of eight pairs of exponentials so many are worked out by multiply-adds: the pipe of exponentials is what a tile of scores waits
