@@ -127,42 +127,49 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
       const uint32_t queries = low_half(at_address(tile_descriptor(16), q_at)), grads = low_half(at_address(tile_descriptor(16), do_at)),
                      ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
-      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
-      const auto scores = [&](int j) {
-        product_of_tiles<kDim>(tmem + 128 * (j & 1), queries, ring + slot_of(2 * j), kScores, steps);
+      const auto at_slot = [&](uint32_t slot) { return slot * (S::kTile >> 4); };
+      const auto scores = [&](int j, uint32_t slot) {
+        product_of_tiles<kDim>(tmem + 128 * (j & 1), queries, ring + at_slot(slot), kScores, steps);
         products_done(s_full + 8 * (j & 1));
       };
-      const auto dp = [&](int j) {
-        product_of_tiles<kDim>(tmem + dp_column, grads, ring + slot_of(2 * j + 1), kScores, steps);
+      const auto dp = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem + dp_column, grads, ring + at_slot(slot), kScores, steps);
         products_done(dp_full);
-        products_done(empty + 8 * ((2 * j + 1) % S::kSlots));
+        products_done(empty + 8 * slot);
       };
-      bool going = warp_wait(q_full, 0, &failed) && item_full(0);
-      if (going && elected()) scores(0);
+      bool going = warp_wait3(q_full, 0, full, 0, 0, 0, &failed);
+      if (going && elected()) scores(0, 0);
       __syncwarp();
-      going = going && warp_wait(do_full, 0, &failed) && item_full(1);
-      if (going && elected()) dp(0);
+      going = going && warp_wait3(do_full, 0, full + 8, 0, 0, 0, &failed);
+      if (going && elected()) dp(1);
       __syncwarp();
-      going = going && (n == 1 || item_full(2));
-      if (going && n > 1 && elected()) scores(1);
+      going = going && (n == 1 || warp_wait(full + 16, 0, &failed));
+      if (going && n > 1 && elected()) scores(1, 2);
       __syncwarp();
+      // one look at barriers between two groups of products: the tensor cores are not far behind the thread that issues them
+      Ring<S::kSlots> k, v, next_k;          // keys of this tile, values of the next, keys of the one after
+      v.next(3);
+      next_k.next(4);
+#pragma unroll 1
       for (int j = 0; j < n && going; j++) {
-        going = (j + 1 >= n || item_full(2 * j + 3)) && (j + 2 >= n || item_full(2 * j + 4)) && warp_wait(ds_full, j & 1, &failed);
+        going = warp_wait3(ds_full, j & 1, j + 1 < n ? full + 8 * v.slot : 0, v.phase, j + 2 < n ? full + 8 * next_k.slot : 0, next_k.phase, &failed);
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          if (j + 1 < n) dp(j + 1);
-          const uint32_t ds = tmem + 128 * (j & 1), k = ring_tokens + slot_of(2 * j);
-          product_over_tokens(tmem + dq_column, ds, k, kResults, j > 0);
-          product_over_tokens(tmem + dq_column, ds + 64, k + kHalfTokens, kResults, true);
-          products_done(empty + 8 * (2 * j % S::kSlots));
-          if (j + 2 < n) scores(j + 2);   // overwrites dS of tile j after it has been read
+          if (j + 1 < n) dp(v.slot);
+          const uint32_t ds = tmem + 128 * (j & 1), b = ring_tokens + at_slot(k.slot);
+          product_over_tokens(tmem + dq_column, ds, b, kResults, j > 0);
+          product_over_tokens(tmem + dq_column, ds + 64, b + kHalfTokens, kResults, true);
+          products_done(empty + 8 * k.slot);
+          if (j + 2 < n) scores(j + 2, next_k.slot);   // overwrites dS of tile j after it has been read
           if (j + 1 == n) products_done(done);
         }
         __syncwarp();
+        k.next(2);
+        v.next(2);
+        next_k.next(2);
       }
     } else if (warp == 10) {
       // -------------------------------------------------- masks: which keys are read, and zeros where they are not
@@ -353,49 +360,57 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
-      const auto item_full = [&](int item) { return warp_wait(full + 8 * (item % S::kSlots), item / S::kSlots & 1, &failed); };
       const uint32_t keys = low_half(at_address(tile_descriptor(16), k_at)), values = low_half(at_address(tile_descriptor(16), v_at)),
                      ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
-      const auto slot_of = [&](int item) { return static_cast<uint32_t>(item % S::kSlots * S::kTile) >> 4; };
-      const auto scores = [&](int i) {
-        product_of_tiles<kDim>(tmem, keys, ring + slot_of(2 * i), kScores, steps);
+      const auto at_slot = [&](uint32_t slot) { return slot * (S::kTile >> 4); };
+      const auto scores = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem, keys, ring + at_slot(slot), kScores, steps);
         products_done(s_full);
       };
-      const auto dp = [&](int i) {
-        product_of_tiles<kDim>(tmem + dp_column, values, ring + slot_of(2 * i + 1), kScores, steps);
+      const auto dp = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem + dp_column, values, ring + at_slot(slot), kScores, steps);
         products_done(dp_full);
       };
-      bool going = warp_wait(k_full, 0, &failed) && item_full(0);
+      bool going = warp_wait3(k_full, 0, full, 0, 0, 0, &failed);
       if (going && elected()) scores(0);
       __syncwarp();
-      going = going && warp_wait(v_full, 0, &failed) && item_full(1);
-      if (going && elected()) dp(0);
+      going = going && warp_wait3(v_full, 0, full + 8, 0, 0, 0, &failed);
+      if (going && elected()) dp(1);
       __syncwarp();
+      Ring<S::kSlots> q, g, next_q, next_g;   // queries and their gradients, of this tile and the next
+      g.next();
+      next_q.next(2);
+      next_g.next(3);
+#pragma unroll 1
       for (int i = 0; i < n && going; i++) {
         const bool more = i + 1 < n;
-        going = (!more || item_full(2 * i + 2)) && warp_wait(p_full, i & 1, &failed);
+        going = warp_wait3(p_full, i & 1, more ? full + 8 * next_q.slot : 0, next_q.phase, 0, 0, &failed);
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          const uint32_t g = ring_tokens + slot_of(2 * i + 1);
-          product_over_tokens(tmem + dv_column, tmem, g, kResults, i > 0);
-          product_over_tokens(tmem + dv_column, tmem + 64, g + kHalfTokens, kResults, true);
-          if (more) scores(i + 1);   // overwrites P after it has been read
-          products_done(empty + 8 * ((2 * i + 1) % S::kSlots));
+          const uint32_t b = ring_tokens + at_slot(g.slot);
+          product_over_tokens(tmem + dv_column, tmem, b, kResults, i > 0);
+          product_over_tokens(tmem + dv_column, tmem + 64, b + kHalfTokens, kResults, true);
+          if (more) scores(next_q.slot);   // overwrites P after it has been read
+          products_done(empty + 8 * g.slot);
         }
         __syncwarp();
-        going = (!more || item_full(2 * i + 3)) && warp_wait(ds_full, i & 1, &failed);
+        going = warp_wait3(ds_full, i & 1, more ? full + 8 * next_g.slot : 0, next_g.phase, 0, 0, &failed);
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          const uint32_t q = ring_tokens + slot_of(2 * i);
-          product_over_tokens(tmem + dk_column, tmem + dp_column, q, kResults, i > 0);
-          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, q + kHalfTokens, kResults, true);
-          if (more) dp(i + 1);
-          products_done(empty + 8 * (2 * i % S::kSlots));
+          const uint32_t b = ring_tokens + at_slot(q.slot);
+          product_over_tokens(tmem + dk_column, tmem + dp_column, b, kResults, i > 0);
+          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, b + kHalfTokens, kResults, true);
+          if (more) dp(next_g.slot);
+          products_done(empty + 8 * q.slot);
           if (!more) products_done(done);
         }
         __syncwarp();
+        q.next(2);
+        g.next(2);
+        next_q.next(2);
+        next_g.next(2);
       }
     } else if (warp == 10) {
       // -------------------------------------------------- what is known of the queries; -infinity makes P = 0 where there is none

@@ -66,9 +66,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 template <int kSlots>
 struct Ring {
   uint32_t slot = 0, phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == kSlots) {
-      slot = 0;
+  __device__ __forceinline__ void next(uint32_t by = 1) {   // by at most kSlots
+    slot += by;
+    if (slot >= kSlots) {
+      slot -= kSlots;
       phase ^= 1;
     }
   }
