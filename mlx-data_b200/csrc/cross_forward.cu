@@ -99,8 +99,12 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
                  p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
 
-  const int q_tiles = (p.q_tokens + 255) / 256;
-  const int q0 = blockIdx.x % q_tiles * 256, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
+  // CTAs of 256 rows first, head by head; those of a ragged end of at most 128 rows, which take less time, after all others, where
+  // they fill the SMs that become free (333 rows, 96 heads: 31.9 us in order of tiles, 29.4 so).
+  const int q_tiles = (p.q_tokens + 255) / 256, end_rows = p.q_tokens - 256 * (q_tiles - 1), whole = end_rows > 128 ? q_tiles : q_tiles - 1;
+  const int id = blockIdx.x, wholes = whole * p.q_heads * p.batch;
+  const int of = id < wholes ? id / whole : id - wholes, q0 = (id < wholes ? id % whole : q_tiles - 1) * 256;
+  const int head = of % p.q_heads, batch = of / p.q_heads;
   const int rows = p.q_tokens - q0 > 128 ? 2 : 1;   // tiles of query rows
   if (threadIdx.x == 0) {
     failed = reach = 0;

@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_back
   __shared__ float weights[2][MLXD_ROTARY_MAX_HEAD_DIM];
   const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), mine = lane / p.lanes, at_once = 32 / p.lanes;
   float2* table = tables[threadIdx.x / 32];
+  asm volatile("griddepcontrol.launch_dependents;");
   const bool is_k = static_cast<int>(blockIdx.x) >= p.q_blocks;
   const Heads in = is_k ? p.k : p.q, gr = is_k ? p.k_grad : p.q_grad, out = is_k ? p.k_out : p.q_out;
   const int heads = is_k ? p.k_heads : p.q_heads;
@@ -422,7 +423,9 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const __grid_constant
   void* out = is_k ? dk : dq;
   if (!out) return;
   float sum = 0;
+  asm volatile("griddepcontrol.wait;" : : : "memory");   // it begins beside the end of the kernel before
   if (at < p.head_dim) {
+#pragma unroll 4
     for (int b = from + warp; b < to; b += 32) sum += p.partial[static_cast<int64_t>(b) * p.head_dim + at];
   }
   sums[warp][lane] = sum;
@@ -684,8 +687,16 @@ extern "C" int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const
       return cudaGetLastError();
     }));
     if (d->q_weight_grad || d->k_weight_grad) {
-      weight_grad_kernel<<<dim3((d->head_dim + 31) / 32, 2), 1024, 0, s>>>(p, blocks, d->q_weight_grad, d->k_weight_grad);
-      MLXD_CUDA(cudaGetLastError());
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3((d->head_dim + 31) / 32, 2);
+      config.blockDim = dim3(1024);
+      config.stream = s;
+      cudaLaunchAttribute early = {};
+      early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      early.val.programmaticStreamSerializationAllowed = 1;
+      config.attrs = &early;
+      config.numAttrs = 1;
+      MLXD_CUDA(cudaLaunchKernelEx(&config, weight_grad_kernel, p, blocks, d->q_weight_grad, d->k_weight_grad));
     }
     return static_cast<int>(MLXD_OK);
   });
