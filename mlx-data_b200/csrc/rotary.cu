@@ -14,7 +14,8 @@ namespace mlxd {
 namespace {
 
 constexpr int kWarps = 4;                                // of a CTA
-constexpr int kBackwardBlocks = 3;                       // CTAs of an SM in the backward pass
+constexpr int kForwardBlocks = 7;                        // CTAs of an SM: 28 warps of 72 registers
+constexpr int kBackwardBlocks = 3;                       // in the backward pass, of 165 registers
 constexpr int kMaxPairs = MLXD_ROTARY_MAX_HEAD_DIM / 2;
 
 struct Heads {
@@ -243,11 +244,13 @@ __device__ void read_weights(const RotaryParams& p, float (&w)[2][MLXD_ROTARY_MA
 // of its heads where tokens are few: each angle of the token once (its sine and cosine are what costs, and all heads share them),
 // then its heads, 32 / lanes at a time, queries first.  The next heads are loaded while these are worked on.  A warp a token and no loop
 // over tokens: CTAs that fit at once, looping, took 65 us instead of 46 (16 x 1024 tokens, 32 heads of 80), since a token's
-// positions and sines are waited for one token after another then.  Measured: 3 x 4099 tokens, 32 heads of 128, float16, norm: 50.6 us,
-// 4.0 TB/s; 16 x 1024 tokens, 32 heads of 80: 48 us, 3.5 TB/s (five of eight lanes own a unit); 19600 tokens, 48 heads of 64, float32:
-// 80 us, 6.0 TB/s; one token of 40 heads 2.8 us.  Bound by the issue of instructions for 16-bit types (about 100 for four heads of 128).
+// positions and sines are waited for one token after another then.  Seven CTAs an SM, by their registers, with the few spills that
+// takes: without a limit (five) 48.0 us, six 46.0, seven 42.0, eight 42.4, nine 44.9 for those; 50.6, 50.6, 45.6 for five, six, seven
+// with the norm (3 x 4099 tokens, 32 heads of 128, float16), 4.4 TB/s.  19600 tokens, 48 heads of 64, float32: 80 us, 6.0 TB/s;
+// one token of 40 heads 2.8 us.  Bound by latency and the issue of instructions for 16-bit types (about 100 for four heads of 128; heads of
+// 80 use five of eight lanes).
 template <class T, int kV, int kUnits, bool kAdjacent, bool kNorm>
-__global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(const __grid_constant__ RotaryParams p) {
   using L = Lane<T, kV, kUnits, kAdjacent>;
   __shared__ float2 tables[kWarps][kMaxPairs];
   __shared__ float weights[2][kNorm ? MLXD_ROTARY_MAX_HEAD_DIM : 1];
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const __grid_consta
 // With g = R^-1(dy), n = x r: dw = sum g n, dx = r (g w - n mean(g w n)); r is worked out again, so that the forward pass keeps nothing.
 // The first p.q_blocks CTAs take the tokens' queries, the others their keys, so that a lane holds the sums of one weight's
 // gradient: over all tokens it meets, then over the lanes and warps of the CTA in a fixed order, one row of p.partial a CTA.
-// Measured: forward and backward of 8 x 2048 tokens, 32 heads of 128, 164 us (4.1 TB/s).  Three CTAs of 165 registers an SM: four
+// Measured: forward and backward of 8 x 2048 tokens, 32 heads of 128, 160 us (4.2 TB/s).  Three CTAs of 165 registers an SM: four
 // (128 registers, spills) took 177, 8-byte vectors, which need fewer, 215.
 template <class T, int kV, int kUnits, bool kAdjacent>
 __global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
