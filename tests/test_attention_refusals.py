@@ -146,3 +146,36 @@ def test_tensors_that_do_not_fit(pkg):
         with pytest.raises(ValueError):
             call()
             pytest.fail("call %d was taken" % i)
+
+
+@pytest.mark.parametrize("entry", ["mlxd_cross_attention", "mlxd_cross_attention_backward"])
+@pytest.mark.parametrize("change,text", [(dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(kv_tokens=(1 << 30) + 1), "2^30"),
+                                         (dict(batch=1 << 10, kv_tokens=1 << 30, q_heads=4, kv_heads=4), "too many keys")])
+def test_cross_limits(pkg, entry, change, text):
+    rc, why = _call(pkg, entry, _cross(pkg._capi, **change))
+    assert rc == pkg._capi.ERR_INVALID and text in why
+
+
+@pytest.mark.gpu
+def test_self_check_word_is_clean(pkg):
+    x = torch.randn(2, 200, 4, 64, device="cuda").to(torch.bfloat16)
+    out, lse = pkg.attention.cross_attention(x, x, x, return_lse=True)
+    pkg.attention.cross_attention_backward(x, x, x, x, out, lse)
+    assert pkg._capi.attention_status(0, torch.cuda.current_stream().cuda_stream) == 0
+    assert pkg._capi.load().mlxd_attention_status(0, None, None) == pkg._capi.ERR_INVALID
+
+
+@pytest.mark.gpu
+def test_keys_end_where_the_mask_does(pkg):
+    """Under a mask whose last keys are not read the call gives what the shorter call gives."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    for tokens in (1, 300):
+        q, k, v = (torch.randn(s, generator=gen, device="cuda").to(torch.float16)
+                   for s in ((2, tokens, 4, 64), (2, 1500, 4, 64), (2, 1500, 4, 64)))
+        for end in (0, 1, 127, 128, 129, 640, 641, 1499):
+            mask = torch.zeros(2, 1500, dtype=torch.bool, device="cuda")
+            mask[:, :end] = True
+            got = pkg.attention.cross_attention(q, k, v, key_mask=mask)
+            want = pkg.attention.cross_attention(q, k, v, lengths=torch.tensor([end, end], device="cuda"))
+            assert torch.equal(got, want)
