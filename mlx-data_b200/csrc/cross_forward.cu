@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
       total += exchange[t][half ^ 1][row];
       if (done) {
         tmem_after_sync();
-        const float by = total > 0 ? 1.0f / total : 0.0f;
+        // only a sum of 0 is a row without keys; one that is not a number stays so, in lse too
+        const float by = total == 0 ? 0.0f : 1.0f / total;
         const uint32_t staged = tiles_at + t * S::kTile;   // the queries are no longer needed
 #pragma unroll
         for (int x = 0; x < kDim / 2; x += 32) {
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         }
         if (p.lse && half == 0 && q0 + 128 * t + row < p.q_tokens) {
           p.lse[(static_cast<int64_t>(batch) * p.q_heads + head) * p.q_tokens + q0 + 128 * t + row] =
-              total > 0 ? top * p.scale + logf(total) : -INFINITY;
+              total == 0 ? -INFINITY : top * p.scale + logf(total);
         }
         fence_async_proxy();
         warp_arrive(staged_full + 8 * t, lane);

@@ -217,8 +217,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) cross_step_kernel(const __grid
 #pragma unroll
       for (int j = 0; j < 8; j++) e[j] += warp_out[i][r][x + j] * by;
     }
-    const float by = sum > 0 ? 1.0f / sum : 0.0f;
-    const float lse = sum > 0 ? most * p.scale + logf(sum) : -INFINITY;
+    // only a sum of 0 is a row without keys; one that is not a number stays so, in lse too, where the joining finds it
+    const float by = sum == 0 ? 0.0f : 1.0f / sum;
+    const float lse = sum == 0 ? -INFINITY : most * p.scale + logf(sum);
     const int64_t stat = (static_cast<int64_t>(batch) * p.q_heads + head) * p.q_tokens + token;
     if (x < p.head_dim) {
       if (sp.splits > 1) {
@@ -251,16 +252,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
   const int parts = (length_of(p, batch) + sp.split_keys - 1) / sp.split_keys;
   asm volatile("griddepcontrol.wait;" : : : "memory");
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 32 * kJoinWarps) top = fmaxf(top, sp.part_lse[i * all + stat]);
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  for (int i = threadIdx.x; i < parts; i += 32 * kJoinWarps) top = max_or_nan(top, sp.part_lse[i * all + stat]);
+  for (int d = 16; d; d >>= 1) top = max_or_nan(top, __shfl_xor_sync(~0u, top, d));
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; i++) top = fmaxf(top, tops[i]);
+  for (int i = 0; i < kJoinWarps; i++) top = max_or_nan(top, tops[i]);
   float4 o = {};
   float total = 0;
   const bool there = 4 * lane < p.head_dim;
-  if (top > -INFINITY) {
+  if (top != -INFINITY) {
 #pragma unroll 4
     for (int i = warp; i < parts; i += kJoinWarps) {
       const float w = exp2_of((sp.part_lse[i * all + stat] - top) * kLog2e);
@@ -283,12 +284,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
     o.z += sums[i][lane].z;
     o.w += sums[i][lane].w;
   }
-  const float by = total > 0 ? 1.0f / total : 0.0f;
+  const float by = total == 0 ? 0.0f : 1.0f / total;
   if (there) {
     T* to = reinterpret_cast<T*>(p.out.data) + batch * p.out.batch + token * p.out.token + head * p.out.head + 4 * lane;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(o.x * by, o.y * by), pack2<T>(o.z * by, o.w * by));
   }
-  if (lane == 0 && p.lse) p.lse[stat] = total > 0 ? top + logf(total) : -INFINITY;
+  if (lane == 0 && p.lse) p.lse[stat] = total == 0 ? -INFINITY : top + logf(total);
 }
 
 // Keys of a CTA: 2048 (sixteen sequences of up to 6404 keys: 57 us, with 1024 60, with 512 66), fewer (down to one round of its warps) while CTAs are fewer than two an SM, more while they are over four

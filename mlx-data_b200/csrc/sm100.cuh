@@ -250,6 +250,13 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
+// The larger of two; what is not a number goes on (fmaxf leaves it out).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // a * b + c for two floats at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;

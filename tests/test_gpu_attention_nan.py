@@ -1,0 +1,51 @@
+"""Numbers that are none in what is read: they reach the rows that read them and no others, whichever way a call takes."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+# batch, tokens, keys, q heads, kv heads, head_dim: single tokens of one part, of some, of more than 32 parts; many queries
+WAYS = [(1, 1, 50, 4, 2, 64), (1, 1, 1601, 32, 8, 128), (1, 1, 6404, 2, 1, 128), (2, 3, 700, 4, 4, 80),
+        (1, 300, 385, 4, 2, 128), (2, 257, 130, 4, 2, 64)]
+
+
+def _inputs(shape, dtype):
+    b, t, n, hq, hk, d = shape
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    return [torch.randn(s, generator=gen, device="cuda").to(dtype) for s in ((b, t, hq, d), (b, n, hk, d), (b, n, hk, d))]
+
+
+def _only(got, clean, rows):
+    """Rows [batch, head, token] are not numbers, in the result and in lse; the others are what they were."""
+    out, lse = got[0].transpose(1, 2), got[1]
+    assert torch.isnan(out[rows]).all() and torch.isnan(lse[rows]).all()
+    assert torch.equal(out[~rows], clean[0].transpose(1, 2)[~rows]) and torch.equal(lse[~rows], clean[1][~rows])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", WAYS)
+def test_nan_in_a_query(pkg, shape, dtype):
+    q, k, v = _inputs(shape, dtype)
+    clean = pkg.attention.cross_attention(q, k, v, return_lse=True)
+    q[-1, -1, 1, 3] = math.nan
+    rows = torch.zeros(clean[1].shape, dtype=torch.bool, device="cuda")
+    rows[-1, 1, -1] = True
+    _only(pkg.attention.cross_attention(q, k, v, return_lse=True), clean, rows)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("key", [2, 19, 45])
+@pytest.mark.parametrize("shape", WAYS)
+def test_nan_in_a_key_that_is_read(pkg, shape, key, value):
+    """A score that is not a number or is infinite leaves its rows without a number: exp(inf - inf)."""
+    q, k, v = _inputs(shape, torch.bfloat16)
+    q = q.abs()
+    clean = pkg.attention.cross_attention(q, k, v, return_lse=True)
+    k[0, key, 0, 5] = value
+    rows = torch.zeros(clean[1].shape, dtype=torch.bool, device="cuda")
+    rows[0, :shape[3] // shape[4]] = True
+    _only(pkg.attention.cross_attention(q, k, v, return_lse=True), clean, rows)
