@@ -282,7 +282,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 // 2^x for two floats at once on the pipe of multiply-adds, which has time where the one for exponentials has not: x = n + f with n the
 // nearest integer (by adding 1.5 * 2^23), 2^f = 1 + f q(f) with the cubic q of least largest relative error on [-1/2, 1/2] (2.9e-6, by
-// exchange), n added to the exponent.  -infinity gives 0; what is not a number gives something that is not finite.
+// exchange), times 2^n, whose bits are n in the exponent.  At most 2^-127 gives 0, -infinity too; what is not a number stays so, by that
+// product (n added to the exponent of q would leave NaN with the bits of the largest finite number).
 __device__ __forceinline__ float2 exp2_by_fma(float2 x) {
   constexpr float kRound = 12582912.0f;
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.0f));
@@ -293,7 +294,8 @@ __device__ __forceinline__ float2 exp2_by_fma(float2 x) {
   q = fma2(f, q, make_float2(0.24024099f, 0.24024099f));
   q = fma2(f, q, make_float2(0.6931242f, 0.6931242f));
   q = fma2(f, q, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+  constexpr int kOne = 127 << 23;
+  return mul2(q, make_float2(__int_as_float((__float_as_int(t.x) << 23) + kOne), __int_as_float((__float_as_int(t.y) << 23) + kOne)));
 }
 
 // Two floats rounded to 16 bits each, the first in the lower half.

@@ -49,3 +49,15 @@ def test_nan_in_a_key_that_is_read(pkg, shape, key, value):
     rows = torch.zeros(clean[1].shape, dtype=torch.bool, device="cuda")
     rows[0, :shape[3] // shape[4]] = True
     _only(pkg.attention.cross_attention(q, k, v, return_lse=True), clean, rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("key", [0, 1, 16, 49, 64, 113, 127, 128, 352])
+def test_nan_in_any_column_of_a_tile(pkg, key, dtype):
+    """Of every eight pairs of keys the first is weighed in another way than the rest."""
+    q, k, v = _inputs((1, 300, 385, 4, 2, 64), dtype)
+    clean = pkg.attention.cross_attention(q, k, v, return_lse=True)
+    k[0, key, 1, 0] = math.nan
+    rows = torch.zeros(clean[1].shape, dtype=torch.bool, device="cuda")
+    rows[0, 2:] = True
+    _only(pkg.attention.cross_attention(q, k, v, return_lse=True), clean, rows)
