@@ -61,3 +61,25 @@ def test_nan_in_any_column_of_a_tile(pkg, key, dtype):
     rows = torch.zeros(clean[1].shape, dtype=torch.bool, device="cuda")
     rows[0, 2:] = True
     _only(pkg.attention.cross_attention(q, k, v, return_lse=True), clean, rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", WAYS)
+def test_gradients_beside_a_score_of_minus_infinity(pkg, shape, dtype):
+    """A key whose scores are all -infinity is a key that is not read, for every gradient but the one that its infinity multiplies."""
+    q, k, v = _inputs(shape, dtype)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    dout = torch.randn_like(q)
+    mask = torch.ones(k.shape[:2], dtype=torch.bool, device="cuda")
+    mask[0, 19] = False
+
+    def both(k, **how):
+        out, lse = pkg.attention.cross_attention(q, k, v, return_lse=True, **how)
+        return out, lse, *pkg.attention.cross_attention_backward(dout, q, k, v, out, lse, **how)
+
+    want = both(k, key_mask=mask)
+    bad = k.clone()
+    bad[0, 19, :, 0] = -math.inf
+    out, lse, dq, dk, dv = both(bad)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert torch.equal(dq[..., 1:], want[2][..., 1:]) and torch.equal(dk, want[3]) and torch.equal(dv, want[4])
