@@ -58,6 +58,10 @@ cudaError_t launch_cross_step(const CrossParams& p, void* workspace, int sms, in
 cudaError_t launch_cross_backward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
 
 #ifdef __CUDACC__
+// What a row's scores c s are added to in the backward pass, so that 2^(c s + base) is its weight.  A row whose scores are all -infinity
+// has no weights: 0, as in the forward pass, not the infinity less infinity that its lse would give.
+__device__ __forceinline__ float row_base(float lse) { return lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f; }
+
 __device__ __forceinline__ int length_of(const CrossParams& p, int b) {
   if (!p.lengths) return p.kv_tokens;
   const int64_t n = p.lengths_dtype == MLXD_I64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
     const float delta = going ? delta_parts[0][row] + delta_parts[1][row] : 0.0f;
     if (there && half == 0) p.delta[stat] = delta;
     // a row that is not there gets P = 0
-    const float base = there ? -p.lse[stat] * kLog2e : -INFINITY;
+    const float base = there ? row_base(p.lse[stat]) : -INFINITY;
     for (int j = 0; j < n && going; j++) {
       const uint32_t mine = tmem + 128 * (j & 1) + 64 * half + lanes;
       uint32_t s[64];
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
         float lse[4], delta[4];
         for (int k = 0; k < 4; k++) {
           const int token = i % q_tiles * 128 + k * 32 + lane;
-          lse[k] = token < p.q_tokens ? -p.lse[first + token] * kLog2e : -INFINITY;
+          lse[k] = token < p.q_tokens ? row_base(p.lse[first + token]) : -INFINITY;
           delta[k] = token < p.q_tokens ? p.delta[first + token] : 0.0f;
         }
         if (i >= 2 && !warp_wait(stats_empty + 8 * (i & 1), (i / 2 - 1) & 1, &failed)) break;

@@ -83,3 +83,27 @@ def test_gradients_beside_a_score_of_minus_infinity(pkg, shape, dtype):
     out, lse, dq, dk, dv = both(bad)
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     assert torch.equal(dq[..., 1:], want[2][..., 1:]) and torch.equal(dk, want[3]) and torch.equal(dv, want[4])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", WAYS)
+def test_gradients_of_rows_without_weights(pkg, shape, dtype):
+    """Scores that are all -infinity give zeros, lse of -infinity and no gradients to keys and values; neighbours keep theirs."""
+    q, k, v = _inputs(shape, dtype)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    dout = torch.randn_like(q)
+
+    def both():
+        out, lse = pkg.attention.cross_attention(q, k, v, return_lse=True)
+        return out, lse, *pkg.attention.cross_attention_backward(dout, q, k, v, out, lse)
+
+    clean = both()
+    k[0, :, 0, 0] = -math.inf
+    group = shape[3] // shape[4]
+    out, lse, dq, dk, dv = both()
+    assert not out[0, :, :group].any() and (lse[0, :group] == -math.inf).all()
+    assert not dk[0, :, 0].any() and not dv[0, :, 0].any()
+    assert not dq[0, :, :group, 1:].any()            # element 0 is 0 times the infinity in the keys
+    for got, want in ((dq, clean[2]), (dk, clean[3]), (dv, clean[4])):
+        heads = group if got is dq else 1
+        assert torch.equal(got[:, :, heads:], want[:, :, heads:]) and torch.equal(got[1:], want[1:])
