@@ -127,6 +127,14 @@ struct Lane {
     }
   }
 
+  // Which of the lane's pairs are turned, a bit each.
+  __device__ uint32_t turned(const RotaryParams& p, int first) const {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) bits |= ((1u << min(max(p.pairs - (first + 32 * k) * kV, 0), kV)) - 1) << (k * kV);
+    return bits;
+  }
+
   // Cosines and sines of the lane's pairs out of the warp's table.
   __device__ void angles(const float2* table, int first, Pairs& u) const {
 #pragma unroll
@@ -227,6 +235,35 @@ __device__ __forceinline__ void put(float* v, int i, float2 x) {
 __device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+// Which pairs of a lane are turned: all of every head; all or none of a lane's; any.
+enum Turned { kAll, kLanes, kAny };
+
+// Turns a lane's pairs where a part of the head passes through.  Elements that pass through stay as they are, bit by bit: a cosine of 1 and
+// a sine of 0 would carry an infinity from one of two to the other.  kLanes: products with the cosines, which are 1, then those with
+// the sines under a predicate; kAny: a choice for every element.  4 x 2048 tokens, 32 heads of 64, bfloat16, 28 and 16 pairs of 32: 12.2
+// and 12.0 us by a predicate, 12.6 and 12.8 by choices (sines of 0: 11.6 and 11.2); 16 pairs of neighbours 13.4 and 11.5 (11.2); in
+// float32, 19600 tokens, 48 heads of 64, neighbours, 79.5 and 81.5 us (80.0).
+template <Turned kTurned, class L>
+__device__ __forceinline__ void turn_part(uint32_t turned, const typename L::Pairs& u, typename L::Pairs& e) {
+#pragma unroll
+  for (int i = 0; i < L::kN; i += 2) {
+    const float2 a = two(e.a, i), c = two(e.b, i), cos = two(u.a, i), sin = two(u.b, i);
+    float2 x = mul2(a, cos), y = mul2(c, cos);
+    if constexpr (kTurned == kLanes) {
+      fma2_if(turned, c, neg2(sin), x);
+      fma2_if(turned, a, sin, y);
+    } else {
+      x = fma2(c, neg2(sin), x);
+      y = fma2(a, sin, y);
+      const bool first = turned >> i & 1, second = turned >> (i + 1) & 1;
+      x = make_float2(first ? x.x : a.x, second ? x.y : a.y);
+      y = make_float2(first ? y.x : c.x, second ? y.y : c.y);
+    }
+    put(e.a, i, x);
+    put(e.b, i, y);
+  }
+}
+
 __device__ float lanes_sum(float v, int lanes) {
   for (int d = lanes >> 1; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
   return v;
@@ -249,7 +286,7 @@ __device__ void read_weights(const RotaryParams& p, float (&w)[2][MLXD_ROTARY_MA
 // with the norm (3 x 4099 tokens, 32 heads of 128, float16), 4.4 TB/s.  19600 tokens, 48 heads of 64, float32: 80 us, 6.0 TB/s;
 // one token of 40 heads 2.8 us.  Bound by latency and the issue of instructions for 16-bit types (about 100 for four heads of 128; heads of
 // 80 use five of eight lanes).
-template <class T, int kV, int kUnits, bool kAdjacent, bool kNorm>
+template <class T, int kV, int kUnits, bool kAdjacent, Turned kTurned, bool kNorm>
 __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(const __grid_constant__ RotaryParams p) {
   using L = Lane<T, kV, kUnits, kAdjacent>;
   __shared__ float2 tables[kWarps][kMaxPairs];
@@ -277,6 +314,7 @@ __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(con
     __syncwarp();
     typename L::Pairs u, w;
     me.angles(table, first, u);
+    const uint32_t turned = kTurned == kAll ? 0 : me.turned(p, first);
 #pragma unroll 1
     for (int is_k = 0; is_k < 2; is_k++) {
       const Heads& in = is_k ? p.k : p.q;
@@ -306,11 +344,15 @@ __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(con
             put(e.b, i, mul2(mul2(two(e.b, i), r), two(w.b, i)));
           }
         }
+        if constexpr (kTurned == kAll) {
 #pragma unroll
-        for (int i = 0; i < L::kN; i += 2) {
-          const float2 a = two(e.a, i), c = two(e.b, i), cos = two(u.a, i), sin = two(u.b, i);
-          put(e.a, i, fma2(c, neg2(sin), mul2(a, cos)));
-          put(e.b, i, fma2(a, sin, mul2(c, cos)));
+          for (int i = 0; i < L::kN; i += 2) {
+            const float2 a = two(e.a, i), c = two(e.b, i), cos = two(u.a, i), sin = two(u.b, i);
+            put(e.a, i, fma2(c, neg2(sin), mul2(a, cos)));
+            put(e.b, i, fma2(a, sin, mul2(c, cos)));
+          }
+        } else {
+          turn_part<kTurned, L>(turned, u, e);
         }
         if (h < heads) me.store(y, e);
         y += out_step;
@@ -324,7 +366,7 @@ __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(con
 // gradient: over all tokens it meets, then over the lanes and warps of the CTA in a fixed order, one row of p.partial a CTA.
 // Measured: forward and backward of 8 x 2048 tokens, 32 heads of 128, 160 us (4.2 TB/s).  Three CTAs of 165 registers an SM: four
 // (128 registers, spills) took 177, 8-byte vectors, which need fewer, 215.
-template <class T, int kV, int kUnits, bool kAdjacent>
+template <class T, int kV, int kUnits, bool kAdjacent, Turned kTurned>
 __global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
   using L = Lane<T, kV, kUnits, kAdjacent>;
   __shared__ float2 tables[kWarps][kMaxPairs];
@@ -339,6 +381,7 @@ __global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_back
   const uint32_t stride = (is_k ? gridDim.x - p.q_blocks : p.q_blocks) * kWarps;
   const L me(p, first);
   read_weights(p, weights);
+  const uint32_t turned = kTurned == kAll ? 0 : me.turned(p, first);
   typename L::Pairs w, dw = {};
   me.gather(weights[is_k], w);
   for (uint32_t row = block * kWarps + threadIdx.x / 32; row < p.rows; row += stride) {
@@ -362,10 +405,11 @@ __global__ void __launch_bounds__(32 * kWarps, kBackwardBlocks) norm_rotary_back
       me.load(x, h + at_once < heads, rx);
       me.load(dy, h + at_once < heads, rg);
       float2 sum = {}, dot = {};
+      if constexpr (kTurned != kAll) turn_part<kTurned, L>(turned, u, g);
 #pragma unroll
       for (int i = 0; i < L::kN; i += 2) {
         const float2 a = two(g.a, i), c = two(g.b, i), cos = two(u.a, i), sin = two(u.b, i), f = two(e.a, i), k = two(e.b, i);
-        const float2 ga = fma2(c, neg2(sin), mul2(a, cos)), gb = fma2(a, sin, mul2(c, cos));
+        const float2 ga = kTurned == kAll ? fma2(c, neg2(sin), mul2(a, cos)) : a, gb = kTurned == kAll ? fma2(a, sin, mul2(c, cos)) : c;
         put(g.a, i, ga);
         put(g.b, i, gb);
         sum = fma2(f, f, fma2(k, k, sum));
@@ -572,13 +616,23 @@ int lanes_of(int units) {
   return lanes;
 }
 
-// Calls f with the instance's constants: vector length, units of a lane, neighbours as pairs.
+// Calls f with the instance's constants: vector length, units of a lane, neighbours as pairs, which pairs are turned.
 template <class T, class F>
 cudaError_t with_instance(const RotaryParams& p, int v, F&& f) {
   constexpr int kWide = 16 / sizeof(T);
   using std::integral_constant;
   const auto go = [&](auto vec, auto units) {
-    return p.adjacent ? f(T(), vec, units, std::true_type()) : f(T(), vec, units, std::false_type());
+    const auto part = [&](auto adjacent, auto kind) {
+      return 2 * p.pairs == p.head_dim ? f(T(), vec, units, adjacent, integral_constant<Turned, kAll>()) : f(T(), vec, units, adjacent, kind);
+    };
+    // a vector of halves is turned or not (vector_of); neighbours may end inside one, single pairs of one lane lie apart
+    using any = integral_constant<Turned, kAny>;
+    using several = integral_constant<Turned, vec() == 1 ? kAny : kLanes>;
+    if (!p.adjacent) return part(std::false_type(), several());
+    if constexpr (sizeof(T) == 4) {
+      if (p.pairs % vec() == 0) return part(std::true_type(), several());
+    }
+    return part(std::true_type(), any());
   };
   if (v == kWide) return go(integral_constant<int, kWide>(), integral_constant<int, 1>());
   if (v == 4) return go(integral_constant<int, 4>(), integral_constant<int, 1>());
@@ -613,10 +667,10 @@ int forward(const char* entry, int device, void* stream, const mlxd_rotary_desc*
   MLXD_ON_DEVICE(device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned blocks = static_cast<unsigned>((p.rows * p.parts + kWarps - 1) / kWarps);
-  const cudaError_t e = with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent) {
+  const cudaError_t e = with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
     using T = decltype(type);
-    if (pass == Pass::kNorm) rotary_kernel<T, vec(), units(), adjacent(), true><<<blocks, 32 * kWarps, 0, s>>>(p);
-    else rotary_kernel<T, vec(), units(), adjacent(), false><<<blocks, 32 * kWarps, 0, s>>>(p);
+    if (pass == Pass::kNorm) rotary_kernel<T, vec(), units(), adjacent(), turned(), true><<<blocks, 32 * kWarps, 0, s>>>(p);
+    else rotary_kernel<T, vec(), units(), adjacent(), turned(), false><<<blocks, 32 * kWarps, 0, s>>>(p);
     return cudaGetLastError();
   });
   return e == cudaSuccess ? MLXD_OK : fail_cuda(e, entry);
@@ -685,8 +739,8 @@ extern "C" int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const
     p.lanes = lanes_of(p.head_dim / 2 / v);
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    MLXD_CUDA(with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent) {
-      norm_rotary_backward_kernel<decltype(type), vec(), units(), adjacent()><<<blocks, 32 * kWarps, 0, s>>>(p);
+    MLXD_CUDA(with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
+      norm_rotary_backward_kernel<decltype(type), vec(), units(), adjacent(), turned()><<<blocks, 32 * kWarps, 0, s>>>(p);
       return cudaGetLastError();
     }));
     if (d->q_weight_grad || d->k_weight_grad) {

@@ -266,6 +266,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+// c += a * b where `is` is not 0, by a predicate: c does not see a and b elsewhere
+__device__ __forceinline__ void fma2_if(uint32_t is, float2 a, float2 b, float2& c) {
+  asm("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\n@p fma.rn.f32x2 %0, %1, %2, %0;\n}"
+      : "+l"(reinterpret_cast<uint64_t&>(c))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "r"(is));
+}
+
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("add.rn.f32x2 %0, %1, %2;"
