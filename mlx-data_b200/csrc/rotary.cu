@@ -730,8 +730,7 @@ extern "C" int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const
     rc = device_sms(device, &sms);
     if (rc != MLXD_OK) return rc;
     backward_blocks(p.rows, p.q_heads, p.k_heads, sms, &p.q_blocks, &blocks);
-    if (!blocks) return static_cast<int>(MLXD_OK);
-    if (!d->workspace || d->workspace_bytes < sizeof(float) * d->head_dim * blocks) {
+    if (blocks && (!d->workspace || d->workspace_bytes < sizeof(float) * d->head_dim * blocks)) {
       return fail(MLXD_ERR_INVALID, std::string(entry) + ": workspace too small");
     }
     p.partial = static_cast<float*>(d->workspace);
@@ -739,10 +738,13 @@ extern "C" int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const
     p.lanes = lanes_of(p.head_dim / 2 / v);
     MLXD_ON_DEVICE(device);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    MLXD_CUDA(with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
-      norm_rotary_backward_kernel<decltype(type), vec(), units(), adjacent(), turned()><<<blocks, 32 * kWarps, 0, s>>>(p);
-      return cudaGetLastError();
-    }));
+    if (blocks) {
+      MLXD_CUDA(with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
+        norm_rotary_backward_kernel<decltype(type), vec(), units(), adjacent(), turned()><<<blocks, 32 * kWarps, 0, s>>>(p);
+        return cudaGetLastError();
+      }));
+    }
+    // without heads too: the sums of nothing
     if (d->q_weight_grad || d->k_weight_grad) {
       cudaLaunchConfig_t config = {};
       config.gridDim = dim3((d->head_dim + 31) / 32, 2);
