@@ -278,7 +278,8 @@ MLXD_API int mlxd_stats_get(mlxd_ctx* ctx, mlxd_stats* out);
  * queued on the caller's CUDA stream (NULL: the default stream) and may be
  * captured into a graph.  Nothing is allocated: the calls that need scratch
  * memory take a workspace, whose contents matter only during the call.  The
- * structs are read before the call returns.  Results do not depend on the
+ * structs are read before the call returns; a pointer that is not aligned to
+ * its elements (a workspace: to 16 bytes) is refused.  Results do not depend on the
  * order in which blocks run: there are no atomic sums. */
 
 /* A [batch, tokens, heads, head_dim] tensor, head_dim contiguous, the other

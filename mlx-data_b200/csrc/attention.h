@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cstdint>
 #include <exception>
 #include <new>
 #include <string>
@@ -20,6 +21,11 @@ inline int dtype_bytes(int dtype) {
     case MLXD_I64: return 8;
     default: return 0;
   }
+}
+
+// Whether a pointer can be read in units of `bytes`; NULL can.
+inline bool on_boundary(const void* p, int bytes) {
+  return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0;
 }
 
 // No exception leaves a C entry point.

@@ -103,6 +103,10 @@ int params_of(const char* entry, const mlxd_cross_desc* d, bool backward, CrossP
     }
   }
   if (backward && b && t && !d->lse) return bad("lse is needed");
+  // a kernel reads and writes whole elements, and a misaligned one is a fault
+  if (!on_boundary(d->lse, 4)) return bad("lse does not start on a multiple of 4 bytes");
+  if (d->lengths && !on_boundary(d->lengths, dtype_bytes(d->lengths_dtype))) return bad("lengths do not start on a multiple of their element's size");
+  if (!on_boundary(d->workspace, 16)) return bad("workspace must start on 16 bytes");
   p = sizes_of(d);
   p.q = heads_of(d->q);
   p.k = heads_of(d->k);

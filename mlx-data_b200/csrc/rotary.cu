@@ -557,6 +557,20 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
     if (d->k_heads && (absent(d->k) || absent(d->k_out))) return bad("k and k_out are needed");
     if (pass == Pass::kBackward && ((d->q_heads && absent(d->q_grad)) || (d->k_heads && absent(d->k_grad)))) return bad("q_grad and k_grad are needed");
   }
+  // a kernel reads and writes whole elements, and a misaligned one is a fault
+  const int bytes = dtype_bytes(d->dtype);
+  for (const mlxd_heads* h : {&d->q, &d->q_out, &d->k, &d->k_out, &d->q_grad, &d->k_grad}) {
+    if (!on_boundary(h->data, bytes)) return bad("a tensor does not start on a multiple of its element's size");
+  }
+  if (!on_boundary(d->positions, dtype_bytes(d->positions_dtype)) || !on_boundary(d->frequencies, 4)) {
+    return bad("positions or frequencies do not start on a multiple of their element's size");
+  }
+  if (pass != Pass::kRotary) {
+    for (const void* w : {d->q_weight, d->k_weight, static_cast<const void*>(d->q_weight_grad), static_cast<const void*>(d->k_weight_grad)}) {
+      if (!on_boundary(w, dtype_bytes(d->weight_dtype))) return bad("a weight or its gradient does not start on a multiple of its element's size");
+    }
+  }
+  if (pass == Pass::kBackward && !on_boundary(d->workspace, 16)) return bad("workspace must start on 16 bytes");
   p.q = heads_of(d->q);
   p.k = heads_of(d->k);
   p.q_out = heads_of(d->q_out);
