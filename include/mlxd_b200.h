@@ -304,7 +304,7 @@ typedef struct mlxd_heads {
  * (same pointer, same strides); other overlaps are not allowed. */
 typedef struct mlxd_rotary_desc {
   int32_t dtype;                 /* of q, k and their results: MLXD_F32, MLXD_BF16 or MLXD_F16 */
-  int32_t batch, tokens, q_heads, k_heads;
+  int32_t batch, tokens, q_heads, k_heads;   /* at most 2^29 heads */
   int32_t head_dim;              /* even, at most MLXD_ROTARY_MAX_HEAD_DIM */
   mlxd_heads q, k, q_out, k_out;
   const void* positions;         /* [n_axes, batch, tokens] */

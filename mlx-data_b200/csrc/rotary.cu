@@ -17,6 +17,7 @@ constexpr int kWarps = 4;                                // of a CTA
 constexpr int kForwardBlocks = 7;                        // CTAs of an SM: 28 warps of 72 registers
 constexpr int kBackwardBlocks = 3;                       // in the backward pass, of 165 registers
 constexpr int kMaxPairs = MLXD_ROTARY_MAX_HEAD_DIM / 2;
+constexpr int kMaxHeads = 1 << 29;                       // of q, and of k: counts of both, and a step beyond the last, fit an int
 
 struct Heads {
   char* data;
@@ -512,6 +513,7 @@ int check_sizes(const char* entry, const mlxd_rotary_desc* d) {
   if (d->head_dim <= 0 || d->head_dim % 2 || d->head_dim > MLXD_ROTARY_MAX_HEAD_DIM) {
     return bad("head_dim must be even, from 2 to " + std::to_string(MLXD_ROTARY_MAX_HEAD_DIM) + " (got " + std::to_string(d->head_dim) + ")");
   }
+  if (d->q_heads > kMaxHeads || d->k_heads > kMaxHeads) return bad("more than 2^29 heads");
   if (static_cast<int64_t>(d->batch) * d->tokens > INT32_MAX) return bad("more than 2^31 - 1 tokens");
   return MLXD_OK;
 }

@@ -63,3 +63,18 @@ def test_cross(pkg, entry):
             setattr(d, k, v)
         rc, why = _call(pkg, entry, d)
         assert rc == capi.ERR_INVALID and ("multiple of" in why or "16 bytes" in why), (change, why)
+
+
+@pytest.mark.parametrize("entry", ENTRIES + ["mlxd_qk_norm_rotary_workspace"])
+@pytest.mark.parametrize("name", ["q_heads", "k_heads"])
+def test_more_heads_than_the_kernels_count(pkg, entry, name):
+    """Numbers of heads near 2^31, whose sums and steps would not fit an int."""
+    capi, lib = pkg._capi, pkg._capi.load()
+    for heads in ((1 << 29) + 1, (1 << 31) - 1):
+        d = _rotary(capi, **{name: heads})
+        if entry.endswith("workspace"):
+            size = ctypes.c_size_t()
+            rc, why = getattr(lib, entry)(0, ctypes.byref(d), ctypes.byref(size)), lib.mlxd_last_error().decode()
+        else:
+            rc, why = _call(pkg, entry, d)
+        assert rc == capi.ERR_INVALID and "2^29 heads" in why
