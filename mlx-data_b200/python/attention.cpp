@@ -12,6 +12,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mlxd_b200.h"
 
@@ -31,6 +32,16 @@ void check(int rc) {
     throw std::invalid_argument(mlxd_last_error());
   }
   throw std::runtime_error(std::string("mlx-data GPU path: ") + mlxd_last_error());
+}
+
+// A Python number; what is none, or does not fit, is a wrong argument like any other.
+template <class T>
+T number(const char* op, const char* name, const py::handle& o) {
+  try {
+    return o.cast<T>();
+  } catch (const py::cast_error&) {
+    bad(op, std::string(name) + (std::is_integral<T>::value ? " must be whole numbers" : " must be a number"));
+  }
 }
 
 // Work is queued on torch's current stream of the tensors' device.
@@ -227,7 +238,7 @@ struct Rotary {
     }
     int64_t pairs = 0;
     for (size_t i = 0; i < n && i < MLXD_ROTARY_MAX_AXES; i++) {
-      pairs += d.sections[i] = sections[i].cast<int32_t>();
+      pairs += d.sections[i] = number<int32_t>(op, "sections", sections[i]);
     }
     frequencies.read(op, "frequencies", frequencies_);
     if (frequencies.kind() != MLXD_F32 || frequencies.dims != 1 || (frequencies.size[0] > 1 && frequencies.stride[0] != 1)) {
@@ -359,7 +370,7 @@ struct Cross {
     d.q_heads = static_cast<int32_t>(q.heads);
     d.kv_heads = static_cast<int32_t>(k.heads);
     d.head_dim = static_cast<int32_t>(q.dim);
-    d.scale = scale.is_none() ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(q.dim))) : scale.cast<float>();
+    d.scale = scale.is_none() ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(q.dim))) : number<float>(op, "scale", scale);
     d.q = q.view();
     d.k = k.view();
     d.v = v.view();
