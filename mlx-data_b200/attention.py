@@ -90,6 +90,13 @@ def _wants_gradient(*tensors):
     return False
 
 
+def _constants(op, **tensors):
+    """Refuses a gradient that would not be worked out, ahead of the autograd functions (the compiled module does so elsewhere)."""
+    for name, t in tensors.items():
+        if _wants_gradient(t):
+            raise ValueError("%s: %s has no gradient here but requires one; pass %s.detach()" % (op, name, name))
+
+
 def rotary(q, k, positions, frequencies, sections, *, inverse=False, adjacent=False, interleaved=False):
     """Turn queries and keys by positions on several axes; returns ``(q, k)`` turned.
 
@@ -99,9 +106,11 @@ def rotary(q, k, positions, frequencies, sections, *, inverse=False, adjacent=Fa
     ``frequencies`` [pairs] float32; ``sections`` the number of pairs of each axis.  Pairs go to the axes in order, or one
     to each axis in turn (``interleaved``).  Pair i turns by float32(position) * frequencies[i], the product rounded to float32.
     Pairs are elements (i, i + pairs), or (2 i, 2 i + 1) (``adjacent``); elements from 2 * pairs on stay as they are.
-    ``inverse`` turns back, which is also the gradient.
+    ``inverse`` turns back, which is also the gradient.  Positions and frequencies have no gradient; ones that require it are
+    refused.
     """
     if _wants_gradient(q, k):
+        _constants("rotary", positions=positions, frequencies=frequencies)
         return _autograd()[0].apply(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
     return _ops.rotary(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
 
@@ -110,9 +119,11 @@ def qk_norm_rotary(q, k, positions, frequencies, sections, q_weight=None, k_weig
                    interleaved=False):
     """x / sqrt(mean(x^2) + eps) * weight for every head of queries and keys, then ``rotary``; returns ``(q, k)``.
 
-    ``q_weight`` and ``k_weight`` [head_dim] of one type, float32, bfloat16 or float16; None stands for ones.
+    ``q_weight`` and ``k_weight`` [head_dim] of one type, float32, bfloat16 or float16; None stands for ones.  ``eps`` is a number,
+    without a gradient.
     """
     if _wants_gradient(q, k, q_weight, k_weight):
+        _constants("qk_norm_rotary", positions=positions, frequencies=frequencies, eps=eps)
         return _autograd()[1].apply(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
     return _ops.qk_norm_rotary(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
 
@@ -130,7 +141,7 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale=None, return_
 
     ``q`` [batch, tokens, q_heads, head_dim]; ``k``, ``v`` [batch, keys, kv_heads, head_dim], bfloat16 or float16; q_heads a
     multiple of kv_heads (query head h reads key head h // (q_heads // kv_heads)); head_dim a multiple of 8, up to 128.
-    ``scale`` is 1 / sqrt(head_dim) unless given.
+    ``scale`` is 1 / sqrt(head_dim) unless given; a number, without a gradient.
     ``lengths`` [batch] int32 or int64: the first so many keys of a sample are read.  ``key_mask`` [batch, keys] bool: keys
     that are False are not read (padding inside a batch of images).  Both may be given.  Whatever lies in k and v where
     nothing is read has no effect.  A sample without a key to read gets zeros.
@@ -138,6 +149,7 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale=None, return_
     [batch, q_heads, tokens], which ``cross_attention_backward`` takes.
     """
     if _wants_gradient(q, k, v):
+        _constants("cross_attention", scale=scale)
         out, lse = _autograd()[2].apply(q, k, v, lengths, key_mask, scale)
         return (out, lse) if return_lse else out
     return _ops.cross_attention(q, k, v, lengths, key_mask, scale, return_lse)

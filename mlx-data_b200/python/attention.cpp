@@ -3,6 +3,7 @@
 // A module of its own because it is built against torch: a call of a few microseconds has no time for reading tensors through
 // their Python methods.  The pipeline's module `_c` knows nothing of torch.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -34,9 +35,19 @@ void check(int rc) {
   throw std::runtime_error(std::string("mlx-data GPU path: ") + mlxd_last_error());
 }
 
+// A gradient that would not be worked out is refused.
+void constant(const char* op, const char* name, const at::Tensor& t) {
+  if (t.requires_grad() && c10::GradMode::is_enabled()) {
+    bad(op, std::string(name) + " has no gradient here but requires one; pass " + name + ".detach()");
+  }
+}
+
 // A Python number; what is none, or does not fit, is a wrong argument like any other.
 template <class T>
 T number(const char* op, const char* name, const py::handle& o) {
+  if (THPVariable_Check(o.ptr())) {
+    constant(op, name, THPVariable_Unpack(o.ptr()));
+  }
   try {
     return o.cast<T>();
   } catch (const py::cast_error&) {
@@ -219,6 +230,7 @@ struct Rotary {
 
   void places(const py::object& positions_, const py::object& frequencies_, const py::sequence& sections, bool adjacent, bool interleaved) {
     positions.read(op, "positions", positions_);
+    constant(op, "positions", positions.t);
     if (positions.dims != q.dims - 1) {
       bad(op, "positions must be [axes, batch, tokens] (or [axes, tokens] beside [tokens, heads, head_dim]), got " + positions.text());
     }
@@ -241,6 +253,7 @@ struct Rotary {
       pairs += d.sections[i] = number<int32_t>(op, "sections", sections[i]);
     }
     frequencies.read(op, "frequencies", frequencies_);
+    constant(op, "frequencies", frequencies.t);
     if (frequencies.kind() != MLXD_F32 || frequencies.dims != 1 || (frequencies.size[0] > 1 && frequencies.stride[0] != 1)) {
       bad(op, "frequencies must be a contiguous float32 vector");
     }
@@ -266,14 +279,14 @@ struct Rotary {
     *at = w.data;
   }
 
-  void weights(const py::object& q_weight_, const py::object& k_weight_, double eps) {
+  void weights(const py::object& q_weight_, const py::object& k_weight_, const py::object& eps) {
     weight("q_weight", q_weight_, q_weight, &d.q_weight);
     weight("k_weight", k_weight_, k_weight, &d.k_weight);
     if (d.q_weight && d.k_weight && q_weight.t.scalar_type() != k_weight.t.scalar_type()) {
       bad(op, "q_weight and k_weight must have one type");
     }
     d.weight_dtype = d.q_weight ? q_weight.kind() : d.k_weight ? k_weight.kind() : MLXD_F32;
-    d.eps = static_cast<float>(eps);
+    d.eps = static_cast<float>(number<double>(op, "eps", eps));
   }
 
   py::tuple results(int (*call)(int, void*, const mlxd_rotary_desc*)) {
@@ -297,7 +310,7 @@ py::tuple rotary(const py::object& q, const py::object& k, const py::object& pos
 }
 
 py::tuple qk_norm_rotary(const py::object& q, const py::object& k, const py::object& positions, const py::object& frequencies,
-                         const py::sequence& sections, const py::object& q_weight, const py::object& k_weight, double eps,
+                         const py::sequence& sections, const py::object& q_weight, const py::object& k_weight, const py::object& eps,
                          bool adjacent, bool interleaved) {
   Rotary r{"qk_norm_rotary"};
   r.inputs(q, k);
@@ -308,7 +321,7 @@ py::tuple qk_norm_rotary(const py::object& q, const py::object& k, const py::obj
 
 py::tuple qk_norm_rotary_backward(const py::object& q_grad, const py::object& k_grad, const py::object& q, const py::object& k,
                                   const py::object& positions, const py::object& frequencies, const py::sequence& sections,
-                                  const py::object& q_weight, const py::object& k_weight, double eps, bool adjacent, bool interleaved) {
+                                  const py::object& q_weight, const py::object& k_weight, const py::object& eps, bool adjacent, bool interleaved) {
   Rotary r{"qk_norm_rotary_backward"};
   r.inputs(q, k);
   r.places(positions, frequencies, sections, adjacent, interleaved);

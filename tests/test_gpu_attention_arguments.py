@@ -25,3 +25,25 @@ def test_scale_that_is_no_number(pkg, scale):
     q, _, _ = _inputs(torch.bfloat16)
     with pytest.raises(ValueError, match="scale"):
         pkg.attention.cross_attention(q, q, q, scale=scale)
+
+
+@pytest.mark.parametrize("which", ["positions", "frequencies", "eps", "scale"])
+@pytest.mark.parametrize("leaf", [True, False])
+def test_gradients_that_are_not_worked_out(pkg, which, leaf):
+    """A tensor that requires a gradient and would get none is refused; without gradients it is an ordinary argument."""
+    A = pkg.attention
+    q, positions, frequencies = _inputs(torch.bfloat16)
+    q.requires_grad_(leaf)                      # alone, and beside inputs whose gradients are worked out
+    eps, scale = torch.tensor(1e-6), torch.tensor(0.1)
+    dict(positions=positions, frequencies=frequencies, eps=eps, scale=scale)[which].requires_grad_()
+    calls = [lambda: A.rotary(q, q, positions, frequencies, (32,)), lambda: A.rotary(q, None, positions, frequencies, (32,), inverse=True),
+             lambda: A.qk_norm_rotary(q, q, positions, frequencies, (32,), None, None, eps)]
+    if which == "eps":
+        calls = calls[2:]
+    if which == "scale":
+        calls = [lambda: A.cross_attention(q, q, q, scale=scale), lambda: A.cross_attention(q, q, q, scale=scale, return_lse=True)]
+    for call in calls:
+        with pytest.raises(ValueError, match=which):
+            call()
+        with torch.no_grad():
+            call()
