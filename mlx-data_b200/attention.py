@@ -6,9 +6,9 @@
 
 All take torch tensors in GPU memory, ``[batch, tokens, heads, head_dim]`` (views of a joint projection too), and queue
 their work on torch's current stream of the tensors' device; results are new contiguous tensors.  They work under
-``torch.autograd``; the functions ``*_backward`` are the same gradients for programs that do without it.  Sums are held in
-float32 and results rounded once to the tensors' type.  The same call gives the same bits again.  Wrong arguments raise
-``ValueError``; there is no CPU path.
+``torch.autograd`` (reverse mode, once; forward mode raises); the functions ``*_backward`` are the same gradients for programs
+that do without it.  Sums are held in float32 and results rounded once to the tensors' type.  The same call gives the same bits
+again.  Wrong arguments raise ``ValueError``; there is no CPU path.
 """
 import importlib
 

@@ -45,7 +45,7 @@ void constant(const char* op, const char* name, const at::Tensor& t) {
 // A Python number; what is none, or does not fit, is a wrong argument like any other.
 template <class T>
 T number(const char* op, const char* name, const py::handle& o) {
-  if (THPVariable_Check(o.ptr())) {
+  if (!PyLong_CheckExact(o.ptr()) && !PyFloat_CheckExact(o.ptr()) && THPVariable_Check(o.ptr())) {
     constant(op, name, THPVariable_Unpack(o.ptr()));
   }
   try {
@@ -84,6 +84,9 @@ struct Tensor {
     t = from;
     if (!t.is_cuda()) {
       bad(op, std::string(name) + " must be in GPU memory (there is no CPU path)");
+    }
+    if (t._fw_grad(0).defined()) {
+      bad(op, std::string(name) + " carries a tangent: there is no forward-mode derivative here");
     }
     if (t.layout() != at::kStrided || t.is_conj() || t.is_neg()) {
       bad(op, std::string(name) + " must be an ordinary strided tensor");

@@ -47,3 +47,30 @@ def test_gradients_that_are_not_worked_out(pkg, which, leaf):
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("requires", [False, True])
+def test_forward_mode_is_refused(pkg, requires):
+    """A tangent would be dropped and read as zero."""
+    A = pkg.attention
+    q, positions, frequencies = _inputs(torch.bfloat16)
+    w = torch.ones(64, device="cuda")
+    fw = torch.autograd.forward_ad
+
+    def calls(dual, f, weight):
+        return [lambda: A.rotary(dual, q, positions, f, (32,)), lambda: A.rotary(q, dual, positions, f, (32,), inverse=True),
+                lambda: A.qk_norm_rotary(dual, None, positions, f, (32,), weight), lambda: A.qk_norm_rotary(q, None, positions, f, (32,), weight),
+                lambda: A.cross_attention(dual, q, q), lambda: A.cross_attention(q, dual, q), lambda: A.cross_attention(q, q, dual)]
+
+    with fw.dual_level():
+        dual = fw.make_dual(q.detach().clone().requires_grad_(requires), torch.ones_like(q))
+        for i, call in enumerate(calls(dual, frequencies, w)):
+            if i != 3:
+                with pytest.raises((ValueError, NotImplementedError) if requires else ValueError):
+                    call()
+        with pytest.raises(ValueError):
+            A.rotary(q, q, positions, fw.make_dual(frequencies, torch.ones_like(frequencies)), (32,))
+        with pytest.raises(ValueError):
+            calls(q, frequencies, fw.make_dual(w, torch.ones_like(w)))[3]()
+        for call in calls(q, frequencies, w):          # nothing carries a tangent
+            call()
