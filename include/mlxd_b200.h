@@ -366,6 +366,8 @@ typedef struct mlxd_cross_desc {
 MLXD_API int mlxd_cross_attention_workspace(int device, const mlxd_cross_desc* d, int backward, size_t* bytes);
 MLXD_API int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cross_desc* d);
 MLXD_API int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d);
+/* The same where lse has a gradient too: lse_grad [batch, q_heads, q_tokens] float32, NULL for none. */
+MLXD_API int mlxd_cross_attention_backward_lse(int device, void* cuda_stream, const mlxd_cross_desc* d, const float* lse_grad);
 
 /* Self-check word of the kernels of cross attention on this device: waits for `cuda_stream`, stores the word in *status
  * (0 = clean; 1: a kernel gave up waiting for its own copies or products, which none does unless the device is at fault),

@@ -110,7 +110,7 @@ EXPORTS = [
     "mlxd_device_alloc", "mlxd_device_free", "mlxd_ctx_set_timing", "mlxd_fused_batch_noalloc",
     "mlxd_noalloc_status", "mlxd_stream_status", "mlxd_device_pci_bus_id",
     "mlxd_rotary", "mlxd_qk_norm_rotary", "mlxd_qk_norm_rotary_workspace", "mlxd_qk_norm_rotary_backward",
-    "mlxd_cross_attention", "mlxd_cross_attention_workspace", "mlxd_cross_attention_backward",
+    "mlxd_cross_attention", "mlxd_cross_attention_workspace", "mlxd_cross_attention_backward", "mlxd_cross_attention_backward_lse",
     "mlxd_attention_status",
 ]
 NOALLOC_MAX_SAMPLES = 1024
@@ -171,6 +171,7 @@ def load():
     lib.mlxd_qk_norm_rotary_workspace.argtypes = [i32, ctypes.POINTER(RotaryDesc), size_p]
     for name in ("mlxd_cross_attention", "mlxd_cross_attention_backward"):
         getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(CrossDesc)]
+    lib.mlxd_cross_attention_backward_lse.argtypes = [i32, vp, ctypes.POINTER(CrossDesc), vp]
     lib.mlxd_cross_attention_workspace.argtypes = [i32, ctypes.POINTER(CrossDesc), i32, size_p]
     lib.mlxd_attention_status.argtypes = [i32, vp, ctypes.POINTER(ctypes.c_int32)]
     _lib = lib

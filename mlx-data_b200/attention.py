@@ -70,14 +70,16 @@ def _autograd():
                 out, lse = _ops.cross_attention(q, k, v, lengths, key_mask, scale, True)
                 ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask)
                 ctx.scale = scale
-                ctx.mark_non_differentiable(lse)
+                ctx.set_materialize_grads(False)
                 return out, lse
 
             @staticmethod
             @torch.autograd.function.once_differentiable
-            def backward(ctx, dout, _):
+            def backward(ctx, dout, dlse):
                 q, k, v, out, lse, lengths, key_mask = ctx.saved_tensors
-                return (*_ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.scale), None, None, None)
+                if dout is None:
+                    dout = torch.zeros_like(out)
+                return (*_ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.scale, dlse), None, None, None)
 
         _functions = Rotary, QkNormRotary, CrossAttention
     return _functions
@@ -146,7 +148,7 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale=None, return_
     that are False are not read (padding inside a batch of images).  Both may be given.  Whatever lies in k and v where
     nothing is read has no effect.  A sample without a key to read gets zeros.
     Returns the result, or with ``return_lse`` also the logarithm of each row's sum of exponentials, float32
-    [batch, q_heads, tokens], which ``cross_attention_backward`` takes.
+    [batch, q_heads, tokens], which ``cross_attention_backward`` takes; it has a gradient like the result.
     """
     if _wants_gradient(q, k, v):
         _constants("cross_attention", scale=scale)
@@ -155,7 +157,7 @@ def cross_attention(q, k, v, *, lengths=None, key_mask=None, scale=None, return_
     return _ops.cross_attention(q, k, v, lengths, key_mask, scale, return_lse)
 
 
-def cross_attention_backward(dout, q, k, v, out, lse, *, lengths=None, key_mask=None, scale=None):
+def cross_attention_backward(dout, q, k, v, out, lse, *, lengths=None, key_mask=None, scale=None, lse_grad=None):
     """Gradients ``(dq, dk, dv)`` of ``cross_attention``: ``out`` and ``lse`` as it returned them, the other arguments as it
-    was given.  Keys that are not read get zeros."""
-    return _ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, scale)
+    was given.  ``lse_grad`` is the gradient of lse, where it has one.  Keys that are not read get zeros."""
+    return _ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, scale, lse_grad)

@@ -19,7 +19,8 @@ struct Heads {
 struct CrossParams {
   Heads q, k, v, out, dout, dq, dk, dv;
   float* lse;
-  float* delta;                 // [batch, q_heads, q_tokens]: sum of dout * out over a row
+  const float* lse_grad;        // backward: the gradient of lse, or null
+  float* delta;                 // [batch, q_heads, q_tokens]: sum of dout * out over a row, less the gradient of its lse
   const void* lengths;
   int lengths_dtype;
   const uint8_t* key_mask;

@@ -211,10 +211,16 @@ extern "C" int mlxd_cross_attention(int device, void* cuda_stream, const mlxd_cr
 }
 
 extern "C" int mlxd_cross_attention_backward(int device, void* cuda_stream, const mlxd_cross_desc* d) {
+  return mlxd_cross_attention_backward_lse(device, cuda_stream, d, nullptr);
+}
+
+extern "C" int mlxd_cross_attention_backward_lse(int device, void* cuda_stream, const mlxd_cross_desc* d, const float* lse_grad) {
   return guarded("cross_attention_backward", [&] {
     CrossParams p;
     int rc = params_of("cross_attention_backward", d, true, p);
     if (rc != MLXD_OK) return rc;
+    if (!on_boundary(lse_grad, 4)) return fail(MLXD_ERR_INVALID, "cross_attention_backward: lse_grad does not start on a multiple of 4 bytes");
+    p.lse_grad = lse_grad;
     size_t need = 0;
     rc = workspace_of(device, p, true, &need);
     if (rc != MLXD_OK) return rc;

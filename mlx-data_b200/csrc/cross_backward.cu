@@ -56,8 +56,9 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, int dim, int 
   tile_stores_read();
 }
 
-// dQ = scale dS K for 128 queries: S = Q K^T, P = exp(S - lse), dP = dO V^T, dS = P (dP - delta).  Two sets of scores, so that the
-// products of the next tile run beside the exponentials of this one.  Also works out delta = sum(dO O) of its rows, which the
+// dQ = scale dS K for 128 queries: S = Q K^T, P = exp(S - lse), dP = dO V^T, dS = P (dP - delta).  lse has the derivative P by S, so its
+// gradient is taken off delta.  Two sets of scores, so that the
+// products of the next tile run beside the exponentials of this one.  Also works out delta = sum(dO O) - dlse of its rows, which the
 // other kernel reads.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
     delta_parts[half][row] = part;
     warp_arrive(delta_full, lane);
     bool going = warp_wait(delta_full, 0, &failed);
-    const float delta = going ? delta_parts[0][row] + delta_parts[1][row] : 0.0f;
+    float delta = going ? delta_parts[0][row] + delta_parts[1][row] : 0.0f;
+    if (p.lse_grad && there) delta -= p.lse_grad[stat];
     if (there && half == 0) p.delta[stat] = delta;
     // a row that is not there gets P = 0
     const float base = there ? row_base(p.lse[stat]) : -INFINITY;

@@ -438,7 +438,7 @@ py::object cross_attention(const py::object& q, const py::object& k, const py::o
 
 py::tuple cross_attention_backward(const py::object& dout, const py::object& q, const py::object& k, const py::object& v,
                                    const py::object& out, const py::object& lse, const py::object& lengths,
-                                   const py::object& key_mask, const py::object& scale) {
+                                   const py::object& key_mask, const py::object& scale, const py::object& lse_grad) {
   Cross c{"cross_attention_backward"};
   c.inputs(q, k, v, lengths, key_mask, scale);
   HeadsTensor o, g;
@@ -455,9 +455,19 @@ py::tuple cross_attention_backward(const py::object& dout, const py::object& q, 
     bad(c.op, "lse must be what cross_attention returned: contiguous float32 [batch, q_heads, tokens]");
   }
   c.d.lse = reinterpret_cast<float*>(l.data);
+  Tensor lg;
+  if (!lse_grad.is_none()) {
+    lg.read(c.op, "lse_grad", lse_grad);
+    if (lg.kind() != MLXD_F32 || lg.t.sizes() != l.t.sizes() || lg.device != c.q.device) {
+      bad(c.op, "lse_grad must have lse's shape, type and device");
+    }
+    if (!lg.t.is_contiguous()) {
+      lg.set(c.op, "lse_grad", at::Tensor(lg.t.contiguous()));
+    }
+  }
   const at::Tensor work = c.workspace(true);
   const at::Tensor dq = empty_like(c.q, &c.d.dq), dk = empty_like(c.k, &c.d.dk), dv = empty_like(c.v, &c.d.dv);
-  check(mlxd_cross_attention_backward(c.q.device, stream_of(c.q.device), &c.d));
+  check(mlxd_cross_attention_backward_lse(c.q.device, stream_of(c.q.device), &c.d, reinterpret_cast<const float*>(lg.data)));
   return py::make_tuple(wrapped(dq), wrapped(dk), wrapped(dv));
 }
 
@@ -475,5 +485,5 @@ PYBIND11_MODULE(_attention, a) {
   a.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lengths"), py::arg("key_mask"),
         py::arg("scale"), py::arg("return_lse"));
   a.def("cross_attention_backward", &cross_attention_backward, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("out"), py::arg("lse"), py::arg("lengths"), py::arg("key_mask"), py::arg("scale"));
+        py::arg("out"), py::arg("lse"), py::arg("lengths"), py::arg("key_mask"), py::arg("scale"), py::arg("lse_grad"));
 }

@@ -78,3 +78,12 @@ def test_more_heads_than_the_kernels_count(pkg, entry, name):
         else:
             rc, why = _call(pkg, entry, d)
         assert rc == capi.ERR_INVALID and "2^29 heads" in why
+
+
+def test_gradient_of_lse(pkg):
+    capi, lib = pkg._capi, pkg._capi.load()
+    heads = capi.Heads(AT, 64 * 64, 64, 64)
+    d = capi.CrossDesc(dtype=capi.BF16, batch=2, q_tokens=4, kv_tokens=6, q_heads=4, kv_heads=2, head_dim=64, scale=0.125, q=heads,
+                       k=heads, v=heads, out=heads, lse=AT, dout=heads, dq=heads, dk=heads, dv=heads, workspace=AT, workspace_bytes=1 << 30)
+    rc = lib.mlxd_cross_attention_backward_lse(0, None, ctypes.byref(d), AT + 2)
+    assert rc == capi.ERR_INVALID and "lse_grad" in lib.mlxd_last_error().decode()
