@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       int issued = 0;
       for (; issued < 2 * n; issued++) {
         const int slot = issued % S::kSlots, use = issued / S::kSlots, i = issued / 2;
+        if (issued == S::kSlots) wait_for_kernels_before();   // no slot is free again before
         if (use && !barrier_wait(empty + 8 * slot, (use - 1) & 1, &failed)) break;
         load_tile<S>(ring_at + slot * S::kTile, issued & 1 ? &maps.dout : &maps.q, i % q_tiles * 128, kv_head * p.group + i / q_tiles, batch, full + 8 * slot);
       }
@@ -379,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       going = going && warp_wait3(v_full, 0, full + 8, 0, 0, 0, &failed);
       if (going && elected()) dp(1);
       __syncwarp();
+      wait_for_kernels_before();
       Ring<S::kSlots> q, g, next_q, next_g;   // queries and their gradients, of this tile and the next
       g.next();
       next_q.next(2);
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       }
     } else if (warp == 10) {
       // -------------------------------------------------- what is known of the queries; -infinity makes P = 0 where there is none
-      asm volatile("griddepcontrol.wait;" : : : "memory");   // delta comes from the kernel before
+      wait_for_kernels_before();   // delta comes from there
       for (int i = 0; i < n; i++) {
         const int64_t first = (static_cast<int64_t>(batch) * p.q_heads + kv_head * p.group + i / q_tiles) * p.q_tokens;
         float* to = reinterpret_cast<float*>(stats[i & 1]);
@@ -446,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
     const int end = p.q_tokens - 128 * (q_tiles - 1) - 64 * half;   // of this thread's queries in the last tile of a head
     int to_last = q_tiles;
     bool going = true;
+    wait_for_kernels_before();
     for (int i = 0; i < n; i++) {
       uint32_t s[64];
       going = warp_wait(stats_full + 8 * (i & 1), i / 2 & 1, &failed) && warp_wait(s_full, i & 1, &failed);

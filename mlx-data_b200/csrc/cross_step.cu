@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
   const int64_t all = static_cast<int64_t>(p.batch) * p.q_heads * p.q_tokens, stat = blockIdx.x;
   const int token = stat % p.q_tokens, head = stat / p.q_tokens % p.q_heads, batch = stat / p.q_tokens / p.q_heads;
   const int parts = (length_of(p, batch) + sp.split_keys - 1) / sp.split_keys;
-  asm volatile("griddepcontrol.wait;" : : : "memory");
+  wait_for_kernels_before();
   float top = -INFINITY;
   for (int i = threadIdx.x; i < parts; i += 32 * kJoinWarps) top = max_or_nan(top, sp.part_lse[i * all + stat]);
   for (int d = 16; d; d >>= 1) top = max_or_nan(top, __shfl_xor_sync(~0u, top, d));

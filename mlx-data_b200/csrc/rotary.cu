@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const __grid_constant
   void* out = is_k ? dk : dq;
   if (!out) return;
   float sum = 0;
-  asm volatile("griddepcontrol.wait;" : : : "memory");   // it begins beside the end of the kernel before
+  wait_for_kernels_before();
   if (at < p.head_dim) {
 #pragma unroll 4
     for (int b = from + warp; b < to; b += 32) sum += p.partial[static_cast<int64_t>(b) * p.head_dim + at];

@@ -89,6 +89,12 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
   if (lane == 0) barrier_arrive(bar);
 }
 
+// Waits for the kernels before, where this one has begun beside their end; nothing limits it, so it comes ahead of the waits that are
+// limited and depend on what it waits for.
+__device__ __forceinline__ void wait_for_kernels_before() {
+  asm volatile("griddepcontrol.wait;" : : : "memory");
+}
+
 // Writes of this thread to shared memory are seen by copies and matrix products that are issued after this (and after a
 // barrier, where another thread issues them).
 __device__ __forceinline__ void fence_async_proxy() {
