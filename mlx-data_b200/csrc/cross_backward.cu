@@ -64,7 +64,7 @@ template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 4 + 2 * kMaskRing + 2];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 4 + 2 * kMaskRing + 1 + 1];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ float delta_parts[2][128];
   __shared__ uint32_t tmem_slot;
@@ -74,13 +74,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 16, ds_full = dp_full + 8, done = ds_full + 8, delta_full = done + 8,
-                 masked = delta_full + 8, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
+                 masked = delta_full + 8, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing, ended = staged_full + 8;
 
   const int q_tiles = (p.q_tokens + 127) / 128;
   const int q0 = blockIdx.x % q_tiles * 128, head = blockIdx.x / q_tiles % p.q_heads, batch = blockIdx.x / q_tiles / p.q_heads;
   if (threadIdx.x == 0) {
     failed = reach = 0;
-    for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, done}) barrier_init(bar, 1);
+    for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, done, ended}) barrier_init(bar, 1);
     for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
         v.next(2);
         next_k.next(2);
       }
+      if (!going) products_end(ended);
     } else if (warp == 10) {
       // -------------------------------------------------- masks: which keys are read, and zeros where they are not
       for (int j = 0; j < n; j++) {
@@ -307,7 +308,7 @@ template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + 1];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + 1 + 1];
   __shared__ float4 stats[2][2][32];      // of the queries of a tile: -lse * log2(e), delta
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, reach;
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
   const uint32_t k_full = smem_address(bars), v_full = k_full + 8, full = k_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, done = ds_full + 8,
-                 stats_full = done + 8, stats_empty = stats_full + 16, staged_full = stats_empty + 16;
+                 stats_full = done + 8, stats_empty = stats_full + 16, staged_full = stats_empty + 16, ended = staged_full + 8;
 
   const int k_tiles = (p.kv_tokens + 127) / 128;
   const int k0 = blockIdx.x % k_tiles * 128, kv_head = blockIdx.x / k_tiles % p.kv_heads, batch = blockIdx.x / k_tiles / p.kv_heads;
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
 
   if (threadIdx.x == 0) {
     failed = reach = 0;
-    for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8}) barrier_init(bar, 1);
+    for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8, ended}) barrier_init(bar, 1);
     for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 8);
     for (const uint32_t bar : {stats_empty, stats_empty + 8}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
@@ -416,6 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
         next_q.next(2);
         next_g.next(2);
       }
+      if (!going) products_end(ended);
     } else if (warp == 10) {
       // -------------------------------------------------- what is known of the queries; -infinity makes P = 0 where there is none
       wait_for_kernels_before();   // delta comes from there

@@ -89,7 +89,7 @@ template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 8 + 2 * kMaskRing + 2];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2 + 1];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ float exchange[2][2][128];   // of a row's two threads: maxima, sums at last
   __shared__ uint32_t tmem_slot;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
-                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing;
+                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing, ended = staged_full + 16;
 
   // CTAs of 256 rows first, head by head; those of a ragged end of at most 128 rows, which take less time, after all others, where
   // they fill the SMs that become free (333 rows, 96 heads: 31.9 us in order of tiles, 29.4 so).
@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   const int rows = p.q_tokens - q0 > 128 ? 2 : 1;   // tiles of query rows
   if (threadIdx.x == 0) {
     failed = reach = 0;
+    barrier_init(ended, 1);
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
         v = next_v;
         k = next_k;
       }
+      if (!going) products_end(ended);
     } else if (warp == 19) {
       // -------------------------------------------------- masks: which keys are read, and zeros where values are not
       for (int j = 0; j < n; j++) {

@@ -249,6 +249,14 @@ __device__ __forceinline__ void products_done(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" : : "r"(bar) : "memory");
 }
 
+// For a warp that issues products and has given up: waits, with a limit, for those under way, which read and write what the CTA is about
+// to free.  `bar` is a barrier of one arrival that nothing else uses.
+__device__ __forceinline__ void products_end(uint32_t bar) {
+  if (elected()) products_done(bar);
+  __syncwarp();
+  for (int i = 0; i < kWaitTries && !barrier_try(bar, 0); i++) {}
+}
+
 // ---------------------------------------------------------------- arithmetic
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
