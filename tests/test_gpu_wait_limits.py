@@ -26,7 +26,10 @@ def seen(tmp_path_factory):
 
 def test_every_warp_gives_up(seen):
     assert seen["gave_up"] == [1, 1, 1, 1] and seen["failed"] == 1
-    assert 0.1 < seen["seconds"] < 20
+
+
+def test_the_limit_is_about_two_seconds(seen):
+    assert 1 < seen["seconds"] < 10, seen["seconds"]
 
 
 def test_products_have_ended(seen):
