@@ -69,6 +69,23 @@ __device__ __forceinline__ int length_of(const CrossParams& p, int b) {
   return static_cast<int>(n < 0 ? 0 : n > p.kv_tokens ? p.kv_tokens : n);
 }
 
+// The number of the CTA, read anew: what follows from it at a kernel's end is worked out again there instead of held in registers (forward,
+// 6 x 333 tokens, 1024 keys, 16 heads of 64: 34.5 us with it held and spills, 32.9 without).
+__device__ __forceinline__ int block_again() {
+  int x;
+  asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(x));
+  return x;
+}
+
+// What a CTA that gave up leaves in rows `first` to `end` - 1 of a head, with all its threads: not a number (of either 16-bit type), instead
+// of whatever the memory held.
+__device__ __forceinline__ void spoil_rows(const Heads& x, int batch, int head, int first, int end, int dim) {
+  for (int row = first + static_cast<int>(threadIdx.x) / 32; row < end; row += static_cast<int>(blockDim.x) / 32) {
+    uint16_t* to = reinterpret_cast<uint16_t*>(x.data) + batch * x.batch + row * x.token + head * x.head;
+    for (int i = threadIdx.x & 31; i < dim; i += 32) to[i] = 0x7fff;
+  }
+}
+
 // The end of a sample's last key that is read, found by the whole CTA from the back: the padding below the images of a batch
 // ends a sample's keys under a mask too.  `reach` (shared) is 0 before, for all threads.
 __device__ __forceinline__ int reach_of(const CrossParams& p, int b, int length, int* reach) {

@@ -299,7 +299,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
   tmem_before_sync();
   __syncthreads();
   if (warp == 9) tmem_free<512>(tmem);
-  if (threadIdx.x == 0 && failed) *p.status = 1;
+  if (failed) {
+    const int id = block_again(), tiles = (p.q_tokens + 127) / 128, from = id % tiles * 128, of = id / tiles;
+    const int end = min(from + 128, p.q_tokens), i = from + static_cast<int>(threadIdx.x);
+    spoil_rows(p.dq, of / p.q_heads, of % p.q_heads, from, end, p.head_dim);
+    // the other kernel's results are not valid either
+    if (i < end) p.delta[static_cast<int64_t>(of) * p.q_tokens + i] = NAN;
+    if (threadIdx.x == 0) *p.status = 1;
+  }
 }
 
 // dV = P^T dO and dK = scale dS^T Q for 128 keys, over the queries of every head that shares them.  Scores lie the other way round
@@ -531,7 +538,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
   tmem_before_sync();
   __syncthreads();
   if (warp == 9) tmem_free<512>(tmem);
-  if (threadIdx.x == 0 && failed) *p.status = 1;
+  if (failed) {
+    const int id = block_again(), tiles = (p.kv_tokens + 127) / 128, from = id % tiles * 128, of = id / tiles;
+    const int end = min(from + 128, p.kv_tokens);
+    spoil_rows(p.dk, of / p.kv_heads, of % p.kv_heads, from, end, p.head_dim);
+    spoil_rows(p.dv, of / p.kv_heads, of % p.kv_heads, from, end, p.head_dim);
+    if (threadIdx.x == 0) *p.status = 1;
+  }
 }
 
 template <class T, int kDim>

@@ -102,9 +102,13 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   // CTAs of 256 rows first, head by head; those of a ragged end of at most 128 rows, which take less time, after all others, where
   // they fill the SMs that become free (333 rows, 96 heads: 31.9 us in order of tiles, 29.4 so).
   const int q_tiles = (p.q_tokens + 255) / 256, end_rows = p.q_tokens - 256 * (q_tiles - 1), whole = end_rows > 128 ? q_tiles : q_tiles - 1;
-  const int id = blockIdx.x, wholes = whole * p.q_heads * p.batch;
-  const int of = id < wholes ? id / whole : id - wholes, q0 = (id < wholes ? id % whole : q_tiles - 1) * 256;
-  const int head = of % p.q_heads, batch = of / p.q_heads;
+  const int wholes = whole * p.q_heads * p.batch;
+  const auto rows_of = [&](int id) {
+    const int of = id < wholes ? id / whole : id - wholes;
+    return make_int3((id < wholes ? id % whole : q_tiles - 1) * 256, of % p.q_heads, of / p.q_heads);
+  };
+  const int3 mine_are = rows_of(blockIdx.x);
+  const int q0 = mine_are.x, head = mine_are.y, batch = mine_are.z;
   const int rows = p.q_tokens - q0 > 128 ? 2 : 1;   // tiles of query rows
   if (threadIdx.x == 0) {
     failed = reach = 0;
@@ -359,7 +363,15 @@ __global__ void __launch_bounds__(kThreads, 1) cross_forward_kernel(const __grid
   tmem_before_sync();
   __syncthreads();
   if (warp == 17) tmem_free<512>(tmem);
-  if (threadIdx.x == 0 && failed) *p.status = 1;
+  if (failed) {
+    const int3 at = rows_of(block_again());
+    const int end = min(at.x + 256, p.q_tokens);
+    spoil_rows(p.out, at.z, at.y, at.x, end, p.head_dim);
+    for (int i = at.x + static_cast<int>(threadIdx.x); p.lse && i < end; i += kThreads) {
+      p.lse[(static_cast<int64_t>(at.z) * p.q_heads + at.y) * p.q_tokens + i] = NAN;
+    }
+    if (threadIdx.x == 0) *p.status = 1;
+  }
 }
 
 template <class T, int kDim>

@@ -34,3 +34,7 @@ def test_the_limit_is_about_two_seconds(seen):
 
 def test_products_have_ended(seen):
     assert seen["ended"] == 1
+
+
+def test_its_rows_are_not_numbers(seen):
+    assert seen["spoiled"] == 128 * 24 and seen["wrong"] == 0
