@@ -370,8 +370,9 @@ MLXD_API int mlxd_cross_attention_backward(int device, void* cuda_stream, const 
 MLXD_API int mlxd_cross_attention_backward_lse(int device, void* cuda_stream, const mlxd_cross_desc* d, const float* lse_grad);
 
 /* Self-check word of the kernels of cross attention on this device: waits for `cuda_stream`, stores the word in *status
- * (0 = clean; 1: a kernel gave up waiting for its own copies or products, which none does unless the device is at fault),
- * clears it, and returns MLXD_ERR_DEVICE when it was set.  Not under capture. */
+ * (0 = clean; 1: a kernel gave up waiting for its own copies or products, which none does unless the device is at fault)
+ * and returns MLXD_ERR_DEVICE when it is set.  The word is one for all streams of the device and stays set for the life of
+ * the process.  The rows that such a kernel was to write hold NaN.  Not under capture. */
 MLXD_API int mlxd_attention_status(int device, void* cuda_stream, int32_t* status);
 
 #ifdef __cplusplus

@@ -237,7 +237,8 @@ def noalloc_status(device, stream):
 
 
 def attention_status(device, stream):
-    """mlxd_attention_status: waits for the stream, returns the self-check word of cross attention's kernels (0 = clean)."""
+    """mlxd_attention_status: waits for the stream, returns the self-check word of cross attention's kernels on the device
+    (0 = clean; once set it stays so)."""
     lib = load()
     word = ctypes.c_int32(-1)
     rc = lib.mlxd_attention_status(device, ctypes.c_void_p(stream), ctypes.byref(word))

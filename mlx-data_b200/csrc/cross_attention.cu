@@ -35,7 +35,7 @@ int check_sizes(const char* entry, const mlxd_cross_desc* d) {
   return MLXD_OK;
 }
 
-// Set by a kernel whose wait for its own copies or products ran out.
+// Set by a kernel whose wait for its own copies or products ran out, and never cleared: whoever asks learns of it, on any stream.
 __device__ int attention_status;
 
 int status_word(int device, int** word) {
@@ -45,7 +45,7 @@ int status_word(int device, int** word) {
   *word = known[device].load(std::memory_order_relaxed);
   if (!*word) {
     void* at = nullptr;
-    MLXD_CUDA(cudaGetSymbolAddress(&at, attention_status));
+    MLXD_CUDA(cudaGetSymbolAddress(&at, static_cast<const void*>(&attention_status)));
     *word = static_cast<int*>(at);
     known[device].store(*word, std::memory_order_relaxed);
   }
@@ -248,7 +248,6 @@ extern "C" int mlxd_attention_status(int device, void* cuda_stream, int32_t* sta
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     int32_t got = 0;
     MLXD_CUDA(cudaMemcpyAsync(&got, word, sizeof(got), cudaMemcpyDeviceToHost, s));
-    MLXD_CUDA(cudaMemsetAsync(word, 0, sizeof(got), s));
     MLXD_CUDA(cudaStreamSynchronize(s));
     *status = got;
     return got ? fail(MLXD_ERR_DEVICE, "attention: a kernel gave up waiting for its own copies or products; its results are not valid") : static_cast<int>(MLXD_OK);
