@@ -47,7 +47,7 @@ cudaError_t allow_shared(int bytes, int device) {
   return e;
 }
 
-int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map);
+int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int heads, int dim, CUtensorMap* map);
 
 cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);
 

@@ -133,7 +133,7 @@ int maps_of(const CrossParams& p, int dtype, bool backward, CrossMaps& m) {
     const auto& x = all[i];
     const int tokens = x.query ? p.q_tokens : p.kv_tokens;
     if (!tokens || (backward && i == 3)) continue;
-    const int rc = cross_map(*x.h, dtype, p.batch, tokens, x.query ? p.q_heads : p.kv_heads, p.head_dim, x.map);
+    const int rc = cross_map(*x.h, dtype, p.device, p.batch, tokens, x.query ? p.q_heads : p.kv_heads, p.head_dim, x.map);
     if (rc != MLXD_OK) return rc;
   }
   return MLXD_OK;
@@ -142,7 +142,7 @@ int maps_of(const CrossParams& p, int dtype, bool backward, CrossMaps& m) {
 }  // namespace
 
 // The driver's encoder, found through the runtime: the library links against no driver library.
-int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int dim, CUtensorMap* map) {
+int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int heads, int dim, CUtensorMap* map) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -161,10 +161,19 @@ int cross_map(const Heads& h, int dtype, int batch, int tokens, int heads, int d
   const auto bytes = [](int64_t stride, int size) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : 16); };
   const cuuint64_t strides[3] = {bytes(h.token, tokens), bytes(h.head, heads), bytes(h.batch, batch)};
   const cuuint32_t box[4] = {64, 128, 1, 1}, steps[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, dtype == MLXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, h.data, sizes,
-                            strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MLXD_ERR_INVALID, "cross_attention: a tensor's strides do not fit a tensor map (status " + std::to_string(r) + ")");
+  const auto make = [&] {
+    return encode(map, dtype == MLXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, h.data, sizes,
+                  strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = make();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // a thread that has not used CUDA before: the runtime binds the device's context to it, the driver's encoder does not
+    MLXD_CUDA(cudaSetDevice(device));
+    r = make();
+  }
+  if (r == CUDA_ERROR_INVALID_VALUE) return fail(MLXD_ERR_INVALID, "cross_attention: a tensor's strides do not fit a tensor map");
+  if (r != CUDA_SUCCESS) return fail(MLXD_ERR_CUDA, "cross_attention: no tensor map (driver status " + std::to_string(r) + ")");
   return MLXD_OK;
 }
 
