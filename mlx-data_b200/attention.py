@@ -22,7 +22,10 @@ class _Operators:
     def __getattr__(self, name):
         global _ops
         importlib.import_module("torch")
-        _ops = importlib.import_module("._attention", __package__)
+        try:
+            _ops = importlib.import_module("._attention", __package__)
+        except ModuleNotFoundError as e:
+            raise ImportError("the attention operators are missing: the package was built without torch; build it again") from e
         return getattr(_ops, name)
 
 
