@@ -6,6 +6,7 @@ the states that text reads: the image's own queries and keys are normalised and 
 are image and not padding (``attention.cross_attention`` with a mask of keys).  Runs a forward and a backward pass, and one step
 of generation.  ``python examples/caption_step.py`` on a GPU.
 """
+import math
 import os
 import sys
 
@@ -16,6 +17,12 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from __graft_entry__ import load_package  # noqa: E402
 
 PATCH, HEADS, KV_HEADS, DIM = 16, 8, 2, 64
+
+
+def resized(h, w, size):
+    """Height and width that ``image_resize_smallest_side`` gives an image: both scaled in float64, halves rounded up."""
+    scale = size / min(h, w)
+    return math.floor(scale * h + 0.5), math.floor(scale * w + 0.5)
 
 
 def image_batch(dx, n, size=224, seed=0):
@@ -31,9 +38,9 @@ def image_batch(dx, n, size=224, seed=0):
         pixels = torch.as_tensor(next(iter(stream))["image"], device="cuda")
     finally:
         dx.core.set_device_output(False)
-    scale = [size / min(s["image"].shape[:2]) for s in samples]
-    grid = [(int(s["image"].shape[0] * f) // PATCH, int(s["image"].shape[1] * f) // PATCH) for s, f in zip(samples, scale)]
-    return pixels, torch.tensor(grid, device="cuda")
+    sizes = [resized(*s["image"].shape[:2], size) for s in samples]
+    assert pixels.shape[1:3] == tuple(max(x) for x in zip(*sizes))   # the largest of the batch, to which the others are padded
+    return pixels, torch.tensor([(h // PATCH, w // PATCH) for h, w in sizes], device="cuda")
 
 
 def patches(pixels, grid):
