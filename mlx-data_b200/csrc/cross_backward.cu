@@ -56,17 +56,52 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, int dim, int 
   tile_stores_read();
 }
 
+// Of a row and this thread's half of the one tile of keys that there is: sums of P dP and of P, over the keys that are read.  Scores and
+// dP stay where they are.  Where a wait runs out the caller's next one does too.
+__device__ __forceinline__ void row_sums(uint32_t at, uint32_t dp_column, uint32_t s_full, uint32_t dp_full, uint32_t masked, bool partial,
+                                         const uint32_t (&mask)[4], int half, float c, float base, volatile int* failed, float* sum,
+                                         float* weights) {
+  if (partial && !warp_wait(masked, 0, failed)) return;
+  const uint32_t words[2] = {partial ? mask[2 * half] : ~0u, partial ? mask[2 * half + 1] : ~0u};
+  const bool single = partial && __popc(mask[0]) + __popc(mask[1]) + __popc(mask[2]) + __popc(mask[3]) == 1;
+  if (!warp_wait(s_full, 0, failed) || !warp_wait(dp_full, 0, failed)) return;
+  tmem_after_sync();
+  float total = 0, part = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    uint32_t s[16], d[16];
+    tmem_load<16>(at + 16 * i, s);
+    tmem_load<16>(at + dp_column + 16 * i, d);
+    tmem_loaded(s);
+    tmem_loaded(d);
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      if (words[i / 2] >> (16 * (i & 1) + k) & 1) {
+        // lse of the forward pass makes the one weight 1 but for a rounding
+        const float w = exp2_of(fmaf(__uint_as_float(s[k]), c, base)), exact = single && w > 0 ? 1.0f : w;
+        total += exact;
+        part = fmaf(exact, __uint_as_float(d[k]), part);
+      }
+    }
+  }
+  *sum = part;
+  *weights = total;
+}
+
 // dQ = scale dS K for 128 queries: S = Q K^T, P = exp(S - lse), dP = dO V^T, dS = P (dP - delta).  lse has the derivative P by S, so its
 // gradient is taken off delta.  Two sets of scores, so that the
 // products of the next tile run beside the exponentials of this one.  Also works out delta = sum(dO O) - dlse of its rows, which the
-// other kernel reads.
+// other kernel reads.  O comes in rounded to 16 bits, and where few keys have weights dS is the small difference of dP and delta: with
+// two keys dQ and dK were off by 0.0052 of their size in bfloat16 (the rounding of results alone: 0.0017).  So where a sample's keys
+// fit one tile, whose P and dP are there before any dS, delta = sum(P dP) / sum(P) of these.  A single key has the weight 1, so that its
+// dS is 0 and no remainder of a rounding.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_constant__ CrossParams p, const __grid_constant__ CrossMaps maps) {
   using S = Sizes<kDim>;
   extern __shared__ __align__(1024) uint8_t shared[];
   __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 4 + 2 * kMaskRing + 1 + 1];
   __shared__ uint32_t mask_words[kMaskRing][4];
-  __shared__ float delta_parts[2][128];
+  __shared__ float delta_parts[2][2][128];   // of a row's two threads: sums, and with one tile of keys those of weights
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, reach;
   asm volatile("griddepcontrol.launch_dependents;");   // the other kernel's CTAs take the SMs that these leave
@@ -211,8 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const int64_t stat = (static_cast<int64_t>(batch) * p.q_heads + head) * p.q_tokens + q0 + row;
     const float c = p.scale * kLog2e;
-    float part = 0;
-    if (there) {   // delta: this thread's half of the elements
+    // a row that is not there gets P = 0
+    const float base = there ? row_base(p.lse[stat]) : -INFINITY;
+    float part = 0, weights = 1;
+    if (n == 1) {
+      row_sums(tmem + 64 * half + lanes, dp_column, s_full, dp_full, masked, partial(0), mask_words[0], half, c, base, &failed, &part, &weights);
+    } else if (there) {   // delta: this thread's half of the elements
       const T* o = reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + (q0 + row) * p.out.token + head * p.out.head;
       const T* g = reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + (q0 + row) * p.dout.token + head * p.dout.head;
 #pragma unroll
@@ -226,14 +265,17 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
         }
       }
     }
-    delta_parts[half][row] = part;
+    delta_parts[0][half][row] = part;
+    delta_parts[1][half][row] = weights;
     warp_arrive(delta_full, lane);
     bool going = warp_wait(delta_full, 0, &failed);
-    float delta = going ? delta_parts[0][row] + delta_parts[1][row] : 0.0f;
+    float delta = going ? delta_parts[0][0][row] + delta_parts[0][1][row] : 0.0f;
+    if (n == 1 && going) {
+      weights = delta_parts[1][0][row] + delta_parts[1][1][row];
+      delta = weights == 0 ? 0.0f : delta / weights;
+    }
     if (p.lse_grad && there) delta -= p.lse_grad[stat];
     if (there && half == 0) p.delta[stat] = delta;
-    // a row that is not there gets P = 0
-    const float base = there ? row_base(p.lse[stat]) : -INFINITY;
     for (int j = 0; j < n && going; j++) {
       const uint32_t mine = tmem + 128 * (j & 1) + 64 * half + lanes;
       uint32_t s[64];
