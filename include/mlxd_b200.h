@@ -342,7 +342,13 @@ MLXD_API int mlxd_qk_norm_rotary_backward(int device, void* cuda_stream, const m
  * 0..kv_tokens are taken as the nearest of them), of these the ones whose byte
  * in key_mask [batch, kv_tokens] is not 0 (NULL: all).  What lies in k and v
  * where nothing is read has no effect, whatever it is.  A sample with no key
- * to read gets zeros, -infinity in lse, and gradients of zero.
+ * to read gets zeros, -infinity in lse, and gradients of zero; a row whose
+ * scores are all -infinity has no weights in either pass.  What is not a number in q, or in a key or
+ * value that is read, makes the rows that read it NaN, and their lse where it
+ * is in a score.
+ *
+ * The weights P and, in the backward pass, dS = P (dP - delta) are rounded to
+ * `dtype`, as operands of the products; sums are float32.
  *
  * lse [batch, q_heads, q_tokens] float32 is the natural logarithm of each
  * row's sum of exponentials; NULL where no backward pass follows. */

@@ -6,7 +6,7 @@
 // 128 scores and 128 results each), weights go back where their scores were and are an operand from there.  While one tile of rows is in
 // the tensor cores the other is with the softmax.  A row belongs to two threads, so that a tile's softmax takes half as long: it and the
 // products of a tile follow one another (about 1600 and 1300 cycles, of which 1024 are products), and a tile waits for both.
-// Measured: 2 x 2048 tokens, 6404 keys, 32 heads on 8, D = 128: 388 us, 1106 TFLOP/s (68 % of the measured rate; 436 us where calls
+// Measured: 2 x 2048 tokens, 6404 keys, 32 heads on 8, D = 128: 393 us, 1094 TFLOP/s (67 % of the measured rate; 446 us where calls
 // follow one another for long and the power cap lowers the clock); D = 64, 4096 keys: 222 us, 619.
 #include "cross.h"
 #include "sm100.cuh"
@@ -22,8 +22,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 2^8: the result is the same quotient, and 2^8 is far from the largest float16.
 constexpr float kSlack = 8.0f;
 // Of eight pairs of exponentials so many are worked out by multiply-adds: the pipe of exponentials is what a tile of scores waits
-// for.  Measured for 0, 1, 2, 3: 388, 376, 382, 398 us (2 x 2048 tokens, 6404 keys, 32 heads of 128), 246, 232, 232, 272 us (4096
-// keys, heads of 64): above one in eight the issue of instructions takes as long.
+// for.  Measured for 0, 1, 2, 3: 398, 393, 392, 400 us (2 x 2048 tokens, 6404 keys, 32 heads of 128), 224, 222, 225, 232 us (4096
+// keys, heads of 64): above one or two in eight the issue of instructions takes as long.
 constexpr int kByFma = 1;
 
 template <int kDim>
@@ -61,8 +61,8 @@ __device__ __forceinline__ float most_of(const uint32_t (&s)[64]) {
   return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
 }
 
-// exp(score - maximum) of 64 scores, as 2^(c s + base): summed in float32, rounded to 16 bits for the products, stored in the
-// first 32 columns of where they came from.
+// exp(score - maximum) of 64 scores, as 2^(c s + base): summed in float32, rounded to 16 bits (the tensor cores take both operands of one
+// 16-bit type; the result's error becomes 1.4 roundings instead of one), stored in the first 32 columns of where they came from.
 template <class T>
 __device__ __forceinline__ void weigh(const uint32_t (&s)[64], float c, float base, float2 (&sum)[2], uint32_t to) {
 #pragma unroll

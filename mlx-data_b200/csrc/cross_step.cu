@@ -3,8 +3,8 @@
 // A CTA takes up to 16 rows (tokens and heads that share a key head) and a stretch of the keys; its four warps take 16 keys each in
 // turn, straight from memory into the registers of 16 x 8 x 16 products, with no detour through shared memory: which elements of a
 // head a product sums over, and which become its columns, is a matter of naming, so a lane's 16-byte loads are its operands.
-// Reading keys and values once is the floor.  Measured: 32 heads on 8, 1601 keys: 7.9 us with the joining of the parts; sixteen
-// sequences of up to 6404 keys: 57 us, 4.7 TB/s (72 % of the measured rate): a CTA's first loads and its last sums are not hidden
+// Reading keys and values once is the floor.  Measured: 32 heads on 8, 1601 keys: 8.0 us with the joining of the parts; sixteen
+// sequences of up to 6404 keys: 58 us, 4.7 TB/s (72 % of the measured rate): a CTA's first loads and its last sums are not hidden
 // (two CTAs of 215 registers an SM).
 #include "cross.h"
 #include "sm100.cuh"
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) cross_step_kernel(const __grid
       for (int h = 0; h < 2; h++) {
         const float x = exp2_of(fmaf(s[h][2 * r], scale, base)), y = exp2_of(fmaf(s[h][2 * r + 1], scale, base));
         total[r] += x + y;
-        w[2 * h + r] = pack2<T>(x, y);
+        w[2 * h + r] = pack2<T>(x, y);   // an operand of the products, so 16 bits; the sum is of the floats
       }
     }
     // column n of product (j, i) is element 64 j + 8 n + i

@@ -283,8 +283,8 @@ __device__ void read_weights(const RotaryParams& p, float (&w)[2][MLXD_ROTARY_MA
 // then its heads, 32 / lanes at a time, queries first.  The next heads are loaded while these are worked on.  A warp a token and no loop
 // over tokens: CTAs that fit at once, looping, took 65 us instead of 46 (16 x 1024 tokens, 32 heads of 80), since a token's
 // positions and sines are waited for one token after another then.  Seven CTAs an SM, by their registers, with the few spills that
-// takes: without a limit (five) 48.0 us, six 46.0, seven 42.0, eight 42.4, nine 44.9 for those; 50.6, 50.6, 45.6 for five, six, seven
-// with the norm (3 x 4099 tokens, 32 heads of 128, float16), 4.4 TB/s.  19600 tokens, 48 heads of 64, float32: 80 us, 6.0 TB/s;
+// takes: without a limit (five) 48.0 us, six 46.0, seven 42.0, eight 42.4, nine 44.9 for those; 50.6, 50.6, 45.7 for five, six, seven
+// with the norm (3 x 4099 tokens, 32 heads of 128, float16), 4.4 TB/s.  19600 tokens, 48 heads of 64, float32: 79 us, 6.1 TB/s;
 // one token of 40 heads 2.8 us.  Bound by latency and the issue of instructions for 16-bit types (about 100 for four heads of 128; heads of
 // 80 use five of eight lanes).
 template <class T, int kV, int kUnits, bool kAdjacent, Turned kTurned, bool kNorm>
