@@ -107,3 +107,22 @@ def test_gradients_of_rows_without_weights(pkg, shape, dtype):
     for got, want in ((dq, clean[2]), (dk, clean[3]), (dv, clean[4])):
         heads = group if got is dq else 1
         assert torch.equal(got[:, :, heads:], want[:, :, heads:]) and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("where", ["q", "dout"])
+@pytest.mark.parametrize("kind", ["lengths", "mask"])
+def test_keys_that_are_not_read_get_zeros(pkg, kind, where, value):
+    """Also in a tile of which a part is read, and beside gradients that are not finite."""
+    q, k, v = _inputs((2, 70, 300, 4, 2, 64), torch.float16)
+    dout = torch.randn_like(q)
+    {"q": q, "dout": dout}[where][:, 5, :, 3] = value
+    read = torch.arange(300, device="cuda") < torch.tensor([100, 200], device="cuda")[:, None]
+    args = dict(lengths=torch.tensor([100, 200], device="cuda"))
+    if kind == "mask":
+        read &= torch.arange(300, device="cuda") % 3 > 0
+        args = dict(key_mask=read)
+    out, lse = pkg.attention.cross_attention(q, k, v, return_lse=True, **args)
+    dq, dk, dv = pkg.attention.cross_attention_backward(dout, q, k, v, out, lse, **args)
+    assert not dk[~read].any() and not dv[~read].any()
+    assert not torch.isfinite(dk[read]).all()
