@@ -45,9 +45,10 @@ def _autograd():
         class Rotary(torch.autograd.Function):
             @staticmethod
             def forward(ctx, q, k, positions, frequencies, sections, inverse, adjacent, interleaved):
+                out = _ops.rotary(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
                 ctx.save_for_backward(positions, frequencies)
-                ctx.how = (sections, not inverse, adjacent, interleaved)
-                return _ops.rotary(q, k, positions, frequencies, sections, inverse, adjacent, interleaved)
+                ctx.how = (tuple(sections), not inverse, adjacent, interleaved)
+                return out
 
             @staticmethod
             @torch.autograd.function.once_differentiable
@@ -57,9 +58,10 @@ def _autograd():
         class QkNormRotary(torch.autograd.Function):
             @staticmethod
             def forward(ctx, q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved):
+                out = _ops.qk_norm_rotary(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
                 ctx.save_for_backward(q, k, positions, frequencies, q_weight, k_weight)
-                ctx.how = (sections, eps, adjacent, interleaved)
-                return _ops.qk_norm_rotary(q, k, positions, frequencies, sections, q_weight, k_weight, eps, adjacent, interleaved)
+                ctx.how = (tuple(sections), float(eps), adjacent, interleaved)
+                return out
 
             @staticmethod
             @torch.autograd.function.once_differentiable
@@ -75,7 +77,7 @@ def _autograd():
             def forward(ctx, q, k, v, lengths, key_mask, scale):
                 out, lse = _ops.cross_attention(q, k, v, lengths, key_mask, scale, True)
                 ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask)
-                ctx.scale = scale
+                ctx.scale = None if scale is None else float(scale)
                 ctx.set_materialize_grads(False)
                 return out, lse
 

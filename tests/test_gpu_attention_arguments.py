@@ -74,3 +74,39 @@ def test_forward_mode_is_refused(pkg, requires):
             calls(q, frequencies, fw.make_dual(w, torch.ones_like(w)))[3]()
         for call in calls(q, frequencies, w):          # nothing carries a tangent
             call()
+
+
+def test_arguments_that_change_between_the_passes(pkg):
+    """The backward pass uses what the forward pass was given: sections in a list, numbers in tensors."""
+    A = pkg.attention
+    q, positions, _ = _inputs()
+    positions = torch.stack((positions[0] + 3, positions[0] + 7))
+    frequencies, w = torch.rand(32, device="cuda"), torch.ones(64, device="cuda")
+    dy = torch.randn_like(q)
+
+    def gradients(change):
+        sections, eps, scale = [8, 24], torch.tensor(1e-2), torch.tensor(0.3)
+        x, z, h = (t.detach().clone().requires_grad_() for t in (q, q, q.bfloat16()))
+        y = A.rotary(x, None, positions, frequencies, sections)[0]
+        n = A.qk_norm_rotary(z, None, positions, frequencies, sections, w, None, eps)[0]
+        c = A.cross_attention(h, h, h, scale=scale)
+        if change:
+            sections[:] = [24, 8]
+            eps.fill_(1.0)
+            scale.fill_(2.0)
+        torch.autograd.backward((y, n, c), (dy, dy, dy.bfloat16()))
+        return x.grad, z.grad, h.grad
+
+    assert all(torch.equal(a, b) for a, b in zip(gradients(True), gradients(False)))
+
+
+def test_wrong_arguments_beside_gradients(pkg):
+    """They are seen before anything is kept for the backward pass."""
+    A = pkg.attention
+    q, positions, frequencies = _inputs()
+    q.requires_grad_()
+    for call in (lambda: A.rotary(q, None, positions.cpu().numpy(), frequencies, (32,)), lambda: A.rotary(q, q.detach().cpu().numpy(), positions, frequencies, (32,)),
+                 lambda: A.qk_norm_rotary(q, None, positions, [1.0] * 32, (32,)), lambda: A.qk_norm_rotary(q, None, positions, frequencies, (32,), 1.0),
+                 lambda: A.cross_attention(q, q, q), lambda: A.cross_attention(q.bfloat16(), q.bfloat16(), q.bfloat16(), lengths=[1])):
+        with pytest.raises(ValueError):
+            call()
