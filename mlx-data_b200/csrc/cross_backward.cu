@@ -31,10 +31,9 @@ __device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* map, i
   for (int x = 0; x < S::kBoxes; x++) tile_load(to + x * kBoxBytes, map, 64 * x, token, head, batch, bar);
 }
 
-// The accumulators of a row, scaled, rounded and put where a store of the tile finds them.  `none`: there are no accumulators; `zero`: the row
-// is zeros whatever they hold.
+// The accumulators of a row, scaled, rounded and put where a store of the tile finds them; zeros where there are none.
 template <class T, int kDim>
-__device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, float by, bool none, bool zero) {
+__device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, float by, bool none) {
 #pragma unroll
   for (int x = 0; x < kDim; x += 32) {
     uint32_t o[32] = {};
@@ -47,7 +46,6 @@ __device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, f
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) w[i] = pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by);
-      if (zero) w[0] = w[1] = w[2] = w[3] = 0;
       const int unit = (x + k) % 64 / 8;
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                    : : "r"(to + (x + k) / 64 * kBoxBytes + row * 128 + ((unit ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
@@ -336,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dq_kernel(const __grid_cons
     if (n && going) going = warp_wait(done, 0, &failed);
     if (going) {
       tmem_after_sync();
-      if (half == 0) stage_row<T, kDim>(tmem + dq_column + lanes, q_at, row, p.scale, n == 0, false);
+      if (half == 0) stage_row<T, kDim>(tmem + dq_column + lanes, q_at, row, p.scale, n == 0);
       fence_async_proxy();
       warp_arrive(staged_full, lane);
       if (threadIdx.x == 0 && barrier_wait(staged_full, 0, &failed)) store_tile<S>(&maps.dq, p.head_dim, q0, head, batch, q_at);
@@ -576,7 +574,14 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
     if (going) {   // the first warpgroup stores dV, the second dK, out of the ring, which is no longer needed
       tmem_after_sync();
       const uint32_t staged = ring_at + half * S::kTile;
-      stage_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, staged, row, half ? p.scale : 1.0f, n == 0, !read);
+      stage_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, staged, row, half ? p.scale : 1.0f, n == 0);
+      if (n && !read) {
+#pragma unroll
+        for (int unit = 0; unit < kDim / 8; unit++) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                       : : "r"(staged + unit / 8 * kBoxBytes + row * 128 + ((unit % 8 ^ (row & 7)) * 16)), "r"(0) : "memory");
+        }
+      }
       fence_async_proxy();
       warp_arrive(staged_full, lane);
       if (row == 0 && barrier_wait(staged_full, 0, &failed)) store_tile<S>(half ? &maps.dk : &maps.dv, p.head_dim, k0, kv_head, batch, staged);
