@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
     const bool read = key < length && (!p.key_mask || p.key_mask[batch * p.key_mask_stride + key]);
     const uint32_t mine = tmem + 64 * half + lanes;
     const int end = p.q_tokens - 128 * (q_tiles - 1) - 64 * half;   // of this thread's queries in the last tile of a head
-    int to_last = q_tiles;
+    int ragged = end < 64 ? q_tiles - 1 : -1;                       // the next such tile that has not all of them
     bool going = true;
     wait_for_kernels_before();
     for (int i = 0; i < n; i++) {
@@ -511,14 +511,12 @@ __global__ void __launch_bounds__(kThreads, 1) cross_dkv_kernel(const __grid_con
       tmem_load<32>(mine, s);
       tmem_load<32>(mine + 32, s + 32);
       tmem_loaded(s);
-      if (--to_last == 0) {
-        to_last = q_tiles;
-        // queries that are not there are zeros, whose scores are not a number where a key holds an infinity
-        if (end < 64) {
+      // queries that are not there are zeros, whose scores are not a number where a key holds an infinity
+      if (i == ragged) {
+        ragged += q_tiles;
 #pragma unroll
-          for (int k = 0; k < 64; k++) {
-            if (k >= end) s[k] = 0;
-          }
+        for (int k = 0; k < 64; k++) {
+          if (k >= end) s[k] = 0;
         }
       }
       const float4* lse = stats[i & 1][0] + 16 * half;
