@@ -3,8 +3,8 @@
 // 128 x 128 x D for the five of the definition.  P and dS are rounded to 16 bits, since the tensor cores take both operands of one 16-bit
 // type: errors of 1.4 roundings instead of one, with delta's share 1.6 at most.  A small dS of float16 is not scaled up ahead of it,
 // since the gradients may come in near the largest float16 by a loss scale, and a large one not held at 65504, so that a loss scaler sees
-// an infinity.  Measured: 2 x 2048 tokens, 4096 keys, 32 heads on 8, D = 128: 900 us, 764 TFLOP/s by the five, 1069 by the seven; D = 64:
-// 629 us.  With few queries (8 x 255 tokens, 1024 keys, 12 heads of 80, padded grids: 83 us) a CTA's beginning and end are most of it:
+// an infinity.  Measured: 2 x 2048 tokens, 4096 keys, 32 heads on 8, D = 128: 897 us, 766 TFLOP/s by the five, 1073 by the seven; D = 64:
+// 625 us.  With few queries (8 x 255 tokens, 1024 keys, 12 heads of 80, padded grids: 83 us) a CTA's beginning and end are most of it:
 // six rounds of CTAs with two tiles of queries each.
 #include "cross.h"
 #include "sm100.cuh"

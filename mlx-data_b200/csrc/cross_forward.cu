@@ -6,7 +6,7 @@
 // 128 scores and 128 results each), weights go back where their scores were and are an operand from there.  While one tile of rows is in
 // the tensor cores the other is with the softmax.  A row belongs to two threads, so that a tile's softmax takes half as long: it and the
 // products of a tile follow one another (about 1600 and 1300 cycles, of which 1024 are products), and a tile waits for both.
-// Measured: 2 x 2048 tokens, 6404 keys, 32 heads on 8, D = 128: 393 us, 1094 TFLOP/s (67 % of the measured rate; 446 us where calls
+// Measured: 2 x 2048 tokens, 6404 keys, 32 heads on 8, D = 128: 393 us, 1094 TFLOP/s (67 % of the measured rate; 440 us where calls
 // follow one another for long and the power cap lowers the clock); D = 64, 4096 keys: 222 us, 619.
 #include "cross.h"
 #include "sm100.cuh"
