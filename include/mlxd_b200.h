@@ -375,7 +375,97 @@ MLXD_API int mlxd_cross_attention_backward(int device, void* cuda_stream, const 
 /* The same where lse has a gradient too: lse_grad [batch, q_heads, q_tokens] float32, NULL for none. */
 MLXD_API int mlxd_cross_attention_backward_lse(int device, void* cuda_stream, const mlxd_cross_desc* d, const float* lse_grad);
 
-/* Self-check word of the kernels of cross attention on this device: waits for `cuda_stream`, stores the word in *status
+/* ---- the text's own attention: a cache in pages, a window in training -------
+ * The place of a token is its number in its sequence, from 0. */
+
+/* A pool of pages [pages, page_size, kv_heads, head_dim], head_dim contiguous, the other strides in elements. */
+typedef struct mlxd_pages {
+  void* data;
+  int64_t stride_page, stride_row, stride_head;
+} mlxd_pages;
+
+/* Keys and values of `batch` sequences in one pool each.  Place s of sample b lies in row s % page_size of page
+ * page_table[b, s / page_size]; an entry outside 0..pages - 1 is no page.  lengths[b] tokens lie there before a call, whose
+ * sample b brings counts[b] new ones (NULL: all `tokens` of the call; values outside 0..tokens are taken as the nearest of them), at the
+ * places lengths[b] to lengths[b] + counts[b] - 1.  Lengths below 0 are taken as 0, places from table_width * page_size on have no page. */
+typedef struct mlxd_cache {
+  mlxd_pages k, v;
+  int32_t pages, page_size;      /* page_size: a power of two from 8 on */
+  const void* page_table;        /* [batch, table_width], rows contiguous */
+  int32_t page_table_dtype;      /* MLXD_I32 or MLXD_I64 */
+  int32_t table_width;           /* table_width * page_size at most 2^30 */
+  int64_t page_table_stride;     /* between two samples */
+  const void* lengths;           /* [batch] */
+  const void* counts;
+  int32_t lengths_dtype, counts_dtype;   /* MLXD_I32 or MLXD_I64 */
+} mlxd_cache;
+
+/* New tokens join a cache: keys are turned as mlxd_rotary turns them (r: all of its rotary part; k_out is not used) and written, with the
+ * values, to their places; queries (r.q_heads may be 0) are turned into q_out.  r.positions NULL: a token's position is its place, on
+ * every axis.  Tokens from counts[b] on, and tokens whose place has no page, are not written; all queries are turned.  Rows of the pool
+ * that no token goes to stay as they are.  Two tokens must not go to one row (a page that is written belongs to one sample), and
+ * the pools overlap neither each other nor what is read. */
+typedef struct mlxd_append_desc {
+  mlxd_rotary_desc r;
+  mlxd_heads v;                  /* like r.k */
+  mlxd_cache cache;
+} mlxd_append_desc;
+
+MLXD_API int mlxd_append_rotary(int device, void* cuda_stream, const mlxd_append_desc* d);
+
+/* Attention over a cache: the call's tokens, which lie in the cache already (mlxd_append_rotary with the same lengths and counts), read
+ * it.  Query i of sample b has the place s = lengths[b] + i and reads the keys at places j <= s, j < lengths[b] + counts[b], with s - j < window
+ * (0: no window) or j < sinks.  With a tree [batch, tokens, tokens] query i reads the new token j where tree[b, i, j] is not 0 and
+ * j < counts[b], and of the cache before them (j < lengths[b]) what the window leaves, s being lengths[b] + the number of new tokens
+ * other than itself that it reads.  Keys at places that have no page are not read.  What lies where no query of the sample reads has no
+ * effect, whatever it is; what is not a number in a value that some queries of a sample read may reach its other queries too.  Queries
+ * without a key to read, those from counts[b] on among them, get zeros and -infinity in lse.
+ * scale, lse [batch, q_heads, tokens], rounding and groups of heads are as in mlxd_cross_desc. */
+typedef struct mlxd_cached_desc {
+  int32_t dtype;                 /* of every tensor here: MLXD_BF16 or MLXD_F16 */
+  int32_t batch, tokens, q_heads, kv_heads;
+  int32_t head_dim;              /* a multiple of 8, at most MLXD_CROSS_MAX_HEAD_DIM */
+  float scale;                   /* positive */
+  int32_t window, sinks;
+  mlxd_heads q, out;             /* data 16-byte aligned, strides multiples of 8; those of the pools too */
+  float* lse;                    /* NULL: not wanted */
+  mlxd_cache cache;
+  const uint8_t* tree;           /* NULL: none; the last dimension contiguous */
+  int64_t tree_stride_batch, tree_stride_token;
+  void* workspace;               /* mlxd_cached_attention_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} mlxd_cached_desc;
+
+MLXD_API int mlxd_cached_attention_workspace(int device, const mlxd_cached_desc* d, size_t* bytes);
+MLXD_API int mlxd_cached_attention(int device, void* cuda_stream, const mlxd_cached_desc* d);
+
+/* Attention of sequences to themselves: query i of sample b reads the keys j <= i with i - j < window (0: no window) or j < sinks, where
+ * i and j are below lengths[b] (NULL: tokens; values outside 0..tokens are taken as the nearest of them).  What lies from there on in any
+ * tensor has no effect; results and gradients there are zeros (-infinity in lse).  What is not a number in a value, or in the backward
+ * pass in a key, query or gradient, may reach other rows of the same sequence and head than those that read it.
+ * The rest is as in mlxd_cross_desc. */
+typedef struct mlxd_window_desc {
+  int32_t dtype;                 /* of every tensor here: MLXD_BF16 or MLXD_F16 */
+  int32_t batch, tokens, q_heads, kv_heads;
+  int32_t head_dim;              /* a multiple of 8, at most MLXD_CROSS_MAX_HEAD_DIM */
+  float scale;                   /* positive */
+  int32_t window, sinks;
+  mlxd_heads q, k, v, out;       /* data 16-byte aligned, strides multiples of 8 */
+  float* lse;
+  const void* lengths;
+  int32_t lengths_dtype;         /* MLXD_I32 or MLXD_I64 */
+  /* backward only: out and lse as the forward pass left them */
+  mlxd_heads dout, dq, dk, dv;
+  const float* lse_grad;         /* [batch, q_heads, tokens], NULL: none */
+  void* workspace;               /* mlxd_window_attention_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} mlxd_window_desc;
+
+MLXD_API int mlxd_window_attention_workspace(int device, const mlxd_window_desc* d, int backward, size_t* bytes);
+MLXD_API int mlxd_window_attention(int device, void* cuda_stream, const mlxd_window_desc* d);
+MLXD_API int mlxd_window_attention_backward(int device, void* cuda_stream, const mlxd_window_desc* d);
+
+/* Self-check word of the kernels of cross, cached and window attention on this device: waits for `cuda_stream`, stores the word in *status
  * (0 = clean; 1: a kernel gave up waiting for its own copies or products, which none does unless the device is at fault)
  * and returns MLXD_ERR_DEVICE when it is set.  The word is one for all streams of the device and stays set for the life of
  * the process.  The rows that such a kernel was to write hold NaN.  Not under capture. */

@@ -91,6 +91,39 @@ class CrossDesc(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_row", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("k", Pages), ("v", Pages), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("page_table", ctypes.c_void_p),
+                ("page_table_dtype", ctypes.c_int32), ("table_width", ctypes.c_int32), ("page_table_stride", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("lengths_dtype", ctypes.c_int32),
+                ("counts_dtype", ctypes.c_int32)]
+
+
+class AppendDesc(ctypes.Structure):
+    _fields_ = [("r", RotaryDesc), ("v", Heads), ("cache", Cache)]
+
+
+_CAUSAL_SIZES = [(n, ctypes.c_int32) for n in ("dtype", "batch", "tokens", "q_heads", "kv_heads", "head_dim")] + [
+    ("scale", ctypes.c_float), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class CachedDesc(ctypes.Structure):
+    _fields_ = _CAUSAL_SIZES + [
+        ("q", Heads), ("out", Heads), ("lse", ctypes.c_void_p), ("cache", Cache), ("tree", ctypes.c_void_p),
+        ("tree_stride_batch", ctypes.c_int64), ("tree_stride_token", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class WindowDesc(ctypes.Structure):
+    _fields_ = _CAUSAL_SIZES + [
+        ("q", Heads), ("k", Heads), ("v", Heads), ("out", Heads), ("lse", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+        ("lengths_dtype", ctypes.c_int32), ("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads), ("lse_grad", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 # numpy mirror of SampleDesc so a whole batch of descriptors is one array
 SAMPLE_DTYPE = np.dtype([
     ("src", np.uint64), ("src_h", np.int32), ("src_w", np.int32),
@@ -111,7 +144,8 @@ EXPORTS = [
     "mlxd_noalloc_status", "mlxd_stream_status", "mlxd_device_pci_bus_id",
     "mlxd_rotary", "mlxd_qk_norm_rotary", "mlxd_qk_norm_rotary_workspace", "mlxd_qk_norm_rotary_backward",
     "mlxd_cross_attention", "mlxd_cross_attention_workspace", "mlxd_cross_attention_backward", "mlxd_cross_attention_backward_lse",
-    "mlxd_attention_status",
+    "mlxd_attention_status", "mlxd_append_rotary", "mlxd_cached_attention", "mlxd_cached_attention_workspace",
+    "mlxd_window_attention", "mlxd_window_attention_backward", "mlxd_window_attention_workspace",
 ]
 NOALLOC_MAX_SAMPLES = 1024
 
@@ -173,6 +207,12 @@ def load():
         getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(CrossDesc)]
     lib.mlxd_cross_attention_backward_lse.argtypes = [i32, vp, ctypes.POINTER(CrossDesc), vp]
     lib.mlxd_cross_attention_workspace.argtypes = [i32, ctypes.POINTER(CrossDesc), i32, size_p]
+    lib.mlxd_append_rotary.argtypes = [i32, vp, ctypes.POINTER(AppendDesc)]
+    lib.mlxd_cached_attention.argtypes = [i32, vp, ctypes.POINTER(CachedDesc)]
+    lib.mlxd_cached_attention_workspace.argtypes = [i32, ctypes.POINTER(CachedDesc), size_p]
+    for name in ("mlxd_window_attention", "mlxd_window_attention_backward"):
+        getattr(lib, name).argtypes = [i32, vp, ctypes.POINTER(WindowDesc)]
+    lib.mlxd_window_attention_workspace.argtypes = [i32, ctypes.POINTER(WindowDesc), i32, size_p]
     lib.mlxd_attention_status.argtypes = [i32, vp, ctypes.POINTER(ctypes.c_int32)]
     _lib = lib
     return lib
@@ -237,7 +277,7 @@ def noalloc_status(device, stream):
 
 
 def attention_status(device, stream):
-    """mlxd_attention_status: waits for the stream, returns the self-check word of cross attention's kernels on the device
+    """mlxd_attention_status: waits for the stream, returns the self-check word of the attention kernels on the device
     (0 = clean; once set it stays so)."""
     lib = load()
     word = ctypes.c_int32(-1)

@@ -3,6 +3,8 @@
 * ``rotary``: positions with several axes (time, row, column) turn queries and keys.
 * ``qk_norm_rotary``: RMS norm of every head of queries and keys, and the rotation, in one pass.
 * ``cross_attention``: queries read the states of images or clips, padding masked out.
+* ``window_attention``: a text reads itself, every token those before it, or a window of them and a few first ones.
+* ``append_rotary`` and ``cached_attention``: the same in generation, over keys and values in the pages of a cache.
 
 All take torch tensors in GPU memory, ``[batch, tokens, heads, head_dim]`` (views of a joint projection too), and queue
 their work on torch's current stream of the tensors' device; results are new contiguous tensors.  They work under
@@ -10,12 +12,13 @@ their work on torch's current stream of the tensors' device; results are new con
 that do without it.  Sums are held in float32 and results rounded once to the tensors' type.  ``cross_attention`` also rounds what its
 products on the tensor cores take, the weights P and in the backward pass dS = P (dP - delta), to the tensors' type, with delta from the
 rounded result where keys are more than 128: errors of 1.4 to 1.6 roundings instead of one.  In float16 a dS beyond 65504 is infinite,
-as a loss scaler expects of a scale that is too high.  The same call gives the same bits again.  Wrong arguments raise ``ValueError``;
+as a loss scaler expects of a scale that is too high.  ``window_attention`` and ``cached_attention`` round alike.  The same call gives the same bits again.  Wrong arguments raise ``ValueError``;
 there is no CPU path.
 """
 import importlib
 
-__all__ = ["rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "cross_attention", "cross_attention_backward"]
+__all__ = ["rotary", "qk_norm_rotary", "qk_norm_rotary_backward", "cross_attention", "cross_attention_backward", "window_attention",
+           "window_attention_backward", "append_rotary", "cached_attention"]
 
 
 
@@ -89,7 +92,25 @@ def _autograd():
                     dout = torch.zeros_like(out)
                 return (*_ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.scale, dlse), None, None, None)
 
-        _functions = Rotary, QkNormRotary, CrossAttention
+        class WindowAttention(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, q, k, v, window, sinks, lengths, scale):
+                out, lse = _ops.window_attention(q, k, v, window, sinks, lengths, scale, True)
+                ctx.save_for_backward(q, k, v, out, lse, lengths)
+                ctx.how = (None if window is None else int(window), int(sinks), None if scale is None else float(scale))
+                ctx.set_materialize_grads(False)
+                return out, lse
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, dout, dlse):
+                q, k, v, out, lse, lengths = ctx.saved_tensors
+                window, sinks, scale = ctx.how
+                if dout is None:
+                    dout = torch.zeros_like(out)
+                return (*_ops.window_attention_backward(dout, q, k, v, out, lse, window, sinks, lengths, scale, dlse), None, None, None, None)
+
+        _functions = Rotary, QkNormRotary, CrossAttention, WindowAttention
     return _functions
 
 
@@ -169,3 +190,59 @@ def cross_attention_backward(dout, q, k, v, out, lse, *, lengths=None, key_mask=
     """Gradients ``(dq, dk, dv)`` of ``cross_attention``: ``out`` and ``lse`` as it returned them, the other arguments as it
     was given.  ``lse_grad`` is the gradient of lse, where it has one.  Keys that are not read get zeros."""
     return _ops.cross_attention_backward(dout, q, k, v, out, lse, lengths, key_mask, scale, lse_grad)
+
+
+def window_attention(q, k, v, *, window=None, sinks=0, lengths=None, scale=None, return_lse=False):
+    """Causal attention of sequences to themselves: token i reads the tokens j <= i with i - j < window, or j < sinks.
+
+    ``q`` [batch, tokens, q_heads, head_dim]; ``k``, ``v`` [batch, tokens, kv_heads, head_dim]; types, heads, head_dim, ``scale`` and
+    ``return_lse`` as in ``cross_attention``.  ``window`` a whole number from 1 on, None: every token before; ``sinks`` first tokens that
+    stay visible.  ``lengths`` [batch] int32 or int64: the first so many tokens of a sample are its sequence; what lies behind them in any
+    tensor has no effect, and results and gradients there are zeros.  An infinity or NaN in a value may reach tokens of its
+    sequence and head that do not read it.
+    """
+    if _wants_gradient(q, k, v):
+        _constants("window_attention", window=window, sinks=sinks, scale=scale)
+        out, lse = _autograd()[3].apply(q, k, v, window, sinks, lengths, scale)
+        return (out, lse) if return_lse else out
+    return _ops.window_attention(q, k, v, window, sinks, lengths, scale, return_lse)
+
+
+def window_attention_backward(dout, q, k, v, out, lse, *, window=None, sinks=0, lengths=None, scale=None, lse_grad=None):
+    """Gradients ``(dq, dk, dv)`` of ``window_attention``: ``out`` and ``lse`` as it returned them, the other arguments as it was
+    given.  ``lse_grad`` is the gradient of lse, where it has one."""
+    return _ops.window_attention_backward(dout, q, k, v, out, lse, window, sinks, lengths, scale, lse_grad)
+
+
+def append_rotary(q, k, v, positions, frequencies, sections, k_pages, v_pages, page_table, lengths, *, counts=None, adjacent=False,
+                  interleaved=False):
+    """New tokens join a cache: keys are turned as by ``rotary`` and written with the values; returns ``q`` turned.
+
+    ``q`` [batch, tokens, q_heads, head_dim] or None, ``k``, ``v`` [batch, tokens, kv_heads, head_dim], ``positions`` [axes, batch,
+    tokens], ``frequencies``, ``sections``, ``adjacent`` and ``interleaved`` as in ``rotary``; ``positions`` None: a token's place in its
+    sequence, on every axis.
+    ``k_pages``, ``v_pages`` [pages, page_size, kv_heads, head_dim] of k's type, written in place; page_size a power of two from 8 on.
+    ``page_table`` [batch, pages of a sample] int32 or int64: place s of sample b lies in row s % page_size of page
+    page_table[b, s // page_size]; an entry that is no page (-1) has no room.  ``lengths`` [batch] int32 or int64: the tokens that the
+    cache holds; the new ones go to the places behind them.  ``counts`` [batch] int32 or int64: of a padded batch, how many of a
+    sample's tokens are new ones; None: all.  Tokens behind these, and those that have no page, are not written; all queries are
+    turned.  Two tokens must not go to one row, and the pools must not overlap the inputs.  There is no gradient: inputs that require one
+    are refused.
+    """
+    return _ops.append_rotary(q, k, v, positions, frequencies, sections, k_pages, v_pages, page_table, lengths, counts, adjacent, interleaved)
+
+
+def cached_attention(q, k_pages, v_pages, page_table, lengths, *, counts=None, tree=None, window=None, sinks=0, scale=None, return_lse=False):
+    """Attention of new tokens over a cache that ``append_rotary`` has put them into, with the same ``lengths`` and ``counts``.
+
+    ``q`` [batch, tokens, q_heads, head_dim], bfloat16 or float16, one token or many; head_dim a multiple of 8, up to 128; q_heads a multiple of
+    kv_heads.  Token i of sample b has the place lengths[b] + i and reads the keys j up to its own place with place - j < window
+    (None: all) or j < sinks.
+    ``tree`` bool [batch, tokens, tokens] or [tokens, tokens], for drafted tokens: token i reads the new token j where tree[i, j], and
+    of the tokens before them what the window leaves, counted from the place lengths[b] + the number of new tokens other than itself that
+    it reads.  Keys that have no page are not read.  What lies where no token of a sample reads has no effect; an infinity or NaN in a
+    value that some read may reach the sample's other tokens.  Tokens that read nothing, those behind counts[b] among them, get
+    zeros.  Returns the result, or with ``return_lse`` also the logarithm of each row's sum of exponentials, float32 [batch,
+    q_heads, tokens].  There is no gradient: inputs that require one are refused.
+    """
+    return _ops.cached_attention(q, k_pages, v_pages, page_table, lengths, counts, tree, window, sinks, scale, return_lse)

@@ -13,6 +13,11 @@
 
 namespace mlxd {
 
+struct Heads {
+  char* data;
+  int64_t batch, token, head;   // strides in elements
+};
+
 // bytes of an element; 0 for a type the operators do not take
 inline int dtype_bytes(int dtype) {
   switch (dtype) {

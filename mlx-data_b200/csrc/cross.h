@@ -8,13 +8,9 @@
 #include <cstdint>
 
 #include "../../include/mlxd_b200.h"
+#include "attention.h"
 
 namespace mlxd {
-
-struct Heads {
-  char* data;
-  int64_t batch, token, head;   // strides in elements
-};
 
 struct CrossParams {
   Heads q, k, v, out, dout, dq, dk, dv;
@@ -36,6 +32,9 @@ struct CrossMaps {
   CUtensorMap q, k, v, out, dout, dq, dk, dv;   // forward: the first four; backward: all but out
 };
 
+// The device's word that a kernel sets whose wait ran out.
+int status_word(int device, int** word);
+
 // Raises a kernel's limit of shared memory, once per device.
 template <auto kKernel>
 cudaError_t allow_shared(int bytes, int device) {
@@ -47,6 +46,9 @@ cudaError_t allow_shared(int bytes, int device) {
   return e;
 }
 
+// A tensor map of 128-byte swizzled boxes of 16-bit elements; strides in elements, the first is not looked at.
+int tile_map(const char* entry, int dtype, int device, void* data, int rank, const uint64_t* sizes, const int64_t* strides, const uint32_t* box,
+             CUtensorMap* map);
 int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int heads, int dim, CUtensorMap* map);
 
 cudaError_t launch_cross_forward(const CrossParams& p, const CrossMaps& maps, int dtype, cudaStream_t stream);

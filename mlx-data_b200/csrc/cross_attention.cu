@@ -9,6 +9,9 @@ namespace mlxd {
 
 namespace {
 
+// Set by a kernel whose wait for its own copies or products ran out, and never cleared: whoever asks learns of it, on any stream.
+__device__ int attention_status;
+
 // Tensors as the copies into shared memory want them: 16-byte units throughout.  Strides of dimensions that are not
 // stepped along do not matter.
 bool aligned(const mlxd_heads& h, int batch, int tokens, int heads) {
@@ -32,23 +35,6 @@ int check_sizes(const char* entry, const mlxd_cross_desc* d) {
     return bad("too many rows");
   }
   if (static_cast<int64_t>(d->batch) * d->kv_heads * ((static_cast<int64_t>(d->kv_tokens) + 127) / 128) > INT32_MAX) return bad("too many keys");
-  return MLXD_OK;
-}
-
-// Set by a kernel whose wait for its own copies or products ran out, and never cleared: whoever asks learns of it, on any stream.
-__device__ int attention_status;
-
-int status_word(int device, int** word) {
-  constexpr int kDevices = 64;
-  static std::atomic<int*> known[kDevices];
-  if (device < 0 || device >= kDevices) return fail(MLXD_ERR_INVALID, "device index out of range");
-  *word = known[device].load(std::memory_order_relaxed);
-  if (!*word) {
-    void* at = nullptr;
-    MLXD_CUDA(cudaGetSymbolAddress(&at, static_cast<const void*>(&attention_status)));
-    *word = static_cast<int*>(at);
-    known[device].store(*word, std::memory_order_relaxed);
-  }
   return MLXD_OK;
 }
 
@@ -141,8 +127,23 @@ int maps_of(const CrossParams& p, int dtype, bool backward, CrossMaps& m) {
 
 }  // namespace
 
+int status_word(int device, int** word) {
+  constexpr int kDevices = 64;
+  static std::atomic<int*> known[kDevices];
+  if (device < 0 || device >= kDevices) return fail(MLXD_ERR_INVALID, "device index out of range");
+  *word = known[device].load(std::memory_order_relaxed);
+  if (!*word) {
+    void* at = nullptr;
+    MLXD_CUDA(cudaGetSymbolAddress(&at, static_cast<const void*>(&attention_status)));
+    *word = static_cast<int*>(at);
+    known[device].store(*word, std::memory_order_relaxed);
+  }
+  return MLXD_OK;
+}
+
 // The driver's encoder, found through the runtime: the library links against no driver library.
-int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int heads, int dim, CUtensorMap* map) {
+int tile_map(const char* entry, int dtype, int device, void* data, int rank, const uint64_t* sizes, const int64_t* strides, const uint32_t* box,
+             CUtensorMap* map) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -156,14 +157,18 @@ int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int 
     encode = reinterpret_cast<Encode>(f);
     known.store(encode, std::memory_order_relaxed);
   }
-  const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
-  // strides of dimensions that are not stepped along may be anything; the encoder wants multiples of 16 bytes
-  const auto bytes = [](int64_t stride, int size) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : 16); };
-  const cuuint64_t strides[3] = {bytes(h.token, tokens), bytes(h.head, heads), bytes(h.batch, batch)};
-  const cuuint32_t box[4] = {64, 128, 1, 1}, steps[4] = {1, 1, 1, 1};
+  cuuint64_t dims[5], bytes[4];
+  cuuint32_t boxes[5];
+  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; i++) {
+    dims[i] = sizes[i];
+    boxes[i] = box[i];
+    // strides of dimensions that are not stepped along may be anything; the encoder wants multiples of 16 bytes
+    if (i) bytes[i - 1] = static_cast<cuuint64_t>(sizes[i] > 1 ? strides[i] * 2 : 16);
+  }
   const auto make = [&] {
-    return encode(map, dtype == MLXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, h.data, sizes,
-                  strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    return encode(map, dtype == MLXD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank), data,
+                  dims, bytes, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = make();
@@ -172,9 +177,16 @@ int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int 
     MLXD_CUDA(cudaSetDevice(device));
     r = make();
   }
-  if (r == CUDA_ERROR_INVALID_VALUE) return fail(MLXD_ERR_INVALID, "cross_attention: a tensor's strides do not fit a tensor map");
-  if (r != CUDA_SUCCESS) return fail(MLXD_ERR_CUDA, "cross_attention: no tensor map (driver status " + std::to_string(r) + ")");
+  if (r == CUDA_ERROR_INVALID_VALUE) return fail(MLXD_ERR_INVALID, std::string(entry) + ": a tensor's strides do not fit a tensor map");
+  if (r != CUDA_SUCCESS) return fail(MLXD_ERR_CUDA, std::string(entry) + ": no tensor map (driver status " + std::to_string(r) + ")");
   return MLXD_OK;
+}
+
+int cross_map(const Heads& h, int dtype, int device, int batch, int tokens, int heads, int dim, CUtensorMap* map) {
+  const uint64_t sizes[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(tokens), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+  const int64_t strides[4] = {1, h.token, h.head, h.batch};
+  const uint32_t box[4] = {64, 128, 1, 1};
+  return tile_map("cross_attention", dtype, device, h.data, 4, sizes, strides, box, map);
 }
 
 }  // namespace mlxd

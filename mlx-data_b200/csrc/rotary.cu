@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "cache.h"
 #include "sm100.cuh"
 
 namespace mlxd {
@@ -18,11 +19,6 @@ constexpr int kForwardBlocks = 7;                        // CTAs of an SM: 28 wa
 constexpr int kBackwardBlocks = 3;                       // in the backward pass, of 165 registers
 constexpr int kMaxPairs = MLXD_ROTARY_MAX_HEAD_DIM / 2;
 constexpr int kMaxHeads = 1 << 29;                       // of q, and of k: counts of both, and a step beyond the last, fit an int
-
-struct Heads {
-  char* data;
-  int64_t batch, token, head;   // strides in elements
-};
 
 struct RotaryParams {
   Heads q, k, q_out, k_out, q_grad, k_grad;
@@ -65,13 +61,18 @@ __device__ float position_at(const RotaryParams& p, int axis, int64_t b, int64_t
 }
 
 // The angle is the float32 product by definition; sincosf reduces arguments of any size.
+__device__ float2 unit_at(const RotaryParams& p, int pair, float position) {
+  if (pair >= p.pairs) return make_float2(1.0f, 0.0f);
+  float2 u;
+  sincosf(__fmul_rn(position, p.frequencies[pair]), &u.y, &u.x);
+  u.y *= p.sign;
+  return u;
+}
+
 __device__ float2 unit_of(const RotaryParams& p, int pair, int64_t b, int64_t s) {
   if (pair >= p.pairs) return make_float2(1.0f, 0.0f);
   const int axis = p.axes[pair >> 4] >> (2 * (pair & 15)) & 3;
-  float2 u;
-  sincosf(__fmul_rn(position_at(p, axis, b, s), p.frequencies[pair]), &u.y, &u.x);
-  u.y *= p.sign;
-  return u;
+  return unit_at(p, pair, position_at(p, axis, b, s));
 }
 
 // Elements of pair i of a head; pairs beyond p.pairs are the elements that pass through, two by two.
@@ -211,6 +212,15 @@ struct Lane {
       }
       *reinterpret_cast<Vec<T, kV>*>(x + at[k][0]) = v[0];
       *reinterpret_cast<Vec<T, kV>*>(x + at[k][1]) = v[1];
+    }
+  }
+
+  __device__ void store_raw(T* x, const Raw& r) const {
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+      if (!owns[k]) continue;
+      *reinterpret_cast<Vec<T, kV>*>(x + at[k][0]) = r.v[k][0];
+      *reinterpret_cast<Vec<T, kV>*>(x + at[k][1]) = r.v[k][1];
     }
   }
 
@@ -362,6 +372,81 @@ __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) rotary_kernel(con
   }
 }
 
+// What joins a cache: values beside the keys, and where both go.
+struct AppendParams {
+  RotaryParams r;               // k_out is not used
+  Heads v, k_pages, v_pages;    // pages: batch is the page, token the row
+  CacheParams cache;
+};
+
+// y = R(x) of queries as above; keys turned and values as they are to their rows in the cache.  One pass, since the alternative reads and
+// writes the turned keys once more and costs two more launches, which is all there is to a single token.  A warp takes a token, or a part
+// of its heads, as above: queries, keys, values; keys and values of tokens that are not written are not read either.
+template <class T, int kV, int kUnits, bool kAdjacent, Turned kTurned>
+__global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) append_rotary_kernel(const __grid_constant__ AppendParams a) {
+  using L = Lane<T, kV, kUnits, kAdjacent>;
+  const RotaryParams& p = a.r;
+  __shared__ float2 tables[kWarps][kMaxPairs];
+  const int lane = threadIdx.x & 31, first = lane & (p.lanes - 1), mine = lane / p.lanes, at_once = 32 / p.lanes;
+  float2* table = tables[threadIdx.x / 32];
+  const L me(p, first);
+  const uint32_t items = static_cast<uint32_t>(p.rows) * p.parts;
+  const uint32_t item = blockIdx.x * kWarps + threadIdx.x / 32;
+  if (item >= items) return;
+  const uint32_t row = p.parts == 1 ? item : item / p.parts, part = item - row * p.parts;
+  const uint32_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
+  const int place = length_of(a.cache, b) + static_cast<int>(s);
+  const int64_t page = static_cast<int>(s) < count_of(a.cache, b, p.tokens) ? page_of(a.cache, b, place) : -1;
+  const int page_row = place & (a.cache.page_size - 1);
+  // rounds of a token: those of its queries, of its keys, of its values; this warp has `from` to `to` - 1 of them
+  const int from = part * p.part_rounds, to = min(p.q_rounds + 2 * p.k_rounds, from + p.part_rounds);
+  if (from < p.q_rounds + p.k_rounds) {   // something to turn
+    for (int i = lane; i < p.head_dim / 2; i += 32) table[i] = p.positions ? unit_of(p, i, b, s) : unit_at(p, i, static_cast<float>(place));
+  }
+  __syncwarp();
+  typename L::Pairs u;
+  me.angles(table, first, u);
+  const uint32_t turned = kTurned == kAll ? 0 : me.turned(p, first);
+  int begin = 0;
+#pragma unroll 1
+  for (int which = 0; which < 3; which++) {
+    const int rounds = which ? p.k_rounds : p.q_rounds, heads = which ? p.k_heads : p.q_heads;
+    const int last = min(to - begin, rounds);
+    int round = max(from - begin, 0);
+    begin += rounds;
+    if (round >= last || (which && page < 0)) continue;
+    const Heads& in = which == 0 ? p.q : which == 1 ? p.k : a.v;
+    const T* x = reinterpret_cast<const T*>(in.data) + b * in.batch + s * in.token;
+    const Heads& out = which == 0 ? p.q_out : which == 1 ? a.k_pages : a.v_pages;
+    T* y = reinterpret_cast<T*>(out.data) + (which ? page * out.batch + page_row * out.token : b * out.batch + s * out.token);
+    typename L::Raw raw = {};
+    int h = round * at_once + mine;
+    me.load(x + h * in.head, h < heads, raw);
+#pragma unroll 1
+    for (; round < last; round++, h += at_once) {
+      if (which == 2) {
+        if (h < heads) me.store_raw(y + h * out.head, raw);
+        me.load(x + (h + at_once) * in.head, round + 1 < last && h + at_once < heads, raw);
+        continue;
+      }
+      typename L::Pairs e;
+      me.widen(raw, e);
+      me.load(x + (h + at_once) * in.head, round + 1 < last && h + at_once < heads, raw);
+      if constexpr (kTurned == kAll) {
+#pragma unroll
+        for (int i = 0; i < L::kN; i += 2) {
+          const float2 l = two(e.a, i), c = two(e.b, i), cos = two(u.a, i), sin = two(u.b, i);
+          put(e.a, i, fma2(c, neg2(sin), mul2(l, cos)));
+          put(e.b, i, fma2(l, sin, mul2(c, cos)));
+        }
+      } else {
+        turn_part<kTurned, L>(turned, u, e);
+      }
+      if (h < heads) me.store(y + h * out.head, e);
+    }
+  }
+}
+
 // With g = R^-1(dy), n = x r: dw = sum g n, dx = r (g w - n mean(g w n)); r is worked out again, so that the forward pass keeps nothing.
 // The first p.q_blocks CTAs take the tokens' queries, the others their keys, so that a lane holds the sums of one weight's
 // gradient: over all tokens it meets, then over the lanes and warps of the CTA in a fixed order, one row of p.partial a CTA.
@@ -503,7 +588,7 @@ void backward_blocks(int64_t rows, int q_heads, int k_heads, int sms, int* q_blo
   *blocks = *q_blocks + share(k_heads);
 }
 
-enum class Pass { kRotary, kNorm, kBackward };
+enum class Pass { kRotary, kNorm, kBackward, kAppend };
 
 int check_sizes(const char* entry, const mlxd_rotary_desc* d) {
   const auto bad = [&](const std::string& what) { return fail(MLXD_ERR_INVALID, std::string(entry) + ": " + what); };
@@ -543,10 +628,11 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
     left[a]--;
     if (d->interleaved) a = (a + 1) % d->n_axes;
   }
-  if (d->positions_dtype != MLXD_I32 && d->positions_dtype != MLXD_I64 && d->positions_dtype != MLXD_F32) {
+  const bool places = pass == Pass::kAppend && !d->positions, norm = pass == Pass::kNorm || pass == Pass::kBackward;
+  if (!places && d->positions_dtype != MLXD_I32 && d->positions_dtype != MLXD_I64 && d->positions_dtype != MLXD_F32) {
     return bad("positions must be int32, int64 or float32");
   }
-  if (pass != Pass::kRotary) {
+  if (norm) {
     if (d->weight_dtype != MLXD_F32 && d->weight_dtype != MLXD_BF16 && d->weight_dtype != MLXD_F16) {
       return bad("weights must be float32, bfloat16 or float16");
     }
@@ -554,9 +640,9 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
   }
   const bool work = d->batch && d->tokens && (d->q_heads || d->k_heads);
   if (work) {
-    if (!d->positions || !d->frequencies) return bad("positions and frequencies are needed");
+    if ((!d->positions && !places) || !d->frequencies) return bad("positions and frequencies are needed");
     if (d->q_heads && (absent(d->q) || absent(d->q_out))) return bad("q and q_out are needed");
-    if (d->k_heads && (absent(d->k) || absent(d->k_out))) return bad("k and k_out are needed");
+    if (pass != Pass::kAppend && d->k_heads && (absent(d->k) || absent(d->k_out))) return bad("k and k_out are needed");
     if (pass == Pass::kBackward && ((d->q_heads && absent(d->q_grad)) || (d->k_heads && absent(d->k_grad)))) return bad("q_grad and k_grad are needed");
   }
   // a kernel reads and writes whole elements, and a misaligned one is a fault
@@ -564,10 +650,10 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
   for (const mlxd_heads* h : {&d->q, &d->q_out, &d->k, &d->k_out, &d->q_grad, &d->k_grad}) {
     if (!on_boundary(h->data, bytes)) return bad("a tensor does not start on a multiple of its element's size");
   }
-  if (!on_boundary(d->positions, dtype_bytes(d->positions_dtype)) || !on_boundary(d->frequencies, 4)) {
+  if ((d->positions && !on_boundary(d->positions, dtype_bytes(d->positions_dtype))) || !on_boundary(d->frequencies, 4)) {
     return bad("positions or frequencies do not start on a multiple of their element's size");
   }
-  if (pass != Pass::kRotary) {
+  if (norm) {
     for (const void* w : {d->q_weight, d->k_weight, static_cast<const void*>(d->q_weight_grad), static_cast<const void*>(d->k_weight_grad)}) {
       if (!on_boundary(w, dtype_bytes(d->weight_dtype))) return bad("a weight or its gradient does not start on a multiple of its element's size");
     }
@@ -604,7 +690,7 @@ int params_of(const char* entry, const mlxd_rotary_desc* d, Pass pass, RotaryPar
 
 // Elements of a vector: 16 bytes where every row and both vectors of a lane start on such a boundary, else 8 bytes (heads
 // of 72 16-bit elements), else single elements.
-int vector_of(const RotaryParams& p, int bytes, bool backward) {
+int vector_of(const RotaryParams& p, int bytes, bool backward, const AppendParams* append = nullptr) {
   for (int v = 16 / bytes; v > 1; v = v == 8 ? 4 : 1) {
     bool fits = p.head_dim / 2 % v == 0 && (p.adjacent || p.pairs % v == 0);
     const auto rows = [&](const Heads& h, int heads) {
@@ -616,7 +702,15 @@ int vector_of(const RotaryParams& p, int bytes, bool backward) {
     rows(p.q, p.q_heads);
     rows(p.k, p.k_heads);
     rows(p.q_out, p.q_heads);
-    rows(p.k_out, p.k_heads);
+    if (append) {
+      rows(append->v, p.k_heads);
+      for (const Heads* h : {&append->k_pages, &append->v_pages}) {
+        rows(*h, p.k_heads);
+        fits = fits && h->batch * bytes % (v * bytes) == 0 && h->token * bytes % (v * bytes) == 0;
+      }
+    } else {
+      rows(p.k_out, p.k_heads);
+    }
     if (backward) {
       rows(p.q_grad, p.q_heads);
       rows(p.k_grad, p.k_heads);
@@ -662,6 +756,20 @@ cudaError_t with_type(int dtype, const RotaryParams& p, int v, F&& f) {
   return with_instance<__nv_bfloat16>(p, v, f);
 }
 
+// How a token's heads lie over warps: they are shared out until there are 32 warps for every SM.  `keys`: rounds of keys, and of what is
+// like them.  Returns the number of CTAs.
+unsigned shares_of(RotaryParams& p, int v, int keys, int sms) {
+  p.lanes = lanes_of(p.head_dim / 2 / v);
+  const int at_once = 32 / p.lanes;
+  p.q_rounds = (p.q_heads + at_once - 1) / at_once;
+  p.k_rounds = (p.k_heads + at_once - 1) / at_once;
+  const int rounds = p.q_rounds + keys * p.k_rounds;
+  const int64_t parts = std::min<int64_t>(rounds, std::max<int64_t>(1, 32 * sms / p.rows));
+  p.part_rounds = static_cast<int>((rounds + parts - 1) / parts);
+  p.parts = (rounds + p.part_rounds - 1) / p.part_rounds;
+  return static_cast<unsigned>((p.rows * p.parts + kWarps - 1) / kWarps);
+}
+
 int forward(const char* entry, int device, void* stream, const mlxd_rotary_desc* d, Pass pass) {
   RotaryParams p;
   int rc = params_of(entry, d, pass, p);
@@ -671,22 +779,48 @@ int forward(const char* entry, int device, void* stream, const mlxd_rotary_desc*
   rc = device_sms(device, &sms);
   if (rc != MLXD_OK) return rc;
   const int v = vector_of(p, dtype_bytes(d->dtype), false);
-  p.lanes = lanes_of(p.head_dim / 2 / v);
-  // a token's heads are shared out among warps until there are 32 warps for every SM
-  const int at_once = 32 / p.lanes;
-  p.q_rounds = (p.q_heads + at_once - 1) / at_once;
-  p.k_rounds = (p.k_heads + at_once - 1) / at_once;
-  const int rounds = p.q_rounds + p.k_rounds;
-  const int64_t parts = std::min<int64_t>(rounds, std::max<int64_t>(1, 32 * sms / p.rows));
-  p.part_rounds = static_cast<int>((rounds + parts - 1) / parts);
-  p.parts = (rounds + p.part_rounds - 1) / p.part_rounds;
+  const unsigned blocks = shares_of(p, v, 1, sms);
   MLXD_ON_DEVICE(device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned blocks = static_cast<unsigned>((p.rows * p.parts + kWarps - 1) / kWarps);
   const cudaError_t e = with_type(d->dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
     using T = decltype(type);
     if (pass == Pass::kNorm) rotary_kernel<T, vec(), units(), adjacent(), turned(), true><<<blocks, 32 * kWarps, 0, s>>>(p);
     else rotary_kernel<T, vec(), units(), adjacent(), turned(), false><<<blocks, 32 * kWarps, 0, s>>>(p);
+    return cudaGetLastError();
+  });
+  return e == cudaSuccess ? MLXD_OK : fail_cuda(e, entry);
+}
+
+int append(const char* entry, int device, void* stream, const mlxd_append_desc* d) {
+  const auto bad = [&](const std::string& what) { return fail(MLXD_ERR_INVALID, std::string(entry) + ": " + what); };
+  if (!d) return bad("no descriptor");
+  AppendParams a;
+  int rc = params_of(entry, &d->r, Pass::kAppend, a.r);
+  if (rc == MLXD_OK) rc = cache_of(entry, d->cache, d->r.batch, &a.cache);
+  if (rc != MLXD_OK) return rc;
+  RotaryParams& p = a.r;
+  if (d->r.inverse) return bad("there is no inverse");
+  if (d->r.tokens >= kMaxPlaces) return bad("2^30 tokens or more");
+  if (p.k_heads < 1) return bad("keys and values are needed");
+  a.v = heads_of(d->v);
+  a.k_pages = pages_of(d->cache.k);
+  a.v_pages = pages_of(d->cache.v);
+  if (!p.rows) return MLXD_OK;
+  if (absent(d->r.k) || absent(d->v)) return bad("k and v are needed");
+  if (d->cache.pages && (!d->cache.k.data || !d->cache.v.data)) return bad("the cache's pages are needed");
+  const int bytes = dtype_bytes(d->r.dtype);
+  for (const Heads* h : {&a.v, &a.k_pages, &a.v_pages}) {
+    if (!on_boundary(h->data, bytes)) return bad("a tensor does not start on a multiple of its element's size");
+  }
+  int sms = 0;
+  rc = device_sms(device, &sms);
+  if (rc != MLXD_OK) return rc;
+  const int v = vector_of(p, bytes, false, &a);
+  const unsigned blocks = shares_of(p, v, 2, sms);
+  MLXD_ON_DEVICE(device);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_type(d->r.dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
+    append_rotary_kernel<decltype(type), vec(), units(), adjacent(), turned()><<<blocks, 32 * kWarps, 0, s>>>(a);
     return cudaGetLastError();
   });
   return e == cudaSuccess ? MLXD_OK : fail_cuda(e, entry);
@@ -716,6 +850,10 @@ extern "C" int mlxd_rotary(int device, void* cuda_stream, const mlxd_rotary_desc
 
 extern "C" int mlxd_qk_norm_rotary(int device, void* cuda_stream, const mlxd_rotary_desc* d) {
   return guarded("qk_norm_rotary", [&] { return forward("qk_norm_rotary", device, cuda_stream, d, Pass::kNorm); });
+}
+
+extern "C" int mlxd_append_rotary(int device, void* cuda_stream, const mlxd_append_desc* d) {
+  return guarded("append_rotary", [&] { return append("append_rotary", device, cuda_stream, d); });
 }
 
 extern "C" int mlxd_qk_norm_rotary_workspace(int device, const mlxd_rotary_desc* d, size_t* bytes) {
