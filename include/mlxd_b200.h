@@ -418,7 +418,8 @@ MLXD_API int mlxd_append_rotary(int device, void* cuda_stream, const mlxd_append
  * (0: no window) or j < sinks.  With a tree [batch, tokens, tokens] query i reads the new token j where tree[b, i, j] is not 0 and
  * j < counts[b], and of the cache before them (j < lengths[b]) what the window leaves, s being lengths[b] + the number of new tokens
  * other than itself that it reads.  Keys at places that have no page are not read.  What lies where no query of the sample reads has no
- * effect, whatever it is; what is not a number in a value that some queries of a sample read may reach its other queries too.  Queries
+ * effect, whatever it is; what is not a number in a value that some queries of a sample read, or under a tree in a value of any of its
+ * new tokens, may reach its other queries too.  Queries
  * without a key to read, those from counts[b] on among them, get zeros and -infinity in lse.
  * scale, lse [batch, q_heads, tokens], rounding and groups of heads are as in mlxd_cross_desc. */
 typedef struct mlxd_cached_desc {

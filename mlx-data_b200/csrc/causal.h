@@ -23,7 +23,40 @@ struct CausalParams {
   int device;
 };
 
-cudaError_t launch_causal_forward(const CausalParams& p, bool paged, int dtype, cudaStream_t stream);
+// How rows lie in tiles of 128: the tokens of a key head's query heads, head by head within a token.
+struct RowTiles {
+  int heads, tokens;            // of a tile
+  int chunks;                   // of a key head's query heads, where they are more than a tile has rows
+  int tiles;                    // of a sample, chunk by chunk
+};
+
+inline RowTiles row_tiles(const CausalParams& p) {
+  RowTiles r;
+  r.heads = p.group < 128 ? p.group : 128;
+  r.tokens = 128 / r.heads;
+  r.chunks = (p.group + r.heads - 1) / r.heads;
+  r.tiles = (p.tokens + r.tokens - 1) / r.tokens;
+  return r;
+}
+
+struct ForwardParams {
+  CausalParams p;
+  RowTiles rows;
+  int splits;                   // of a sample's keys
+  int halves;                   // a CTA has one tile of rows, whose keys its two halves take tile by tile in turns
+  int parts;                    // splits * (halves ? 2 : 1); 1: results are final
+  float* part_out;              // [parts][batch, q_heads, tokens][head_dim]
+  float* part_lse;              // [parts][batch, q_heads, tokens]
+};
+
+struct CausalMaps {
+  CUtensorMap q, k, v, out, dout, dq, dk, dv;   // forward: the first four
+};
+
+// Splits and parts of a call, but for where the parts lie.
+ForwardParams forward_plan(const CausalParams& p, bool paged, int sms);
+size_t forward_workspace(const ForwardParams& f);
+cudaError_t launch_causal_forward(const ForwardParams& f, const CausalMaps& maps, bool paged, int dtype, cudaStream_t stream);
 cudaError_t launch_causal_backward(const CausalParams& p, int dtype, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -1,4 +1,5 @@
 // Attention over a cache and attention in a window: entry points, checks, launches.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -73,6 +74,47 @@ int tensor_of(const char* entry, const char* name, const Heads& h, int64_t batch
   return MLXD_OK;
 }
 
+// Maps of queries and results: boxes of 64 elements of a tile's rows.
+int rows_map(const char* entry, const CausalParams& p, const RowTiles& r, const Heads& h, int dtype, CUtensorMap* map) {
+  const uint64_t sizes[5] = {static_cast<uint64_t>(p.head_dim), static_cast<uint64_t>(p.group), static_cast<uint64_t>(p.tokens),
+                             static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.batch)};
+  const int64_t strides[5] = {1, h.head, h.token, h.head * p.group, h.batch};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(r.heads), static_cast<uint32_t>(r.tokens), 1, 1};
+  return tile_map(entry, dtype, p.device, h.data, 5, sizes, strides, box, map);
+}
+
+// Of keys and values: boxes of 64 elements of 128 tokens, or of as many as a page has.
+int keys_map(const char* entry, const CausalParams& p, const Heads& h, int64_t major, int64_t minor, int dtype, CUtensorMap* map) {
+  const uint64_t sizes[4] = {static_cast<uint64_t>(p.head_dim), static_cast<uint64_t>(minor), static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(major)};
+  const int64_t strides[4] = {1, h.token, h.head, h.batch};
+  const uint32_t box[4] = {64, p.cache.page_size ? static_cast<uint32_t>(std::min(p.cache.page_size, 128)) : 128u, 1, 1};
+  return tile_map(entry, dtype, p.device, h.data, 4, sizes, strides, box, map);
+}
+
+int forward(const char* entry, CausalParams& p, int dtype, bool paged, void* workspace, size_t workspace_bytes, int device, void* stream) {
+  p.device = device;
+  int sms = 0;
+  int rc = device_sms(device, &sms);
+  if (rc != MLXD_OK) return rc;
+  ForwardParams f = forward_plan(p, paged, sms);
+  const size_t need = forward_workspace(f);
+  if (need && (!workspace || workspace_bytes < need)) return fail(MLXD_ERR_INVALID, std::string(entry) + ": workspace too small");
+  MLXD_ON_DEVICE(device);
+  rc = status_word(device, &f.p.status);
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.tokens;
+  f.part_out = static_cast<float*>(workspace);
+  f.part_lse = f.part_out + (need ? f.parts * rows * p.head_dim : 0);
+  CausalMaps maps;
+  const int64_t major = paged ? p.cache.pages : p.batch, minor = paged ? p.cache.page_size : p.tokens;
+  if (rc == MLXD_OK) rc = rows_map(entry, p, f.rows, p.q, dtype, &maps.q);
+  if (rc == MLXD_OK) rc = rows_map(entry, p, f.rows, p.out, dtype, &maps.out);
+  if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.k, major, minor, dtype, &maps.k);   // without pages there is nothing to read
+  if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.v, major, minor, dtype, &maps.v);
+  if (rc != MLXD_OK) return rc;
+  MLXD_CUDA(launch_causal_forward(f, maps, paged, dtype, static_cast<cudaStream_t>(stream)));
+  return MLXD_OK;
+}
+
 size_t delta_bytes(const CausalParams& p) { return sizeof(float) * p.batch * p.q_heads * p.tokens; }
 
 int cached_params(const char* entry, const mlxd_cached_desc* d, CausalParams& p) {
@@ -133,13 +175,22 @@ int window_call(const char* entry, int device, void* stream, const mlxd_window_d
   int rc = window_params(entry, d, backward, p);
   if (rc != MLXD_OK) return rc;
   if (!p.batch || !p.tokens) return MLXD_OK;
+  if (!backward) return forward(entry, p, d->dtype, false, d->workspace, d->workspace_bytes, device, stream);
   MLXD_ON_DEVICE(device);
   p.device = device;
   rc = status_word(device, &p.status);
   if (rc != MLXD_OK) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  MLXD_CUDA(backward ? launch_causal_backward(p, d->dtype, s) : launch_causal_forward(p, false, d->dtype, s));
+  MLXD_CUDA(launch_causal_backward(p, d->dtype, static_cast<cudaStream_t>(stream)));
   return MLXD_OK;
+}
+
+int forward_bytes(const CausalParams& p, bool paged, int device, size_t* bytes) {
+  *bytes = 0;
+  if (!p.batch || !p.tokens) return MLXD_OK;
+  int sms = 0;
+  const int rc = device_sms(device, &sms);
+  if (rc == MLXD_OK) *bytes = forward_workspace(forward_plan(p, paged, sms));
+  return rc;
 }
 
 }  // namespace
@@ -164,11 +215,11 @@ int cache_of(const char* entry, const mlxd_cache& c, int batch, CacheParams* p) 
   p->lengths = c.lengths;
   p->counts = c.counts;
   p->table_stride = c.page_table_stride;
-  p->table_width = c.table_width;
+  p->table_width = c.pages ? c.table_width : 0;   // a pool of no pages has no places
   p->pages = c.pages;
   p->page_size = c.page_size;
   p->page_shift = __builtin_ctz(static_cast<unsigned>(c.page_size));
-  p->capacity = c.table_width * c.page_size;
+  p->capacity = p->table_width * c.page_size;
   p->table_dtype = c.page_table_dtype;
   p->lengths_dtype = c.lengths_dtype;
   p->counts_dtype = c.counts_dtype;
@@ -182,26 +233,22 @@ using namespace mlxd;
 extern "C" int mlxd_cached_attention_workspace(int device, const mlxd_cached_desc* d, size_t* bytes) {
   return guarded("cached_attention_workspace", [&] {
     CausalParams p;
-    const int rc = sizes_of("cached_attention_workspace", d, p);
+    int rc = sizes_of("cached_attention_workspace", d, p);
     if (rc != MLXD_OK) return rc;
     if (!bytes) return fail(MLXD_ERR_INVALID, "cached_attention_workspace: no place for the result");
-    *bytes = 0;
-    return static_cast<int>(MLXD_OK);
+    rc = cache_of("cached_attention_workspace", d->cache, d->batch, &p.cache);
+    if (rc != MLXD_OK) return rc;
+    return forward_bytes(p, true, device, bytes);
   });
 }
 
 extern "C" int mlxd_cached_attention(int device, void* cuda_stream, const mlxd_cached_desc* d) {
   return guarded("cached_attention", [&] {
     CausalParams p;
-    int rc = cached_params("cached_attention", d, p);
+    const int rc = cached_params("cached_attention", d, p);
     if (rc != MLXD_OK) return rc;
     if (!p.batch || !p.tokens) return static_cast<int>(MLXD_OK);
-    MLXD_ON_DEVICE(device);
-    p.device = device;
-    rc = status_word(device, &p.status);
-    if (rc != MLXD_OK) return rc;
-    MLXD_CUDA(launch_causal_forward(p, true, d->dtype, static_cast<cudaStream_t>(cuda_stream)));
-    return static_cast<int>(MLXD_OK);
+    return forward("cached_attention", p, d->dtype, true, d->workspace, d->workspace_bytes, device, cuda_stream);
   });
 }
 
@@ -211,8 +258,8 @@ extern "C" int mlxd_window_attention_workspace(int device, const mlxd_window_des
     const int rc = sizes_of("window_attention_workspace", d, p);
     if (rc != MLXD_OK) return rc;
     if (!bytes) return fail(MLXD_ERR_INVALID, "window_attention_workspace: no place for the result");
-    *bytes = backward ? delta_bytes(p) : 0;
-    return static_cast<int>(MLXD_OK);
+    *bytes = delta_bytes(p);
+    return backward ? static_cast<int>(MLXD_OK) : forward_bytes(p, false, device, bytes);
   });
 }
 
