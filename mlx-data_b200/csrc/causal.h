@@ -10,7 +10,6 @@ struct CausalParams {
   Heads q, k, v, out, dout, dq, dk, dv;   // k, v of a cache: batch is the page, token the row
   float* lse;
   const float* lse_grad;        // backward: the gradient of lse, or null
-  float* delta;                 // backward: [batch, q_heads, tokens]
   CacheParams cache;            // cached attention
   const uint8_t* tree;          // cached attention: null without one
   int64_t tree_batch, tree_token;
@@ -57,7 +56,8 @@ struct CausalMaps {
 ForwardParams forward_plan(const CausalParams& p, bool paged, int sms);
 size_t forward_workspace(const ForwardParams& f);
 cudaError_t launch_causal_forward(const ForwardParams& f, const CausalMaps& maps, bool paged, int dtype, cudaStream_t stream);
-cudaError_t launch_causal_backward(const CausalParams& p, int dtype, cudaStream_t stream);
+size_t backward_workspace(const CausalParams& p);
+cudaError_t launch_causal_backward(const CausalParams& p, void* workspace, const CausalMaps& maps, int dtype, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // A sample: its queries are at the places held to held + fresh - 1, keys lie at 0 to end - 1.
@@ -74,6 +74,12 @@ __device__ __forceinline__ Sequence sequence_of(const CausalParams& p, int b) {
   int n = p.tokens;
   if (p.lengths) n = static_cast<int>(min(max(integer_at(p.lengths, p.lengths_dtype, b), int64_t{0}), static_cast<int64_t>(n)));
   return {0, n, n};
+}
+
+// Bits `from` to `to` - 1 of the 64 that begin at `first`.
+__device__ __forceinline__ uint64_t bits_of(int first, int from, int to) {
+  const int lo = max(from - first, 0), hi = min(to - first, 64);
+  return lo < hi ? (~uint64_t{0} >> (64 - (hi - lo))) << lo : 0;
 }
 
 // What a query reads: keys below `sinks`, and those from `from` to `to` - 1; with a tree those of its row behind `to`.

@@ -115,8 +115,6 @@ int forward(const char* entry, CausalParams& p, int dtype, bool paged, void* wor
   return MLXD_OK;
 }
 
-size_t delta_bytes(const CausalParams& p) { return sizeof(float) * p.batch * p.q_heads * p.tokens; }
-
 int cached_params(const char* entry, const mlxd_cached_desc* d, CausalParams& p) {
   const auto bad = [&](const std::string& what) { return fail(MLXD_ERR_INVALID, std::string(entry) + ": " + what); };
   int rc = sizes_of(entry, d, p);
@@ -163,9 +161,7 @@ int window_params(const char* entry, const mlxd_window_desc* d, bool backward, C
   if (backward) {
     if (p.batch && p.tokens && !d->lse) return bad("lse is needed");
     if (!on_boundary(d->lse_grad, 4)) return bad("lse_grad does not start on a multiple of 4 bytes");
-    const size_t need_bytes = delta_bytes(p);
-    if (need_bytes && (!d->workspace || d->workspace_bytes < need_bytes)) return bad("workspace too small");
-    p.delta = static_cast<float*>(d->workspace);
+    if (p.batch && p.tokens && (!d->workspace || d->workspace_bytes < backward_workspace(p))) return bad("workspace too small");
   }
   return MLXD_OK;
 }
@@ -179,8 +175,15 @@ int window_call(const char* entry, int device, void* stream, const mlxd_window_d
   MLXD_ON_DEVICE(device);
   p.device = device;
   rc = status_word(device, &p.status);
+  const RowTiles rows = row_tiles(p);
+  CausalMaps maps;
+  const struct { const Heads* h; bool query; CUtensorMap* map; } all[] = {{&p.q, true, &maps.q},   {&p.dout, true, &maps.dout}, {&p.dq, true, &maps.dq}, {&p.k, false, &maps.k},
+                                                                          {&p.v, false, &maps.v}, {&p.dk, false, &maps.dk},    {&p.dv, false, &maps.dv}};
+  for (const auto& x : all) {
+    if (rc == MLXD_OK) rc = x.query ? rows_map(entry, p, rows, *x.h, d->dtype, x.map) : keys_map(entry, p, *x.h, p.batch, p.tokens, d->dtype, x.map);
+  }
   if (rc != MLXD_OK) return rc;
-  MLXD_CUDA(launch_causal_backward(p, d->dtype, static_cast<cudaStream_t>(stream)));
+  MLXD_CUDA(launch_causal_backward(p, d->workspace, maps, d->dtype, static_cast<cudaStream_t>(stream)));
   return MLXD_OK;
 }
 
@@ -258,8 +261,9 @@ extern "C" int mlxd_window_attention_workspace(int device, const mlxd_window_des
     const int rc = sizes_of("window_attention_workspace", d, p);
     if (rc != MLXD_OK) return rc;
     if (!bytes) return fail(MLXD_ERR_INVALID, "window_attention_workspace: no place for the result");
-    *bytes = delta_bytes(p);
-    return backward ? static_cast<int>(MLXD_OK) : forward_bytes(p, false, device, bytes);
+    if (!backward) return forward_bytes(p, false, device, bytes);
+    *bytes = p.batch && p.tokens ? backward_workspace(p) : 0;
+    return static_cast<int>(MLXD_OK);
   });
 }
 

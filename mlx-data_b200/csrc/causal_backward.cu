@@ -1,4 +1,10 @@
-// Gradients of window attention: a warp for each query and head, then a warp for each key and head.
+// Gradients of window attention: one kernel for queries, one for keys and values.  As in cross attention each works out the scores
+// again, so that every sum has one owner and the same order in every call (no atomics, seven products of 128 x 128 x D for the five of the
+// definition), and P and dS are rounded to 16 bits as operands of the products.  Rows are tokens and the query heads that share a key
+// head, as in the forward pass.  First tokens that stay visible are keys of every query behind them: their tiles' rows are split among
+// CTAs, whose parts a third kernel adds in order.
+#include <algorithm>
+
 #include "causal.h"
 #include "sm100.cuh"
 
@@ -6,103 +12,823 @@ namespace mlxd {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kThreads = 384;          // two warpgroups for what lies between the products, then warps for copies, products, helpers
+constexpr int kMaskRing = 4;           // queries: tiles of keys in the ring are no more
+constexpr int kRowRing = 8;            // keys: items in the ring are no more
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <class T>
-__device__ __forceinline__ void load4(const Heads& x, int b, int i, int head, int lane, bool there, float (&to)[4]) {
-  const T* at = reinterpret_cast<const T*>(x.data) + b * x.batch + i * x.token + head * x.head + 4 * lane;
-  const uint2 v = there ? *reinterpret_cast<const uint2*>(at) : make_uint2(0, 0);
-  const float2 lo = unpack2<T>(v.x), hi = unpack2<T>(v.y);
-  to[0] = lo.x, to[1] = lo.y, to[2] = hi.x, to[3] = hi.y;
+template <int kDim>
+struct Sizes {
+  static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
+  static constexpr int kBoxes = kDim / 64;
+  static constexpr int kSlots = kDim == 128 ? 5 : 8;       // of the ring
+  static constexpr int kShared = (2 + kSlots) * kTile;
+};
+
+struct BackwardParams {
+  CausalParams p;
+  RowTiles rows;
+  float2* stats;                // [batch, kv_heads, tokens, group]: -lse log2(e) and delta of a row
+  float* partial;               // [sink_parts][batch, kv_heads][sink_tiles][dk, dv][128][head_dim]
+  int sink_tiles, sink_parts;   // tiles of keys whose rows are split into so many parts; 1: none is
+};
+
+// Keys or values: 128 tokens.
+template <class S>
+__device__ __forceinline__ void load_keys(uint32_t to, const CUtensorMap* map, int token, int head, int batch, uint32_t bar) {
+  barrier_expect(bar, S::kTile);
+  for (int x = 0; x < S::kBoxes; x++) tile_load(to + x * kBoxBytes, map, 64 * x, token, head, batch, bar);
 }
 
-template <class T>
-__device__ __forceinline__ void store4(const Heads& x, int b, int i, int head, int lane, bool there, const float (&v)[4], float by) {
-  T* at = reinterpret_cast<T*>(x.data) + b * x.batch + i * x.token + head * x.head + 4 * lane;
-  if (there) *reinterpret_cast<uint2*>(at) = make_uint2(pack2<T>(v[0] * by, v[1] * by), pack2<T>(v[2] * by, v[3] * by));
+// Queries or gradients of results: a tile of rows.
+template <class S>
+__device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, const RowTiles& r, int chunk, int token, int kv_head, int batch, uint32_t bar) {
+  barrier_expect(bar, S::kBoxes * r.heads * r.tokens * 128);
+  for (int x = 0; x < S::kBoxes; x++) tile_load(to + x * kBoxBytes, map, 64 * x, chunk * r.heads, token, kv_head, batch, bar);
 }
 
-__device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
-  float x = a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
-  for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-  return x;
+__device__ __forceinline__ void store_zeros(uint32_t at) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" : : "r"(at), "r"(0) : "memory");
 }
 
-// dQ = scale dS K, dS = P (dP - delta), delta = sum(dO O) - dlse, which the other kernel reads.
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) causal_dq_kernel(const __grid_constant__ CausalParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  if (row >= static_cast<int64_t>(p.batch) * p.q_heads * p.tokens) return;
-  const int i = row % p.tokens, head = row / p.tokens % p.q_heads, b = row / p.tokens / p.q_heads, kv_head = head / p.group;
-  const bool there = 4 * lane < p.head_dim;
-  const Sequence s = sequence_of<false>(p, b);
-  float dq[4] = {};
-  if (i < s.fresh) {
-    float q[4], o[4], g[4];
-    load4<T>(p.q, b, i, head, lane, there, q);
-    load4<T>(p.out, b, i, head, lane, there, o);
-    load4<T>(p.dout, b, i, head, lane, there, g);
-    const float delta = dot4(o, g) - (p.lse_grad ? p.lse_grad[row] : 0.0f), base = row_base(p.lse[row]);
-    if (lane == 0) p.delta[row] = delta;
-    const Reach r = reach_of(p, s, i, i + 1);
-    for (int j = r.sinks ? 0 : r.from; j < r.to; j = j + 1 == r.sinks ? r.from : j + 1) {
-      float k[4], v[4];
-      load4<T>(p.k, b, j, kv_head, lane, there, k);
-      load4<T>(p.v, b, j, kv_head, lane, there, v);
-      const float ds = exp2_of(dot4(q, k) * p.scale * kLog2e + base) * (dot4(g, v) - delta);
-      for (int e = 0; e < 4; e++) dq[e] += ds * k[e];
+// The accumulators of a row, scaled, rounded and put where a store of the tile finds them; zeros where there are none.
+template <class T, int kDim>
+__device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, float by, bool none) {
+#pragma unroll
+  for (int x = 0; x < kDim; x += 32) {
+    uint32_t o[32] = {};
+    if (!none) {
+      tmem_load<32>(tmem + x, o);
+      tmem_loaded(o);
+    }
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by);
+      const int unit = (x + k) % 64 / 8;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                   : : "r"(to + (x + k) / 64 * kBoxBytes + row * 128 + ((unit ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
   }
-  store4<T>(p.dq, b, i, head, lane, there, dq, p.scale);
 }
 
-// dV = P^T dO, dK = scale dS^T Q, over the queries of every head that shares the key.
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps) causal_dkv_kernel(const __grid_constant__ CausalParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-  if (row >= static_cast<int64_t>(p.batch) * p.kv_heads * p.tokens) return;
-  const int j = row % p.tokens, kv_head = row / p.tokens % p.kv_heads, b = row / p.tokens / p.kv_heads;
-  const bool there = 4 * lane < p.head_dim;
-  const Sequence s = sequence_of<false>(p, b);
-  float dk[4] = {}, dv[4] = {};
-  if (j < s.fresh) {
-    float k[4], v[4];
-    load4<T>(p.k, b, j, kv_head, lane, there, k);
-    load4<T>(p.v, b, j, kv_head, lane, there, v);
-    const int end = j < p.sinks || p.window > s.fresh - j ? s.fresh : j + p.window;
-    for (int head = kv_head * p.group; head < (kv_head + 1) * p.group; head++) {
-      for (int i = j; i < end; i++) {
-        const int64_t stat = (static_cast<int64_t>(b) * p.q_heads + head) * p.tokens + i;
-        float q[4], g[4];
-        load4<T>(p.q, b, i, head, lane, there, q);
-        load4<T>(p.dout, b, i, head, lane, there, g);
-        const float w = exp2_of(dot4(q, k) * p.scale * kLog2e + row_base(p.lse[stat])), ds = w * (dot4(g, v) - p.delta[stat]);
-        for (int e = 0; e < 4; e++) {
-          dv[e] += w * g[e];
-          dk[e] += ds * q[e];
-        }
+// Of a row and this thread's half of a tile of keys: sums of P dP and of P, over the keys that are read.  Scores and dP stay where they are.
+__device__ __forceinline__ void row_sums(uint32_t scores_at, uint32_t dp_at, uint64_t read, bool single, float c, float base, float* sum, float* weights) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    uint32_t s[16], d[16];
+    tmem_load<16>(scores_at + 16 * i, s);
+    tmem_load<16>(dp_at + 16 * i, d);
+    tmem_loaded(s);
+    tmem_loaded(d);
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      if (read >> (16 * i + k) & 1) {
+        // lse of the forward pass makes the one weight 1 but for a rounding
+        const float w = exp2_of(fmaf(__uint_as_float(s[k]), c, base)), exact = single && w > 0 ? 1.0f : w;
+        *weights += exact;
+        *sum = fmaf(exact, __uint_as_float(d[k]), *sum);
       }
     }
   }
-  store4<T>(p.dk, b, j, kv_head, lane, there, dk, p.scale);
-  store4<T>(p.dv, b, j, kv_head, lane, there, dv, 1.0f);
 }
 
+struct RowJob {
+  int q0, chunk, kv_head, batch;
+};
+
+// The last tiles of rows first: without a window they have the most keys.
+__device__ __forceinline__ RowJob row_job_of(const BackwardParams& f, int id) {
+  RowJob j;
+  j.kv_head = id % f.p.kv_heads;
+  id /= f.p.kv_heads;
+  j.batch = id % f.p.batch;
+  id /= f.p.batch;
+  j.chunk = id % f.rows.chunks;
+  j.q0 = (f.rows.tiles - 1 - id / f.rows.chunks) * f.rows.tokens;
+  return j;
+}
+
+// dQ = scale dS K for a tile of rows: S = Q K^T, P = exp(S - lse), dP = dO V^T, dS = P (dP - delta), delta = sum(dO O) - dlse.  Two sets of
+// scores, so that the products of the next tile run beside the exponentials of this one.  What the other kernel needs of a row it leaves
+// in the order in which that one reads it.
+// O comes in rounded to 16 bits, and where few keys have weights dS is the small difference of dP and delta.  So where the keys of a tile's
+// rows fit two tiles, whose P and dP are there before any dS (the second dP where dQ will be), delta = sum(P dP) / sum(P) of these:
+// 255 tokens in float16, dQ off by 0.00036 of its size by O, 0.0003 so (0.00021 by the rounding of results alone).  A single key has the
+// weight 1, so that its dS is 0 and no remainder of a rounding.
+template <class T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
+  using S = Sizes<kDim>;
+  const CausalParams& p = f.p;
+  extern __shared__ __align__(1024) uint8_t shared[];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 5 + kMaskRing + 1 + 1];
+  __shared__ float delta_parts[2][2][128];   // of a row's two threads: sums, and with few keys those of weights
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  asm volatile("griddepcontrol.launch_dependents;");   // the other kernel's CTAs take the SMs that these leave
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
+  const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
+  const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
+                 s_full = empty + 8 * S::kSlots, dp_full = s_full + 16, ds_full = dp_full + 8, done = ds_full + 8, delta_full = done + 8,
+                 dp2_full = delta_full + 8, landed = dp2_full + 8, staged_full = landed + 8 * kMaskRing, ended = staged_full + 8;
+  const RowJob job = row_job_of(f, blockIdx.x);
+  const int batch = job.batch, kv_head = job.kv_head;
+  const Sequence seq = sequence_of<false>(p, batch);
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, dp2_full, done, ended}) barrier_init(bar, 1);
+    for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 8);
+    for (int i = 0; i < S::kSlots; i++) {
+      barrier_init(full + 8 * i, 1);
+      barrier_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kMaskRing; i++) barrier_init(landed + 8 * i, 1);
+    barrier_init_done();
+  }
+  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tmem = tmem_slot, dp_column = 256, dq_column = 384;   // scores in 0 and 128
+  // what the tile's rows read, in tiles of keys: first ones, then the window's
+  const int end_token = min(job.q0 + f.rows.tokens, seq.fresh);
+  const Reach all = job.q0 < end_token ? reach_of(p, seq, job.q0, end_token) : Reach{0, 0, 0};
+  const int sink_tiles = (all.sinks + 127) / 128, main_first = max(all.from / 128, sink_tiles);
+  const int n = sink_tiles + max((all.to + 127) / 128 - main_first, 0);
+  const auto tile_of = [&](int j) { return j < sink_tiles ? j : j - sink_tiles + main_first; };
+  const auto partial = [&](int j) {
+    const int lo = tile_of(j) * 128, hi = lo + 128;
+    return !(hi <= all.sinks || (lo >= all.from && hi <= all.to));
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 8 && lane == 0 && n) {
+      // -------------------------------------------------- copies: keys of tile 0, values of tile 0, keys of tile 1, ...
+      load_rows<S>(q_at, &maps.q, f.rows, job.chunk, job.q0, kv_head, batch, q_full);
+      load_rows<S>(do_at, &maps.dout, f.rows, job.chunk, job.q0, kv_head, batch, do_full);
+      int issued = 0, r = 0;
+      for (; issued < 2 * n; issued++) {
+        const int slot = issued % S::kSlots, use = issued / S::kSlots, j = issued / 2;
+        if (use && !barrier_wait(empty + 8 * slot, (use - 1) & 1, &failed)) break;
+        // keys of a tile that is not read as a whole go by way of the mask warp
+        const bool by_masks = !(issued & 1) && partial(j);
+        load_keys<S>(ring_at + slot * S::kTile, issued & 1 ? &maps.v : &maps.k, tile_of(j) * 128, kv_head, batch, by_masks ? landed + 8 * (r % kMaskRing) : full + 8 * slot);
+        r += by_masks;
+      }
+      if (failed) {   // what is under way still lands before the CTA ends
+        for (int i = 0; i < kWaitTries && !(barrier_try(q_full, 0) && barrier_try(do_full, 0)); i++) {}
+        r = 0;
+        for (int k = 0; k < issued; k++) {
+          const bool by_masks = !(k & 1) && partial(k / 2);
+          const uint32_t bar = by_masks ? landed + 8 * (r % kMaskRing) : full + 8 * (k % S::kSlots), parity = (by_masks ? r / kMaskRing : k / S::kSlots) & 1;
+          r += by_masks;
+          if (k < issued - S::kSlots) continue;
+          for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
+        }
+      }
+    } else if (warp == 9 && n) {
+      // -------------------------------------------------- products
+      constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
+      const int steps = (p.head_dim + 15) / 16;
+      const uint32_t queries = low_half(at_address(tile_descriptor(16), q_at)), grads = low_half(at_address(tile_descriptor(16), do_at)),
+                     ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
+      const auto at_slot = [&](uint32_t slot) { return slot * (S::kTile >> 4); };
+      const auto scores = [&](int j, uint32_t slot) {
+        product_of_tiles<kDim>(tmem + 128 * (j & 1), queries, ring + at_slot(slot), kScores, steps);
+        products_done(s_full + 8 * (j & 1));
+      };
+      const auto dp = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem + dp_column, grads, ring + at_slot(slot), kScores, steps);
+        products_done(dp_full);
+        products_done(empty + 8 * slot);
+      };
+      bool going = warp_wait3(q_full, 0, full, 0, 0, 0, &failed);
+      if (going && elected()) scores(0, 0);
+      __syncwarp();
+      going = going && warp_wait3(do_full, 0, full + 8, 0, 0, 0, &failed);
+      if (going && elected()) dp(1);
+      __syncwarp();
+      going = going && (n == 1 || warp_wait(full + 16, 0, &failed));
+      if (going && n > 1 && elected()) scores(1, 2);
+      __syncwarp();
+      if (n == 2) {
+        going = going && warp_wait(full + 24, 0, &failed);
+        if (going && elected()) {
+          product_of_tiles<kDim>(tmem + dq_column, grads, ring + at_slot(3), kScores, steps);
+          products_done(dp2_full);
+        }
+        __syncwarp();
+        going = going && warp_wait(ds_full, 0, &failed);
+        tmem_after_sync();
+        if (going && elected()) {
+          for (int j = 0; j < 2; j++) {
+            product_over_tokens(tmem + dq_column, tmem + 128 * j, ring_tokens + at_slot(2 * j), kResults, j > 0);
+            product_over_tokens(tmem + dq_column, tmem + 128 * j + 64, ring_tokens + at_slot(2 * j) + kHalfTokens, kResults, true);
+          }
+          products_done(done);
+        }
+        __syncwarp();
+      }
+      // one look at barriers between two groups of products: the tensor cores are not far behind the thread that issues them
+      Ring<S::kSlots> k, v, next_k;          // keys of this tile, values of the next, keys of the one after
+      v.next(3);
+      next_k.next(4);
+#pragma unroll 1
+      for (int j = 0; j < n && n != 2 && going; j++) {
+        going = warp_wait3(ds_full, j & 1, j + 1 < n ? full + 8 * v.slot : 0, v.phase, j + 2 < n ? full + 8 * next_k.slot : 0, next_k.phase, &failed);
+        if (!going) break;
+        tmem_after_sync();
+        if (elected()) {
+          if (j + 1 < n) dp(v.slot);
+          const uint32_t ds = tmem + 128 * (j & 1), b = ring_tokens + at_slot(k.slot);
+          product_over_tokens(tmem + dq_column, ds, b, kResults, j > 0);
+          product_over_tokens(tmem + dq_column, ds + 64, b + kHalfTokens, kResults, true);
+          products_done(empty + 8 * k.slot);
+          if (j + 2 < n) scores(j + 2, next_k.slot);   // overwrites dS of tile j after it has been read
+          if (j + 1 == n) products_done(done);
+        }
+        __syncwarp();
+        k.next(2);
+        v.next(2);
+        next_k.next(2);
+      }
+      if (!going) products_end(ended);
+    } else if (warp == 10) {
+      // -------------------------------------------------- masks: zeros where keys are not read by any row
+      int r = 0;
+      for (int j = 0; j < n; j++) {
+        if (!partial(j)) continue;
+        const int item = 2 * j, first = tile_of(j) * 128;
+        if (!warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed)) break;
+        const uint32_t keys = ring_at + item % S::kSlots * S::kTile;
+        for (int row = lane / 8; row < 128; row += 4) {   // 8 lanes a row of 128 bytes
+          const int key = first + row;
+          if (key < all.sinks || (key >= all.from && key < all.to)) continue;
+          for (int x = 0; x < S::kBoxes; x++) store_zeros(keys + x * kBoxBytes + row * 128 + (lane & 7) * 16);
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(full + 8 * (item % S::kSlots));
+        r++;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------------------------------------------- a row belongs to two threads, one for each half of the keys of a tile
+    const int half = warp / 4, row = threadIdx.x & 127;
+    const int token = job.q0 + row / f.rows.heads, in_group = job.chunk * f.rows.heads + row % f.rows.heads, head = kv_head * p.group + in_group;
+    const bool there = row < f.rows.heads * f.rows.tokens && token < p.tokens && in_group < p.group, reads = there && token < seq.fresh;
+    const Reach mine = reads ? reach_of(p, seq, token, token + 1) : Reach{0, 0, 0};
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const int64_t stat = (static_cast<int64_t>(batch) * p.q_heads + head) * p.tokens + token;
+    // a row that reads nothing gets P = 0
+    const float base = reads ? row_base(p.lse[stat]) : -INFINITY;
+    float part = 0, weights = 1;
+    bool going = true;
+    if (n == 1 || n == 2) {
+      weights = 0;
+      const bool single = mine.sinks + mine.to - mine.from == 1;
+      for (int j = 0; j < n && going; j++) {
+        going = warp_wait(s_full + 8 * j, 0, &failed) && warp_wait(j ? dp2_full : dp_full, 0, &failed);
+        if (!going) break;
+        tmem_after_sync();
+        const int first_key = tile_of(j) * 128 + 64 * half;
+        const uint64_t read = bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks);
+        row_sums(tmem + 128 * j + 64 * half + lanes, tmem + (j ? dq_column : dp_column) + 64 * half + lanes, read, single, c, base, &part, &weights);
+      }
+    } else if (reads) {   // delta: this thread's half of the elements
+      const T* o = reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + token * p.out.token + head * p.out.head;
+      const T* g = reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + token * p.dout.token + head * p.dout.head;
+#pragma unroll
+      for (int x = 0; x < kDim / 2; x += 8) {
+        const int at = half * (kDim / 2) + x;
+        if (at < p.head_dim) {
+          const uint4 a = *reinterpret_cast<const uint4*>(o + at), b = *reinterpret_cast<const uint4*>(g + at);
+          const T *u = reinterpret_cast<const T*>(&a), *v = reinterpret_cast<const T*>(&b);
+#pragma unroll
+          for (int i = 0; i < 8; i++) part += static_cast<float>(u[i]) * static_cast<float>(v[i]);
+        }
+      }
+    }
+    delta_parts[0][half][row] = part;
+    delta_parts[1][half][row] = weights;
+    warp_arrive(delta_full, lane);
+    going = warp_wait(delta_full, 0, &failed) && going;
+    float delta = going ? delta_parts[0][0][row] + delta_parts[0][1][row] : 0.0f;
+    if (n <= 2 && going) {
+      weights = delta_parts[1][0][row] + delta_parts[1][1][row];
+      delta = weights == 0 ? 0.0f : delta / weights;
+    }
+    if (p.lse_grad && reads) delta -= p.lse_grad[stat];
+    if (there && half == 0) {
+      f.stats[((static_cast<int64_t>(batch) * p.kv_heads + kv_head) * p.tokens + token) * p.group + in_group] = make_float2(base, delta);
+    }
+    for (int j = 0; j < n && going; j++) {
+      const uint32_t scores_at = tmem + 128 * (j & 1) + 64 * half + lanes;
+      uint32_t s[64];
+      going = warp_wait(s_full + 8 * (j & 1), j / 2 & 1, &failed);
+      if (!going) break;
+      tmem_after_sync();
+      tmem_load<32>(scores_at, s);
+      tmem_load<32>(scores_at + 32, s + 32);
+      tmem_loaded(s);
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        const float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), make_float2(c, c), make_float2(base, base));
+        s[k] = __float_as_uint(exp2_of(x.x));
+        s[k + 1] = __float_as_uint(exp2_of(x.y));
+      }
+      const int first_key = tile_of(j) * 128 + 64 * half;
+      const uint64_t read = bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks);
+      const bool every = __all_sync(~0u, read == ~uint64_t{0});
+      const bool second = n == 2 && j == 1;
+      going = second || warp_wait(dp_full, j & 1, &failed);
+      if (!going) break;
+      tmem_after_sync();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        uint32_t d[32], packed[16];
+        tmem_load<32>(tmem + (second ? dq_column : dp_column) + 64 * half + 32 * i + lanes, d);
+        tmem_loaded(d);
+        if (every) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float2 x = add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-delta, -delta));
+            const float2 y = mul2(x, make_float2(__uint_as_float(s[32 * i + k]), __uint_as_float(s[32 * i + k + 1])));
+            packed[k / 2] = pack2<T>(y.x, y.y);
+          }
+        } else {
+          const uint32_t word = static_cast<uint32_t>(read >> (32 * i));
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float x = word >> k & 1 ? (__uint_as_float(d[k]) - delta) * __uint_as_float(s[32 * i + k]) : 0.0f;
+            const float y = word >> (k + 1) & 1 ? (__uint_as_float(d[k + 1]) - delta) * __uint_as_float(s[32 * i + k + 1]) : 0.0f;
+            packed[k / 2] = pack2<T>(x, y);
+          }
+        }
+        tmem_store<16>(scores_at + 16 * i, packed);
+      }
+      tmem_stored();
+      tmem_before_sync();
+      if (n != 2 || second) warp_arrive(ds_full, lane);
+    }
+    if (n && going) going = warp_wait(done, 0, &failed);
+    if (going) {
+      tmem_after_sync();
+      if (half == 0) stage_row<T, kDim>(tmem + dq_column + lanes, q_at, row, p.scale, n == 0);
+      fence_async_proxy();
+      warp_arrive(staged_full, lane);
+      if (threadIdx.x == 0 && barrier_wait(staged_full, 0, &failed)) {
+        for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(&maps.dq, 64 * x, job.chunk * f.rows.heads, job.q0, kv_head, batch, q_at + x * kBoxBytes);
+        tile_stores_read();
+      }
+    }
+  }
+  __syncwarp();
+  tmem_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_free<512>(tmem);
+  if (failed) {   // not a number, instead of whatever the memory held; the other kernel's results are not valid either
+    const RowJob at = row_job_of(f, block_again());
+    for (int i = threadIdx.x / 32; i < f.rows.tokens * f.rows.heads; i += kThreads / 32) {
+      const int token = at.q0 + i / f.rows.heads, head = at.chunk * f.rows.heads + i % f.rows.heads;
+      if (token >= p.tokens || head >= p.group) continue;
+      uint16_t* to = reinterpret_cast<uint16_t*>(p.dq.data) + at.batch * p.dq.batch + token * p.dq.token + (at.kv_head * p.group + head) * p.dq.head;
+      for (int e = lane; e < p.head_dim; e += 32) to[e] = 0x7fff;
+      if (lane == 0) f.stats[((static_cast<int64_t>(at.batch) * p.kv_heads + at.kv_head) * p.tokens + token) * p.group + head] = make_float2(NAN, NAN);
+    }
+    if (threadIdx.x == 0) *p.status = 1;
+  }
+}
+
+struct KeyJob {
+  int tile, part, kv_head, batch;
+};
+
+// Tiles of first tokens, which have the most rows, first; then in order: without a window the first have the most.
+__device__ __forceinline__ KeyJob key_job_of(const BackwardParams& f, int id) {
+  KeyJob j;
+  j.kv_head = id % f.p.kv_heads;
+  id /= f.p.kv_heads;
+  j.batch = id % f.p.batch;
+  id /= f.p.batch;
+  const int split = f.sink_tiles * f.sink_parts;
+  j.tile = id < split ? id / f.sink_parts : id - split + f.sink_tiles;
+  j.part = id < split ? id % f.sink_parts : 0;
+  return j;
+}
+
+// dV = P^T dO and dK = scale dS^T Q for 128 keys, over the rows that read some of them.  Scores lie the other way round (a key a lane), so
+// that P^T and dS^T are operands as they are.
+template <class T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
+  using S = Sizes<kDim>;
+  const CausalParams& p = f.p;
+  extern __shared__ __align__(1024) uint8_t shared[];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + kRowRing + 1 + 1];
+  __shared__ float4 stats[2][2][32];      // of the rows of a tile: -lse * log2(e), delta
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
+  const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
+  const uint32_t k_full = smem_address(bars), v_full = k_full + 8, full = k_full + 16, empty = full + 8 * S::kSlots,
+                 s_full = empty + 8 * S::kSlots, dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, done = ds_full + 8,
+                 stats_full = done + 8, stats_empty = stats_full + 16, landed = stats_empty + 16, staged_full = landed + 8 * kRowRing, ended = staged_full + 8;
+  const KeyJob job = key_job_of(f, blockIdx.x);
+  const int k0 = job.tile * 128, kv_head = job.kv_head, batch = job.batch, tile_rows = f.rows.tokens * f.rows.heads;
+  const int length = sequence_of<false>(p, batch).fresh;
+
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8, ended}) barrier_init(bar, 1);
+    for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 8);
+    for (const uint32_t bar : {stats_empty, stats_empty + 8}) barrier_init(bar, 8);
+    for (int i = 0; i < S::kSlots; i++) {
+      barrier_init(full + 8 * i, 1);
+      barrier_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kRowRing; i++) barrier_init(landed + 8 * i, 1);
+    barrier_init_done();
+  }
+  // a box may have fewer rows than a tile: the others are summed over too, and no copy writes them
+  for (int i = threadIdx.x; i < (128 - tile_rows) * 8 * S::kBoxes * S::kSlots; i += kThreads) {
+    const int box = i / ((128 - tile_rows) * 8), unit = i % ((128 - tile_rows) * 8);
+    store_zeros(ring_at + box * kBoxBytes + tile_rows * 128 + unit * 16);
+  }
+  fence_async_proxy();
+  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tmem = tmem_slot, dp_column = 128, dv_column = 256, dk_column = 384;   // scores in 0
+  // tiles of rows that read the keys, chunk by chunk: this CTA has `begin` to `begin` + n - 1 of them
+  const int rows_end = k0 < p.sinks || p.window >= length ? length : min(length, k0 + 127 + p.window), first_tile = k0 / f.rows.tokens;
+  const int whole = k0 < length ? ((rows_end + f.rows.tokens - 1) / f.rows.tokens - first_tile) * f.rows.chunks : 0;
+  const bool split = job.tile < f.sink_tiles && f.sink_parts > 1;
+  const int share = split ? (whole + f.sink_parts - 1) / f.sink_parts : whole;
+  const int begin = min(job.part * share, whole), n = min(share, whole - begin);
+  const auto token_of = [&](int i) { return (first_tile + (begin + i) / f.rows.chunks) * f.rows.tokens; };
+  const auto chunk_of = [&](int i) { return (begin + i) % f.rows.chunks; };
+  // a tile in which the sequence ends before the tensor does: rows behind it are cleared
+  const auto partial = [&](int i) { return length < p.tokens && token_of(i) + f.rows.tokens > length; };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 8 && lane == 0 && n) {
+      // -------------------------------------------------- copies: queries of tile 0, their gradients, queries of tile 1, ...
+      load_keys<S>(k_at, &maps.k, k0, kv_head, batch, k_full);
+      load_keys<S>(v_at, &maps.v, k0, kv_head, batch, v_full);
+      int issued = 0, r = 0;
+      for (; issued < 2 * n; issued++) {
+        const int slot = issued % S::kSlots, use = issued / S::kSlots, i = issued / 2;
+        if (issued == S::kSlots) wait_for_kernels_before();   // no slot is free again before
+        if (use && !barrier_wait(empty + 8 * slot, (use - 1) & 1, &failed)) break;
+        const bool by_masks = partial(i);
+        load_rows<S>(ring_at + slot * S::kTile, issued & 1 ? &maps.dout : &maps.q, f.rows, chunk_of(i), token_of(i), kv_head, batch,
+                     by_masks ? landed + 8 * (r % kRowRing) : full + 8 * slot);
+        r += by_masks;
+      }
+      if (failed) {   // what is under way still lands before the CTA ends
+        for (int i = 0; i < kWaitTries && !(barrier_try(k_full, 0) && barrier_try(v_full, 0)); i++) {}
+        r = 0;
+        for (int k = 0; k < issued; k++) {
+          const bool by_masks = partial(k / 2);
+          const uint32_t bar = by_masks ? landed + 8 * (r % kRowRing) : full + 8 * (k % S::kSlots), parity = (by_masks ? r / kRowRing : k / S::kSlots) & 1;
+          r += by_masks;
+          if (k < issued - S::kSlots) continue;
+          for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
+        }
+      }
+    } else if (warp == 9 && n) {
+      // -------------------------------------------------- products
+      constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
+      const int steps = (p.head_dim + 15) / 16;
+      const uint32_t keys = low_half(at_address(tile_descriptor(16), k_at)), values = low_half(at_address(tile_descriptor(16), v_at)),
+                     ring = low_half(at_address(tile_descriptor(16), ring_at)), ring_tokens = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
+      const auto at_slot = [&](uint32_t slot) { return slot * (S::kTile >> 4); };
+      const auto scores = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem, keys, ring + at_slot(slot), kScores, steps);
+        products_done(s_full);
+      };
+      const auto dp = [&](uint32_t slot) {
+        product_of_tiles<kDim>(tmem + dp_column, values, ring + at_slot(slot), kScores, steps);
+        products_done(dp_full);
+      };
+      bool going = warp_wait3(k_full, 0, full, 0, 0, 0, &failed);
+      if (going && elected()) scores(0);
+      __syncwarp();
+      going = going && warp_wait3(v_full, 0, full + 8, 0, 0, 0, &failed);
+      if (going && elected()) dp(1);
+      __syncwarp();
+      wait_for_kernels_before();
+      Ring<S::kSlots> q, g, next_q, next_g;   // queries and their gradients, of this tile and the next
+      g.next();
+      next_q.next(2);
+      next_g.next(3);
+#pragma unroll 1
+      for (int i = 0; i < n && going; i++) {
+        const bool more = i + 1 < n;
+        going = warp_wait3(p_full, i & 1, more ? full + 8 * next_q.slot : 0, next_q.phase, 0, 0, &failed);
+        if (!going) break;
+        tmem_after_sync();
+        if (elected()) {
+          const uint32_t b = ring_tokens + at_slot(g.slot);
+          product_over_tokens(tmem + dv_column, tmem, b, kResults, i > 0);
+          product_over_tokens(tmem + dv_column, tmem + 64, b + kHalfTokens, kResults, true);
+          if (more) scores(next_q.slot);   // overwrites P after it has been read
+          products_done(empty + 8 * g.slot);
+        }
+        __syncwarp();
+        going = warp_wait3(ds_full, i & 1, more ? full + 8 * next_g.slot : 0, next_g.phase, 0, 0, &failed);
+        if (!going) break;
+        tmem_after_sync();
+        if (elected()) {
+          const uint32_t b = ring_tokens + at_slot(q.slot);
+          product_over_tokens(tmem + dk_column, tmem + dp_column, b, kResults, i > 0);
+          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, b + kHalfTokens, kResults, true);
+          if (more) dp(next_g.slot);
+          products_done(empty + 8 * q.slot);
+          if (!more) products_done(done);
+        }
+        __syncwarp();
+        q.next(2);
+        g.next(2);
+        next_q.next(2);
+        next_g.next(2);
+      }
+      if (!going) products_end(ended);
+    } else if (warp == 10) {
+      // -------------------------------------------------- what is known of the rows; -infinity makes P = 0 where there is none
+      wait_for_kernels_before();
+      for (int i = 0; i < n; i++) {
+        const int token = token_of(i), chunk = chunk_of(i);
+        const float2* from = f.stats + ((static_cast<int64_t>(batch) * p.kv_heads + kv_head) * p.tokens + token) * p.group;
+        float* to = reinterpret_cast<float*>(stats[i & 1]);
+        float2 x[4];
+        for (int k = 0; k < 4; k++) {
+          const int row = k * 32 + lane, t = row / f.rows.heads, head = chunk * f.rows.heads + row % f.rows.heads;
+          x[k] = row < tile_rows && token + t < length && head < p.group ? from[static_cast<int64_t>(t) * p.group + head] : make_float2(-INFINITY, 0.0f);
+        }
+        if (i >= 2 && !warp_wait(stats_empty + 8 * (i & 1), (i / 2 - 1) & 1, &failed)) break;
+        for (int k = 0; k < 4; k++) {
+          to[k * 32 + lane] = x[k].x;
+          to[128 + k * 32 + lane] = x[k].y;
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(stats_full + 8 * (i & 1));
+      }
+    } else if (warp == 11) {
+      // -------------------------------------------------- zeros in rows behind the sequence
+      int r = 0;
+      for (int item = 0; item < 2 * n; item++) {
+        const int i = item / 2;
+        if (!partial(i)) continue;
+        if (!warp_wait(landed + 8 * (r % kRowRing), r / kRowRing & 1, &failed)) break;
+        const uint32_t at = ring_at + item % S::kSlots * S::kTile;
+        for (int row = max(length - token_of(i), 0) * f.rows.heads + lane / 8; row < tile_rows; row += 4) {
+          for (int x = 0; x < S::kBoxes; x++) store_zeros(at + x * kBoxBytes + row * 128 + (lane & 7) * 16);
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(full + 8 * (item % S::kSlots));
+        r++;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------------------------------------------- a key belongs to two threads, one for each half of the rows of a tile
+    const int half = warp / 4, row = threadIdx.x & 127, key = k0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const bool there = key < length;
+    const int tokens_end = key < p.sinks || p.window >= length ? length : min(length, key + p.window);   // of the queries that read the key
+    const uint32_t mine = tmem + 64 * half + lanes;
+    bool going = true;
+    wait_for_kernels_before();
+    for (int i = 0; i < n; i++) {
+      uint32_t s[64];
+      going = warp_wait(stats_full + 8 * (i & 1), i / 2 & 1, &failed) && warp_wait(s_full, i & 1, &failed);
+      if (!going) break;
+      tmem_after_sync();
+      tmem_load<32>(mine, s);
+      tmem_load<32>(mine + 32, s + 32);
+      tmem_loaded(s);
+      const float4* lse = stats[i & 1][0] + 16 * half;
+      const float4* delta = stats[i & 1][1] + 16 * half;
+      const int token = token_of(i), lo = min(max(key - token, 0), f.rows.tokens), hi = there ? min(max(tokens_end - token, 0), f.rows.tokens) : 0;
+      // rows beyond a box are zeros with P = 0 by their stats, so a whole tile needs no bits
+      const uint64_t read = bits_of(64 * half, lo * f.rows.heads, hi == f.rows.tokens ? 128 : hi * f.rows.heads);
+      const bool every = __all_sync(~0u, read == ~uint64_t{0});
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        uint32_t packed[16];
+        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 l = lse[8 * x + k / 4];
+          uint32_t* e = s + 32 * x + k;
+          const float2 a = fma2(make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])), make_float2(c, c), make_float2(l.x, l.y));
+          const float2 b = fma2(make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])), make_float2(c, c), make_float2(l.z, l.w));
+          const float v[4] = {exp2_of(a.x), exp2_of(a.y), exp2_of(b.x), exp2_of(b.y)};
+#pragma unroll
+          for (int y = 0; y < 4; y++) e[y] = __float_as_uint(v[y]);
+          if (!every) {
+#pragma unroll
+            for (int y = 0; y < 4; y++) e[y] = word >> (k + y) & 1 ? e[y] : 0u;
+          }
+          packed[k / 2] = pack2<T>(__uint_as_float(e[0]), __uint_as_float(e[1]));
+          packed[k / 2 + 1] = pack2<T>(__uint_as_float(e[2]), __uint_as_float(e[3]));
+        }
+        tmem_store<16>(mine + 16 * x, packed);
+      }
+      tmem_stored();
+      tmem_before_sync();
+      warp_arrive(p_full, lane);
+      going = warp_wait(dp_full, i & 1, &failed);
+      if (!going) break;
+      tmem_after_sync();
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        uint32_t d[32], packed[16];
+        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
+        tmem_load<32>(mine + dp_column + 32 * x, d);
+        tmem_loaded(d);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 l = delta[8 * x + k / 4];
+          const uint32_t* e = s + 32 * x + k;
+          float2 a = mul2(add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-l.x, -l.y)),
+                          make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])));
+          float2 b = mul2(add2(make_float2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), make_float2(-l.z, -l.w)),
+                          make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])));
+          if (!every) {   // not 0 times an infinity
+            a.x = word >> k & 1 ? a.x : 0.0f;
+            a.y = word >> (k + 1) & 1 ? a.y : 0.0f;
+            b.x = word >> (k + 2) & 1 ? b.x : 0.0f;
+            b.y = word >> (k + 3) & 1 ? b.y : 0.0f;
+          }
+          packed[k / 2] = pack2<T>(a.x, a.y);
+          packed[k / 2 + 1] = pack2<T>(b.x, b.y);
+        }
+        tmem_store<16>(mine + dp_column + 16 * x, packed);
+      }
+      warp_arrive(stats_empty + 8 * (i & 1), lane);
+      tmem_stored();
+      tmem_before_sync();
+      warp_arrive(ds_full, lane);
+    }
+    if (n && going) going = warp_wait(done, 0, &failed);
+    if (going && split) {   // the first warpgroup writes dV, the second dK
+      tmem_after_sync();
+      float* to = f.partial + ((((static_cast<int64_t>(job.part) * p.batch + batch) * p.kv_heads + kv_head) * f.sink_tiles + job.tile) * 2 + (half ? 0 : 1)) * 128 * p.head_dim + row * p.head_dim;
+#pragma unroll
+      for (int x = 0; x < kDim; x += 32) {
+        uint32_t o[32] = {};
+        if (n) {
+          tmem_load<32>(tmem + (half ? dk_column : dv_column) + lanes + x, o);
+          tmem_loaded(o);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          if (x + k < p.head_dim) *reinterpret_cast<float4*>(to + x + k) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+        }
+      }
+    } else if (going) {   // the first warpgroup stores dV, the second dK, out of the ring, which is no longer needed
+      tmem_after_sync();
+      const uint32_t staged = ring_at + half * S::kTile;
+      stage_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, staged, row, half ? p.scale : 1.0f, n == 0);
+      if (n && !there) {   // keys behind the sequence get zeros, whatever they are
+#pragma unroll
+        for (int unit = 0; unit < kDim / 8; unit++) store_zeros(staged + unit / 8 * kBoxBytes + row * 128 + ((unit % 8 ^ (row & 7)) * 16));
+      }
+      fence_async_proxy();
+      warp_arrive(staged_full, lane);
+      if (row == 0 && barrier_wait(staged_full, 0, &failed)) {
+        for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(half ? &maps.dk : &maps.dv, 64 * x, k0, kv_head, batch, staged + x * kBoxBytes);
+        tile_stores_read();
+      }
+    }
+  }
+  __syncwarp();
+  tmem_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_free<512>(tmem);
+  if (failed) {
+    const KeyJob at = key_job_of(f, block_again());
+    const int from = at.tile * 128, end = min(from + 128, p.tokens);
+    if (at.tile < f.sink_tiles && f.sink_parts > 1) {
+      float* to = f.partial + (((static_cast<int64_t>(at.part) * p.batch + at.batch) * p.kv_heads + at.kv_head) * f.sink_tiles + at.tile) * 256 * p.head_dim;
+      for (int i = threadIdx.x; i < 256 * p.head_dim; i += kThreads) to[i] = NAN;
+    } else {
+      spoil_rows(p.dk, at.batch, at.kv_head, from, end, p.head_dim);
+      spoil_rows(p.dv, at.batch, at.kv_head, from, end, p.head_dim);
+    }
+    if (threadIdx.x == 0) *p.status = 1;
+  }
+}
+
+// The parts of first tokens' gradients, added in order: a CTA a tile, dk or dv, some of its rows.
+constexpr int kSumRows = 16;
+
 template <class T>
-cudaError_t launch(const CausalParams& p, cudaStream_t stream) {
-  const auto blocks = [&](int heads) { return static_cast<unsigned>((static_cast<int64_t>(p.batch) * heads * p.tokens + kWarps - 1) / kWarps); };
-  causal_dq_kernel<T><<<blocks(p.q_heads), 32 * kWarps, 0, stream>>>(p);
-  causal_dkv_kernel<T><<<blocks(p.kv_heads), 32 * kWarps, 0, stream>>>(p);
-  return cudaGetLastError();
+__global__ void __launch_bounds__(128) causal_sum_kernel(const __grid_constant__ BackwardParams f) {
+  const CausalParams& p = f.p;
+  int id = blockIdx.x;
+  const int rows = id % (128 / kSumRows) * kSumRows;
+  id /= 128 / kSumRows;
+  const int which = id % 2;     // dk, dv
+  id /= 2;
+  const int tile = id % f.sink_tiles, of = id / f.sink_tiles, kv_head = of % p.kv_heads, batch = of / p.kv_heads;
+  const int length = sequence_of<false>(p, batch).fresh;
+  const Heads& out = which ? p.dv : p.dk;
+  const float by = which ? 1.0f : p.scale;
+  const int64_t step = static_cast<int64_t>(p.batch) * p.kv_heads * f.sink_tiles * 256 * p.head_dim;
+  const float* from = f.partial + ((static_cast<int64_t>(of) * f.sink_tiles + tile) * 2 + which) * 128 * p.head_dim;
+  wait_for_kernels_before();
+  for (int i = threadIdx.x; i < kSumRows * p.head_dim / 4; i += 128) {
+    const int row = rows + 4 * i / p.head_dim, e = 4 * i % p.head_dim, key = tile * 128 + row;
+    if (key >= p.tokens) continue;
+    float4 sum = {};
+    if (key < length) {
+      for (int part = 0; part < f.sink_parts; part++) {
+        const float4 x = *reinterpret_cast<const float4*>(from + part * step + row * p.head_dim + e);
+        sum.x += x.x;
+        sum.y += x.y;
+        sum.z += x.z;
+        sum.w += x.w;
+      }
+    }
+    T* to = reinterpret_cast<T*>(out.data) + batch * out.batch + key * out.token + kv_head * out.head + e;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(sum.x * by, sum.y * by), pack2<T>(sum.z * by, sum.w * by));
+  }
+}
+
+template <class... Args>
+cudaError_t launch_behind(void (*kernel)(Args...), int64_t blocks, int threads, int bytes, cudaStream_t stream, std::common_type_t<Args>... args) {
+  // begins while the last CTAs of the kernel before run; what it needs of that one it waits for on the device
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+BackwardParams backward_plan(const CausalParams& p) {
+  BackwardParams f = {};
+  f.p = p;
+  f.rows = row_tiles(p);
+  f.sink_parts = 1;
+  if (p.sinks && p.window < p.tokens) {
+    f.sink_tiles = (std::min(p.sinks, p.tokens) + 127) / 128;
+    // parts as long as the rows of other tiles, and not too short
+    const int64_t others = (static_cast<int64_t>(p.window) + 127) / f.rows.tokens + 2, all = f.rows.tiles;
+    f.sink_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(32, all / std::max<int64_t>(others, 16))));
+  }
+  return f;
+}
+
+size_t stats_bytes(const CausalParams& p) { return (sizeof(float2) * p.batch * p.q_heads * p.tokens + 15) / 16 * 16; }
+
+template <class T, int kDim>
+cudaError_t launch(const BackwardParams& f, const CausalMaps& maps, cudaStream_t stream) {
+  constexpr int bytes = Sizes<kDim>::kShared;
+  const CausalParams& p = f.p;
+  cudaError_t e = allow_shared<causal_dq_kernel<T, kDim>>(bytes, p.device);
+  if (e == cudaSuccess) e = allow_shared<causal_dkv_kernel<T, kDim>>(bytes, p.device);
+  if (e != cudaSuccess) return e;
+  const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.batch;
+  causal_dq_kernel<T, kDim><<<static_cast<unsigned>(heads * f.rows.tiles * f.rows.chunks), kThreads, bytes, stream>>>(f, maps);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  e = launch_behind(causal_dkv_kernel<T, kDim>, heads * ((p.tokens + 127) / 128 + f.sink_tiles * (f.sink_parts - 1)), kThreads, bytes, stream, f, maps);
+  if (e != cudaSuccess || f.sink_parts == 1) return e;
+  return launch_behind(causal_sum_kernel<T>, heads * f.sink_tiles * 2 * (128 / kSumRows), 128, 0, stream, f);
 }
 
 }  // namespace
 
-cudaError_t launch_causal_backward(const CausalParams& p, int dtype, cudaStream_t stream) {
-  return dtype == MLXD_F16 ? launch<__half>(p, stream) : launch<__nv_bfloat16>(p, stream);
+size_t backward_workspace(const CausalParams& p) {
+  const BackwardParams f = backward_plan(p);
+  const size_t partial = f.sink_parts > 1 ? sizeof(float) * f.sink_parts * p.batch * p.kv_heads * f.sink_tiles * 256 * p.head_dim : 0;
+  return stats_bytes(p) + partial;
+}
+
+cudaError_t launch_causal_backward(const CausalParams& p, void* workspace, const CausalMaps& maps, int dtype, cudaStream_t stream) {
+  BackwardParams f = backward_plan(p);
+  f.stats = static_cast<float2*>(workspace);
+  f.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(p));
+  if (dtype == MLXD_F16) return p.head_dim > 64 ? launch<__half, 128>(f, maps, stream) : launch<__half, 64>(f, maps, stream);
+  return p.head_dim > 64 ? launch<__nv_bfloat16, 128>(f, maps, stream) : launch<__nv_bfloat16, 64>(f, maps, stream);
 }
 
 }  // namespace mlxd

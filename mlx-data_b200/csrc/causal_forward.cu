@@ -29,12 +29,6 @@ struct Sizes {
   static constexpr int kShared = (2 + kSlots) * kTile;
 };
 
-// Bits `from` to `to` - 1 of the 64 that begin at `first`.
-__device__ __forceinline__ uint64_t bits_of(int first, int from, int to) {
-  const int lo = max(from - first, 0), hi = min(to - first, 64);
-  return lo < hi ? (~uint64_t{0} >> (64 - (hi - lo))) << lo : 0;
-}
-
 __device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[64]) {
   tmem_load<32>(at, s);
   tmem_load<32>(at + 32, s + 32);

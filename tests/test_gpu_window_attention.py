@@ -251,3 +251,17 @@ def test_refusals(pkg):
     x = q.clone().requires_grad_()
     with pytest.raises(ValueError, match="scale has no gradient"):
         A.window_attention(x, k, v, scale=torch.tensor(0.1, requires_grad=True))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,window", [(1, None), (1, 5), (700, 1)])
+def test_single_keys_have_no_gradient_of_scores(pkg, dtype, tokens, window):
+    """A query that reads one key has the weight 1 whatever the score: dq and dk are exactly 0, and a gradient of lse comes through alone."""
+    A = pkg.attention
+    q, k, v, dout = make(dtype, 3, tokens, 8, 2, 128, seed=2)
+    out, lse = A.window_attention(q, k, v, window=window, return_lse=True)
+    assert torch.equal(out, v.repeat_interleave(4, 2))
+    dq, dk, dv = A.window_attention_backward(dout, q, k, v, out, lse, window=window)
+    assert not dq.any() and not dk.any()
+    want = dout.double().view(3, tokens, 2, 4, 128)
+    ao.within(dv, want.sum(3), co.U[dtype] * 1.01 * want.sum(3).abs() + 8 * co.F32 * want.abs().sum(3) + co.TINY[dtype])
