@@ -42,7 +42,9 @@ struct ForwardParams {
   CausalParams p;
   RowTiles rows;
   int splits;                   // of a sample's keys
-  int halves;                   // a CTA has one tile of rows, whose keys its two halves take tile by tile in turns
+  int steps;                    // few rows, by the kernel for these:
+  int cluster;                  // so many CTAs share a split's keys and join what they have
+  int halves;                   // else: a CTA has one tile of rows, whose keys its two halves take tile by tile in turns
   int parts;                    // splits * (halves ? 2 : 1); 1: results are final
   float* part_out;              // [parts][batch, q_heads, tokens][head_dim]
   float* part_lse;              // [parts][batch, q_heads, tokens]
@@ -55,6 +57,8 @@ struct CausalMaps {
 // Splits and parts of a call, but for where the parts lie.
 ForwardParams forward_plan(const CausalParams& p, bool paged, int sms);
 size_t forward_workspace(const ForwardParams& f);
+cudaError_t launch_causal_step(const ForwardParams& f, int dtype, cudaStream_t stream);
+cudaError_t launch_causal_join(const ForwardParams& f, int dtype, cudaStream_t stream);
 cudaError_t launch_causal_forward(const ForwardParams& f, const CausalMaps& maps, bool paged, int dtype, cudaStream_t stream);
 size_t backward_workspace(const CausalParams& p);
 cudaError_t launch_causal_backward(const CausalParams& p, void* workspace, const CausalMaps& maps, int dtype, cudaStream_t stream);

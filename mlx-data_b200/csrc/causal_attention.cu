@@ -104,15 +104,24 @@ int forward(const char* entry, CausalParams& p, int dtype, bool paged, void* wor
   const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.tokens;
   f.part_out = static_cast<float*>(workspace);
   f.part_lse = f.part_out + (need ? f.parts * rows * p.head_dim : 0);
+  const auto join = [&] {
+    if (f.parts > 1) MLXD_CUDA(launch_causal_join(f, dtype, static_cast<cudaStream_t>(stream)));
+    return static_cast<int>(MLXD_OK);
+  };
+  if (rc != MLXD_OK) return rc;
+  if (f.steps) {
+    MLXD_CUDA(launch_causal_step(f, dtype, static_cast<cudaStream_t>(stream)));
+    return join();
+  }
   CausalMaps maps;
   const int64_t major = paged ? p.cache.pages : p.batch, minor = paged ? p.cache.page_size : p.tokens;
-  if (rc == MLXD_OK) rc = rows_map(entry, p, f.rows, p.q, dtype, &maps.q);
+  rc = rows_map(entry, p, f.rows, p.q, dtype, &maps.q);
   if (rc == MLXD_OK) rc = rows_map(entry, p, f.rows, p.out, dtype, &maps.out);
   if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.k, major, minor, dtype, &maps.k);   // without pages there is nothing to read
   if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.v, major, minor, dtype, &maps.v);
   if (rc != MLXD_OK) return rc;
   MLXD_CUDA(launch_causal_forward(f, maps, paged, dtype, static_cast<cudaStream_t>(stream)));
-  return MLXD_OK;
+  return join();
 }
 
 int cached_params(const char* entry, const mlxd_cached_desc* d, CausalParams& p) {

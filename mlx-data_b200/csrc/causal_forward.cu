@@ -585,9 +585,12 @@ cudaError_t launch(const ForwardParams& f, const CausalMaps& maps, cudaStream_t 
   const int step = f.halves ? 1 : 2;
   const unsigned blocks = static_cast<unsigned>((f.rows.tiles + step - 1) / step) * f.rows.chunks * f.splits * p.kv_heads * p.batch;
   causal_forward_kernel<T, kDim, kPaged><<<blocks, kThreads, bytes, stream>>>(f, maps);
-  if (f.parts == 1) return cudaGetLastError();
-  const cudaError_t launched = cudaGetLastError();
-  if (launched != cudaSuccess) return launched;
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_join(const ForwardParams& f, cudaStream_t stream) {
+  const CausalParams& p = f.p;
   // begins while the parts are being worked out and waits for them on the device
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + kJoinWarps - 1) / kJoinWarps));
@@ -612,8 +615,19 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
   ForwardParams f = {};
   f.p = p;
   f.rows = row_tiles(p);
-  f.halves = paged && f.rows.tiles == 1;
-  f.splits = 1;
+  f.splits = f.cluster = 1;
+  const int64_t sixteens = (static_cast<int64_t>(p.tokens) * p.group + 15) / 16, heads = static_cast<int64_t>(p.batch) * p.kv_heads;
+  f.steps = paged && sixteens <= 1 && heads <= 65535;
+  f.halves = paged && !f.steps && f.rows.tiles == 1;
+  if (f.steps) {
+    int64_t reach = p.cache.capacity;
+    if (p.window != INT32_MAX) reach = std::min(reach, static_cast<int64_t>(p.window) + p.tokens + std::min(p.sinks, p.cache.capacity) + 32);
+    const int64_t rounds = std::max<int64_t>(1, reach / 64);    // of a CTA's four warps
+    while (f.cluster < 8 && heads * f.cluster < 2 * sms && f.cluster * 2 <= rounds) f.cluster *= 2;
+    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(2 * sms / (heads * f.cluster), rounds / (f.cluster * 8))));
+    f.parts = f.splits;
+    return f;
+  }
   const int64_t ctas = static_cast<int64_t>((f.rows.tiles + (f.halves ? 0 : 1)) / (f.halves ? 1 : 2)) * f.rows.chunks * p.batch * p.kv_heads;
   if (paged) {
     // tiles of keys that a CTA may have
@@ -629,6 +643,10 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
 size_t forward_workspace(const ForwardParams& f) {
   const CausalParams& p = f.p;
   return f.parts > 1 ? sizeof(float) * f.parts * p.batch * p.q_heads * p.tokens * (p.head_dim + 1) : 0;
+}
+
+cudaError_t launch_causal_join(const ForwardParams& f, int dtype, cudaStream_t stream) {
+  return dtype == MLXD_F16 ? launch_join<__half>(f, stream) : launch_join<__nv_bfloat16>(f, stream);
 }
 
 cudaError_t launch_causal_forward(const ForwardParams& f, const CausalMaps& maps, bool paged, int dtype, cudaStream_t stream) {
