@@ -38,6 +38,9 @@ inline RowTiles row_tiles(const CausalParams& p) {
   return r;
 }
 
+// CTAs of an SM in the kernel for few rows: eight rows a block.
+constexpr int step_ctas(int dim, int blocks) { return dim > 64 ? (blocks == 1 ? 3 : 2) : (blocks == 1 ? 4 : 3); }
+
 struct ForwardParams {
   CausalParams p;
   RowTiles rows;

@@ -617,14 +617,15 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
   f.rows = row_tiles(p);
   f.splits = f.cluster = 1;
   const int64_t sixteens = (static_cast<int64_t>(p.tokens) * p.group + 15) / 16, heads = static_cast<int64_t>(p.batch) * p.kv_heads;
-  f.steps = paged && sixteens <= 1 && heads <= 65535;
+  f.steps = paged && sixteens <= 1 && p.kv_heads <= 65535 && p.batch * int64_t{64} <= 65535;
   f.halves = paged && !f.steps && f.rows.tiles == 1;
   if (f.steps) {
     int64_t reach = p.cache.capacity;
     if (p.window != INT32_MAX) reach = std::min(reach, static_cast<int64_t>(p.window) + p.tokens + std::min(p.sinks, p.cache.capacity) + 32);
     const int64_t rounds = std::max<int64_t>(1, reach / 64);    // of a CTA's four warps
-    while (f.cluster < 8 && heads * f.cluster < 2 * sms && f.cluster * 2 <= rounds) f.cluster *= 2;
-    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(2 * sms / (heads * f.cluster), rounds / (f.cluster * 8))));
+    const int64_t slots = static_cast<int64_t>(step_ctas(p.head_dim, p.tokens * p.group <= 8 ? 1 : 2)) * sms;
+    while (f.cluster < 8 && 2 * heads * f.cluster <= slots && f.cluster * 2 <= rounds) f.cluster *= 2;
+    f.splits = static_cast<int>(std::max<int64_t>(1, std::min({reach / (f.cluster * 1500), 8 * slots / (heads * f.cluster), int64_t{64}})));
     f.parts = f.splits;
     return f;
   }

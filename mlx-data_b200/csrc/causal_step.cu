@@ -14,7 +14,6 @@ namespace mlxd {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kRows = 16;
 constexpr int kKeys = 16;              // of a warp at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;         // as in the kernel for many queries
@@ -73,48 +72,52 @@ __device__ __forceinline__ float4 remote_float4(uint32_t at) {
   return v;
 }
 
-template <int kDim>
+template <int kDim, int kBlocks>
 struct StepSizes {
   static constexpr int kUnits = kDim / 32;         // 16-byte units of a key that a lane holds
   static constexpr int kHalves = kDim / 64;        // and of a value
-  static constexpr int kStages = kDim == 128 ? 3 : 6;
+  static constexpr int kCtas = step_ctas(kDim, kBlocks);   // of an SM, by registers
+  static constexpr int kStages = (kDim == 128 ? 6 : 12) / kCtas;
   static constexpr int kStage = (2 * kUnits + 4 * kHalves) * 512;   // bytes of a warp's 16 keys and values
   static constexpr int kQueue = kWarps * kStages * kStage;
   // after the keys, in the same place: the warps' sums, then the CTA's
   static constexpr int kStride = kDim + 4;
-  static constexpr int kWarpSums = kWarps * kRows * kStride * 4;
-  static constexpr int kShared = kQueue > kWarpSums + kRows * kStride * 4 ? kQueue : kWarpSums + kRows * kStride * 4;
+  static constexpr int kSums = (kWarps + 1) * 8 * kBlocks * kStride * 4;
+  static constexpr int kShared = kQueue > kSums ? kQueue : kSums;
 };
 
-template <class T, int kDim>
-__global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __grid_constant__ ForwardParams f) {
-  using Z = StepSizes<kDim>;
-  constexpr int kUnits = Z::kUnits, kHalves = Z::kHalves;
+// kBlocks: columns of eight rows.  Scores lie keys by rows, S^T = K Q^T, and results elements by rows, O^T = V^T P^T, so that eight rows (a token
+// of up to eight heads) cost half of what sixteen do.
+template <class T, int kDim, int kBlocks>
+__global__ void __launch_bounds__(32 * kWarps, step_ctas(kDim, kBlocks)) causal_step_kernel(const __grid_constant__ ForwardParams f) {
+  using Z = StepSizes<kDim, kBlocks>;
+  constexpr int kUnits = Z::kUnits, kHalves = Z::kHalves, kRows = 8 * kBlocks;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
   __shared__ Reach reaches[kRows];
   __shared__ float warp_top[kWarps][kRows], warp_total[kWarps][kRows], cta_top[kRows], cta_total[kRows];
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, c = lane & 3;
-  const int kv_head = blockIdx.y % p.kv_heads, batch = blockIdx.y / p.kv_heads, row0 = blockIdx.z * kRows, rows = p.tokens * p.group;
+  // neighbours are the key heads of the same keys, which lie side by side in a page
+  const int kv_head = blockIdx.y, split = blockIdx.z % f.splits, batch = blockIdx.z / f.splits, rows = p.tokens * p.group;
   const Sequence seq = sequence_of<true>(p, batch);
 
-  uint32_t q[2][kUnits][4];            // rows g and 8 + g; lane (g, c) holds the units c, c + 4, ...
+  uint32_t q[kBlocks][kUnits][4];      // rows g, 8 + g; lane (g, c) holds the units c, c + 4, ...
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const int row = row0 + 8 * h + g, token = row / p.group;
+  for (int b = 0; b < kBlocks; b++) {
+    const int row = 8 * b + g, token = row / p.group;
     const T* from = reinterpret_cast<const T*>(p.q.data) + batch * p.q.batch + token * p.q.token + (kv_head * p.group + row % p.group) * p.q.head;
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       const uint4 x = row < rows && 32 * i + 8 * c < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i + 8 * c)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int w = 0; w < 4; w++) q[h][i][w] = word_of(x, w);
+      for (int w = 0; w < 4; w++) q[b][i][w] = word_of(x, w);
     }
   }
 
   // ---------------------------------------------------- what each row reads: eight threads a row
-  {
-    const int row = row0 + threadIdx.x / 8, token = row / p.group;
+  if (threadIdx.x < 8 * kRows) {
+    const int row = threadIdx.x / 8, token = row / p.group;
     const bool reads = row < rows && token < seq.fresh;
     int place = seq.held + token, to = min(place + 1, seq.end);
     if (p.tree) {
@@ -125,14 +128,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
       place = seq.held + others;
       to = min(seq.held, seq.end);
     }
-    if (threadIdx.x % 8 == 0) reaches[threadIdx.x / 8] = reads ? reach_of(p, seq, place, to) : Reach{-1, 0, 0};
+    if (threadIdx.x % 8 == 0) reaches[row] = reads ? reach_of(p, seq, place, to) : Reach{-1, 0, 0};
   }
   __syncthreads();
   // of all rows: what some row reads, and what every row reads
-  Reach all = {0, INT32_MAX, 0}, every = {INT32_MAX, 0, INT32_MAX};
-  const int mine = lane < kRows ? lane : 0;
+  Reach all, every;
   {
-    const Reach r = reaches[mine];
+    const Reach r = reaches[lane % kRows];
     const bool reads = r.sinks >= 0;
     all.sinks = __reduce_max_sync(~0u, reads ? r.sinks : 0);
     all.from = __reduce_min_sync(~0u, reads ? r.from : INT32_MAX);
@@ -140,8 +142,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
     every.sinks = __reduce_min_sync(~0u, reads ? r.sinks : INT32_MAX);
     every.from = __reduce_max_sync(~0u, reads ? r.from : 0);
     every.to = __reduce_min_sync(~0u, reads ? r.to : INT32_MAX);
-    const bool any = __any_sync(~0u, reads);
-    if (any && p.tree) {               // the new tokens are read by the tree alone
+    if (__any_sync(~0u, reads) && p.tree) {   // the new tokens are read by the tree alone
       all.from = min(all.from, min(seq.held, seq.end));
       all.to = seq.end;
     }
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
   const int sink_list = (all.sinks + kKeys - 1) / kKeys, main_first = max(all.from / kKeys, sink_list);
   const int whole = sink_list + (all.to > all.from ? max((all.to + kKeys - 1) / kKeys - main_first, 0) : 0);
   const int shares = f.splits * f.cluster, share = (whole + shares - 1) / shares;
-  const int first = min(static_cast<int>(blockIdx.x) * share, whole), n = min(share, whole - first);
+  const int first = min((split * f.cluster + static_cast<int>(blockIdx.x)) * share, whole), n = min(share, whole - first);
   const auto key_of = [&](int j) { return (j + first < sink_list ? j + first : j + first - sink_list + main_first) * kKeys; };
 
   // ---------------------------------------------------- copies
@@ -162,33 +163,38 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
     return mine < n ? page_of(p.cache, batch, key_of(mine) + 8 * (lane & 1)) : -1;
   };
   const uint32_t queue = smem_address(shared) + warp * Z::kStages * Z::kStage + lane * 16;
-  const T* const key_pool = reinterpret_cast<const T*>(p.k.data) + kv_head * p.k.head;
-  const T* const value_pool = reinterpret_cast<const T*>(p.v.data) + kv_head * p.v.head;
+  // lane (g, c) takes of the keys g and 8 + g the units c, c + 4, ..., of the values 2 c, 2 c + 1, 2 c + 8, 2 c + 9 the units g, g + 8
+  const T* const key_pool = reinterpret_cast<const T*>(p.k.data) + kv_head * p.k.head + g * p.k.token + 8 * c;
+  const T* const value_pool = reinterpret_cast<const T*>(p.v.data) + kv_head * p.v.head + 2 * c * p.v.token + 8 * g;
   int pages = pages_from(warp), next_pages = pages_from(warp + 16 * kWarps), copied = warp, round = 0;
   uint32_t holes = 0;                  // two bits a stage: halves without a page
   const auto copy = [&](int stage) {   // round `copied` of this warp, which may be none
-    const int at = key_of(copied), here = round & 15;
+    const int here = round & 15;
     const int page0 = __shfl_sync(~0u, pages, 2 * here), page1 = __shfl_sync(~0u, pages, 2 * here + 1);
     if (copied < n) {
-      const int row = at & (p.cache.page_size - 1), row1 = (at + 8) & (p.cache.page_size - 1);
+      const int at = key_of(copied), row0 = at & (p.cache.page_size - 1), row1 = (at + 8) & (p.cache.page_size - 1);
       const uint32_t to = queue + stage * Z::kStage;
-      const auto read = [&](int key) { return key < all.sinks || (key >= all.from && key < all.to); };
+      const bool inside = (at >= all.from && at + kKeys <= all.to) || at + kKeys <= all.sinks;   // every key is read by some row
+      const auto read = [&](int key) { return inside || key < all.sinks || (key >= all.from && key < all.to); };
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int page = h ? page1 : page0;
-        const T* from = key_pool + static_cast<int64_t>(max(page, 0)) * p.k.batch + ((h ? row1 : row) + g) * p.k.token + 8 * c;
+        const int page = h ? page1 : page0, row = h ? row1 : row0;
+        const T* const keys = key_pool + max(page, 0) * p.k.batch + row * p.k.token;
+        const T* const values = value_pool + max(page, 0) * p.v.batch + row * p.v.token;
         const bool there = page >= 0 && read(at + 8 * h + g);
 #pragma unroll
-        for (int i = 0; i < kUnits; i++) copy_unit(to + (h * kUnits + i) * 512, there && 32 * i + 8 * c < p.head_dim ? from + 32 * i : key_pool, there && 32 * i + 8 * c < p.head_dim);
-      }
+        for (int i = 0; i < kUnits; i++) {
+          const bool whole = there && 32 * i + 8 * c < p.head_dim;
+          copy_unit(to + (h * kUnits + i) * 512, whole ? keys + 32 * i : key_pool, whole);
+        }
 #pragma unroll
-      for (int h = 0; h < 4; h++) {    // keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9; units g, g + 8
-        const int page = h / 2 ? page1 : page0, key = 2 * c + (h & 1);
-        const T* from = value_pool + static_cast<int64_t>(max(page, 0)) * p.v.batch + ((h / 2 ? row1 : row) + key) * p.v.token + 8 * g;
-        const bool there = page >= 0 && read(at + 8 * (h / 2) + key);
+        for (int e = 0; e < 2; e++) {
+          const bool there = page >= 0 && read(at + 8 * h + 2 * c + e);
 #pragma unroll
-        for (int i = 0; i < kHalves; i++) {
-          copy_unit(to + (2 * kUnits + h * kHalves + i) * 512, there && 64 * i + 8 * g < p.head_dim ? from + 64 * i : value_pool, there && 64 * i + 8 * g < p.head_dim);
+          for (int i = 0; i < kHalves; i++) {
+            const bool whole = there && 64 * i + 8 * g < p.head_dim;
+            copy_unit(to + (2 * kUnits + (2 * h + e) * kHalves + i) * 512, whole ? values + e * p.v.token + 64 * i : value_pool, whole);
+          }
         }
       }
       holes = (holes & ~(3u << (2 * stage))) | (static_cast<uint32_t>((page0 < 0) | (page1 < 0) << 1) << (2 * stage));
@@ -204,21 +210,92 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
   for (int i = 0; i < Z::kStages; i++) copy(i);
 
   const float scale = p.scale * kLog2e;
-  float top[2] = {-INFINITY, -INFINITY}, total[2] = {};
-  float o[kHalves][8][4] = {};
+  float top[kBlocks][2], total[kBlocks][2] = {};   // of rows 2 c, 2 c + 1 (and 8 more)
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) top[b][0] = top[b][1] = -INFINITY;
+  constexpr int kProducts = kDim / 16;
+  float o[kBlocks][kProducts][4] = {};
   int stage = 0;
   for (int j = warp; j < n; j += kWarps) {
     asm volatile("cp.async.wait_group %0;" : : "n"(Z::kStages - 1) : "memory");
     const uint32_t from = queue + stage * Z::kStage;
-    float s[2][4] = {};
+    float s[kBlocks][4] = {}, s2[kBlocks][4] = {};   // keys g (values 0, 1) and 8 + g (2, 3) of rows 2 c, 2 c + 1
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int i = 0; i < kUnits; i++) {
+      const uint4 k0 = shared_unit(from + i * 512), k1 = shared_unit(from + (kUnits + i) * 512);
+      const uint32_t a[4] = {k0.x, k1.x, k0.y, k1.y}, b[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
-      for (int i = 0; i < kUnits; i++) {
-        const uint4 k = shared_unit(from + (h * kUnits + i) * 512);
-        const uint32_t a[4] = {q[0][i][0], q[1][i][0], q[0][i][1], q[1][i][1]}, b[4] = {q[0][i][2], q[1][i][2], q[0][i][3], q[1][i][3]};
-        product16<T>(s[h], a, k.x, k.y);
-        product16<T>(s[h], b, k.z, k.w);
+      for (int x = 0; x < kBlocks; x++) {
+        product16<T>(s[x], a, q[x][i][0], q[x][i][1]);
+        product16<T>(s2[x], b, q[x][i][2], q[x][i][3]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kBlocks; x++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[x][e] += s2[x][e];
+    }
+    const int at = key_of(j);
+    const uint32_t missing = holes >> (2 * stage) & 3;
+    if (missing || !((at >= every.from && at + kKeys <= every.to) || at + kKeys <= every.sinks)) {
+#pragma unroll
+      for (int x = 0; x < kBlocks; x++) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const int row = 8 * x + 2 * c + r;
+          const Reach reach = reaches[row];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int key = at + 8 * h + g;
+            bool read = key < reach.sinks || (key >= reach.from && key < reach.to);
+            if (p.tree && reach.sinks >= 0 && key >= seq.held && key < seq.end) read = p.tree[batch * p.tree_batch + row / p.group * p.tree_token + key - seq.held];
+            if (!read || (missing >> h & 1)) s[x][2 * h + r] = -INFINITY;
+          }
+        }
+      }
+    }
+    // a row's reference is moved where some lane's score has grown by more than 2^8 in weight
+    float now[kBlocks][2];
+    bool grows = false;
+#pragma unroll
+    for (int x = 0; x < kBlocks; x++) {
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        now[x][r] = fmaxf(s[x][r], s[x][2 + r]);
+        grows = grows || (now[x][r] - top[x][r]) * scale > kSlack;
+      }
+    }
+    if (__any_sync(~0u, grows)) {
+#pragma unroll
+      for (int x = 0; x < kBlocks; x++) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          float most = now[x][r];
+          for (int d = 4; d < 32; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+          const bool moves = (most - top[x][r]) * scale > kSlack;   // also from -infinity; not where both are
+          const float keep = moves ? exp2_of((top[x][r] - most) * scale) : 1.0f;
+          top[x][r] = moves ? most : top[x][r];
+          total[x][r] *= keep;
+#pragma unroll
+          for (int i = 0; i < kProducts; i++) {
+            o[x][i][r] *= keep;
+            o[x][i][2 + r] *= keep;
+          }
+        }
+      }
+    }
+    uint32_t w[kBlocks][2];
+#pragma unroll
+    for (int x = 0; x < kBlocks; x++) {
+      const float base[2] = {top[x][0] == -INFINITY ? 0.0f : -top[x][0] * scale, top[x][1] == -INFINITY ? 0.0f : -top[x][1] * scale};
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const float y = exp2_of(fmaf(s[x][2 * h], scale, base[0])), z = exp2_of(fmaf(s[x][2 * h + 1], scale, base[1]));
+        total[x][0] += y;
+        total[x][1] += z;
+        // an operand of the products, so 16 bits (the sum is of the floats), keys by rows to rows by keys
+        const uint32_t packed = pack2<T>(y, z);
+        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w[x][h]) : "r"(packed));
       }
     }
     uint4 v[4][kHalves];
@@ -227,69 +304,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < kHalves; i++) v[h][i] = shared_unit(from + (2 * kUnits + h * kHalves + i) * 512);
     }
-    // a lane has rows g (values 0, 1) and 8 + g (2, 3) of keys 2 c, 2 c + 1 and 8 more
-    const int at = key_of(j);
-    const uint32_t missing = holes >> (2 * stage) & 3;
-    if (missing || !((at >= every.from && at + kKeys <= every.to) || at + kKeys <= every.sinks)) {
+    // Heads of 128: rows g and 8 + g of product i are the elements 8 g + i and 64 + 8 g + i; of 64: 8 g + 2 i and 8 g + 2 i + 1.
 #pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const Reach reach = reaches[8 * r + g];
-        const int token = (row0 + 8 * r + g) / p.group;
+    for (int i = 0; i < kProducts; i++) {
+      const int e0 = kHalves == 2 ? i : 2 * i, e1 = kHalves == 2 ? i : 2 * i + 1;
+      const auto pair = [&](int h, int half, int e) { return __byte_perm(word_of(v[h][half], e / 2), word_of(v[h + 1][half], e / 2), e & 1 ? 0x7632 : 0x5410); };
+      const uint32_t a[4] = {pair(0, 0, e0), pair(0, kHalves - 1, e1), pair(2, 0, e0), pair(2, kHalves - 1, e1)};
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int key = at + 8 * h + 2 * c + e;
-            bool read = key < reach.sinks || (key >= reach.from && key < reach.to);
-            if (p.tree && reach.sinks >= 0 && key >= seq.held && key < seq.end) read = p.tree[batch * p.tree_batch + token * p.tree_token + key - seq.held];
-            if (!read || (missing >> h & 1)) s[h][2 * r + e] = -INFINITY;
-          }
-        }
-      }
-    }
-    uint32_t w[4];
-    float now[2];
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      now[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-      now[r] = fmaxf(now[r], __shfl_xor_sync(~0u, now[r], 1));
-      now[r] = fmaxf(now[r], __shfl_xor_sync(~0u, now[r], 2));
-    }
-    const bool grows0 = (now[0] - top[0]) * scale > kSlack, grows1 = (now[1] - top[1]) * scale > kSlack;
-    if (__any_sync(~0u, grows0 || grows1)) {
-      const float keep[2] = {grows0 ? exp2_of((top[0] - now[0]) * scale) : 1.0f, grows1 ? exp2_of((top[1] - now[1]) * scale) : 1.0f};
-      top[0] = grows0 ? now[0] : top[0];
-      top[1] = grows1 ? now[1] : top[1];
-      total[0] *= keep[0];
-      total[1] *= keep[1];
-#pragma unroll
-      for (int x = 0; x < kHalves; x++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[x][i][e] *= keep[e / 2];
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const float base = top[r] == -INFINITY ? 0.0f : -top[r] * scale;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const float x = exp2_of(fmaf(s[h][2 * r], scale, base)), y = exp2_of(fmaf(s[h][2 * r + 1], scale, base));
-        total[r] += x + y;
-        w[2 * h + r] = pack2<T>(x, y);   // an operand of the products, so 16 bits; the sum is of the floats
-      }
-    }
-    // column n of product (x, i) is element 64 x + 8 n + i
-#pragma unroll
-    for (int x = 0; x < kHalves; x++) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int order = i & 1 ? 0x7632 : 0x5410;
-        product16<T>(o[x][i], w, __byte_perm(word_of(v[0][x], i / 2), word_of(v[1][x], i / 2), order),
-                     __byte_perm(word_of(v[2][x], i / 2), word_of(v[3][x], i / 2), order));
-      }
+      for (int x = 0; x < kBlocks; x++) product16<T>(o[x][i], a, w[x][0], w[x][1]);
     }
     copy(stage);
     stage = stage + 1 == Z::kStages ? 0 : stage + 1;
@@ -301,27 +323,31 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
   float* const warp_out = reinterpret_cast<float*>(shared);
   float* const cta_out = warp_out + kWarps * kRows * Z::kStride;
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    total[r] += __shfl_xor_sync(~0u, total[r], 1);
-    total[r] += __shfl_xor_sync(~0u, total[r], 2);
-    if (c == 0) {
-      warp_top[warp][8 * r + g] = top[r];
-      warp_total[warp][8 * r + g] = total[r];
-    }
+  for (int x = 0; x < kBlocks; x++) {
 #pragma unroll
-    for (int x = 0; x < kHalves; x++) {
+    for (int r = 0; r < 2; r++) {
+      for (int d = 4; d < 32; d *= 2) total[x][r] += __shfl_xor_sync(~0u, total[x][r], d);
+      const int row = 8 * x + 2 * c + r;
+      if (g == 0) {
+        warp_top[warp][row] = top[x][r];
+        warp_total[warp][row] = total[x][r];
+      }
+      float* to = warp_out + (warp * kRows + row) * Z::kStride + 8 * g;
+      if constexpr (kHalves == 2) {
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        float* to = warp_out + (warp * kRows + 8 * r + g) * Z::kStride + 64 * x + 8 * (2 * c + m);
-        *reinterpret_cast<float4*>(to) = make_float4(o[x][0][2 * r + m], o[x][1][2 * r + m], o[x][2][2 * r + m], o[x][3][2 * r + m]);
-        *reinterpret_cast<float4*>(to + 4) = make_float4(o[x][4][2 * r + m], o[x][5][2 * r + m], o[x][6][2 * r + m], o[x][7][2 * r + m]);
+        for (int e = 0; e < 2; e++) {
+          *reinterpret_cast<float4*>(to + 64 * e) = make_float4(o[x][0][2 * e + r], o[x][1][2 * e + r], o[x][2][2 * e + r], o[x][3][2 * e + r]);
+          *reinterpret_cast<float4*>(to + 64 * e + 4) = make_float4(o[x][4][2 * e + r], o[x][5][2 * e + r], o[x][6][2 * e + r], o[x][7][2 * e + r]);
+        }
+      } else {
+        *reinterpret_cast<float4*>(to) = make_float4(o[x][0][r], o[x][0][2 + r], o[x][1][r], o[x][1][2 + r]);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(o[x][2][r], o[x][2][2 + r], o[x][3][r], o[x][3][2 + r]);
       }
     }
   }
   __syncthreads();
   constexpr int kLanes = kDim / 4;     // threads of a row, 4 elements each
-  const int here = min(rows - row0, kRows);
-  for (int i = threadIdx.x; i < here * kLanes; i += 32 * kWarps) {
+  for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
     const int r = i / kLanes, x = i % kLanes * 4;
     float most = warp_top[0][r], sum = 0;
 #pragma unroll
@@ -350,8 +376,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
   else __syncthreads();
   const uint32_t rank = f.cluster > 1 ? cluster_rank() : 0;
   const uint32_t out_at = smem_address(cta_out), top_at = smem_address(cta_top), total_at = smem_address(cta_total);
-  for (int i = rank * 32 * kWarps + threadIdx.x; i < here * kLanes; i += 32 * kWarps * f.cluster) {
-    const int r = i / kLanes, x = i % kLanes * 4, row = row0 + r, token = row / p.group, head = kv_head * p.group + row % p.group;
+  for (int i = rank * 32 * kWarps + threadIdx.x; i < rows * kLanes; i += 32 * kWarps * f.cluster) {
+    const int r = i / kLanes, x = i % kLanes * 4, token = r / p.group, head = kv_head * p.group + r % p.group;
     float most = -INFINITY, sum = 0;
     for (int k = 0; k < f.cluster; k++) most = fmaxf(most, remote_float(of_rank(top_at + 4 * r, k)));
     const float base = most == -INFINITY ? 0.0f : most;
@@ -373,7 +399,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
     const float lse = sum == 0 ? -INFINITY : most * p.scale + logf(sum);
     const int64_t stat = (static_cast<int64_t>(batch) * p.q_heads + head) * p.tokens + token;
     if (f.splits > 1) {
-      const int64_t part = blockIdx.x / f.cluster * static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + stat;
+      const int64_t part = split * static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + stat;
       *reinterpret_cast<float4*>(f.part_out + part * p.head_dim + x) = e;
       if (x == 0) f.part_lse[part] = lse;
     } else {
@@ -385,14 +411,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) causal_step_kernel(const __gri
   if (f.cluster > 1) cluster_meet();   // nobody leaves while others read what it has
 }
 
-template <class T, int kDim>
+template <class T, int kDim, int kBlocks>
 cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
-  constexpr int bytes = StepSizes<kDim>::kShared;
+  constexpr int bytes = StepSizes<kDim, kBlocks>::kShared;
   const CausalParams& p = f.p;
-  const cudaError_t e = allow_shared<causal_step_kernel<T, kDim>>(bytes, p.device);
+  const cudaError_t e = allow_shared<causal_step_kernel<T, kDim, kBlocks>>(bytes, p.device);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(f.splits * f.cluster, p.batch * p.kv_heads, (static_cast<unsigned>(p.tokens) * p.group + kRows - 1) / kRows);
+  config.gridDim = dim3(f.cluster, p.kv_heads, f.splits * p.batch);
   config.blockDim = dim3(32 * kWarps);
   config.dynamicSmemBytes = bytes;
   config.stream = stream;
@@ -402,14 +428,19 @@ cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
   config.numAttrs = f.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&config, causal_step_kernel<T, kDim>, f);
+  return cudaLaunchKernelEx(&config, causal_step_kernel<T, kDim, kBlocks>, f);
+}
+
+template <class T>
+cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
+  if (f.p.tokens * f.p.group <= 8) return f.p.head_dim > 64 ? launch<T, 128, 1>(f, stream) : launch<T, 64, 1>(f, stream);
+  return f.p.head_dim > 64 ? launch<T, 128, 2>(f, stream) : launch<T, 64, 2>(f, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_causal_step(const ForwardParams& f, int dtype, cudaStream_t stream) {
-  if (dtype == MLXD_F16) return f.p.head_dim > 64 ? launch<__half, 128>(f, stream) : launch<__half, 64>(f, stream);
-  return f.p.head_dim > 64 ? launch<__nv_bfloat16, 128>(f, stream) : launch<__nv_bfloat16, 64>(f, stream);
+  return dtype == MLXD_F16 ? launch<__half>(f, stream) : launch<__nv_bfloat16>(f, stream);
 }
 
 }  // namespace mlxd
