@@ -25,8 +25,8 @@ template <int kDim>
 struct Sizes {
   static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
   static constexpr int kBoxes = kDim / 64;
-  static constexpr int kSlots = kDim == 128 ? 5 : 8;       // of the ring of keys and values
-  static constexpr int kShared = (2 + kSlots) * kTile;
+  static constexpr int kSlots = kDim == 128 ? 4 : 8;       // of the ring of keys and values
+  static constexpr int kShared = (3 + kSlots) * kTile;     // and queries of two tiles, results of one
 };
 
 __device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[64]) {
@@ -87,14 +87,30 @@ __device__ __forceinline__ bool warp_wait_all(uint32_t bar0, uint32_t parity0, u
   return (!bar0 || warp_wait(bar0, parity0, failed)) && (!bar1 || warp_wait(bar1, parity1, failed)) && (!bar2 || warp_wait(bar2, parity2, failed));
 }
 
-// What a CTA does: up to two tiles of rows from token q0 on, or one in halves, of a key head's query heads, and which part of the keys.
+// A wait for what comes behind so many tiles, each with limited waits of its own.
+__device__ __forceinline__ bool patient_wait(uint32_t bar, uint32_t parity, int tiles, volatile int* failed) {
+  for (int tile = 0; tile <= tiles; tile++) {
+    for (int i = 0; i < kWaitTries; i++) {
+      if (barrier_try(bar, parity)) return true;
+      if (*failed) return false;
+    }
+  }
+  *failed = 1;
+  return false;
+}
+
+// A job: up to two tiles of rows from token q0 on, or one in halves, of a key head's query heads, and which part of the keys.
 struct Job {
   int q0, chunk, kv_head, batch, split;
 };
 
+__host__ __device__ inline int64_t jobs_of(const ForwardParams& f) {
+  const int step = f.halves ? 1 : 2;
+  return static_cast<int64_t>((f.rows.tiles + step - 1) / step) * f.rows.chunks * f.splits * f.p.kv_heads * f.p.batch;
+}
+
 // The last tiles of rows first: without a window they have the most keys.
-template <class F>
-__device__ __forceinline__ Job job_of(const F& f, int id) {
+__device__ __forceinline__ Job job_of(const ForwardParams& f, int id) {
   const CausalParams& p = f.p;
   const int step = f.halves ? 1 : 2, tiles = (f.rows.tiles + step - 1) / step;
   Job j;
@@ -109,30 +125,96 @@ __device__ __forceinline__ Job job_of(const F& f, int id) {
   return j;
 }
 
+// What is to be done for a job, in tiles of 128 keys: those that its rows read are first ones and then the window's, and the job has n of
+// this list from `first` on.
+struct Work {
+  Job job;
+  Sequence seq;
+  int row_tiles;
+  Reach of[2], all;             // what the rows of each tile read, and of both
+  int sink_tiles, main_first, first, n;
+
+  __device__ __forceinline__ int tile(int j) const { return j + first < sink_tiles ? j + first : j + first - sink_tiles + main_first; }
+
+  // Whether rows that read `r` read some key of tile j.
+  __device__ __forceinline__ bool touches(const Reach& r, int j) const {
+    const int lo = tile(j) * 128;
+    return lo < r.sinks || (lo < r.to && lo + 128 > r.from && r.to > r.from);
+  }
+
+  // Whether values of tile j that no row reads need no clearing: there are none in a cache, or none behind the sequence, whose tensor's end
+  // is zeros by itself.
+  template <bool kPaged>
+  __device__ __forceinline__ bool whole(int j, int tokens) const {
+    const int lo = tile(j) * 128, hi = lo + 128;
+    if (!kPaged) return hi <= seq.end || seq.end == tokens;
+    return hi <= all.sinks || (lo >= all.from && hi <= all.to);
+  }
+};
+
+// `first_place`: with a tree, the first place that the rows of each tile have.
+template <bool kPaged>
+__device__ __forceinline__ Work work_of(const ForwardParams& f, int id, const volatile int* first_place) {
+  const CausalParams& p = f.p;
+  Work w;
+  w.job = job_of(f, id);
+  w.seq = sequence_of<kPaged>(p, w.job.batch);
+  w.row_tiles = f.halves || p.tokens - w.job.q0 <= f.rows.tokens ? 1 : 2;
+  const auto reach_of_tile = [&](int u) {
+    const int first = w.job.q0 + u * f.rows.tokens, end = min(min(first + f.rows.tokens, p.tokens), w.seq.fresh);
+    if (first >= end) return Reach{0, 0, 0};
+    if (!kPaged || !p.tree) return reach_of(p, w.seq, w.seq.held + first, min(w.seq.held + end, w.seq.end));
+    Reach a = reach_of(p, w.seq, first_place[u], w.seq.end);
+    a.from = min(a.from, min(w.seq.held, w.seq.end));   // the new tokens are read by the tree alone
+    a.sinks = min(a.sinks, a.from);
+    return a;
+  };
+  w.of[0] = reach_of_tile(0);
+  w.of[1] = f.halves ? w.of[0] : reach_of_tile(1);
+  // tile 0 begins first, tile 1 ends last, where it reads at all
+  w.all = w.of[0];
+  if (w.of[1].to > w.of[1].from || w.of[1].sinks) {
+    w.all.from = min(w.all.from, w.of[1].from);
+    w.all.to = max(w.all.to, w.of[1].to);
+    w.all.sinks = min(max(w.all.sinks, w.of[1].sinks), w.all.from);
+  }
+  w.sink_tiles = (w.all.sinks + 127) / 128;
+  w.main_first = max(w.all.from / 128, w.sink_tiles);
+  const int whole = w.sink_tiles + (w.all.to > w.all.from ? max((w.all.to + 127) / 128 - w.main_first, 0) : 0);
+  const int share = f.splits == 1 ? whole : (whole + f.splits - 1) / f.splits;
+  w.first = min(w.job.split * share, whole);
+  w.n = min(share, whole - w.first);
+  return w;
+}
+
+// A CTA takes one job after another, every gridDim.x-th: copies and products of the next begin while the results of the one before are
+// written (window attention; a cache has as many CTAs as jobs, since which of its pages are none is found by the whole CTA).
 template <class T, int kDim, bool kPaged>
 __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __grid_constant__ ForwardParams f, const __grid_constant__ CausalMaps maps) {
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2 + 1];
+  __shared__ uint64_t bars[4 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2 + 1 + 1];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ float exchange[2][2][128];   // of a row's two threads: maxima, sums at last
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed, holes, first_place[2];
+  __shared__ int failed, holes, first_place[2], gave_up[2][4];
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
-  const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
-  const uint32_t q_full = smem_address(bars), full = q_full + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
-                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing, ended = staged_full + 16;
-  const Job job = job_of(f, blockIdx.x);
-  const int batch = job.batch, kv_head = job.kv_head, tile_tokens = f.rows.tokens, tile_heads = f.rows.heads;
-  const Sequence seq = sequence_of<kPaged>(p, batch);
+  const uint32_t tiles_at = smem_address(shared), staged = tiles_at + 2 * S::kTile, ring_at = staged + S::kTile;
+  const uint32_t q_full = smem_address(bars), q_empty = q_full + 16, full = q_empty + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
+                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing,
+                 staged_empty = staged_full + 16, ended = staged_empty + 8;
+  const int tile_tokens = f.rows.tokens, tile_heads = f.rows.heads, jobs = static_cast<int>(jobs_of(f));
   if (threadIdx.x == 0) {
     failed = holes = 0;
+    for (int i = 0; i < 8; i++) gave_up[i / 4][i % 4] = 0;
     first_place[0] = first_place[1] = INT32_MAX;
     barrier_init(ended, 1);
+    barrier_init(staged_empty, 1);
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
+      barrier_init(q_empty + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
       barrier_init(p_full + 8 * t, 8);
       barrier_init(o_full + 8 * t, 1);
@@ -153,257 +235,282 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = tmem_slot, o_column = 256;   // scores of tile t in columns 128 t, results in 256 + 128 t
-
-  // ---------------------------------------------------- rows: this thread's, where it is one of the softmax
+  // ---------------------------------------------------- this thread's row, where it is one of the softmax
   const int t = warp / 8, half = warp / 4 % 2, part = warp % 4, row = 32 * part + lane;
-  const int row_token = job.q0 + (f.halves ? 0 : t * tile_tokens) + row / tile_heads, in_group = job.chunk * tile_heads + row % tile_heads;
-  const bool there = warp < 16 && row < tile_heads * tile_tokens && row_token < p.tokens && in_group < p.group;   // the row is in the result
-  const bool reads = there && row_token < seq.fresh;
-  Reach mine = {0, 0, 0};
-  const uint8_t* tree = nullptr;
-  if (reads) {
-    int place = seq.held + row_token, to = min(place + 1, seq.end);
-    if (p.tree) {
-      tree = p.tree + batch * p.tree_batch + row_token * p.tree_token;
-      place = seq.held;
-      to = min(seq.held, seq.end);
-      for (int j = 0; j < seq.fresh; j++) place += j != row_token && tree[j];
-    }
-    mine = reach_of(p, seq, place, to);
-    if (p.tree) atomicMin(&first_place[t], place);
-  }
-  if (p.tree) __syncthreads();
-  // what the rows of tile u read, in tiles of keys: those below `sinks`, and `from` to `to` - 1
-  const auto reach_of_tile = [&](int u) {
-    const int first = job.q0 + (f.halves ? 0 : u * tile_tokens), end = min(min(first + tile_tokens, p.tokens), seq.fresh);
-    if (first >= end) return Reach{0, 0, 0};
-    if (!p.tree) return reach_of(p, seq, seq.held + first, min(seq.held + end, seq.end));
-    Reach a = reach_of(p, seq, first_place[f.halves ? 0 : u], seq.end);
-    a.from = min(a.from, min(seq.held, seq.end));   // the new tokens are read by the tree alone
-    a.sinks = min(a.sinks, a.from);
-    return a;
-  };
-  const int row_tiles = f.halves || p.tokens - job.q0 <= tile_tokens ? 1 : 2;
-  const Reach of_tile[2] = {reach_of_tile(0), f.halves ? reach_of_tile(0) : row_tiles == 2 ? reach_of_tile(1) : Reach{0, 0, 0}};
-  // of the CTA: tile 0 begins first, tile 1 ends last, where it reads at all
-  Reach all = of_tile[0];
-  if (of_tile[1].to > of_tile[1].from || of_tile[1].sinks) {
-    if (all.to > all.from || all.sinks) {
-      all.from = min(all.from, of_tile[1].from);
-      all.to = max(all.to, of_tile[1].to);
-      all.sinks = min(max(all.sinks, of_tile[1].sinks), all.from);
-    } else {
-      all = of_tile[1];
-    }
-  }
-  // the list of tiles of keys: first ones, then the window's; this CTA has `first` to `first` + n - 1 of it
-  const int sink_tiles = (all.sinks + 127) / 128, main_first = max(all.from / 128, sink_tiles), main_end = all.to > all.from ? (all.to + 127) / 128 : 0;
-  const int whole = sink_tiles + max(main_end - main_first, 0), share = (whole + f.splits - 1) / f.splits;
-  const int first = min(job.split * share, whole), n = min(share, whole - first);
-  const auto tile_of = [&](int j) { return j + first < sink_tiles ? j + first : j + first - sink_tiles + main_first; };
-  const auto active = [&](int u, int j) {
-    if (f.halves) return (j & 1) == u;
-    const int tile = tile_of(j);
-    const Reach& r = of_tile[u];
-    return tile * 128 < r.sinks || (tile * 128 < r.to && tile * 128 + 128 > r.from && r.to > r.from);
-  };
-  // a tile whose keys are not all read by some row
-  const auto partial = [&](int j) {
-    const int lo = tile_of(j) * 128, hi = lo + 128;
-    return holes || !(hi <= all.sinks || (lo >= all.from && hi <= all.to));
-  };
-  if (kPaged) {   // pages that are none, among those that are read
-    const int entries = max(128 >> p.cache.page_shift, 1), wide = max(p.cache.page_shift - 7, 0);
-    for (int e = threadIdx.x; e < n * entries; e += kThreads) {
-      const int tile = tile_of(e / entries), entry = entries > 1 ? tile * entries + e % entries : tile >> wide;
-      const int place = max(entry << p.cache.page_shift, tile * 128), end = min((entry + 1) << p.cache.page_shift, tile * 128 + 128);
-      const bool needed = place < all.sinks || (place < all.to && end > all.from);
-      if (needed && (entry >= p.cache.table_width || page_at(p.cache, batch, entry) < 0)) holes = 1;
+  const int row_token = (f.halves ? 0 : t * tile_tokens) + row / tile_heads, row_head = row % tile_heads;
+  int tree_place = 0;
+  if (kPaged && p.tree) {
+    const Job job = job_of(f, blockIdx.x);
+    const Sequence seq = sequence_of<kPaged>(p, job.batch);
+    const int token = job.q0 + row_token;
+    if (warp < 16 && row < tile_heads * tile_tokens && token < seq.fresh) {
+      const uint8_t* tree = p.tree + job.batch * p.tree_batch + token * p.tree_token;
+      tree_place = seq.held;
+      for (int j = 0; j < seq.fresh; j++) tree_place += j != token && tree[j];
+      atomicMin(&first_place[f.halves ? 0 : t], tree_place);
     }
     __syncthreads();
   }
+  if (kPaged) {   // pages that are none, among those that are read
+    const Work w = work_of<kPaged>(f, blockIdx.x, first_place);
+    const int entries = max(128 >> p.cache.page_shift, 1), wide = max(p.cache.page_shift - 7, 0);
+    for (int e = threadIdx.x; e < w.n * entries; e += kThreads) {
+      const int tile = w.tile(e / entries), entry = entries > 1 ? tile * entries + e % entries : tile >> wide;
+      const int place = max(entry << p.cache.page_shift, tile * 128), end = min((entry + 1) << p.cache.page_shift, tile * 128 + 128);
+      const bool needed = place < w.all.sinks || (place < w.all.to && end > w.all.from);
+      if (needed && (entry >= p.cache.table_width || page_at(p.cache, w.job.batch, entry) < 0)) holes = 1;
+    }
+    __syncthreads();
+  }
+  const bool gaps = kPaged && holes;
 
   if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16 && n) {
+    if (warp == 16) {
       // -------------------------------------------------- copies: a lane has a page's box, or all of a tile's; lane 0 waits
-      const int q_tiles = f.halves ? 1 : row_tiles;
-      if (lane == 0) {
-        for (int u = 0; u < q_tiles; u++) {
-          barrier_expect(q_full + 8 * u, S::kBoxes * tile_heads * tile_tokens * 128);
-          for (int x = 0; x < S::kBoxes; x++) {
-            tile_load(tiles_at + u * S::kTile + x * kBoxBytes, &maps.q, 64 * x, job.chunk * tile_heads, job.q0 + u * tile_tokens, kv_head, batch, q_full + 8 * u);
+      const int pages = kPaged ? max(128 >> p.cache.page_shift, 1) : 1, x = lane / pages, page = lane % pages;   // of a tile; this lane's
+      const bool copies = x < S::kBoxes;
+      uint32_t issued = 0, partials = 0, queries[2] = {0, 0}, how = 0;   // how: four bits a slot, which barrier its copy goes to
+      bool going = true;
+      for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
+        const Work w = work_of<kPaged>(f, id, first_place);
+        if (!w.n) continue;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          if (u >= w.row_tiles || !going) break;
+          if (queries[u]) going = warp_wait(q_empty + 8 * u, (queries[u] - 1) & 1, &failed);
+          if (!going) break;
+          if (lane == 0) {
+            barrier_expect(q_full + 8 * u, S::kBoxes * tile_heads * tile_tokens * 128);
+            for (int y = 0; y < S::kBoxes; y++) {
+              tile_load(tiles_at + u * S::kTile + y * kBoxBytes, &maps.q, 64 * y, w.job.chunk * tile_heads, w.job.q0 + u * tile_tokens, w.job.kv_head, w.job.batch, q_full + 8 * u);
+            }
+          }
+          queries[u]++;
+        }
+        const auto major_of = [&](int j) {
+          if (!kPaged) return w.job.batch;
+          const int place = w.tile(j) * 128 + (page << (pages > 1 ? p.cache.page_shift : 0));
+          return j < w.n && copies && place < p.cache.capacity ? page_of(p.cache, w.job.batch, place) : -1;
+        };
+        int major = major_of(0);
+        for (int i = 0; i < 2 * w.n && going; i++) {   // keys of tile 0, values of tile 0, keys of tile 1, ...
+          const int j = i / 2;
+          const uint32_t slot = issued % S::kSlots, use = issued / S::kSlots;
+          if (use) going = warp_wait(empty + 8 * slot, (use - 1) & 1, &failed);
+          if (!going) break;
+          // values of a tile that is not read as a whole go by way of the mask warp
+          const bool by_masks = i & 1 && (gaps || !w.template whole<kPaged>(j, p.tokens));
+          const uint32_t bar = by_masks ? landed + 8 * (partials % kMaskRing) : full + 8 * slot;
+          if (lane == 0) barrier_expect(bar, S::kTile);
+          __syncwarp();
+          how = (how & ~(15u << (4 * slot))) | ((by_masks ? 8 | (partials % (2 * kMaskRing)) : use & 1) << (4 * slot));
+          if (copies) {
+            const int minor = kPaged ? (pages > 1 ? 0 : (w.tile(j) * 128) & (p.cache.page_size - 1)) : w.tile(j) * 128;
+            tile_load(ring_at + slot * S::kTile + x * kBoxBytes + page * (kBoxBytes / pages), i & 1 ? &maps.v : &maps.k, 64 * x, minor, w.job.kv_head, major, bar);
+          }
+          issued++;
+          if (i & 1) {
+            partials += by_masks;
+            major = major_of(j + 1);
           }
         }
       }
-      const int pages = kPaged ? max(128 >> p.cache.page_shift, 1) : 1, x = lane / pages, page = lane % pages;   // of a tile; this lane's
-      const bool copies = x < S::kBoxes;
-      const auto major_of = [&](int j) {
-        if (!kPaged) return batch;
-        const int place = tile_of(j) * 128 + (page << (pages > 1 ? p.cache.page_shift : 0));
-        return j < n && copies && place < p.cache.capacity ? page_of(p.cache, batch, place) : -1;
-      };
-      int issued = 0, partials = 0, major = major_of(0);
-      bool going = true;
-      for (; issued < 2 * n; issued++) {   // keys of tile 0, values of tile 0, keys of tile 1, ...
-        const int slot = issued % S::kSlots, use = issued / S::kSlots, j = issued / 2;
-        if (use) going = warp_wait(empty + 8 * slot, (use - 1) & 1, &failed);
-        if (!going) break;
-        // values of a tile that is not read as a whole go by way of the mask warp
-        const bool by_masks = issued & 1 && partial(j);
-        const uint32_t bar = by_masks ? landed + 8 * (partials % kMaskRing) : full + 8 * slot;
-        if (lane == 0) barrier_expect(bar, S::kTile);
-        __syncwarp();
-        if (copies) {
-          const int minor = kPaged ? (pages > 1 ? 0 : (tile_of(j) * 128) & (p.cache.page_size - 1)) : tile_of(j) * 128;
-          tile_load(ring_at + slot * S::kTile + x * kBoxBytes + page * (kBoxBytes / pages), issued & 1 ? &maps.v : &maps.k, 64 * x, minor, kv_head, major, bar);
-        }
-        if (issued & 1) {
-          partials += by_masks;
-          major = major_of(j + 1);
-        }
-      }
       if (!going && lane == 0) {   // what is under way still lands before the CTA ends
-        for (int u = 0; u < q_tiles; u++) {
-          for (int i = 0; i < kWaitTries && !barrier_try(q_full + 8 * u, 0); i++) {}
+        for (int u = 0; u < 2; u++) {
+          for (int i = 0; queries[u] && i < kWaitTries && !barrier_try(q_full + 8 * u, (queries[u] - 1) & 1); i++) {}
         }
-        int r = 0;
-        for (int k = 0; k < issued; k++) {
-          const bool by_masks = k & 1 && partial(k / 2);
-          const uint32_t bar = by_masks ? landed + 8 * (r % kMaskRing) : full + 8 * (k % S::kSlots);
-          const uint32_t parity = (by_masks ? r / kMaskRing : k / S::kSlots) & 1;
-          r += by_masks;
-          if (k < issued - S::kSlots) continue;
+        for (uint32_t k = 0; k < min(issued, static_cast<uint32_t>(S::kSlots)); k++) {
+          const uint32_t of = how >> (4 * k) & 15;
+          const uint32_t bar = of & 8 ? landed + 8 * (of % kMaskRing) : full + 8 * k, parity = of & 8 ? of / kMaskRing & 1 : of;
           for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
         }
       }
-    } else if (warp == 17 && n) {
+    } else if (warp == 17) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
-      const int steps = (p.head_dim + 15) / 16, users = f.halves ? 2 : row_tiles;
+      const int steps = (p.head_dim + 15) / 16;
       const uint32_t queries = low_half(at_address(tile_descriptor(16), tiles_at)), keys = low_half(at_address(tile_descriptor(16), ring_at)),
                      values = low_half(at_address(tile_descriptor(kBoxBytes), ring_at));
       const auto scores = [&](int u, uint32_t slot) {   // S = Q K^T
         product_of_tiles<kDim>(tmem + 128 * u, queries + (f.halves ? 0 : u * (S::kTile >> 4)), keys + slot * (S::kTile >> 4), kScores, steps);
         products_done(s_full + 8 * u);
       };
-      Ring<S::kSlots> at;                               // the item that is needed next
-      bool going = warp_wait(full, 0, &failed);
-      for (int u = 0; u < users && going; u++) {
-        if (!f.halves || u == 0) going = warp_wait(q_full + 8 * u, 0, &failed);
-        if (going && elected()) {
-          if (active(u, 0)) scores(u, 0);
-          if (u + 1 == users) products_done(empty + 0);
+      Ring<S::kSlots> k;                                // the item that is needed next
+      uint32_t done[2] = {0, 0}, loaded[2] = {0, 0};    // tiles of keys that each tile of rows has taken; its loads of queries
+      bool going = true;
+      for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
+        const Work w = work_of<kPaged>(f, id, first_place);
+        if (!w.n) continue;
+        const int n = w.n, users = f.halves ? 2 : w.row_tiles;
+        const auto active = [&](int u, int j) { return f.halves ? (j & 1) == u : w.touches(w.of[u], j); };
+        int last_of[2] = {n - 1, n - 1};                // each one's last tile of keys
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          while (last_of[u] >= 0 && !active(u, last_of[u])) last_of[u]--;
         }
-        __syncwarp();
-      }
-      at.next();
-      // The tensor cores run a product or two behind the thread that issues them, so between two groups of products there is one
-      // look at barriers and no more: with the last group of a tile of keys, at those of the next one's tiles too.
-      Ring<S::kSlots> v = at, k = at;
-      k.next();
-      going = going && warp_wait_all(full + 8 * v.slot, v.phase, n > 1 ? full + 8 * k.slot : 0, k.phase, 0, 0, &failed);
-      uint32_t done[2] = {0, 0};                        // tiles of keys that each tile of rows has taken
-      int last_of[2] = {n - 1, n - 1};                  // the last one
-      for (int u = 0; u < users; u++) {
-        while (last_of[u] >= 0 && !active(u, last_of[u])) last_of[u]--;
-      }
-#pragma unroll 1
-      for (int j = 0; j < n && going; j++) {
-        Ring<S::kSlots> next_v = k, next_k;
-        next_v.next();
-        next_k = next_v;
-        next_k.next();
+        bool begun[2] = {false, false};
+        going = warp_wait(full + 8 * k.slot, k.phase, &failed);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           if (u >= users || !going) break;
-          // O += P V, P where the scores were, when both halves of the keys have been weighed
-          const uint32_t o = tmem + o_column + 128 * u, values_at = values + v.slot * (S::kTile >> 4);
-          const bool last = u + 1 == users, weighs = active(u, j), more = j + 1 < n && active(u, j + 1);
-          going = warp_wait_all(weighs ? p_full + 8 * u : 0, done[u] & 1, last && j + 1 < n ? full + 8 * next_v.slot : 0, next_v.phase,
-                                last && j + 2 < n ? full + 8 * next_k.slot : 0, next_k.phase, &failed);
-          if (!going) break;
-          tmem_after_sync();
-          if (elected()) {
-            if (weighs) {
-              product_over_tokens(o, tmem + 128 * u, values_at, kResults, done[u] > 0);
-              product_over_tokens(o, tmem + 128 * u + 64, values_at + kHalfTokens, kResults, true);
-              if (j == last_of[u]) products_done(o_full + 8 * u);
-            }
-            if (last) products_done(empty + 8 * v.slot);
-            // products run in the order in which they are issued: these scores overwrite P after it has been read
-            if (more) scores(u, k.slot);
-            if (last && j + 1 < n) products_done(empty + 8 * k.slot);
+          if (!f.halves || u == 0) going = warp_wait(q_full + 8 * u, loaded[u]++ & 1, &failed);
+          if (going && elected()) {
+            if (active(u, 0)) scores(u, k.slot);
+            // without another tile, or with none at all, the queries are no longer needed
+            if (last_of[u] <= 0 && !f.halves) products_done(q_empty + 8 * u);
+            if (u + 1 == users) products_done(empty + 8 * k.slot);
           }
           __syncwarp();
-          done[u] += weighs;
         }
-        v = next_v;
-        k = next_k;
-      }
-      if (!going) products_end(ended);
-    } else if (warp == 19) {
-      // -------------------------------------------------- masks: which keys are read, and zeros where values are not
-      int r = 0;
-      for (int j = 0; j < n; j++) {
-        if (!partial(j)) continue;
-        uint32_t words[4];
-        for (int i = 0; i < 4; i++) {
-          const int key = tile_of(j) * 128 + i * 32 + lane;
-          bool read = key < all.sinks || (key >= all.from && key < all.to);
-          if (kPaged && read && holes) read = page_of(p.cache, batch, key) >= 0;
-          words[i] = __ballot_sync(~0u, read);
-        }
-        const int item = 2 * j + 1;
-        if (!warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed)) break;
-        const uint32_t values = ring_at + item % S::kSlots * S::kTile;
-        for (int i = 0; i < 4; i++) {
-          if (lane == 0) mask_words[r % kMaskRing][i] = words[i];
-          // 8 lanes a row of 128 bytes
-          for (int v = lane / 8; v < 32; v += 4) {
-            if (words[i] >> v & 1) continue;
-            for (int x = 0; x < S::kBoxes; x++) {
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
-                           : : "r"(values + x * kBoxBytes + (32 * i + v) * 128 + (lane & 7) * 16), "r"(0) : "memory");
+        if (!going) break;
+        // The tensor cores run a product or two behind the thread that issues them, so between two groups of products there is one
+        // look at barriers and no more: with the last group of a tile of keys, at those of the next one's tiles too.
+        Ring<S::kSlots> v = k;
+        v.next();
+        k = v;
+        k.next();
+        going = warp_wait_all(full + 8 * v.slot, v.phase, n > 1 ? full + 8 * k.slot : 0, k.phase, 0, 0, &failed);
+#pragma unroll 1
+        for (int j = 0; j < n && going; j++) {
+          Ring<S::kSlots> next_v = k, next_k;
+          next_v.next();
+          next_k = next_v;
+          next_k.next();
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            if (u >= users || !going) break;
+            // O += P V, P where the scores were, when both halves of the keys have been weighed
+            const uint32_t o = tmem + o_column + 128 * u, values_at = values + v.slot * (S::kTile >> 4);
+            const bool last = u + 1 == users, weighs = active(u, j), more = j + 1 < n && active(u, j + 1);
+            going = warp_wait_all(weighs ? p_full + 8 * u : 0, done[u] & 1, last && j + 1 < n ? full + 8 * next_v.slot : 0, next_v.phase,
+                                  last && j + 2 < n ? full + 8 * next_k.slot : 0, next_k.phase, &failed);
+            if (!going) break;
+            tmem_after_sync();
+            if (elected()) {
+              if (weighs) {
+                product_over_tokens(o, tmem + 128 * u, values_at, kResults, begun[u]);
+                product_over_tokens(o, tmem + 128 * u + 64, values_at + kHalfTokens, kResults, true);
+                if (j == last_of[u]) products_done(o_full + 8 * u);
+              }
+              if (last) products_done(empty + 8 * v.slot);
+              // products run in the order in which they are issued: these scores overwrite P after it has been read
+              if (more) scores(u, k.slot);
+              if (j + 1 == last_of[u] && !f.halves) products_done(q_empty + 8 * u);
+              if (last && j + 1 < n) products_done(empty + 8 * k.slot);
             }
+            __syncwarp();
+            done[u] += weighs;
+            begun[u] = begun[u] || weighs;
+          }
+          if (j + 1 < n) {
+            v = next_v;
+            k = next_k;
           }
         }
-        fence_async_proxy();
-        __syncwarp();
-        if (lane == 0) {
-          barrier_arrive(full + 8 * (item % S::kSlots));
-          barrier_arrive(masked + 8 * (r % kMaskRing));
+        // k is the key item of a tile behind the last: the next job's first
+      }
+      if (!going) products_end(ended);
+    } else if (warp == 18 && f.parts == 1 && lane == 0) {
+      // -------------------------------------------------- results: a warp of its own, since a store takes longer than a tile's softmax
+      uint32_t stores[2] = {0, 0};
+      bool going = true;
+      for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
+        const Work w = work_of<kPaged>(f, id, first_place);
+        const Job& job = w.job;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          if (u >= w.row_tiles || !going) break;
+          going = patient_wait(staged_full + 8 * u, stores[u]++ & 1, w.n, &failed);
+          if (!going) break;
+          for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) {
+            tile_store(&maps.out, 64 * x, job.chunk * tile_heads, job.q0 + u * tile_tokens, job.kv_head, job.batch, staged + x * kBoxBytes);
+          }
+          tile_stores_read();
+          barrier_arrive(staged_empty);
         }
-        r++;
+      }
+    } else if (warp == 19) {
+      // -------------------------------------------------- masks: which keys are read, and zeros where values are not
+      uint32_t r = 0, item = 1;                         // partial tiles; values in the ring
+      bool going = true;
+      for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
+        const Work w = work_of<kPaged>(f, id, first_place);
+        for (int j = 0; j < w.n && going; j++, item += 2) {
+          if (!gaps && w.template whole<kPaged>(j, p.tokens)) continue;
+          uint32_t words[4];
+          for (int i = 0; i < 4; i++) {
+            const int key = w.tile(j) * 128 + i * 32 + lane;
+            bool read = kPaged ? key < w.all.sinks || (key >= w.all.from && key < w.all.to) : key < w.seq.end;
+            if (gaps && read) read = page_of(p.cache, w.job.batch, key) >= 0;
+            words[i] = __ballot_sync(~0u, read);
+          }
+          going = warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed);
+          if (!going) break;
+          const uint32_t values = ring_at + item % S::kSlots * S::kTile;
+          for (int i = 0; i < 4; i++) {
+            if (lane == 0) mask_words[r % kMaskRing][i] = words[i];
+            // 8 lanes a row of 128 bytes
+            for (int v = lane / 8; v < 32; v += 4) {
+              if (words[i] >> v & 1) continue;
+              for (int x = 0; x < S::kBoxes; x++) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                             : : "r"(values + x * kBoxBytes + (32 * i + v) * 128 + (lane & 7) * 16), "r"(0) : "memory");
+              }
+            }
+          }
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) {
+            barrier_arrive(full + 8 * (item % S::kSlots));
+            barrier_arrive(masked + 8 * (r % kMaskRing));
+          }
+          r++;
+        }
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ---------------------------------------------------- softmax: a row belongs to two threads, one for each half of the keys of a tile
-    // A wait that ran out does not end the loop: the two warps of a row's threads meet at a barrier for every tile.
+    // A wait that ran out does not end a job: the two warps of a row's threads meet at a barrier for every tile.
     const uint32_t lanes = static_cast<uint32_t>(32 * part) << 16;
     const uint32_t scores_at = tmem + 128 * t + 64 * half + lanes, result = tmem + o_column + 128 * t + half * (kDim / 2) + lanes;
-    if (f.halves || t < row_tiles) {
-      const float c = p.scale * kLog2e;
+    const float c = p.scale * kLog2e;
+    uint32_t done = 0, ends = 0, stagings = 0;   // tiles of keys and jobs of this tile of rows; results of both tiles
+    volatile int* const stop = &gave_up[t][part];
+    for (int id = blockIdx.x; id < jobs; id += gridDim.x) {
+      const Work w = work_of<kPaged>(f, id, first_place);
+      const bool here = f.halves || t < w.row_tiles;
+      const uint32_t staging = stagings + (f.halves ? 0 : t);
+      stagings += w.row_tiles;
+      if (!here) continue;
+      const int token = w.job.q0 + row_token, in_group = w.job.chunk * tile_heads + row_head;
+      const bool there = row < tile_heads * tile_tokens && token < p.tokens && in_group < p.group;   // the row is in the result
+      const bool reads = there && token < w.seq.fresh;
+      const bool tree = kPaged && p.tree;
+      Reach mine = {0, 0, 0};
+      if (reads) mine = tree ? reach_of(p, w.seq, tree_place, min(w.seq.held, w.seq.end)) : reach_of(p, w.seq, w.seq.held + token, min(w.seq.held + token + 1, w.seq.end));
+      const Reach tile_reach = t ? w.of[1] : w.of[0];
       float top = -INFINITY, total = 0;
-      int done = 0;
+      bool begun = false;
 #pragma unroll 1
-      for (int j = 0; j < n; j++) {
-        if (!active(t, j)) continue;
+      for (int j = 0; j < w.n; j++) {
+        if (f.halves ? (j & 1) != t : !w.touches(tile_reach, j)) continue;
         uint32_t s[64];
         warp_wait(s_full + 8 * t, done & 1, &failed);
         tmem_after_sync();
         load_scores(scores_at, s);
-        const int first_key = tile_of(j) * 128 + 64 * half;
+        const int first_key = w.tile(j) * 128 + 64 * half;
         const bool whole_tile = (first_key >= mine.from && first_key + 64 <= mine.to) || first_key + 64 <= mine.sinks;
-        if (!__all_sync(~0u, whole_tile) || holes) {
+        if (!__all_sync(~0u, whole_tile) || gaps) {
           uint64_t read = bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks);
-          if (tree) {
-            for (int k = max(first_key, seq.held); k < min(first_key + 64, seq.end); k++) {
-              if (tree[k - seq.held]) read |= uint64_t{1} << (k - first_key);
+          if (tree && reads) {
+            const uint8_t* of_row = p.tree + w.job.batch * p.tree_batch + token * p.tree_token;
+            for (int k = max(first_key, w.seq.held); k < min(first_key + 64, w.seq.end); k++) {
+              if (of_row[k - w.seq.held]) read |= uint64_t{1} << (k - first_key);
             }
           }
-          if (holes) {
+          if (gaps) {
             warp_wait(masked + 8 * (j % kMaskRing), j / kMaskRing & 1, &failed);
             const uint32_t* words = mask_words[j % kMaskRing] + 2 * half;
             read &= words[0] | static_cast<uint64_t>(words[1]) << 32;
@@ -415,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
         exchange[t][half][row] = now;
         asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");
         now = fmaxf(now, exchange[t][half ^ 1][row]);
-        if (done == 0) {
+        if (!begun) {
           top = now;
         } else {
           const bool grows = (now - top) * c > kSlack;   // also from -infinity; not where both are
@@ -444,66 +551,61 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
         tmem_before_sync();
         warp_arrive(p_full + 8 * t, lane);
         done++;
+        begun = true;
       }
-      const bool valid = !done || warp_wait(o_full + 8 * t, 0, &failed);
+      if (begun && !warp_wait(o_full + 8 * t, ends++ & 1, &failed)) *stop = 1;
+      if (f.parts == 1 && staging && !warp_wait(staged_empty, (staging - 1) & 1, &failed)) *stop = 1;
       exchange[t][half][row] = total;
       asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");
       total += exchange[t][half ^ 1][row];
-      if (valid) {
-        tmem_after_sync();
-        // only a sum of 0 is a row without keys; one that is not a number stays so, in lse too
-        const float by = total == 0 ? 0.0f : 1.0f / total;
-        const float lse = total == 0 ? -INFINITY : top * p.scale + logf(total);
-        const int64_t stat = (static_cast<int64_t>(batch) * p.q_heads + kv_head * p.group + in_group) * p.tokens + row_token;
-        const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.tokens, slot = f.halves ? 2 * job.split + t : job.split;
-        const uint32_t staged = tiles_at + t * S::kTile;   // the queries are no longer needed
-        const bool any = __any_sync(~0u, total != 0);
+      const bool stops = *stop;        // both warps of a row's threads end here, or neither
+      asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");   // the next job writes there
+      if (stops) break;
+      tmem_after_sync();
+      // only a sum of 0 is a row without keys; one that is not a number stays so, in lse too
+      const float by = total == 0 ? 0.0f : 1.0f / total;
+      const float lse = total == 0 ? -INFINITY : top * p.scale + logf(total);
+      const int64_t stat = (static_cast<int64_t>(w.job.batch) * p.q_heads + w.job.kv_head * p.group + in_group) * p.tokens + token;
+      const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.tokens, slot = f.halves ? 2 * w.job.split + t : w.job.split;
 #pragma unroll
-        for (int x = 0; x < kDim / 2; x += 32) {
-          uint32_t o[32] = {};
-          if (done) {
-            tmem_load<32>(result + x, o);
-            tmem_loaded(o);
-          }
-          if (f.parts > 1) {
-            if (there && total != 0) {   // a part without keys is not read when they are joined
-              float* to = f.part_out + (slot * rows + stat) * p.head_dim + half * (kDim / 2) + x;
+      for (int x = 0; x < kDim / 2; x += 32) {
+        uint32_t o[32] = {};
+        if (begun) {
+          tmem_load<32>(result + x, o);
+          tmem_loaded(o);
+        }
+        if (f.parts > 1) {
+          if (there && total != 0) {   // a part without keys is not read when they are joined
+            float* to = f.part_out + (slot * rows + stat) * p.head_dim + half * (kDim / 2) + x;
 #pragma unroll
-              for (int k = 0; k < 32; k += 4) {
-                if (half * (kDim / 2) + x + k < p.head_dim) {
-                  *reinterpret_cast<float4*>(to + k) = make_float4(__uint_as_float(o[k]) * by, __uint_as_float(o[k + 1]) * by, __uint_as_float(o[k + 2]) * by, __uint_as_float(o[k + 3]) * by);
-                }
+            for (int k = 0; k < 32; k += 4) {
+              if (half * (kDim / 2) + x + k < p.head_dim) {
+                *reinterpret_cast<float4*>(to + k) = make_float4(__uint_as_float(o[k]) * by, __uint_as_float(o[k + 1]) * by, __uint_as_float(o[k + 2]) * by, __uint_as_float(o[k + 3]) * by);
               }
             }
-            continue;
           }
+          continue;
+        }
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint32_t w[4];
+        for (int k = 0; k < 32; k += 8) {
+          uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              // what a row without keys has summed is nothing, whatever stands there
-              w[i] = any && total != 0 ? pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by) : 0u;
-            }
-            const int column = half * (kDim / 2) + x + k;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                         : : "r"(staged + column / 64 * kBoxBytes + row * 128 + ((column % 64 / 8 ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          for (int i = 0; i < 4; i++) {
+            // what a row without keys has summed is nothing, whatever stands there
+            v[i] = total != 0 ? pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by) : 0u;
           }
+          const int column = half * (kDim / 2) + x + k;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       : : "r"(staged + column / 64 * kBoxBytes + row * 128 + ((column % 64 / 8 ^ (row & 7)) * 16)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
         }
-        if (half == 0 && there) {
-          if (f.parts > 1) f.part_lse[slot * rows + stat] = lse;
-          else if (p.lse) p.lse[stat] = lse;
-        }
-        if (f.parts == 1) {
-          fence_async_proxy();
-          warp_arrive(staged_full + 8 * t, lane);
-          if (row == 0 && half == 0 && barrier_wait(staged_full + 8 * t, 0, &failed)) {
-            for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) {
-              tile_store(&maps.out, 64 * x, job.chunk * tile_heads, job.q0 + t * tile_tokens, kv_head, batch, staged + x * kBoxBytes);
-            }
-            tile_stores_read();
-          }
-        }
+      }
+      if (half == 0 && there) {
+        if (f.parts > 1) f.part_lse[slot * rows + stat] = lse;
+        else if (p.lse) p.lse[stat] = lse;
+      }
+      if (f.parts == 1) {
+        fence_async_proxy();
+        warp_arrive(staged_full + 8 * t, lane);
       }
     }
   }
@@ -511,23 +613,25 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   tmem_before_sync();
   __syncthreads();
   if (warp == 17) tmem_free<512>(tmem);
-  if (failed) {   // not a number, instead of whatever the memory held
-    const Job at = job_of(f, block_again());
-    const int step = f.halves ? 1 : 2, rows = step * f.rows.tokens * f.rows.heads;
-    for (int i = threadIdx.x / 32; i < rows; i += kThreads / 32) {
-      const int token = at.q0 + i / f.rows.heads, head = at.chunk * f.rows.heads + i % f.rows.heads;
-      if (token >= p.tokens || head >= p.group) continue;
-      const int64_t stat = (static_cast<int64_t>(at.batch) * p.q_heads + at.kv_head * p.group + head) * p.tokens + token;
-      if (f.parts > 1) {
-        for (int u = 0; u < (f.halves ? 2 : 1); u++) {
-          const int64_t part_row = (f.halves ? 2 * at.split + u : at.split) * static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + stat;
-          for (int e = lane; e < p.head_dim; e += 32) f.part_out[part_row * p.head_dim + e] = NAN;
-          if (lane == 0) f.part_lse[part_row] = NAN;
+  if (failed) {   // not a number, instead of whatever the memory held, in all that the CTA was to write
+    for (int id = block_again(); id < jobs; id += gridDim.x) {
+      const Job at = job_of(f, id);
+      const int step = f.halves ? 1 : 2, rows = step * f.rows.tokens * f.rows.heads;
+      for (int i = threadIdx.x / 32; i < rows; i += kThreads / 32) {
+        const int token = at.q0 + i / f.rows.heads, head = at.chunk * f.rows.heads + i % f.rows.heads;
+        if (token >= p.tokens || head >= p.group) continue;
+        const int64_t stat = (static_cast<int64_t>(at.batch) * p.q_heads + at.kv_head * p.group + head) * p.tokens + token;
+        if (f.parts > 1) {
+          for (int u = 0; u < (f.halves ? 2 : 1); u++) {
+            const int64_t part_row = (f.halves ? 2 * at.split + u : at.split) * static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + stat;
+            for (int e = lane; e < p.head_dim; e += 32) f.part_out[part_row * p.head_dim + e] = NAN;
+            if (lane == 0) f.part_lse[part_row] = NAN;
+          }
+        } else {
+          uint16_t* to = reinterpret_cast<uint16_t*>(p.out.data) + at.batch * p.out.batch + token * p.out.token + (at.kv_head * p.group + head) * p.out.head;
+          for (int e = lane; e < p.head_dim; e += 32) to[e] = 0x7fff;
+          if (p.lse && lane == 0) p.lse[stat] = NAN;
         }
-      } else {
-        uint16_t* to = reinterpret_cast<uint16_t*>(p.out.data) + at.batch * p.out.batch + token * p.out.token + (at.kv_head * p.group + head) * p.out.head;
-        for (int e = lane; e < p.head_dim; e += 32) to[e] = 0x7fff;
-        if (p.lse && lane == 0) p.lse[stat] = NAN;
       }
     }
     if (threadIdx.x == 0) *p.status = 1;
@@ -582,9 +686,10 @@ cudaError_t launch(const ForwardParams& f, const CausalMaps& maps, cudaStream_t 
   const CausalParams& p = f.p;
   const cudaError_t e = allow_shared<causal_forward_kernel<T, kDim, kPaged>>(bytes, p.device);
   if (e != cudaSuccess) return e;
-  const int step = f.halves ? 1 : 2;
-  const unsigned blocks = static_cast<unsigned>((f.rows.tiles + step - 1) / step) * f.rows.chunks * f.splits * p.kv_heads * p.batch;
-  causal_forward_kernel<T, kDim, kPaged><<<blocks, kThreads, bytes, stream>>>(f, maps);
+  int sms = 0;
+  if (device_sms(p.device, &sms) != MLXD_OK) return cudaErrorInvalidDevice;
+  const int64_t jobs = jobs_of(f);
+  causal_forward_kernel<T, kDim, kPaged><<<static_cast<unsigned>(kPaged ? jobs : std::min<int64_t>(jobs, sms)), kThreads, bytes, stream>>>(f, maps);
   return cudaGetLastError();
 }
 
