@@ -54,7 +54,7 @@ struct ForwardParams {
 };
 
 struct CausalMaps {
-  CUtensorMap q, k, v, out, dout, dq, dk, dv;   // forward: the first four
+  CUtensorMap q, k, v, dout, dq, dk, dv;   // forward: the first three
 };
 
 // Splits and parts of a call, but for where the parts lie.

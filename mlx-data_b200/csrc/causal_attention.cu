@@ -116,7 +116,6 @@ int forward(const char* entry, CausalParams& p, int dtype, bool paged, void* wor
   CausalMaps maps;
   const int64_t major = paged ? p.cache.pages : p.batch, minor = paged ? p.cache.page_size : p.tokens;
   rc = rows_map(entry, p, f.rows, p.q, dtype, &maps.q);
-  if (rc == MLXD_OK) rc = rows_map(entry, p, f.rows, p.out, dtype, &maps.out);
   if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.k, major, minor, dtype, &maps.k);   // without pages there is nothing to read
   if (rc == MLXD_OK && major) rc = keys_map(entry, p, p.v, major, minor, dtype, &maps.v);
   if (rc != MLXD_OK) return rc;

@@ -25,8 +25,8 @@ template <int kDim>
 struct Sizes {
   static constexpr int kTile = 128 * kDim * 2;             // bytes of 128 tokens
   static constexpr int kBoxes = kDim / 64;
-  static constexpr int kSlots = kDim == 128 ? 4 : 8;       // of the ring of keys and values
-  static constexpr int kShared = (3 + kSlots) * kTile;     // and queries of two tiles, results of one
+  static constexpr int kSlots = kDim == 128 ? 5 : 8;       // of the ring of keys and values
+  static constexpr int kShared = (2 + kSlots) * kTile;     // and queries of two tiles
 };
 
 __device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[64]) {
@@ -87,16 +87,15 @@ __device__ __forceinline__ bool warp_wait_all(uint32_t bar0, uint32_t parity0, u
   return (!bar0 || warp_wait(bar0, parity0, failed)) && (!bar1 || warp_wait(bar1, parity1, failed)) && (!bar2 || warp_wait(bar2, parity2, failed));
 }
 
-// A wait for what comes behind so many tiles, each with limited waits of its own.
-__device__ __forceinline__ bool patient_wait(uint32_t bar, uint32_t parity, int tiles, volatile int* failed) {
-  for (int tile = 0; tile <= tiles; tile++) {
-    for (int i = 0; i < kWaitTries; i++) {
-      if (barrier_try(bar, parity)) return true;
-      if (*failed) return false;
-    }
+// 16 packed elements of a row, 32 bytes: one store where they start on such a boundary, so that whole sectors are written.
+__device__ __forceinline__ void store_row_part(void* to, const uint32_t (&v)[8], int units) {
+  if (units >= 2 && reinterpret_cast<uintptr_t>(to) % 32 == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 : : "l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    return;
   }
-  *failed = 1;
-  return false;
+  if (units >= 1) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+  if (units >= 2) *(reinterpret_cast<uint4*>(to) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
 }
 
 // A job: up to two tiles of rows from token q0 on, or one in halves, of a key head's query heads, and which part of the keys.
@@ -194,31 +193,28 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[4 + 2 * S::kSlots + 6 + 2 * kMaskRing + 2 + 1 + 1];
+  __shared__ uint64_t bars[4 + 2 * S::kSlots + 6 + 2 * kMaskRing + 1];
   __shared__ uint32_t mask_words[kMaskRing][4];
   __shared__ float exchange[2][2][128];   // of a row's two threads: maxima, sums at last
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, holes, first_place[2], gave_up[2][4];
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
-  const uint32_t tiles_at = smem_address(shared), staged = tiles_at + 2 * S::kTile, ring_at = staged + S::kTile;
+  const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + 2 * S::kTile;
   const uint32_t q_full = smem_address(bars), q_empty = q_full + 16, full = q_empty + 16, empty = full + 8 * S::kSlots, s_full = empty + 8 * S::kSlots,
-                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, staged_full = landed + 8 * kMaskRing,
-                 staged_empty = staged_full + 16, ended = staged_empty + 8;
+                 p_full = s_full + 16, o_full = p_full + 16, masked = o_full + 16, landed = masked + 8 * kMaskRing, ended = landed + 8 * kMaskRing;
   const int tile_tokens = f.rows.tokens, tile_heads = f.rows.heads, jobs = static_cast<int>(jobs_of(f));
   if (threadIdx.x == 0) {
     failed = holes = 0;
     for (int i = 0; i < 8; i++) gave_up[i / 4][i % 4] = 0;
     first_place[0] = first_place[1] = INT32_MAX;
     barrier_init(ended, 1);
-    barrier_init(staged_empty, 1);
     for (int t = 0; t < 2; t++) {
       barrier_init(q_full + 8 * t, 1);
       barrier_init(q_empty + 8 * t, 1);
       barrier_init(s_full + 8 * t, 1);
       barrier_init(p_full + 8 * t, 8);
       barrier_init(o_full + 8 * t, 1);
-      barrier_init(staged_full + 8 * t, 8);
     }
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
@@ -411,25 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
         // k is the key item of a tile behind the last: the next job's first
       }
       if (!going) products_end(ended);
-    } else if (warp == 18 && f.parts == 1 && lane == 0) {
-      // -------------------------------------------------- results: a warp of its own, since a store takes longer than a tile's softmax
-      uint32_t stores[2] = {0, 0};
-      bool going = true;
-      for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
-        const Work w = work_of<kPaged>(f, id, first_place);
-        const Job& job = w.job;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          if (u >= w.row_tiles || !going) break;
-          going = patient_wait(staged_full + 8 * u, stores[u]++ & 1, w.n, &failed);
-          if (!going) break;
-          for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) {
-            tile_store(&maps.out, 64 * x, job.chunk * tile_heads, job.q0 + u * tile_tokens, job.kv_head, job.batch, staged + x * kBoxBytes);
-          }
-          tile_stores_read();
-          barrier_arrive(staged_empty);
-        }
-      }
     } else if (warp == 19) {
       // -------------------------------------------------- masks: which keys are read, and zeros where values are not
       uint32_t r = 0, item = 1;                         // partial tiles; values in the ring
@@ -476,14 +453,11 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
     const uint32_t lanes = static_cast<uint32_t>(32 * part) << 16;
     const uint32_t scores_at = tmem + 128 * t + 64 * half + lanes, result = tmem + o_column + 128 * t + half * (kDim / 2) + lanes;
     const float c = p.scale * kLog2e;
-    uint32_t done = 0, ends = 0, stagings = 0;   // tiles of keys and jobs of this tile of rows; results of both tiles
+    uint32_t done = 0, ends = 0;       // tiles of keys and jobs of this tile of rows
     volatile int* const stop = &gave_up[t][part];
     for (int id = blockIdx.x; id < jobs; id += gridDim.x) {
       const Work w = work_of<kPaged>(f, id, first_place);
-      const bool here = f.halves || t < w.row_tiles;
-      const uint32_t staging = stagings + (f.halves ? 0 : t);
-      stagings += w.row_tiles;
-      if (!here) continue;
+      if (!f.halves && t >= w.row_tiles) continue;
       const int token = w.job.q0 + row_token, in_group = w.job.chunk * tile_heads + row_head;
       const bool there = row < tile_heads * tile_tokens && token < p.tokens && in_group < p.group;   // the row is in the result
       const bool reads = there && token < w.seq.fresh;
@@ -554,7 +528,6 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
         begun = true;
       }
       if (begun && !warp_wait(o_full + 8 * t, ends++ & 1, &failed)) *stop = 1;
-      if (f.parts == 1 && staging && !warp_wait(staged_empty, (staging - 1) & 1, &failed)) *stop = 1;
       exchange[t][half][row] = total;
       asm volatile("bar.sync %0, 64;" : : "r"(1 + 4 * t + part) : "memory");
       total += exchange[t][half ^ 1][row];
@@ -586,26 +559,22 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
           }
           continue;
         }
+        T* const to = reinterpret_cast<T*>(p.out.data) + w.job.batch * p.out.batch + token * p.out.token + (w.job.kv_head * p.group + in_group) * p.out.head;
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          uint32_t v[4];
+        for (int k = 0; k < 32; k += 16) {
+          uint32_t v[8];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
+          for (int i = 0; i < 8; i++) {
             // what a row without keys has summed is nothing, whatever stands there
             v[i] = total != 0 ? pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by) : 0u;
           }
           const int column = half * (kDim / 2) + x + k;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                       : : "r"(staged + column / 64 * kBoxBytes + row * 128 + ((column % 64 / 8 ^ (row & 7)) * 16)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+          if (there) store_row_part(to + column, v, (p.head_dim - column) / 8);
         }
       }
       if (half == 0 && there) {
         if (f.parts > 1) f.part_lse[slot * rows + stat] = lse;
         else if (p.lse) p.lse[stat] = lse;
-      }
-      if (f.parts == 1) {
-        fence_async_proxy();
-        warp_arrive(staged_full + 8 * t, lane);
       }
     }
   }
