@@ -54,7 +54,7 @@ struct ForwardParams {
 };
 
 struct CausalMaps {
-  CUtensorMap q, k, v, dout, dq, dk, dv;   // forward: the first three
+  CUtensorMap q, k, v, dout;   // forward: the first three
 };
 
 // Splits and parts of a call, but for where the parts lie.
@@ -87,6 +87,17 @@ __device__ __forceinline__ Sequence sequence_of(const CausalParams& p, int b) {
 __device__ __forceinline__ uint64_t bits_of(int first, int from, int to) {
   const int lo = max(from - first, 0), hi = min(to - first, 64);
   return lo < hi ? (~uint64_t{0} >> (64 - (hi - lo))) << lo : 0;
+}
+
+// 16 packed elements of a row, 32 bytes: one store where they start on such a boundary, so that whole sectors are written.
+__device__ __forceinline__ void store_row_part(void* to, const uint32_t (&v)[8], int units) {
+  if (units >= 2 && reinterpret_cast<uintptr_t>(to) % 32 == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 : : "l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    return;
+  }
+  if (units >= 1) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+  if (units >= 2) *(reinterpret_cast<uint4*>(to) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
 }
 
 // What a query reads: keys below `sinks`, and those from `from` to `to` - 1; with a tree those of its row behind `to`.

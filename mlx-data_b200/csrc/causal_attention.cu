@@ -185,8 +185,8 @@ int window_call(const char* entry, int device, void* stream, const mlxd_window_d
   rc = status_word(device, &p.status);
   const RowTiles rows = row_tiles(p);
   CausalMaps maps;
-  const struct { const Heads* h; bool query; CUtensorMap* map; } all[] = {{&p.q, true, &maps.q},   {&p.dout, true, &maps.dout}, {&p.dq, true, &maps.dq}, {&p.k, false, &maps.k},
-                                                                          {&p.v, false, &maps.v}, {&p.dk, false, &maps.dk},    {&p.dv, false, &maps.dv}};
+  const struct { const Heads* h; bool query; CUtensorMap* map; } all[] = {
+      {&p.q, true, &maps.q}, {&p.dout, true, &maps.dout}, {&p.k, false, &maps.k}, {&p.v, false, &maps.v}};
   for (const auto& x : all) {
     if (rc == MLXD_OK) rc = x.query ? rows_map(entry, p, rows, *x.h, d->dtype, x.map) : keys_map(entry, p, *x.h, p.batch, p.tokens, d->dtype, x.map);
   }

@@ -12,7 +12,7 @@ namespace mlxd {
 
 namespace {
 
-constexpr int kThreads = 384;          // two warpgroups for what lies between the products, then warps for copies, products, helpers
+constexpr int kThreads = 640;          // four warpgroups for what lies between the products, then warps for copies, products, helpers
 constexpr int kMaskRing = 4;           // queries: tiles of keys in the ring are no more
 constexpr int kRowRing = 8;            // keys: items in the ring are no more
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,32 +51,49 @@ __device__ __forceinline__ void store_zeros(uint32_t at) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" : : "r"(at), "r"(0) : "memory");
 }
 
-// The accumulators of a row, scaled, rounded and put where a store of the tile finds them; zeros where there are none.
-template <class T, int kDim>
-__device__ __forceinline__ void stage_row(uint32_t tmem, uint32_t to, int row, float by, bool none) {
+// Elements `from` to `from` + kCount - 1 of a row of accumulators, scaled, rounded and written; zeros where there are none.
+template <class T, int kCount>
+__device__ __forceinline__ void write_row(uint32_t tmem, T* to, int from, int dim, float by, bool there, bool none) {
 #pragma unroll
-  for (int x = 0; x < kDim; x += 32) {
-    uint32_t o[32] = {};
+  for (int x = 0; x < kCount; x += 16) {
+    uint32_t o[16], v[8] = {};
     if (!none) {
-      tmem_load<32>(tmem + x, o);
+      tmem_load<16>(tmem + from + x, o);
       tmem_loaded(o);
-    }
 #pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = pack2<T>(__uint_as_float(o[k + 2 * i]) * by, __uint_as_float(o[k + 2 * i + 1]) * by);
-      const int unit = (x + k) % 64 / 8;
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                   : : "r"(to + (x + k) / 64 * kBoxBytes + row * 128 + ((unit ^ (row & 7)) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      for (int i = 0; i < 8; i++) v[i] = pack2<T>(__uint_as_float(o[2 * i]) * by, __uint_as_float(o[2 * i + 1]) * by);
     }
+    if (there) store_row_part(to + from + x, v, (dim - from - x) / 8);
   }
 }
 
-// Of a row and this thread's half of a tile of keys: sums of P dP and of P, over the keys that are read.  Scores and dP stay where they are.
-__device__ __forceinline__ void row_sums(uint32_t scores_at, uint32_t dp_at, uint64_t read, bool single, float c, float base, float* sum, float* weights) {
+// The same where some rows are zeros: those for which `sums` is false.
+template <class T, int kCount>
+__device__ __forceinline__ void write_row_or_zeros(uint32_t tmem, T* to, int from, int dim, float by, bool there, bool sums, bool none) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int x = 0; x < kCount; x += 16) {
+    uint32_t o[16], v[8] = {};
+    if (!none) {
+      tmem_load<16>(tmem + from + x, o);
+      tmem_loaded(o);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = sums ? pack2<T>(__uint_as_float(o[2 * i]) * by, __uint_as_float(o[2 * i + 1]) * by) : 0u;
+    }
+    if (there) store_row_part(to + from + x, v, (dim - from - x) / 8);
+  }
+}
+
+// D (+)= A B over 128 tokens: A 128 x 128 in tensor memory, 16 columns of every 32, as the four threads of a row leave it; B a tile.
+__device__ __forceinline__ void product_over_quarters(uint32_t d, uint32_t a, uint32_t b, uint32_t how, bool add) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) product_from_tmem(d, a + 32 * (k / 2) + 8 * (k % 2), b + (2048 * k >> 4), how, add || k > 0);
+}
+
+// Of a row and this thread's quarter of a tile of keys: sums of P dP and of P, over the keys that are read.  Scores and dP stay where they
+// are.
+__device__ __forceinline__ void row_sums(uint32_t scores_at, uint32_t dp_at, uint32_t read, bool single, float c, float base, float* sum, float* weights) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
     uint32_t s[16], d[16];
     tmem_load<16>(scores_at + 16 * i, s);
     tmem_load<16>(dp_at + 16 * i, d);
@@ -122,8 +139,8 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 5 + kMaskRing + 1 + 1];
-  __shared__ float delta_parts[2][2][128];   // of a row's two threads: sums, and with few keys those of weights
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 2 + 5 + kMaskRing + 1];
+  __shared__ float delta_parts[4][128];   // of a row's four threads
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   asm volatile("griddepcontrol.launch_dependents;");   // the other kernel's CTAs take the SMs that these leave
@@ -131,14 +148,14 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 16, ds_full = dp_full + 8, done = ds_full + 8, delta_full = done + 8,
-                 dp2_full = delta_full + 8, landed = dp2_full + 8, staged_full = landed + 8 * kMaskRing, ended = staged_full + 8;
+                 dp2_full = delta_full + 8, landed = dp2_full + 8, ended = landed + 8 * kMaskRing;
   const RowJob job = row_job_of(f, blockIdx.x);
   const int batch = job.batch, kv_head = job.kv_head;
   const Sequence seq = sequence_of<false>(p, batch);
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, dp2_full, done, ended}) barrier_init(bar, 1);
-    for (const uint32_t bar : {ds_full, delta_full, staged_full}) barrier_init(bar, 8);
+    for (const uint32_t bar : {ds_full, delta_full}) barrier_init(bar, 16);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
       barrier_init(empty + 8 * i, 1);
@@ -146,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
     for (int i = 0; i < kMaskRing; i++) barrier_init(landed + 8 * i, 1);
     barrier_init_done();
   }
-  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  if (warp == 17) tmem_alloc<512>(smem_address(&tmem_slot));
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
@@ -162,9 +179,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
     return !(hi <= all.sinks || (lo >= all.from && hi <= all.to));
   };
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    if (warp == 8 && lane == 0 && n) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16 && lane == 0 && n) {
       // -------------------------------------------------- copies: keys of tile 0, values of tile 0, keys of tile 1, ...
       load_rows<S>(q_at, &maps.q, f.rows, job.chunk, job.q0, kv_head, batch, q_full);
       load_rows<S>(do_at, &maps.dout, f.rows, job.chunk, job.q0, kv_head, batch, do_full);
@@ -188,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
           for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
         }
       }
-    } else if (warp == 9 && n) {
+    } else if (warp == 17 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
@@ -224,8 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         tmem_after_sync();
         if (going && elected()) {
           for (int j = 0; j < 2; j++) {
-            product_over_tokens(tmem + dq_column, tmem + 128 * j, ring_tokens + at_slot(2 * j), kResults, j > 0);
-            product_over_tokens(tmem + dq_column, tmem + 128 * j + 64, ring_tokens + at_slot(2 * j) + kHalfTokens, kResults, true);
+            product_over_quarters(tmem + dq_column, tmem + 128 * j, ring_tokens + at_slot(2 * j), kResults, j > 0);
           }
           products_done(done);
         }
@@ -242,9 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         tmem_after_sync();
         if (elected()) {
           if (j + 1 < n) dp(v.slot);
-          const uint32_t ds = tmem + 128 * (j & 1), b = ring_tokens + at_slot(k.slot);
-          product_over_tokens(tmem + dq_column, ds, b, kResults, j > 0);
-          product_over_tokens(tmem + dq_column, ds + 64, b + kHalfTokens, kResults, true);
+          product_over_quarters(tmem + dq_column, tmem + 128 * (j & 1), ring_tokens + at_slot(k.slot), kResults, j > 0);
           products_done(empty + 8 * k.slot);
           if (j + 2 < n) scores(j + 2, next_k.slot);   // overwrites dS of tile j after it has been read
           if (j + 1 == n) products_done(done);
@@ -255,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         next_k.next(2);
       }
       if (!going) products_end(ended);
-    } else if (warp == 10) {
+    } else if (warp == 18) {
       // -------------------------------------------------- masks: zeros where keys are not read by any row
       int r = 0;
       for (int j = 0; j < n; j++) {
@@ -275,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---------------------------------------------------- a row belongs to two threads, one for each half of the keys of a tile
-    const int half = warp / 4, row = threadIdx.x & 127;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---------------------------------------------------- a row belongs to four threads, one for each quarter of the keys of a tile
+    const int quarter = warp / 4, row = threadIdx.x & 127;
     const int token = job.q0 + row / f.rows.heads, in_group = job.chunk * f.rows.heads + row % f.rows.heads, head = kv_head * p.group + in_group;
     const bool there = row < f.rows.heads * f.rows.tokens && token < p.tokens && in_group < p.group, reads = there && token < seq.fresh;
     const Reach mine = reads ? reach_of(p, seq, token, token + 1) : Reach{0, 0, 0};
@@ -295,16 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         going = warp_wait(s_full + 8 * j, 0, &failed) && warp_wait(j ? dp2_full : dp_full, 0, &failed);
         if (!going) break;
         tmem_after_sync();
-        const int first_key = tile_of(j) * 128 + 64 * half;
-        const uint64_t read = bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks);
-        row_sums(tmem + 128 * j + 64 * half + lanes, tmem + (j ? dq_column : dp_column) + 64 * half + lanes, read, single, c, base, &part, &weights);
+        const int first_key = tile_of(j) * 128 + 32 * quarter;
+        const uint32_t read = static_cast<uint32_t>(bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks));
+        row_sums(tmem + 128 * j + 32 * quarter + lanes, tmem + (j ? dq_column : dp_column) + 32 * quarter + lanes, read, single, c, base, &part, &weights);
       }
-    } else if (reads) {   // delta: this thread's half of the elements
+    } else if (reads) {   // delta: this thread's quarter of the elements
       const T* o = reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + token * p.out.token + head * p.out.head;
       const T* g = reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + token * p.dout.token + head * p.dout.head;
 #pragma unroll
-      for (int x = 0; x < kDim / 2; x += 8) {
-        const int at = half * (kDim / 2) + x;
+      for (int x = 0; x < kDim / 4; x += 8) {
+        const int at = quarter * (kDim / 4) + x;
         if (at < p.head_dim) {
           const uint4 a = *reinterpret_cast<const uint4*>(o + at), b = *reinterpret_cast<const uint4*>(g + at);
           const T *u = reinterpret_cast<const T*>(&a), *v = reinterpret_cast<const T*>(&b);
@@ -313,64 +327,60 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         }
       }
     }
-    delta_parts[0][half][row] = part;
-    delta_parts[1][half][row] = weights;
+    // with few keys the sums of weights too, in the ring's last place, which these do not reach
+    float(*const weight_parts)[128] = reinterpret_cast<float(*)[128]>(shared + (1 + S::kSlots) * S::kTile);
+    delta_parts[quarter][row] = part;
+    if (n <= 2) weight_parts[quarter][row] = weights;
     warp_arrive(delta_full, lane);
     going = warp_wait(delta_full, 0, &failed) && going;
-    float delta = going ? delta_parts[0][0][row] + delta_parts[0][1][row] : 0.0f;
+    const auto of_row = [&](const float(*parts)[128]) { return (parts[0][row] + parts[1][row]) + (parts[2][row] + parts[3][row]); };
+    float delta = going ? of_row(delta_parts) : 0.0f;
     if (n <= 2 && going) {
-      weights = delta_parts[1][0][row] + delta_parts[1][1][row];
+      weights = of_row(weight_parts);
       delta = weights == 0 ? 0.0f : delta / weights;
     }
     if (p.lse_grad && reads) delta -= p.lse_grad[stat];
-    if (there && half == 0) {
+    if (there && quarter == 0) {
       f.stats[((static_cast<int64_t>(batch) * p.kv_heads + kv_head) * p.tokens + token) * p.group + in_group] = make_float2(base, delta);
     }
     for (int j = 0; j < n && going; j++) {
-      const uint32_t scores_at = tmem + 128 * (j & 1) + 64 * half + lanes;
-      uint32_t s[64];
+      const uint32_t scores_at = tmem + 128 * (j & 1) + 32 * quarter + lanes;
+      uint32_t s[32], d[32], packed[16];
       going = warp_wait(s_full + 8 * (j & 1), j / 2 & 1, &failed);
       if (!going) break;
       tmem_after_sync();
       tmem_load<32>(scores_at, s);
-      tmem_load<32>(scores_at + 32, s + 32);
       tmem_loaded(s);
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
+      for (int k = 0; k < 32; k += 2) {
         const float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), make_float2(c, c), make_float2(base, base));
         s[k] = __float_as_uint(exp2_of(x.x));
         s[k + 1] = __float_as_uint(exp2_of(x.y));
       }
-      const int first_key = tile_of(j) * 128 + 64 * half;
-      const uint64_t read = bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks);
-      const bool every = __all_sync(~0u, read == ~uint64_t{0});
+      const int first_key = tile_of(j) * 128 + 32 * quarter;
+      const uint32_t read = static_cast<uint32_t>(bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks));
       const bool second = n == 2 && j == 1;
       going = second || warp_wait(dp_full, j & 1, &failed);
       if (!going) break;
       tmem_after_sync();
+      tmem_load<32>(tmem + (second ? dq_column : dp_column) + 32 * quarter + lanes, d);
+      tmem_loaded(d);
+      if (__all_sync(~0u, read == ~0u)) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        uint32_t d[32], packed[16];
-        tmem_load<32>(tmem + (second ? dq_column : dp_column) + 64 * half + 32 * i + lanes, d);
-        tmem_loaded(d);
-        if (every) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float2 x = add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-delta, -delta));
-            const float2 y = mul2(x, make_float2(__uint_as_float(s[32 * i + k]), __uint_as_float(s[32 * i + k + 1])));
-            packed[k / 2] = pack2<T>(y.x, y.y);
-          }
-        } else {
-          const uint32_t word = static_cast<uint32_t>(read >> (32 * i));
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float x = word >> k & 1 ? (__uint_as_float(d[k]) - delta) * __uint_as_float(s[32 * i + k]) : 0.0f;
-            const float y = word >> (k + 1) & 1 ? (__uint_as_float(d[k + 1]) - delta) * __uint_as_float(s[32 * i + k + 1]) : 0.0f;
-            packed[k / 2] = pack2<T>(x, y);
-          }
+        for (int k = 0; k < 32; k += 2) {
+          const float2 x = add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-delta, -delta));
+          const float2 y = mul2(x, make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])));
+          packed[k / 2] = pack2<T>(y.x, y.y);
         }
-        tmem_store<16>(scores_at + 16 * i, packed);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float x = read >> k & 1 ? (__uint_as_float(d[k]) - delta) * __uint_as_float(s[k]) : 0.0f;
+          const float y = read >> (k + 1) & 1 ? (__uint_as_float(d[k + 1]) - delta) * __uint_as_float(s[k + 1]) : 0.0f;
+          packed[k / 2] = pack2<T>(x, y);
+        }
       }
+      tmem_store<16>(scores_at, packed);
       tmem_stored();
       tmem_before_sync();
       if (n != 2 || second) warp_arrive(ds_full, lane);
@@ -378,19 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
     if (n && going) going = warp_wait(done, 0, &failed);
     if (going) {
       tmem_after_sync();
-      if (half == 0) stage_row<T, kDim>(tmem + dq_column + lanes, q_at, row, p.scale, n == 0);
-      fence_async_proxy();
-      warp_arrive(staged_full, lane);
-      if (threadIdx.x == 0 && barrier_wait(staged_full, 0, &failed)) {
-        for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(&maps.dq, 64 * x, job.chunk * f.rows.heads, job.q0, kv_head, batch, q_at + x * kBoxBytes);
-        tile_stores_read();
-      }
+      T* const to = reinterpret_cast<T*>(p.dq.data) + batch * p.dq.batch + token * p.dq.token + head * p.dq.head;
+      write_row<T, kDim / 4>(tmem + dq_column + lanes, to, quarter * (kDim / 4), p.head_dim, p.scale, there, n == 0);
     }
   }
   __syncwarp();
   tmem_before_sync();
   __syncthreads();
-  if (warp == 9) tmem_free<512>(tmem);
+  if (warp == 17) tmem_free<512>(tmem);
   if (failed) {   // not a number, instead of whatever the memory held; the other kernel's results are not valid either
     const RowJob at = row_job_of(f, block_again());
     for (int i = threadIdx.x / 32; i < f.rows.tokens * f.rows.heads; i += kThreads / 32) {
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
-  __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + kRowRing + 1 + 1];
+  __shared__ uint64_t bars[2 + 2 * S::kSlots + 5 + 4 + kRowRing + 1];
   __shared__ float4 stats[2][2][32];      // of the rows of a tile: -lse * log2(e), delta
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
   const uint32_t k_full = smem_address(bars), v_full = k_full + 8, full = k_full + 16, empty = full + 8 * S::kSlots,
                  s_full = empty + 8 * S::kSlots, dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, done = ds_full + 8,
-                 stats_full = done + 8, stats_empty = stats_full + 16, landed = stats_empty + 16, staged_full = landed + 8 * kRowRing, ended = staged_full + 8;
+                 stats_full = done + 8, stats_empty = stats_full + 16, landed = stats_empty + 16, ended = landed + 8 * kRowRing;
   const KeyJob job = key_job_of(f, blockIdx.x);
   const int k0 = job.tile * 128, kv_head = job.kv_head, batch = job.batch, tile_rows = f.rows.tokens * f.rows.heads;
   const int length = sequence_of<false>(p, batch).fresh;
@@ -445,8 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8, ended}) barrier_init(bar, 1);
-    for (const uint32_t bar : {p_full, ds_full, staged_full}) barrier_init(bar, 8);
-    for (const uint32_t bar : {stats_empty, stats_empty + 8}) barrier_init(bar, 8);
+    for (const uint32_t bar : {p_full, ds_full, stats_empty, stats_empty + 8}) barrier_init(bar, 16);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
       barrier_init(empty + 8 * i, 1);
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
     store_zeros(ring_at + box * kBoxBytes + tile_rows * 128 + unit * 16);
   }
   fence_async_proxy();
-  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
+  if (warp == 17) tmem_alloc<512>(smem_address(&tmem_slot));
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
@@ -476,9 +480,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   // a tile in which the sequence ends before the tensor does: rows behind it are cleared
   const auto partial = [&](int i) { return length < p.tokens && token_of(i) + f.rows.tokens > length; };
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    if (warp == 8 && lane == 0 && n) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16 && lane == 0 && n) {
       // -------------------------------------------------- copies: queries of tile 0, their gradients, queries of tile 1, ...
       load_keys<S>(k_at, &maps.k, k0, kv_head, batch, k_full);
       load_keys<S>(v_at, &maps.v, k0, kv_head, batch, v_full);
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
           for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
         }
       }
-    } else if (warp == 9 && n) {
+    } else if (warp == 17 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
@@ -536,9 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          const uint32_t b = ring_tokens + at_slot(g.slot);
-          product_over_tokens(tmem + dv_column, tmem, b, kResults, i > 0);
-          product_over_tokens(tmem + dv_column, tmem + 64, b + kHalfTokens, kResults, true);
+          product_over_quarters(tmem + dv_column, tmem, ring_tokens + at_slot(g.slot), kResults, i > 0);
           if (more) scores(next_q.slot);   // overwrites P after it has been read
           products_done(empty + 8 * g.slot);
         }
@@ -547,9 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          const uint32_t b = ring_tokens + at_slot(q.slot);
-          product_over_tokens(tmem + dk_column, tmem + dp_column, b, kResults, i > 0);
-          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, b + kHalfTokens, kResults, true);
+          product_over_quarters(tmem + dk_column, tmem + dp_column, ring_tokens + at_slot(q.slot), kResults, i > 0);
           if (more) dp(next_g.slot);
           products_done(empty + 8 * q.slot);
           if (!more) products_done(done);
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         next_g.next(2);
       }
       if (!going) products_end(ended);
-    } else if (warp == 10) {
+    } else if (warp == 18) {
       // -------------------------------------------------- what is known of the rows; -infinity makes P = 0 where there is none
       wait_for_kernels_before();
       for (int i = 0; i < n; i++) {
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) barrier_arrive(stats_full + 8 * (i & 1));
       }
-    } else if (warp == 11) {
+    } else if (warp == 19) {
       // -------------------------------------------------- zeros in rows behind the sequence
       int r = 0;
       for (int item = 0; item < 2 * n; item++) {
@@ -599,124 +599,106 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---------------------------------------------------- a key belongs to two threads, one for each half of the rows of a tile
-    const int half = warp / 4, row = threadIdx.x & 127, key = k0 + row;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---------------------------------------------------- a key belongs to four threads, one for each quarter of the rows of a tile
+    const int quarter = warp / 4, row = threadIdx.x & 127, key = k0 + row;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const float c = p.scale * kLog2e;
     const bool there = key < length;
     const int tokens_end = key < p.sinks || p.window >= length ? length : min(length, key + p.window);   // of the queries that read the key
-    const uint32_t mine = tmem + 64 * half + lanes;
+    const uint32_t mine = tmem + 32 * quarter + lanes;
     bool going = true;
     wait_for_kernels_before();
     for (int i = 0; i < n; i++) {
-      uint32_t s[64];
+      uint32_t s[32], d[32], packed[16];
       going = warp_wait(stats_full + 8 * (i & 1), i / 2 & 1, &failed) && warp_wait(s_full, i & 1, &failed);
       if (!going) break;
       tmem_after_sync();
       tmem_load<32>(mine, s);
-      tmem_load<32>(mine + 32, s + 32);
       tmem_loaded(s);
-      const float4* lse = stats[i & 1][0] + 16 * half;
-      const float4* delta = stats[i & 1][1] + 16 * half;
+      const float4* lse = stats[i & 1][0] + 8 * quarter;
+      const float4* delta = stats[i & 1][1] + 8 * quarter;
       const int token = token_of(i), lo = min(max(key - token, 0), f.rows.tokens), hi = there ? min(max(tokens_end - token, 0), f.rows.tokens) : 0;
       // rows beyond a box are zeros with P = 0 by their stats, so a whole tile needs no bits
-      const uint64_t read = bits_of(64 * half, lo * f.rows.heads, hi == f.rows.tokens ? 128 : hi * f.rows.heads);
-      const bool every = __all_sync(~0u, read == ~uint64_t{0});
+      const uint32_t read = static_cast<uint32_t>(bits_of(32 * quarter, lo * f.rows.heads, hi == f.rows.tokens ? 128 : hi * f.rows.heads));
+      const bool every = __all_sync(~0u, read == ~0u);
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-        uint32_t packed[16];
-        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
+      for (int k = 0; k < 32; k += 4) {
+        const float4 l = lse[k / 4];
+        uint32_t* e = s + k;
+        const float2 a = fma2(make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])), make_float2(c, c), make_float2(l.x, l.y));
+        const float2 b = fma2(make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])), make_float2(c, c), make_float2(l.z, l.w));
+        const float v[4] = {exp2_of(a.x), exp2_of(a.y), exp2_of(b.x), exp2_of(b.y)};
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 l = lse[8 * x + k / 4];
-          uint32_t* e = s + 32 * x + k;
-          const float2 a = fma2(make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])), make_float2(c, c), make_float2(l.x, l.y));
-          const float2 b = fma2(make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])), make_float2(c, c), make_float2(l.z, l.w));
-          const float v[4] = {exp2_of(a.x), exp2_of(a.y), exp2_of(b.x), exp2_of(b.y)};
-#pragma unroll
-          for (int y = 0; y < 4; y++) e[y] = __float_as_uint(v[y]);
-          if (!every) {
-#pragma unroll
-            for (int y = 0; y < 4; y++) e[y] = word >> (k + y) & 1 ? e[y] : 0u;
-          }
-          packed[k / 2] = pack2<T>(__uint_as_float(e[0]), __uint_as_float(e[1]));
-          packed[k / 2 + 1] = pack2<T>(__uint_as_float(e[2]), __uint_as_float(e[3]));
-        }
-        tmem_store<16>(mine + 16 * x, packed);
+        for (int y = 0; y < 4; y++) e[y] = every || (read >> (k + y) & 1) ? __float_as_uint(v[y]) : 0u;
+        packed[k / 2] = pack2<T>(__uint_as_float(e[0]), __uint_as_float(e[1]));
+        packed[k / 2 + 1] = pack2<T>(__uint_as_float(e[2]), __uint_as_float(e[3]));
       }
+      tmem_store<16>(mine, packed);
       tmem_stored();
       tmem_before_sync();
       warp_arrive(p_full, lane);
       going = warp_wait(dp_full, i & 1, &failed);
       if (!going) break;
       tmem_after_sync();
+      tmem_load<32>(mine + dp_column, d);
+      tmem_loaded(d);
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-        uint32_t d[32], packed[16];
-        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
-        tmem_load<32>(mine + dp_column + 32 * x, d);
-        tmem_loaded(d);
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 l = delta[8 * x + k / 4];
-          const uint32_t* e = s + 32 * x + k;
-          float2 a = mul2(add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-l.x, -l.y)),
-                          make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])));
-          float2 b = mul2(add2(make_float2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), make_float2(-l.z, -l.w)),
-                          make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])));
-          if (!every) {   // not 0 times an infinity
-            a.x = word >> k & 1 ? a.x : 0.0f;
-            a.y = word >> (k + 1) & 1 ? a.y : 0.0f;
-            b.x = word >> (k + 2) & 1 ? b.x : 0.0f;
-            b.y = word >> (k + 3) & 1 ? b.y : 0.0f;
-          }
-          packed[k / 2] = pack2<T>(a.x, a.y);
-          packed[k / 2 + 1] = pack2<T>(b.x, b.y);
+      for (int k = 0; k < 32; k += 4) {
+        const float4 l = delta[k / 4];
+        const uint32_t* e = s + k;
+        float2 a = mul2(add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-l.x, -l.y)),
+                        make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])));
+        float2 b = mul2(add2(make_float2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), make_float2(-l.z, -l.w)),
+                        make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])));
+        if (!every) {   // not 0 times an infinity
+          a.x = read >> k & 1 ? a.x : 0.0f;
+          a.y = read >> (k + 1) & 1 ? a.y : 0.0f;
+          b.x = read >> (k + 2) & 1 ? b.x : 0.0f;
+          b.y = read >> (k + 3) & 1 ? b.y : 0.0f;
         }
-        tmem_store<16>(mine + dp_column + 16 * x, packed);
+        packed[k / 2] = pack2<T>(a.x, a.y);
+        packed[k / 2 + 1] = pack2<T>(b.x, b.y);
       }
+      tmem_store<16>(mine + dp_column, packed);
       warp_arrive(stats_empty + 8 * (i & 1), lane);
       tmem_stored();
       tmem_before_sync();
       warp_arrive(ds_full, lane);
     }
     if (n && going) going = warp_wait(done, 0, &failed);
-    if (going && split) {   // the first warpgroup writes dV, the second dK
+    // the first two warpgroups write dV, the others dK, half of the elements each
+    const bool is_k = quarter / 2, none = n == 0;
+    const int from = quarter % 2 * (kDim / 2);
+    const uint32_t sums = tmem + (is_k ? dk_column : dv_column) + lanes;
+    if (going && split) {
       tmem_after_sync();
-      float* to = f.partial + ((((static_cast<int64_t>(job.part) * p.batch + batch) * p.kv_heads + kv_head) * f.sink_tiles + job.tile) * 2 + (half ? 0 : 1)) * 128 * p.head_dim + row * p.head_dim;
+      float* to = f.partial + ((((static_cast<int64_t>(job.part) * p.batch + batch) * p.kv_heads + kv_head) * f.sink_tiles + job.tile) * 2 + (is_k ? 0 : 1)) * 128 * p.head_dim + row * p.head_dim;
 #pragma unroll
-      for (int x = 0; x < kDim; x += 32) {
-        uint32_t o[32] = {};
-        if (n) {
-          tmem_load<32>(tmem + (half ? dk_column : dv_column) + lanes + x, o);
+      for (int x = 0; x < kDim / 2; x += 16) {
+        uint32_t o[16] = {};
+        if (!none) {
+          tmem_load<16>(sums + from + x, o);
           tmem_loaded(o);
         }
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          if (x + k < p.head_dim) *reinterpret_cast<float4*>(to + x + k) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+        for (int k = 0; k < 16; k += 4) {
+          if (from + x + k < p.head_dim) *reinterpret_cast<float4*>(to + from + x + k) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
         }
       }
-    } else if (going) {   // the first warpgroup stores dV, the second dK, out of the ring, which is no longer needed
+    } else if (going) {
       tmem_after_sync();
-      const uint32_t staged = ring_at + half * S::kTile;
-      stage_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, staged, row, half ? p.scale : 1.0f, n == 0);
-      if (n && !there) {   // keys behind the sequence get zeros, whatever they are
-#pragma unroll
-        for (int unit = 0; unit < kDim / 8; unit++) store_zeros(staged + unit / 8 * kBoxBytes + row * 128 + ((unit % 8 ^ (row & 7)) * 16));
-      }
-      fence_async_proxy();
-      warp_arrive(staged_full, lane);
-      if (row == 0 && barrier_wait(staged_full, 0, &failed)) {
-        for (int x = 0; x < S::kBoxes && 64 * x < p.head_dim; x++) tile_store(half ? &maps.dk : &maps.dv, 64 * x, k0, kv_head, batch, staged + x * kBoxBytes);
-        tile_stores_read();
-      }
+      const Heads& out = is_k ? p.dk : p.dv;
+      T* const to = reinterpret_cast<T*>(out.data) + batch * out.batch + key * out.token + kv_head * out.head;
+      // keys behind the sequence get zeros, whatever they are; their accumulators are zeros but for what is not a number
+      if (__all_sync(~0u, there)) write_row<T, kDim / 2>(sums, to, from, p.head_dim, is_k ? p.scale : 1.0f, true, none);
+      else write_row_or_zeros<T, kDim / 2>(sums, to, from, p.head_dim, is_k ? p.scale : 1.0f, key < p.tokens, there && !none, none);
     }
   }
   __syncwarp();
   tmem_before_sync();
   __syncthreads();
-  if (warp == 9) tmem_free<512>(tmem);
+  if (warp == 17) tmem_free<512>(tmem);
   if (failed) {
     const KeyJob at = key_job_of(f, block_again());
     const int from = at.tile * 128, end = min(from + 128, p.tokens);

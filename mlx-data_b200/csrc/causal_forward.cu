@@ -87,17 +87,6 @@ __device__ __forceinline__ bool warp_wait_all(uint32_t bar0, uint32_t parity0, u
   return (!bar0 || warp_wait(bar0, parity0, failed)) && (!bar1 || warp_wait(bar1, parity1, failed)) && (!bar2 || warp_wait(bar2, parity2, failed));
 }
 
-// 16 packed elements of a row, 32 bytes: one store where they start on such a boundary, so that whole sectors are written.
-__device__ __forceinline__ void store_row_part(void* to, const uint32_t (&v)[8], int units) {
-  if (units >= 2 && reinterpret_cast<uintptr_t>(to) % 32 == 0) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 : : "l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-    return;
-  }
-  if (units >= 1) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-  if (units >= 2) *(reinterpret_cast<uint4*>(to) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
-}
-
 // A job: up to two tiles of rows from token q0 on, or one in halves, of a key head's query heads, and which part of the keys.
 struct Job {
   int q0, chunk, kv_head, batch, split;
@@ -338,8 +327,46 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
       for (int id = blockIdx.x; id < jobs && going; id += gridDim.x) {
         const Work w = work_of<kPaged>(f, id, first_place);
         if (!w.n) continue;
-        const int n = w.n, users = f.halves ? 2 : w.row_tiles;
-        const auto active = [&](int u, int j) { return f.halves ? (j & 1) == u : w.touches(w.of[u], j); };
+        const int n = w.n, users = w.row_tiles;
+        const auto active = [&](int u, int j) { return w.touches(w.of[u], j); };
+        if (f.halves) {
+          // Tile j is the half j % 2's: its scores are issued two tiles ahead, behind the products that read the weights they overwrite.
+          // There is one job, so items are numbered from 0.
+          const auto slot_of = [&](int item) { return static_cast<uint32_t>(item) % S::kSlots; };
+          const auto wait_of = [&](int item) { return full + 8 * slot_of(item); };
+          const auto phase_of = [&](int item) { return static_cast<uint32_t>(item) / S::kSlots & 1; };
+          going = warp_wait(q_full, 0, &failed);
+          for (int j = 0; j < 2 && j < n && going; j++) {
+            going = warp_wait(wait_of(2 * j), phase_of(2 * j), &failed);
+            if (going && elected()) {
+              scores(j, slot_of(2 * j));
+              products_done(empty + 8 * slot_of(2 * j));
+            }
+            __syncwarp();
+          }
+#pragma unroll 1
+          for (int j = 0; j < n && going; j++) {
+            const int u = j & 1;
+            const bool more = j + 2 < n;
+            going = warp_wait_all(p_full + 8 * u, j >> 1 & 1, wait_of(2 * j + 1), phase_of(2 * j + 1), more ? wait_of(2 * j + 4) : 0, phase_of(2 * j + 4), &failed);
+            if (!going) break;
+            tmem_after_sync();
+            if (elected()) {
+              const uint32_t o = tmem + o_column + 128 * u, values_at = values + slot_of(2 * j + 1) * (S::kTile >> 4);
+              product_over_tokens(o, tmem + 128 * u, values_at, kResults, j >= 2);
+              product_over_tokens(o, tmem + 128 * u + 64, values_at + kHalfTokens, kResults, true);
+              products_done(empty + 8 * slot_of(2 * j + 1));
+              if (more) {
+                scores(u, slot_of(2 * j + 4));
+                products_done(empty + 8 * slot_of(2 * j + 4));
+              } else {
+                products_done(o_full + 8 * u);
+              }
+            }
+            __syncwarp();
+          }
+          break;
+        }
         int last_of[2] = {n - 1, n - 1};                // each one's last tile of keys
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -350,11 +377,11 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           if (u >= users || !going) break;
-          if (!f.halves || u == 0) going = warp_wait(q_full + 8 * u, loaded[u]++ & 1, &failed);
+          going = warp_wait(q_full + 8 * u, loaded[u]++ & 1, &failed);
           if (going && elected()) {
             if (active(u, 0)) scores(u, k.slot);
             // without another tile, or with none at all, the queries are no longer needed
-            if (last_of[u] <= 0 && !f.halves) products_done(q_empty + 8 * u);
+            if (last_of[u] <= 0) products_done(q_empty + 8 * u);
             if (u + 1 == users) products_done(empty + 8 * k.slot);
           }
           __syncwarp();
@@ -392,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
               if (last) products_done(empty + 8 * v.slot);
               // products run in the order in which they are issued: these scores overwrite P after it has been read
               if (more) scores(u, k.slot);
-              if (j + 1 == last_of[u] && !f.halves) products_done(q_empty + 8 * u);
+              if (j + 1 == last_of[u]) products_done(q_empty + 8 * u);
               if (last && j + 1 < n) products_done(empty + 8 * k.slot);
             }
             __syncwarp();
@@ -708,8 +735,7 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
     // tiles of keys that a CTA may have
     int64_t most = (p.cache.capacity + 127) / 128;
     if (p.window != INT32_MAX) most = std::min(most, (static_cast<int64_t>(p.window) + 2 * f.rows.tokens + 127) / 128 + 1 + (std::min(p.sinks, p.cache.capacity) + 127) / 128);
-    const int64_t want = f.halves ? 4 * sms : sms;
-    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min<int64_t>(want / ctas, 64))));
+    f.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min<int64_t>(sms / ctas, 64))));
   }
   f.parts = f.splits * (f.halves ? 2 : 1);
   return f;

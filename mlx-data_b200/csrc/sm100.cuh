@@ -120,11 +120,6 @@ __device__ __forceinline__ void tile_load(uint32_t to, const CUtensorMap* map, i
       : : "r"(to), "l"(map), "r"(element), "r"(head), "r"(token), "r"(kv_head), "r"(batch), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tile_store(const CUtensorMap* map, int element, int head, int token, int kv_head, int batch, uint32_t from) {
-  asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4, %5}], [%6];"
-               : : "l"(map), "r"(element), "r"(head), "r"(token), "r"(kv_head), "r"(batch), "r"(from) : "memory");
-}
-
 __device__ __forceinline__ void tile_stores_read() {
   asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;" : : : "memory");
 }
