@@ -12,7 +12,9 @@ namespace mlxd {
 
 namespace {
 
-constexpr int kThreads = 640;          // four warpgroups for what lies between the products, then warps for copies, products, helpers
+// Warpgroups for what lies between the products, then warps for copies, products, helpers.  Queries: four, each row four threads'; keys: two
+// of twice the registers (8192 tokens, window 2048, 32 heads on 8: queries 498 and 502 us, keys 594 and 514).
+constexpr int kRowThreads = 640, kKeyThreads = 384;
 constexpr int kMaskRing = 4;           // queries: tiles of keys in the ring are no more
 constexpr int kRowRing = 8;            // keys: items in the ring are no more
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,25 +53,10 @@ __device__ __forceinline__ void store_zeros(uint32_t at) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" : : "r"(at), "r"(0) : "memory");
 }
 
-// Elements `from` to `from` + kCount - 1 of a row of accumulators, scaled, rounded and written; zeros where there are none.
+// Elements `from` to `from` + kCount - 1 of a row of accumulators, scaled, rounded and written; zeros where the row has no sums, or nothing
+// was summed at all (`none`, of the whole CTA).
 template <class T, int kCount>
-__device__ __forceinline__ void write_row(uint32_t tmem, T* to, int from, int dim, float by, bool there, bool none) {
-#pragma unroll
-  for (int x = 0; x < kCount; x += 16) {
-    uint32_t o[16], v[8] = {};
-    if (!none) {
-      tmem_load<16>(tmem + from + x, o);
-      tmem_loaded(o);
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = pack2<T>(__uint_as_float(o[2 * i]) * by, __uint_as_float(o[2 * i + 1]) * by);
-    }
-    if (there) store_row_part(to + from + x, v, (dim - from - x) / 8);
-  }
-}
-
-// The same where some rows are zeros: those for which `sums` is false.
-template <class T, int kCount>
-__device__ __forceinline__ void write_row_or_zeros(uint32_t tmem, T* to, int from, int dim, float by, bool there, bool sums, bool none) {
+__device__ __forceinline__ void write_row(uint32_t tmem, T* to, int from, int dim, float by, bool there, bool sums, bool none) {
 #pragma unroll
   for (int x = 0; x < kCount; x += 16) {
     uint32_t o[16], v[8] = {};
@@ -135,7 +122,7 @@ __device__ __forceinline__ RowJob row_job_of(const BackwardParams& f, int id) {
 // 255 tokens in float16, dQ off by 0.00036 of its size by O, 0.0003 so (0.00021 by the rounding of results alone).  A single key has the
 // weight 1, so that its dS is 0 and no remainder of a rounding.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
+__global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
@@ -313,29 +300,39 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
         const uint32_t read = static_cast<uint32_t>(bits_of(first_key, mine.from, mine.to) | bits_of(first_key, 0, mine.sinks));
         row_sums(tmem + 128 * j + 32 * quarter + lanes, tmem + (j ? dq_column : dp_column) + 32 * quarter + lanes, read, single, c, base, &part, &weights);
       }
-    } else if (reads) {   // delta: this thread's quarter of the elements
-      const T* o = reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + token * p.out.token + head * p.out.head;
-      const T* g = reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + token * p.dout.token + head * p.dout.head;
+    } else if (n) {
+      // delta: a warp takes two rows at a time, 16 bytes a lane (each thread its own row: 6.7 us of a CTA's 36, at 17 tiles of keys)
 #pragma unroll
-      for (int x = 0; x < kDim / 4; x += 8) {
-        const int at = quarter * (kDim / 4) + x;
-        if (at < p.head_dim) {
-          const uint4 a = *reinterpret_cast<const uint4*>(o + at), b = *reinterpret_cast<const uint4*>(g + at);
-          const T *u = reinterpret_cast<const T*>(&a), *v = reinterpret_cast<const T*>(&b);
+      for (int i = 0; i < 4; i++) {
+        const int of = warp * 8 + 2 * i + lane / 16, at = lane % 16 * 8;
+        const int t = job.q0 + of / f.rows.heads, g = job.chunk * f.rows.heads + of % f.rows.heads, h = kv_head * p.group + g;
+        float sum = 0;
+        if (of < f.rows.heads * f.rows.tokens && t < seq.fresh && g < p.group && at < p.head_dim) {
+          const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + t * p.out.token + h * p.out.head + at));
+          const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + t * p.dout.token + h * p.dout.head + at));
+          const uint32_t u[4] = {a.x, a.y, a.z, a.w}, v[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int i = 0; i < 8; i++) part += static_cast<float>(u[i]) * static_cast<float>(v[i]);
+          for (int k = 0; k < 4; k++) {
+            const float2 x = unpack2<T>(u[k]), y = unpack2<T>(v[k]);
+            sum += x.x * y.x + x.y * y.y;
+          }
         }
+        for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane % 16 == 0) delta_parts[0][of] = sum;
       }
     }
     // with few keys the sums of weights too, in the ring's last place, which these do not reach
     float(*const weight_parts)[128] = reinterpret_cast<float(*)[128]>(shared + (1 + S::kSlots) * S::kTile);
-    delta_parts[quarter][row] = part;
-    if (n <= 2) weight_parts[quarter][row] = weights;
+    if (n <= 2) {
+      delta_parts[quarter][row] = part;
+      weight_parts[quarter][row] = weights;
+    }
     warp_arrive(delta_full, lane);
     going = warp_wait(delta_full, 0, &failed) && going;
     const auto of_row = [&](const float(*parts)[128]) { return (parts[0][row] + parts[1][row]) + (parts[2][row] + parts[3][row]); };
-    float delta = going ? of_row(delta_parts) : 0.0f;
+    float delta = going && reads ? delta_parts[0][row] : 0.0f;
     if (n <= 2 && going) {
+      delta = of_row(delta_parts);
       weights = of_row(weight_parts);
       delta = weights == 0 ? 0.0f : delta / weights;
     }
@@ -389,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
     if (going) {
       tmem_after_sync();
       T* const to = reinterpret_cast<T*>(p.dq.data) + batch * p.dq.batch + token * p.dq.token + head * p.dq.head;
-      write_row<T, kDim / 4>(tmem + dq_column + lanes, to, quarter * (kDim / 4), p.head_dim, p.scale, there, n == 0);
+      write_row<T, kDim / 4>(tmem + dq_column + lanes, to, quarter * (kDim / 4), p.head_dim, p.scale, there, true, n == 0);
     }
   }
   __syncwarp();
@@ -398,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dq_kernel(const __grid_con
   if (warp == 17) tmem_free<512>(tmem);
   if (failed) {   // not a number, instead of whatever the memory held; the other kernel's results are not valid either
     const RowJob at = row_job_of(f, block_again());
-    for (int i = threadIdx.x / 32; i < f.rows.tokens * f.rows.heads; i += kThreads / 32) {
+    for (int i = threadIdx.x / 32; i < f.rows.tokens * f.rows.heads; i += kRowThreads / 32) {
       const int token = at.q0 + i / f.rows.heads, head = at.chunk * f.rows.heads + i % f.rows.heads;
       if (token >= p.tokens || head >= p.group) continue;
       uint16_t* to = reinterpret_cast<uint16_t*>(p.dq.data) + at.batch * p.dq.batch + token * p.dq.token + (at.kv_head * p.group + head) * p.dq.head;
@@ -429,7 +426,7 @@ __device__ __forceinline__ KeyJob key_job_of(const BackwardParams& f, int id) {
 // dV = P^T dO and dK = scale dS^T Q for 128 keys, over the rows that read some of them.  Scores lie the other way round (a key a lane), so
 // that P^T and dS^T are operands as they are.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
+__global__ void __launch_bounds__(kKeyThreads, 1) causal_dkv_kernel(const __grid_constant__ BackwardParams f, const __grid_constant__ CausalMaps maps) {
   using S = Sizes<kDim>;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
@@ -450,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8, ended}) barrier_init(bar, 1);
-    for (const uint32_t bar : {p_full, ds_full, stats_empty, stats_empty + 8}) barrier_init(bar, 16);
+    for (const uint32_t bar : {p_full, ds_full, stats_empty, stats_empty + 8}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
       barrier_init(full + 8 * i, 1);
       barrier_init(empty + 8 * i, 1);
@@ -459,12 +456,12 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
     barrier_init_done();
   }
   // a box may have fewer rows than a tile: the others are summed over too, and no copy writes them
-  for (int i = threadIdx.x; i < (128 - tile_rows) * 8 * S::kBoxes * S::kSlots; i += kThreads) {
+  for (int i = threadIdx.x; i < (128 - tile_rows) * 8 * S::kBoxes * S::kSlots; i += kKeyThreads) {
     const int box = i / ((128 - tile_rows) * 8), unit = i % ((128 - tile_rows) * 8);
     store_zeros(ring_at + box * kBoxBytes + tile_rows * 128 + unit * 16);
   }
   fence_async_proxy();
-  if (warp == 17) tmem_alloc<512>(smem_address(&tmem_slot));
+  if (warp == 9) tmem_alloc<512>(smem_address(&tmem_slot));
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
@@ -480,9 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
   // a tile in which the sequence ends before the tensor does: rows behind it are cleared
   const auto partial = [&](int i) { return length < p.tokens && token_of(i) + f.rows.tokens > length; };
 
-  if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16 && lane == 0 && n) {
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 8 && lane == 0 && n) {
       // -------------------------------------------------- copies: queries of tile 0, their gradients, queries of tile 1, ...
       load_keys<S>(k_at, &maps.k, k0, kv_head, batch, k_full);
       load_keys<S>(v_at, &maps.v, k0, kv_head, batch, v_full);
@@ -507,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
           for (int i = 0; i < kWaitTries && !barrier_try(bar, parity); i++) {}
         }
       }
-    } else if (warp == 17 && n) {
+    } else if (warp == 9 && n) {
       // -------------------------------------------------- products
       constexpr uint32_t kScores = product_descriptor<T>(128, 128, false), kResults = product_descriptor<T>(128, kDim, true);
       const int steps = (p.head_dim + 15) / 16;
@@ -540,7 +537,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          product_over_quarters(tmem + dv_column, tmem, ring_tokens + at_slot(g.slot), kResults, i > 0);
+          const uint32_t b = ring_tokens + at_slot(g.slot);
+          product_over_tokens(tmem + dv_column, tmem, b, kResults, i > 0);
+          product_over_tokens(tmem + dv_column, tmem + 64, b + kHalfTokens, kResults, true);
           if (more) scores(next_q.slot);   // overwrites P after it has been read
           products_done(empty + 8 * g.slot);
         }
@@ -549,7 +548,9 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         if (!going) break;
         tmem_after_sync();
         if (elected()) {
-          product_over_quarters(tmem + dk_column, tmem + dp_column, ring_tokens + at_slot(q.slot), kResults, i > 0);
+          const uint32_t b = ring_tokens + at_slot(q.slot);
+          product_over_tokens(tmem + dk_column, tmem + dp_column, b, kResults, i > 0);
+          product_over_tokens(tmem + dk_column, tmem + dp_column + 64, b + kHalfTokens, kResults, true);
           if (more) dp(next_g.slot);
           products_done(empty + 8 * q.slot);
           if (!more) products_done(done);
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         next_g.next(2);
       }
       if (!going) products_end(ended);
-    } else if (warp == 18) {
+    } else if (warp == 10) {
       // -------------------------------------------------- what is known of the rows; -infinity makes P = 0 where there is none
       wait_for_kernels_before();
       for (int i = 0; i < n; i++) {
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) barrier_arrive(stats_full + 8 * (i & 1));
       }
-    } else if (warp == 19) {
+    } else if (warp == 11) {
       // -------------------------------------------------- zeros in rows behind the sequence
       int r = 0;
       for (int item = 0; item < 2 * n; item++) {
@@ -599,112 +600,122 @@ __global__ void __launch_bounds__(kThreads, 1) causal_dkv_kernel(const __grid_co
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    // ---------------------------------------------------- a key belongs to four threads, one for each quarter of the rows of a tile
-    const int quarter = warp / 4, row = threadIdx.x & 127, key = k0 + row;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------------------------------------------- a key belongs to two threads, one for each half of the rows of a tile
+    const int half = warp / 4, row = threadIdx.x & 127, key = k0 + row;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const float c = p.scale * kLog2e;
     const bool there = key < length;
     const int tokens_end = key < p.sinks || p.window >= length ? length : min(length, key + p.window);   // of the queries that read the key
-    const uint32_t mine = tmem + 32 * quarter + lanes;
+    const uint32_t mine = tmem + 64 * half + lanes;
     bool going = true;
     wait_for_kernels_before();
     for (int i = 0; i < n; i++) {
-      uint32_t s[32], d[32], packed[16];
+      uint32_t s[64];
       going = warp_wait(stats_full + 8 * (i & 1), i / 2 & 1, &failed) && warp_wait(s_full, i & 1, &failed);
       if (!going) break;
       tmem_after_sync();
       tmem_load<32>(mine, s);
+      tmem_load<32>(mine + 32, s + 32);
       tmem_loaded(s);
-      const float4* lse = stats[i & 1][0] + 8 * quarter;
-      const float4* delta = stats[i & 1][1] + 8 * quarter;
+      const float4* lse = stats[i & 1][0] + 16 * half;
+      const float4* delta = stats[i & 1][1] + 16 * half;
       const int token = token_of(i), lo = min(max(key - token, 0), f.rows.tokens), hi = there ? min(max(tokens_end - token, 0), f.rows.tokens) : 0;
       // rows beyond a box are zeros with P = 0 by their stats, so a whole tile needs no bits
-      const uint32_t read = static_cast<uint32_t>(bits_of(32 * quarter, lo * f.rows.heads, hi == f.rows.tokens ? 128 : hi * f.rows.heads));
-      const bool every = __all_sync(~0u, read == ~0u);
+      const uint64_t read = bits_of(64 * half, lo * f.rows.heads, hi == f.rows.tokens ? 128 : hi * f.rows.heads);
+      const bool every = __all_sync(~0u, read == ~uint64_t{0});
 #pragma unroll
-      for (int k = 0; k < 32; k += 4) {
-        const float4 l = lse[k / 4];
-        uint32_t* e = s + k;
-        const float2 a = fma2(make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])), make_float2(c, c), make_float2(l.x, l.y));
-        const float2 b = fma2(make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])), make_float2(c, c), make_float2(l.z, l.w));
-        const float v[4] = {exp2_of(a.x), exp2_of(a.y), exp2_of(b.x), exp2_of(b.y)};
+      for (int x = 0; x < 2; x++) {
+        uint32_t packed[16];
+        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
 #pragma unroll
-        for (int y = 0; y < 4; y++) e[y] = every || (read >> (k + y) & 1) ? __float_as_uint(v[y]) : 0u;
-        packed[k / 2] = pack2<T>(__uint_as_float(e[0]), __uint_as_float(e[1]));
-        packed[k / 2 + 1] = pack2<T>(__uint_as_float(e[2]), __uint_as_float(e[3]));
+        for (int k = 0; k < 32; k += 4) {
+          const float4 l = lse[8 * x + k / 4];
+          uint32_t* e = s + 32 * x + k;
+          const float2 a = fma2(make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])), make_float2(c, c), make_float2(l.x, l.y));
+          const float2 b = fma2(make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])), make_float2(c, c), make_float2(l.z, l.w));
+          const float v[4] = {exp2_of(a.x), exp2_of(a.y), exp2_of(b.x), exp2_of(b.y)};
+#pragma unroll
+          for (int y = 0; y < 4; y++) e[y] = __float_as_uint(v[y]);
+          if (!every) {
+#pragma unroll
+            for (int y = 0; y < 4; y++) e[y] = word >> (k + y) & 1 ? e[y] : 0u;
+          }
+          packed[k / 2] = pack2<T>(__uint_as_float(e[0]), __uint_as_float(e[1]));
+          packed[k / 2 + 1] = pack2<T>(__uint_as_float(e[2]), __uint_as_float(e[3]));
+        }
+        tmem_store<16>(mine + 16 * x, packed);
       }
-      tmem_store<16>(mine, packed);
       tmem_stored();
       tmem_before_sync();
       warp_arrive(p_full, lane);
       going = warp_wait(dp_full, i & 1, &failed);
       if (!going) break;
       tmem_after_sync();
-      tmem_load<32>(mine + dp_column, d);
-      tmem_loaded(d);
 #pragma unroll
-      for (int k = 0; k < 32; k += 4) {
-        const float4 l = delta[k / 4];
-        const uint32_t* e = s + k;
-        float2 a = mul2(add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-l.x, -l.y)),
-                        make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])));
-        float2 b = mul2(add2(make_float2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), make_float2(-l.z, -l.w)),
-                        make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])));
-        if (!every) {   // not 0 times an infinity
-          a.x = read >> k & 1 ? a.x : 0.0f;
-          a.y = read >> (k + 1) & 1 ? a.y : 0.0f;
-          b.x = read >> (k + 2) & 1 ? b.x : 0.0f;
-          b.y = read >> (k + 3) & 1 ? b.y : 0.0f;
+      for (int x = 0; x < 2; x++) {
+        uint32_t d[32], packed[16];
+        const uint32_t word = static_cast<uint32_t>(read >> (32 * x));
+        tmem_load<32>(mine + dp_column + 32 * x, d);
+        tmem_loaded(d);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 l = delta[8 * x + k / 4];
+          const uint32_t* e = s + 32 * x + k;
+          float2 a = mul2(add2(make_float2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), make_float2(-l.x, -l.y)),
+                          make_float2(__uint_as_float(e[0]), __uint_as_float(e[1])));
+          float2 b = mul2(add2(make_float2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), make_float2(-l.z, -l.w)),
+                          make_float2(__uint_as_float(e[2]), __uint_as_float(e[3])));
+          if (!every) {   // not 0 times an infinity
+            a.x = word >> k & 1 ? a.x : 0.0f;
+            a.y = word >> (k + 1) & 1 ? a.y : 0.0f;
+            b.x = word >> (k + 2) & 1 ? b.x : 0.0f;
+            b.y = word >> (k + 3) & 1 ? b.y : 0.0f;
+          }
+          packed[k / 2] = pack2<T>(a.x, a.y);
+          packed[k / 2 + 1] = pack2<T>(b.x, b.y);
         }
-        packed[k / 2] = pack2<T>(a.x, a.y);
-        packed[k / 2 + 1] = pack2<T>(b.x, b.y);
+        tmem_store<16>(mine + dp_column + 16 * x, packed);
       }
-      tmem_store<16>(mine + dp_column, packed);
       warp_arrive(stats_empty + 8 * (i & 1), lane);
       tmem_stored();
       tmem_before_sync();
       warp_arrive(ds_full, lane);
     }
     if (n && going) going = warp_wait(done, 0, &failed);
-    // the first two warpgroups write dV, the others dK, half of the elements each
-    const bool is_k = quarter / 2, none = n == 0;
-    const int from = quarter % 2 * (kDim / 2);
-    const uint32_t sums = tmem + (is_k ? dk_column : dv_column) + lanes;
-    if (going && split) {
+    if (going && split) {   // the first warpgroup writes dV, the second dK
       tmem_after_sync();
-      float* to = f.partial + ((((static_cast<int64_t>(job.part) * p.batch + batch) * p.kv_heads + kv_head) * f.sink_tiles + job.tile) * 2 + (is_k ? 0 : 1)) * 128 * p.head_dim + row * p.head_dim;
+      float* to = f.partial + ((((static_cast<int64_t>(job.part) * p.batch + batch) * p.kv_heads + kv_head) * f.sink_tiles + job.tile) * 2 + (half ? 0 : 1)) * 128 * p.head_dim + row * p.head_dim;
 #pragma unroll
-      for (int x = 0; x < kDim / 2; x += 16) {
-        uint32_t o[16] = {};
-        if (!none) {
-          tmem_load<16>(sums + from + x, o);
+      for (int x = 0; x < kDim; x += 32) {
+        uint32_t o[32] = {};
+        if (n) {
+          tmem_load<32>(tmem + (half ? dk_column : dv_column) + lanes + x, o);
           tmem_loaded(o);
         }
 #pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-          if (from + x + k < p.head_dim) *reinterpret_cast<float4*>(to + from + x + k) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+        for (int k = 0; k < 32; k += 4) {
+          if (x + k < p.head_dim) *reinterpret_cast<float4*>(to + x + k) = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
         }
       }
-    } else if (going) {
+    } else if (going) {   // the first warpgroup writes dV, the second dK
       tmem_after_sync();
-      const Heads& out = is_k ? p.dk : p.dv;
+      const Heads& out = half ? p.dk : p.dv;
       T* const to = reinterpret_cast<T*>(out.data) + batch * out.batch + key * out.token + kv_head * out.head;
       // keys behind the sequence get zeros, whatever they are; their accumulators are zeros but for what is not a number
-      if (__all_sync(~0u, there)) write_row<T, kDim / 2>(sums, to, from, p.head_dim, is_k ? p.scale : 1.0f, true, none);
-      else write_row_or_zeros<T, kDim / 2>(sums, to, from, p.head_dim, is_k ? p.scale : 1.0f, key < p.tokens, there && !none, none);
+      write_row<T, kDim>(tmem + (half ? dk_column : dv_column) + lanes, to, 0, p.head_dim, half ? p.scale : 1.0f, key < p.tokens, there && n > 0, n == 0);
     }
   }
   __syncwarp();
   tmem_before_sync();
   __syncthreads();
-  if (warp == 17) tmem_free<512>(tmem);
+  if (warp == 9) tmem_free<512>(tmem);
   if (failed) {
     const KeyJob at = key_job_of(f, block_again());
     const int from = at.tile * 128, end = min(from + 128, p.tokens);
     if (at.tile < f.sink_tiles && f.sink_parts > 1) {
       float* to = f.partial + (((static_cast<int64_t>(at.part) * p.batch + at.batch) * p.kv_heads + at.kv_head) * f.sink_tiles + at.tile) * 256 * p.head_dim;
-      for (int i = threadIdx.x; i < 256 * p.head_dim; i += kThreads) to[i] = NAN;
+      for (int i = threadIdx.x; i < 256 * p.head_dim; i += kKeyThreads) to[i] = NAN;
     } else {
       spoil_rows(p.dk, at.batch, at.kv_head, from, end, p.head_dim);
       spoil_rows(p.dv, at.batch, at.kv_head, from, end, p.head_dim);
@@ -789,10 +800,10 @@ cudaError_t launch(const BackwardParams& f, const CausalMaps& maps, cudaStream_t
   if (e == cudaSuccess) e = allow_shared<causal_dkv_kernel<T, kDim>>(bytes, p.device);
   if (e != cudaSuccess) return e;
   const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.batch;
-  causal_dq_kernel<T, kDim><<<static_cast<unsigned>(heads * f.rows.tiles * f.rows.chunks), kThreads, bytes, stream>>>(f, maps);
+  causal_dq_kernel<T, kDim><<<static_cast<unsigned>(heads * f.rows.tiles * f.rows.chunks), kRowThreads, bytes, stream>>>(f, maps);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = launch_behind(causal_dkv_kernel<T, kDim>, heads * ((p.tokens + 127) / 128 + f.sink_tiles * (f.sink_parts - 1)), kThreads, bytes, stream, f, maps);
+  e = launch_behind(causal_dkv_kernel<T, kDim>, heads * ((p.tokens + 127) / 128 + f.sink_tiles * (f.sink_parts - 1)), kKeyThreads, bytes, stream, f, maps);
   if (e != cudaSuccess || f.sink_parts == 1) return e;
   return launch_behind(causal_sum_kernel<T>, heads * f.sink_tiles * 2 * (128 / kSumRows), 128, 0, stream, f);
 }
