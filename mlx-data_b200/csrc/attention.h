@@ -7,6 +7,7 @@
 #include <exception>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mlxd_b200.h"
 #include "context.h"
@@ -50,6 +51,28 @@ int guarded(const char* entry, F&& body) {
     return MLXD_ERR_INVALID;
   }
 }
+
+#ifdef __CUDACC__
+// Launches a kernel that begins while the last CTAs of the kernel before it in the stream run, and that waits on the device
+// (griddepcontrol.wait, in every CTA) for that one's end before it touches what others write or read.
+template <class... Args>
+cudaError_t launch_behind(void (*kernel)(Args...), dim3 grid, int threads, int bytes, cudaStream_t stream, int cluster, std::common_type_t<Args>... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute how[2] = {};
+  how[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  how[0].val.programmaticStreamSerializationAllowed = 1;
+  how[1].id = cudaLaunchAttributeClusterDimension;
+  how[1].val.clusterDim.x = cluster;
+  how[1].val.clusterDim.y = how[1].val.clusterDim.z = 1;
+  config.attrs = how;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+#endif
 
 // SMs of a device, looked up once per device.
 int device_sms(int device, int* sms);

@@ -130,7 +130,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
   __shared__ float delta_parts[4][128];   // of a row's four threads
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
-  asm volatile("griddepcontrol.launch_dependents;");   // the other kernel's CTAs take the SMs that these leave
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
@@ -138,7 +137,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
                  dp2_full = delta_full + 8, landed = dp2_full + 8, ended = landed + 8 * kMaskRing;
   const RowJob job = row_job_of(f, blockIdx.x);
   const int batch = job.batch, kv_head = job.kv_head;
-  const Sequence seq = sequence_of<false>(p, batch);
   if (threadIdx.x == 0) {
     failed = 0;
     for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, dp2_full, done, ended}) barrier_init(bar, 1);
@@ -155,6 +153,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
   __syncthreads();
   tmem_after_sync();
   const uint32_t tmem = tmem_slot, dp_column = 256, dq_column = 384;   // scores in 0 and 128
+  wait_for_kernels_before();
+  // The other kernel's CTAs take the SMs that these leave.  They read the inputs before they wait for this kernel, so not ahead of here.
+  asm volatile("griddepcontrol.launch_dependents;");
+  const Sequence seq = sequence_of<false>(p, batch);
   // what the tile's rows read, in tiles of keys: first ones, then the window's
   const int end_token = min(job.q0 + f.rows.tokens, seq.fresh);
   const Reach all = job.q0 < end_token ? reach_of(p, seq, job.q0, end_token) : Reach{0, 0, 0};
@@ -760,22 +762,6 @@ __global__ void __launch_bounds__(128) causal_sum_kernel(const __grid_constant__
   }
 }
 
-template <class... Args>
-cudaError_t launch_behind(void (*kernel)(Args...), int64_t blocks, int threads, int bytes, cudaStream_t stream, std::common_type_t<Args>... args) {
-  // begins while the last CTAs of the kernel before run; what it needs of that one it waits for on the device
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = bytes;
-  config.stream = stream;
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 BackwardParams backward_plan(const CausalParams& p) {
   BackwardParams f = {};
   f.p = p;
@@ -800,12 +786,12 @@ cudaError_t launch(const BackwardParams& f, const CausalMaps& maps, cudaStream_t
   if (e == cudaSuccess) e = allow_shared<causal_dkv_kernel<T, kDim>>(bytes, p.device);
   if (e != cudaSuccess) return e;
   const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.batch;
-  causal_dq_kernel<T, kDim><<<static_cast<unsigned>(heads * f.rows.tiles * f.rows.chunks), kRowThreads, bytes, stream>>>(f, maps);
-  e = cudaGetLastError();
+  e = launch_behind(causal_dq_kernel<T, kDim>, dim3(static_cast<unsigned>(heads * f.rows.tiles * f.rows.chunks)), kRowThreads, bytes, stream, 1, f, maps);
   if (e != cudaSuccess) return e;
-  e = launch_behind(causal_dkv_kernel<T, kDim>, heads * ((p.tokens + 127) / 128 + f.sink_tiles * (f.sink_parts - 1)), kKeyThreads, bytes, stream, f, maps);
+  e = launch_behind(causal_dkv_kernel<T, kDim>, dim3(static_cast<unsigned>(heads * ((p.tokens + 127) / 128 + f.sink_tiles * (f.sink_parts - 1)))), kKeyThreads, bytes,
+                    stream, 1, f, maps);
   if (e != cudaSuccess || f.sink_parts == 1) return e;
-  return launch_behind(causal_sum_kernel<T>, heads * f.sink_tiles * 2 * (128 / kSumRows), 128, 0, stream, f);
+  return launch_behind(causal_sum_kernel<T>, dim3(static_cast<unsigned>(heads * f.sink_tiles * 2 * (128 / kSumRows))), 128, 0, stream, 1, f);
 }
 
 }  // namespace

@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
+  wait_for_kernels_before();
   const uint32_t tmem = tmem_slot, o_column = 256;   // scores of tile t in columns 128 t, results in 256 + 128 t
   // ---------------------------------------------------- this thread's row, where it is one of the softmax
   const int t = warp / 8, half = warp / 4 % 2, part = warp % 4, row = 32 * part + lane;
@@ -685,24 +686,14 @@ cudaError_t launch(const ForwardParams& f, const CausalMaps& maps, cudaStream_t 
   int sms = 0;
   if (device_sms(p.device, &sms) != MLXD_OK) return cudaErrorInvalidDevice;
   const int64_t jobs = jobs_of(f);
-  causal_forward_kernel<T, kDim, kPaged><<<static_cast<unsigned>(kPaged ? jobs : std::min<int64_t>(jobs, sms)), kThreads, bytes, stream>>>(f, maps);
-  return cudaGetLastError();
+  return launch_behind(causal_forward_kernel<T, kDim, kPaged>, dim3(static_cast<unsigned>(kPaged ? jobs : std::min<int64_t>(jobs, sms))), kThreads, bytes, stream, 1, f, maps);
 }
 
 template <class T>
 cudaError_t launch_join(const ForwardParams& f, cudaStream_t stream) {
   const CausalParams& p = f.p;
-  // begins while the parts are being worked out and waits for them on the device
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + kJoinWarps - 1) / kJoinWarps));
-  config.blockDim = dim3(32 * kJoinWarps);
-  config.stream = stream;
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, causal_join_kernel<T>, f);
+  return launch_behind(causal_join_kernel<T>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.q_heads * p.tokens + kJoinWarps - 1) / kJoinWarps)),
+                       32 * kJoinWarps, 0, stream, 1, f);
 }
 
 template <class T, int kDim>
@@ -723,10 +714,18 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
   if (f.steps) {
     int64_t reach = p.cache.capacity;
     if (p.window != INT32_MAX) reach = std::min(reach, static_cast<int64_t>(p.window) + p.tokens + std::min(p.sinks, p.cache.capacity) + 32);
-    const int64_t rounds = std::max<int64_t>(1, reach / 64);    // of a CTA's four warps
-    const int64_t slots = static_cast<int64_t>(step_ctas(p.head_dim, p.tokens * p.group <= 8 ? 1 : 2)) * sms;
-    while (f.cluster < 8 && 2 * heads * f.cluster <= slots && f.cluster * 2 <= rounds) f.cluster *= 2;
-    f.splits = static_cast<int>(std::max<int64_t>(1, std::min({reach / (f.cluster * 1500), 8 * slots / (heads * f.cluster), int64_t{64}})));
+    // Shares of a key head's keys: up to 320 CTAs in all, of 128 keys at least, dealt to clusters of up to eight; long stretches are cut at
+    // 1500 keys and by splits alone, since samples are of different lengths and clusters wait for places side by side.  us for clusters x
+    // splits: 8 heads, 1602 keys 8x1 9.9, 4x4 9.6, 1x1 28.1; 6001 keys 8x1 20.4, 8x4 13.8, 1x32 19.8; 24001 keys 8x1 59.9, 8x4 27.5;
+    // 160 heads, windows of 1028 keys 1x1 28.8, 2x1 18.6, 4x1 20.3; 128 heads, up to 24001 keys 2x1 372, 8x2 241, 1x16 221, 1x32 232.
+    int64_t shares = std::max<int64_t>(1, std::min(320 / heads, reach / 128));
+    if (reach / shares > 1500) {
+      const int64_t slots = static_cast<int64_t>(step_ctas(p.head_dim, p.tokens * p.group <= 8 ? 1 : 2)) * sms;
+      f.splits = static_cast<int>(std::max(shares, std::min({reach / 1500, 8 * slots / heads, int64_t{64}})));
+    } else {
+      while (f.cluster < 8 && f.cluster * 2 <= shares) f.cluster *= 2;
+      f.splits = static_cast<int>(shares / f.cluster);
+    }
     f.parts = f.splits;
     return f;
   }

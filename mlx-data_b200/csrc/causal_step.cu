@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(32 * kWarps, step_ctas(kDim, kBlocks)) causal_
   __shared__ Reach reaches[kRows];
   __shared__ float warp_top[kWarps][kRows], warp_total[kWarps][kRows], cta_top[kRows], cta_total[kRows];
   asm volatile("griddepcontrol.launch_dependents;");
+  wait_for_kernels_before();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, c = lane & 3;
   // neighbours are the key heads of the same keys, which lie side by side in a page
   const int kv_head = blockIdx.y, split = blockIdx.z % f.splits, batch = blockIdx.z / f.splits, rows = p.tokens * p.group;
@@ -417,18 +418,7 @@ cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
   const CausalParams& p = f.p;
   const cudaError_t e = allow_shared<causal_step_kernel<T, kDim, kBlocks>>(bytes, p.device);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(f.cluster, p.kv_heads, f.splits * p.batch);
-  config.blockDim = dim3(32 * kWarps);
-  config.dynamicSmemBytes = bytes;
-  config.stream = stream;
-  cudaLaunchAttribute cluster = {};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = f.cluster;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = f.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&config, causal_step_kernel<T, kDim, kBlocks>, f);
+  return launch_behind(causal_step_kernel<T, kDim, kBlocks>, dim3(f.cluster, p.kv_heads, f.splits * p.batch), 32 * kWarps, bytes, stream, f.cluster, f);
 }
 
 template <class T>

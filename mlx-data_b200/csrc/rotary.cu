@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) append_rotary_ker
   const L me(p, first);
   const uint32_t items = static_cast<uint32_t>(p.rows) * p.parts;
   const uint32_t item = blockIdx.x * kWarps + threadIdx.x / 32;
+  wait_for_kernels_before();
   if (item >= items) return;
   const uint32_t row = p.parts == 1 ? item : item / p.parts, part = item - row * p.parts;
   const uint32_t b = row / static_cast<uint32_t>(p.tokens), s = row - b * p.tokens;
@@ -820,8 +821,7 @@ int append(const char* entry, int device, void* stream, const mlxd_append_desc* 
   MLXD_ON_DEVICE(device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(d->r.dtype, p, v, [&](auto type, auto vec, auto units, auto adjacent, auto turned) {
-    append_rotary_kernel<decltype(type), vec(), units(), adjacent(), turned()><<<blocks, 32 * kWarps, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_behind(append_rotary_kernel<decltype(type), vec(), units(), adjacent(), turned()>, dim3(blocks), 32 * kWarps, 0, s, 1, a);
   });
   return e == cudaSuccess ? MLXD_OK : fail_cuda(e, entry);
 }
