@@ -54,7 +54,8 @@ int guarded(const char* entry, F&& body) {
 
 #ifdef __CUDACC__
 // Launches a kernel that begins while the last CTAs of the kernel before it in the stream run, and that waits on the device
-// (griddepcontrol.wait, in every CTA) for that one's end before it touches what others write or read.
+// (griddepcontrol.wait, in every CTA) for that one's end before it touches what others write or read.  Such a kernel reads by ordinary
+// loads, not by those for memory that nobody writes while it runs.
 template <class... Args>
 cudaError_t launch_behind(void (*kernel)(Args...), dim3 grid, int threads, int bytes, cudaStream_t stream, int cluster, std::common_type_t<Args>... args) {
   cudaLaunchConfig_t config = {};

@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
         const int t = job.q0 + of / f.rows.heads, g = job.chunk * f.rows.heads + of % f.rows.heads, h = kv_head * p.group + g;
         float sum = 0;
         if (of < f.rows.heads * f.rows.tokens && t < seq.fresh && g < p.group && at < p.head_dim) {
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + t * p.out.token + h * p.out.head + at));
-          const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + t * p.dout.token + h * p.dout.head + at));
+          const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.out.data) + batch * p.out.batch + t * p.out.token + h * p.out.head + at);
+          const uint4 b = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.dout.data) + batch * p.dout.batch + t * p.dout.token + h * p.dout.head + at);
           const uint32_t u[4] = {a.x, a.y, a.z, a.w}, v[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
           for (int k = 0; k < 4; k++) {

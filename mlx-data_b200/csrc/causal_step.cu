@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(32 * kWarps, step_ctas(kDim, kBlocks)) causal_
     const T* from = reinterpret_cast<const T*>(p.q.data) + batch * p.q.batch + token * p.q.token + (kv_head * p.group + row % p.group) * p.q.head;
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const uint4 x = row < rows && 32 * i + 8 * c < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(from + 32 * i + 8 * c)) : make_uint4(0, 0, 0, 0);
+      const uint4 x = row < rows && 32 * i + 8 * c < p.head_dim ? *reinterpret_cast<const uint4*>(from + 32 * i + 8 * c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int w = 0; w < 4; w++) q[b][i][w] = word_of(x, w);
     }
