@@ -734,17 +734,23 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
   if (f.steps) {
     int64_t reach = p.cache.capacity;
     if (p.window != INT32_MAX) reach = std::min(reach, static_cast<int64_t>(p.window) + p.tokens + std::min(p.sinks, p.cache.capacity) + 32);
-    // Shares of a key head's keys: up to 320 CTAs in all, of 128 keys at least, dealt to clusters of up to eight; long stretches are cut at
-    // 1500 keys and by splits alone, since samples are of different lengths and clusters wait for places side by side.  us for clusters x
-    // splits: 8 heads, 1602 keys 8x1 9.9, 4x4 9.6, 1x1 28.1; 6001 keys 8x1 20.4, 8x4 13.8, 1x32 19.8; 24001 keys 8x1 59.9, 8x4 27.5;
-    // 160 heads, windows of 1028 keys 1x1 28.8, 2x1 18.6, 4x1 20.3; 128 heads, up to 24001 keys 2x1 372, 8x2 241, 1x16 221, 1x32 232.
-    int64_t shares = std::max<int64_t>(1, std::min(320 / heads, reach / 128));
-    if (reach / shares > 1500) {
-      const int64_t slots = static_cast<int64_t>(step_ctas(p.head_dim, p.tokens * p.group <= 8 ? 1 : 2)) * sms;
-      f.splits = static_cast<int>(std::max(shares, std::min({reach / 1500, 8 * slots / heads, int64_t{64}})));
-    } else {
-      while (f.cluster < 8 && f.cluster * 2 <= shares) f.cluster *= 2;
-      f.splits = static_cast<int>(shares / f.cluster);
+    // A CTA for each SM at most, joined within clusters of up to eight, where that leaves it 800 keys or fewer.  Else shares of a key head's
+    // keys: up to 320 CTAs in all, of 128 keys at least, dealt to clusters; long stretches are cut at 1500 keys and by splits alone,
+    // since samples are of different lengths and clusters wait for places side by side.  us for clusters x splits, the first ones of each
+    // alone on their SMs: 8 heads, 1602 keys 8x1 8.0, 8x2 14.7, 4x4 9.8; 6001 keys 8x1 14.9, 8x4 13.7; 24001 keys 8x1 41.7, 8x4 27.9;
+    // 32 heads, 1505 keys 4x1 7.9, 8x1 10.6; 3001 keys 4x1 14.8, 8x1 18.7; 160 heads, windows of 1028 keys 1x1 28.7, 2x1 18.6, 4x1 20.3;
+    // 128 heads, up to 24001 keys 1x1 276, 2x1 371, 8x2 238, 1x16 223.
+    while (f.cluster < 8 && 2 * heads * f.cluster <= sms && f.cluster * 2 <= reach / 128) f.cluster *= 2;
+    if (heads * f.cluster > sms || reach > 800 * f.cluster) {
+      f.cluster = 1;
+      const int64_t shares = std::max<int64_t>(1, std::min(320 / heads, reach / 128));
+      if (reach / shares > 1500) {
+        const int64_t slots = static_cast<int64_t>(step_ctas(p.head_dim, p.tokens * p.group <= 8 ? 1 : 2)) * sms;
+        f.splits = static_cast<int>(std::max(shares, std::min({reach / 1500, 8 * slots / heads, int64_t{64}})));
+      } else {
+        while (f.cluster < 8 && f.cluster * 2 <= shares) f.cluster *= 2;
+        f.splits = static_cast<int>(shares / f.cluster);
+      }
     }
     f.parts = f.splits;
     return f;

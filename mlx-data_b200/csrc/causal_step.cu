@@ -1,9 +1,9 @@
 // Cached attention of few rows - single tokens of a generation, short drafts - where reading keys and values is all the work.
 //
-// A CTA takes up to 16 rows (tokens and the query heads that share a key head) and a stretch of the keys; its four warps take 16 keys each
+// A CTA takes up to 16 rows (tokens and the query heads that share a key head) and a stretch of the keys; its warps take 16 keys each
 // in turn, as operands of 16 x 8 x 16 products.  Which elements of a head a product sums over, and which become its columns, is a
 // matter of naming, so what a lane copies in units of 16 bytes is its own operands: copies go into a queue in shared memory that every lane
-// has for itself, three rounds deep, and nothing waits for another lane.  Keys that are not read, or have no page, arrive as zeros.  The
+// has for itself, two or three rounds deep, and nothing waits for another lane.  Keys that are not read, or have no page, arrive as zeros.  The
 // CTAs of a cluster share a stretch of keys and join their sums through each other's shared memory; where that is not enough CTAs, keys are
 // split among clusters too, and a second kernel joins the parts.
 //
@@ -18,7 +18,6 @@ namespace mlxd {
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kKeys = 16;              // of a warp at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;         // as in the kernel for many queries
@@ -77,12 +76,15 @@ __device__ __forceinline__ float4 remote_float4(uint32_t at) {
   return v;
 }
 
-template <int kDim, int kBlocks>
+// kAlone: no more CTAs than SMs, so one CTA of an SM has twice the warps: a round of a warp takes 1 to 2 us, most of it one instruction
+// waiting for another, and only other warps fill that.
+template <int kDim, int kBlocks, bool kAlone>
 struct StepSizes {
+  static constexpr int kWarps = kAlone ? 8 : 4;
   static constexpr int kUnits = kDim / 32;         // 16-byte units of a key that a lane holds
   static constexpr int kHalves = kDim / 64;        // and of a value
-  static constexpr int kCtas = step_ctas(kDim, kBlocks);   // of an SM, by registers
-  static constexpr int kStages = (kDim == 128 ? 6 : 12) / kCtas;
+  static constexpr int kCtas = kAlone ? 1 : step_ctas(kDim, kBlocks);   // of an SM, by registers
+  static constexpr int kStages = kAlone ? 256 / kDim : (kDim == 128 ? 6 : 12) / kCtas;
   static constexpr int kStage = (2 * kUnits + 4 * kHalves) * 512;   // bytes of a warp's 16 keys and values
   static constexpr int kQueue = kWarps * kStages * kStage;
   // after the keys, in the same place: the warps' sums, then the CTA's
@@ -93,10 +95,11 @@ struct StepSizes {
 
 // kBlocks: columns of eight rows.  Scores lie keys by rows, S^T = K Q^T, and results elements by rows, O^T = V^T P^T, so that eight rows (a token
 // of up to eight heads) cost half of what sixteen do.
-template <class T, int kDim, int kBlocks>
-__global__ void __launch_bounds__(32 * kWarps, step_ctas(kDim, kBlocks)) causal_step_kernel(const __grid_constant__ ForwardParams f) {
-  using Z = StepSizes<kDim, kBlocks>;
-  constexpr int kUnits = Z::kUnits, kHalves = Z::kHalves, kRows = 8 * kBlocks;
+template <class T, int kDim, int kBlocks, bool kAlone>
+__global__ void __launch_bounds__(32 * StepSizes<kDim, kBlocks, kAlone>::kWarps, StepSizes<kDim, kBlocks, kAlone>::kCtas)
+    causal_step_kernel(const __grid_constant__ ForwardParams f) {
+  using Z = StepSizes<kDim, kBlocks, kAlone>;
+  constexpr int kWarps = Z::kWarps, kUnits = Z::kUnits, kHalves = Z::kHalves, kRows = 8 * kBlocks;
   const CausalParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t shared[];
   __shared__ Reach reaches[kRows];
@@ -417,13 +420,21 @@ __global__ void __launch_bounds__(32 * kWarps, step_ctas(kDim, kBlocks)) causal_
   if (f.cluster > 1) cluster_meet();   // nobody leaves while others read what it has
 }
 
+template <class T, int kDim, int kBlocks, bool kAlone>
+cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
+  constexpr int bytes = StepSizes<kDim, kBlocks, kAlone>::kShared;
+  const CausalParams& p = f.p;
+  const cudaError_t e = allow_shared<causal_step_kernel<T, kDim, kBlocks, kAlone>>(bytes, p.device);
+  if (e != cudaSuccess) return e;
+  return launch_behind(causal_step_kernel<T, kDim, kBlocks, kAlone>, dim3(f.cluster, p.kv_heads, f.splits * p.batch), 32 * StepSizes<kDim, kBlocks, kAlone>::kWarps, bytes, stream, f.cluster, f);
+}
+
 template <class T, int kDim, int kBlocks>
 cudaError_t launch(const ForwardParams& f, cudaStream_t stream) {
-  constexpr int bytes = StepSizes<kDim, kBlocks>::kShared;
-  const CausalParams& p = f.p;
-  const cudaError_t e = allow_shared<causal_step_kernel<T, kDim, kBlocks>>(bytes, p.device);
-  if (e != cudaSuccess) return e;
-  return launch_behind(causal_step_kernel<T, kDim, kBlocks>, dim3(f.cluster, p.kv_heads, f.splits * p.batch), 32 * kWarps, bytes, stream, f.cluster, f);
+  int sms = 0;
+  if (device_sms(f.p.device, &sms) != MLXD_OK) return cudaErrorInvalidDevice;
+  const int64_t ctas = static_cast<int64_t>(f.cluster) * f.splits * f.p.batch * f.p.kv_heads;
+  return ctas <= sms ? launch<T, kDim, kBlocks, true>(f, stream) : launch<T, kDim, kBlocks, false>(f, stream);
 }
 
 template <class T>
