@@ -7,7 +7,7 @@
 // CTAs of a cluster share a stretch of keys and join their sums through each other's shared memory; where that is not enough CTAs, keys are
 // split among clusters too, and a second kernel joins the parts.
 //
-// Reading keys and values once is the floor.  Measured: 32 heads on 8 of 128, 1602 keys: 9.7 us (one of 17 keys 5.3: launch, lengths, pages,
+// Reading keys and values once is the floor.  Measured: 32 heads on 8 of 128, 1602 keys: 8.0 us (17 keys 5.2: launch, lengths, pages,
 // keys, one after another); sixteen sequences of up to 24001 keys 222-232 us, 4.8 TB/s (74 % of the measured rate), wherever pages lie and
 // however long they are; forty sequences, windows of 1024, 16 heads on 4 of 64: 19 us.  Copies of 16 bytes keep half of the cycles of L1
 // busy; beginnings and ends of CTAs take the rest.
