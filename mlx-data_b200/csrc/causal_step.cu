@@ -374,9 +374,10 @@ __global__ void __launch_bounds__(32 * StepSizes<kDim, kBlocks, kAlone>::kWarps,
       e.w += a.w * by;
     }
     *reinterpret_cast<float4*>(cta_out + r * Z::kStride + x) = e;
-    if (x == 0) {
-      cta_top[r] = most;
-      cta_total[r] = reaches[r].sinks < 0 ? 0.0f : sum;   // a row that reads nothing
+    if (x == 0) {   // a row that reads nothing has neither, whatever its scores were: tiles that every other row reads are not masked for it
+      const bool reads = reaches[r].sinks >= 0;
+      cta_top[r] = reads ? most : -INFINITY;
+      cta_total[r] = reads ? sum : 0.0f;
     }
   }
 
