@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
     if (going) {
       tmem_after_sync();
       T* const to = reinterpret_cast<T*>(p.dq.data) + batch * p.dq.batch + token * p.dq.token + head * p.dq.head;
-      write_row<T, kDim / 4>(tmem + dq_column + lanes, to, quarter * (kDim / 4), p.head_dim, p.scale, there, true, n == 0);
+      // rows behind the sequence get zeros: 0 times a key that is not a number, or infinite, has made their accumulators NaN
+      write_row<T, kDim / 4>(tmem + dq_column + lanes, to, quarter * (kDim / 4), p.head_dim, p.scale, there, reads, n == 0);
     }
   }
   __syncwarp();
