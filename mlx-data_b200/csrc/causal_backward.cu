@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
   __shared__ float delta_parts[4][128];   // of a row's four threads
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
+  __shared__ uint32_t progress;           // copies begun
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t q_at = smem_address(shared), do_at = q_at + S::kTile, ring_at = do_at + S::kTile;
   const uint32_t q_full = smem_address(bars), do_full = q_full + 8, full = q_full + 16, empty = full + 8 * S::kSlots,
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
   const int batch = job.batch, kv_head = job.kv_head;
   if (threadIdx.x == 0) {
     failed = 0;
+    progress = 0;
     for (const uint32_t bar : {q_full, do_full, s_full, s_full + 8, dp_full, dp2_full, done, ended}) barrier_init(bar, 1);
     for (const uint32_t bar : {ds_full, delta_full}) barrier_init(bar, 16);
     for (int i = 0; i < S::kSlots; i++) {
@@ -186,6 +188,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
         // keys of a tile that is not read as a whole go by way of the mask warp
         const bool by_masks = !(issued & 1) && partial(j);
         load_keys<S>(ring_at + slot * S::kTile, issued & 1 ? &maps.v : &maps.k, tile_of(j) * 128, kv_head, batch, by_masks ? landed + 8 * (r % kMaskRing) : full + 8 * slot);
+        *static_cast<volatile uint32_t*>(&progress) = issued + 1;
         r += by_masks;
       }
       if (failed) {   // what is under way still lands before the CTA ends
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) causal_dq_kernel(const __grid_
       for (int j = 0; j < n; j++) {
         if (!partial(j)) continue;
         const int item = 2 * j, first = tile_of(j) * 128;
-        if (!warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed)) break;
+        if (!warp_wait_behind(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed, &progress)) break;
         const uint32_t keys = ring_at + item % S::kSlots * S::kTile;
         for (int row = lane / 8; row < 128; row += 4) {   // 8 lanes a row of 128 bytes
           const int key = first + row;
@@ -442,6 +445,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) causal_dkv_kernel(const __grid
   __shared__ float4 stats[2][2][32];      // of the rows of a tile: -lse * log2(e), delta
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
+  __shared__ uint32_t progress;           // copies begun
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t k_at = smem_address(shared), v_at = k_at + S::kTile, ring_at = v_at + S::kTile;
@@ -454,6 +458,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) causal_dkv_kernel(const __grid
 
   if (threadIdx.x == 0) {
     failed = 0;
+    progress = 0;
     for (const uint32_t bar : {k_full, v_full, s_full, dp_full, done, stats_full, stats_full + 8, ended}) barrier_init(bar, 1);
     for (const uint32_t bar : {p_full, ds_full, stats_empty, stats_empty + 8}) barrier_init(bar, 8);
     for (int i = 0; i < S::kSlots; i++) {
@@ -499,6 +504,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) causal_dkv_kernel(const __grid
         const bool by_masks = partial(i);
         load_rows<S>(ring_at + slot * S::kTile, issued & 1 ? &maps.dout : &maps.q, f.rows, chunk_of(i), token_of(i), kv_head, batch,
                      by_masks ? landed + 8 * (r % kRowRing) : full + 8 * slot);
+        *static_cast<volatile uint32_t*>(&progress) = issued + 1;
         r += by_masks;
       }
       if (failed) {   // what is under way still lands before the CTA ends
@@ -596,7 +602,8 @@ __global__ void __launch_bounds__(kKeyThreads, 1) causal_dkv_kernel(const __grid
       for (int item = 0; item < 2 * n; item++) {
         const int i = item / 2;
         if (!partial(i)) continue;
-        if (!warp_wait(landed + 8 * (r % kRowRing), r / kRowRing & 1, &failed)) break;
+        if (item >= S::kSlots) wait_for_kernels_before();   // its copy begins behind that; those of items before do not
+        if (!warp_wait_behind(landed + 8 * (r % kRowRing), r / kRowRing & 1, &failed, &progress)) break;
         const uint32_t at = ring_at + item % S::kSlots * S::kTile;
         for (int row = max(length - token_of(i), 0) * f.rows.heads + lane / 8; row < tile_rows; row += 4) {
           for (int x = 0; x < S::kBoxes; x++) store_zeros(at + x * kBoxBytes + row * 128 + (lane & 7) * 16);

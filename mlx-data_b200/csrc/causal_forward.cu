@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   __shared__ float exchange[2][2][128];   // of a row's two threads: maxima, sums at last
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, holes, first_place[2], gave_up[2][4];
+  __shared__ uint32_t progress;           // copies begun
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const uint32_t tiles_at = smem_address(shared), ring_at = tiles_at + (f.halves && S::kHalfSlots > S::kSlots ? 1 : 2) * S::kTile;
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
   const uint32_t slots = f.halves ? S::kHalfSlots : S::kSlots;
   if (threadIdx.x == 0) {
     failed = holes = 0;
+    progress = 0;
     for (int i = 0; i < 8; i++) gave_up[i / 4][i % 4] = 0;
     first_place[0] = first_place[1] = INT32_MAX;
     barrier_init(ended, 1);
@@ -315,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
             tile_load(ring_at + slot * S::kTile + x * kBoxBytes + page * (kBoxBytes / pages), i & 1 ? &maps.v : &maps.k, 64 * x, minor, w.job.kv_head, major, bar);
           }
           issued++;
+          if (lane == 0) *static_cast<volatile uint32_t*>(&progress) = issued;
           if (i & 1) {
             partials += by_masks;
             major = major_of(j + 1);
@@ -469,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1) causal_forward_kernel(const __gri
             if (gaps && read) read = page_of(p.cache, w.job.batch, key) >= 0;
             words[i] = __ballot_sync(~0u, read);
           }
-          going = warp_wait(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed);
+          // the next such tile may be at the end of the last job
+          going = warp_wait_behind(landed + 8 * (r % kMaskRing), r / kMaskRing & 1, &failed, &progress);
           if (!going) break;
           const uint32_t values = ring_at + item % slots * S::kTile;
           for (int i = 0; i < 4; i++) {

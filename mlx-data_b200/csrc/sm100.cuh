@@ -62,6 +62,21 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(~0u, barrier_wait(bar, parity, failed));
 }
 
+// The same for a warp whose turn is far off while others of its CTA work towards it: `progress` counts what they have begun, and the limit
+// begins anew whenever it has moved.  It ends too, since those have limits of their own and finitely much to begin.
+__device__ __forceinline__ bool warp_wait_behind(uint32_t bar, uint32_t parity, volatile int* failed, volatile uint32_t* progress) {
+  bool done = barrier_try(bar, parity);
+  uint32_t seen = *progress;
+  for (int i = 0; i < kWaitTries && !done && !*failed; i++) {
+    done = barrier_try(bar, parity);
+    const uint32_t now = *progress;
+    if (now != seen) i = 0;
+    seen = now;
+  }
+  if (!done) *failed = 1;
+  return __all_sync(~0u, done);
+}
+
 // Where one is in a ring of kSlots slots: the slot, and the parity of its use.
 template <int kSlots>
 struct Ring {
