@@ -22,6 +22,7 @@ namespace {
 constexpr int kRowThreads = 640, kKeyThreads = 384;
 constexpr int kMaskRing = 4;           // queries: tiles of keys in the ring are no more
 constexpr int kRowRing = 8;            // keys: items in the ring are no more
+constexpr int kSplitCtas = 1024;       // CTAs that share the rows of first tokens' tiles
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int kDim>
@@ -782,9 +783,13 @@ BackwardParams backward_plan(const CausalParams& p) {
   f.sink_parts = 1;
   if (p.sinks && p.window < p.tokens) {
     f.sink_tiles = (std::min(p.sinks, p.tokens) + 127) / 128;
-    // parts as long as the rows of other tiles, and not too short
+    // Parts as long as the rows of other tiles, and not too short; no more than kSplitCtas CTAs in all, which fill the device several times
+    // over, since each leaves a tile of float32 sums (134 MB for heads of 128).  Both passes of the backward, 32 heads on 8: 32768 tokens,
+    // window 512, 16384 first ones 22.1 ms with one part (0.4 GB more than the tensors), 27.0 with 32 (4.7 GB); 16 x 8192 tokens, window
+    // 128, 4 first ones 4.38 ms with 8 parts, 4.47 with 16.
     const int64_t others = (static_cast<int64_t>(p.window) + 127) / f.rows.tokens + 2, all = f.rows.tiles;
-    f.sink_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(32, all / std::max<int64_t>(others, 16))));
+    const int64_t most = std::min<int64_t>(32, kSplitCtas / (static_cast<int64_t>(p.batch) * p.kv_heads * f.sink_tiles));
+    f.sink_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, all / std::max<int64_t>(others, 16))));
   }
   return f;
 }
