@@ -3,7 +3,7 @@
 // A CTA takes up to 16 rows (tokens and the query heads that share a key head) and a stretch of the keys; its warps take 16 keys each
 // in turn, as operands of 16 x 8 x 16 products.  Which elements of a head a product sums over, and which become its columns, is a
 // matter of naming, so what a lane copies in units of 16 bytes is its own operands: copies go into a queue in shared memory that every lane
-// has for itself, two or three rounds deep, and nothing waits for another lane.  Keys that are not read, or have no page, arrive as zeros.  The
+// has for itself, two to four rounds deep, and nothing waits for another lane.  Keys that are not read, or have no page, arrive as zeros.  The
 // CTAs of a cluster share a stretch of keys and join their sums through each other's shared memory; where that is not enough CTAs, keys are
 // split among clusters too, and a second kernel joins the parts.
 //
@@ -85,6 +85,7 @@ struct StepSizes {
   static constexpr int kHalves = kDim / 64;        // and of a value
   static constexpr int kCtas = kAlone ? 1 : step_ctas(kDim, kBlocks);   // of an SM, by registers
   static constexpr int kStages = kAlone ? 256 / kDim : (kDim == 128 ? 6 : 12) / kCtas;
+  static_assert(2 * kStages <= 32, "two bits of a word for each");   // `holes`
   static constexpr int kStage = (2 * kUnits + 4 * kHalves) * 512;   // bytes of a warp's 16 keys and values
   static constexpr int kQueue = kWarps * kStages * kStage;
   // after the keys, in the same place: the warps' sums, then the CTA's
