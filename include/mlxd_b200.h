@@ -417,7 +417,9 @@ MLXD_API int mlxd_append_rotary(int device, void* cuda_stream, const mlxd_append
  * it.  Query i of sample b has the place s = lengths[b] + i and reads the keys at places j <= s, j < lengths[b] + counts[b], with s - j < window
  * (0: no window) or j < sinks.  With a tree [batch, tokens, tokens] query i reads the new token j where tree[b, i, j] is not 0 and
  * j < counts[b], and of the cache before them (j < lengths[b]) what the window leaves, s being lengths[b] + the number of new tokens
- * other than itself that it reads.  Keys at places that have no page are not read.  What lies where no query of the sample reads has no
+ * other than itself that it reads.  New tokens are read by the tree alone: where a branch is longer than the window, a tree without the
+ * ancestors that lie a window or more behind (but with those below `sinks`) makes its rows those of mlxd_window_attention.  Keys at places
+ * that have no page are not read.  What lies where no query of the sample reads has no
  * effect, whatever it is; what is not a number in a value that some queries of a sample read, or under a tree in a value of any of its
  * new tokens, may reach its other queries too.  Queries
  * without a key to read, those from counts[b] on among them, get zeros and -infinity in lse.

@@ -240,7 +240,9 @@ def cached_attention(q, k_pages, v_pages, page_table, lengths, *, counts=None, t
     (None: all) or j < sinks.
     ``tree`` bool [batch, tokens, tokens] or [tokens, tokens], for drafted tokens: token i reads the new token j where tree[i, j], and
     of the tokens before them what the window leaves, counted from the place lengths[b] + the number of new tokens other than itself that
-    it reads.  Keys that have no page are not read.  What lies where no token of a sample reads has no effect; an infinity or NaN in a
+    it reads.  New tokens are read by the tree alone, whatever the window: of a branch longer than the window a caller takes the tokens that
+    lie a window or more behind out of a row (but first tokens that stay visible) to get what ``window_attention`` would read.  Keys that
+    have no page are not read.  What lies where no token of a sample reads has no effect; an infinity or NaN in a
     value that some read, or under a tree in that of any new token, may reach the sample's other tokens.  Tokens that read nothing, those behind counts[b] among them, get
     zeros.  Returns the result, or with ``return_lse`` also the logarithm of each row's sum of exponentials, float32 [batch,
     q_heads, tokens].  There is no gradient: inputs that require one are refused.
