@@ -12,8 +12,9 @@ their work on torch's current stream of the tensors' device; results are new con
 that do without it.  Sums are held in float32 and results rounded once to the tensors' type.  ``cross_attention`` also rounds what its
 products on the tensor cores take, the weights P and in the backward pass dS = P (dP - delta), to the tensors' type, with delta from the
 rounded result where keys are more than 128: errors of 1.4 to 1.6 roundings instead of one.  In float16 a dS beyond 65504 is infinite,
-as a loss scaler expects of a scale that is too high.  ``window_attention`` and ``cached_attention`` round alike.  The same call gives the same bits again.  Wrong arguments raise ``ValueError``;
-there is no CPU path.
+as a loss scaler expects of a scale that is too high.  ``cached_attention`` and ``window_attention`` round alike, the latter with delta from
+the rounded result where the 128 rows of a tile (tokens times the query heads of a key head) read more than two tiles of 128 keys.  The
+same call gives the same bits again.  Wrong arguments raise ``ValueError``; there is no CPU path.
 """
 import importlib
 
@@ -221,7 +222,8 @@ def append_rotary(q, k, v, positions, frequencies, sections, k_pages, v_pages, p
     ``q`` [batch, tokens, q_heads, head_dim] or None, ``k``, ``v`` [batch, tokens, kv_heads, head_dim], ``positions`` [axes, batch,
     tokens], ``frequencies``, ``sections``, ``adjacent`` and ``interleaved`` as in ``rotary``; ``positions`` None: a token's place in its
     sequence, on every axis.
-    ``k_pages``, ``v_pages`` [pages, page_size, kv_heads, head_dim] of k's type, written in place; page_size a power of two from 8 on.
+    ``k_pages``, ``v_pages`` [pages, page_size, kv_heads, head_dim] of k's type, written in place; page_size a power of two from 8 on.  Pools
+    of float32, and of heads of more than 128 or not a multiple of 8, are for readers of one's own: ``cached_attention`` does not take them.
     ``page_table`` [batch, pages of a sample] int32 or int64: place s of sample b lies in row s % page_size of page
     page_table[b, s // page_size]; an entry that is no page (-1) has no room.  ``lengths`` [batch] int32 or int64: the tokens that the
     cache holds; the new ones go to the places behind them.  ``counts`` [batch] int32 or int64: of a padded batch, how many of a

@@ -733,6 +733,8 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
   f.rows = row_tiles(p);
   f.splits = f.cluster = 1;
   const int64_t sixteens = (static_cast<int64_t>(p.tokens) * p.group + 15) / 16, heads = static_cast<int64_t>(p.batch) * p.kv_heads;
+  // Samples and splits lie along the grid's third dimension, up to 64 splits each; more samples go by tiles of 128 rows, of which a single
+  // token leaves most empty (8 heads on 2 of 128, up to 1501 keys: 1023 samples 204 us, 1024 381; up to 101 keys 30 and 148).
   f.steps = paged && sixteens <= 1 && p.kv_heads <= 65535 && p.batch * int64_t{64} <= 65535;
   f.halves = paged && !f.steps && f.rows.tiles == 1;
   if (f.steps) {
@@ -740,10 +742,10 @@ ForwardParams forward_plan(const CausalParams& p, bool paged, int sms) {
     if (p.window != INT32_MAX) reach = std::min(reach, static_cast<int64_t>(p.window) + p.tokens + std::min(p.sinks, p.cache.capacity) + 32);
     // A CTA for each SM at most, joined within clusters of up to eight, where that leaves it 800 keys or fewer.  Else shares of a key head's
     // keys: up to 320 CTAs in all, of 128 keys at least, dealt to clusters; long stretches are cut at 1500 keys and by splits alone,
-    // since samples are of different lengths and clusters wait for places side by side.  us for clusters x splits, the first ones of each
-    // alone on their SMs: 8 heads, 1602 keys 8x1 8.0, 8x2 14.7, 4x4 9.8; 6001 keys 8x1 14.9, 8x4 13.7; 24001 keys 8x1 41.7, 8x4 27.9;
-    // 32 heads, 1505 keys 4x1 7.9, 8x1 10.6; 3001 keys 4x1 14.8, 8x1 18.7; 160 heads, windows of 1028 keys 1x1 28.7, 2x1 18.6, 4x1 20.3;
-    // 128 heads, up to 24001 keys 1x1 276, 2x1 371, 8x2 238, 1x16 223.
+    // since samples are of different lengths and clusters wait for places side by side.  us for clusters x splits, what this takes first:
+    // 8 heads, 1602 keys 8x1 8.0, 8x2 14.7, 4x4 9.8; 32 heads, 1505 keys 4x1 7.9, 8x1 10.6; 3001 keys 4x1 14.8, 8x1 18.7; 128 heads, up to
+    // 24001 keys 1x16 220, 1x1 276, 2x1 371, 8x2 238.  Not the best everywhere: 8 heads, 6001 keys 8x1 15.0, 8x4 13.7, 4x4 13.3; 24001 keys
+    // 8x5 30.6, 8x1 41.7, 8x4 27.9, 4x4 27.5; 160 heads, windows of 1028 keys 2x1 18.7, 1x1 28.7, 4x1 20.3, 1x2 17.3.
     while (f.cluster < 8 && 2 * heads * f.cluster <= sms && f.cluster * 2 <= reach / 128) f.cluster *= 2;
     if (heads * f.cluster > sms || reach > 800 * f.cluster) {
       f.cluster = 1;
