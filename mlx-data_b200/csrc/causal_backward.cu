@@ -4,8 +4,8 @@
 // head, as in the forward pass.  First tokens that stay visible are keys of every query behind them: their tiles' rows are split among
 // CTAs, whose parts a third kernel adds in order.
 //
-// 10 D operations a pair by the definition, 14 D here.  Measured: 8192 tokens, 32 heads on 8 of 128, window 2048, 4 first tokens: 471 us
-// for queries (tensor pipe active for 42 %), 519 for keys (52 %); with the forward pass, 16384 tokens: 2694-2765 us, 670 TFLOP/s by
+// 10 D operations a pair by the definition, 14 D here.  Measured: 8192 tokens, 32 heads on 8 of 128, window 2048, 4 first tokens: 471-484
+// us for queries (tensor pipe active for 41 %), 514-519 for keys (52 %); with the forward pass, 16384 tokens: 2694-2770 us, 650 TFLOP/s by
 // the definition.  Bound by shared memory and by the chain of a tile: products of 128 x 128 x 16 read 128 bytes a cycle where both
 // operands lie there, so a tile of the first kernel takes 1800 cycles of it with its copies, of 2840 measured.
 #include <algorithm>

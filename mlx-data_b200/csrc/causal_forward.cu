@@ -11,7 +11,7 @@
 // tile of keys, and 3300 to 3600 as measured: products read both operands from shared memory, 128 bytes a cycle, which copies and
 // exchanges share, and a tile's softmax (1600 to 1900 cycles) and products follow one another.  A job's first and last tiles, of which a
 // part is masked, and its results cost about 4 us more.  Measured: 2 x 4099 tokens, 32 heads on 8 of 128, window 1024, 4 first tokens
-// 173-177 us, 690 TFLOP/s (43 % of the measured rate); a chunk of 2048 tokens behind 6404 keys 268-277 us, 910; eight trees of 25 drafts
+// 173-178 us, 680 TFLOP/s (42 % of the measured rate); a chunk of 2048 tokens behind 6404 keys 268-277 us, 910; eight trees of 25 drafts
 // over up to 8217 keys 68 us, 3.1 TB/s, of which CTAs stream for 36.  Stores of results by tile copies took 3000 to 6000 cycles a tile
 // and held up the softmax, or, from a warp of their own, the next tile's: rows go from registers, 32 bytes a thread.
 #include <algorithm>
